@@ -22,6 +22,7 @@ _i = ctypes.c_int
 _f = ctypes.c_float
 _sz = ctypes.c_size_t
 _ip = ctypes.POINTER(ctypes.c_int)
+_szp = ctypes.POINTER(ctypes.c_size_t)
 
 # name -> (restype, argtypes); mirrors include/tagi_hip.h one to one
 SIGNATURES = {
@@ -66,6 +67,17 @@ SIGNATURES = {
     "tagi_batchnorm2d_fwd": (_i, [_vp] * 8 + [_i, _f, _i, _i, _i] + [_vp] * 3),
     "tagi_batchnorm2d_fwd_res": (_i, [_vp] * 10 + [_i, _f, _i, _i, _i] + [_vp] * 3),
     "tagi_batchnorm2d_bwd": (_i, [_vp] * 9 + [_f] + [_i] * 6 + [_vp] * 7),
+    "tagi_layernorm_fwd": (_i, [_vp] * 6 + [_i, _f, _i, _i] + [_vp] * 5),
+    "tagi_layernorm_bwd_scratch": (_i, [_i, _i, _szp]),
+    "tagi_layernorm_bwd": (_i, [_vp] * 9 + [_f] + [_i] * 5 + [_vp] * 8),
+    "tagi_grouped_linear_fwd": (_i, [_vp] * 8 + [_i] * 6 + [_vp] * 3),
+    "tagi_grouped_linear_fwd_act": (_i, [_vp] * 8 + [_i] * 7 + [_vp] * 4),
+    "tagi_grouped_linear_bwd": (_i, [_vp] * 9 + [_i] * 8 + [_vp] * 7),
+    "tagi_moe_route_scratch": (_i, [_i, _i, _szp]),
+    "tagi_moe_route": (_i, [_vp] * 2 + [_i] * 3 + [_vp] * 9),
+    "tagi_moe_combine_fwd": (_i, [_vp] * 5 + [_i] * 4 + [_vp] * 3),
+    "tagi_moe_combine_bwd": (_i, [_vp] * 7 + [_i] * 5 + [_vp] * 5),
+    "tagi_moe_gather_bwd": (_i, [_vp] * 6 + [_i] * 4 + [_vp] * 3),
     "tagi_avgpool2d_build_idx": (_i, [_i] * 6 + [_ip] * 5),
     "tagi_avgpool2d_fwd": (_i, [_vp] * 3 + [_i] * 4 + [_vp] * 3),
     "tagi_avgpool2d_bwd_dz": (_i, [_vp] * 4 + [_i] * 7 + [_vp] * 3),
@@ -143,6 +155,20 @@ def tune(key, value):
 
 def cap_factor(batch_size, prev=1.0):
     return float(lib.tagi_cap_factor(int(batch_size), float(prev)))
+
+
+def layernorm_bwd_scratch(n, B):
+    """Bytes of scratch that tagi_layernorm_bwd needs for the parameter innovations."""
+    size = ctypes.c_size_t(0)
+    check(lib.tagi_layernorm_bwd_scratch(n, B, ctypes.byref(size)))
+    return size.value
+
+
+def moe_route_scratch(T, E):
+    """Bytes of scratch that tagi_moe_route needs."""
+    size = ctypes.c_size_t(0)
+    check(lib.tagi_moe_route_scratch(T, E, ctypes.byref(size)))
+    return size.value
 
 
 def conv2d_out_size(kernel, stride, wi, hi, pad, pad_type):

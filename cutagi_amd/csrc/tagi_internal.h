@@ -307,6 +307,53 @@ hipError_t launch_conv2d_bwd_db(const float *var_b, const float *dmu, const floa
                                 int fo, int woho, int chunks, float *scratch, float *dmu_b,
                                 float *dvar_b, hipStream_t stream);
 
+// LayerNorm (tagi_layernorm.hip): mu_b / var_b / jcb may be null
+size_t layernorm_bwd_scratch_floats(int n, int B);
+hipError_t launch_layernorm_fwd(const float *mu_w, const float *var_w, const float *mu_b,
+                                const float *var_b, const float *mu_a, const float *var_a,
+                                float epsilon, int n, int B, float *mu_s, float *var_s,
+                                float *mu_z, float *var_z, hipStream_t stream);
+hipError_t launch_layernorm_bwd(const float *mu_w, const float *var_w, const float *var_b,
+                                const float *mu_a, const float *jcb, const float *mu_s,
+                                const float *var_s, const float *dmu_out, const float *dvar_out,
+                                float epsilon, int n, int B, int state_update, int param_update,
+                                float *scratch, float *dmu, float *dvar, float *dmu_w,
+                                float *dvar_w, float *dmu_b, float *dvar_b, hipStream_t stream);
+
+// Mixture of experts (tagi_moe.hip)
+size_t moe_route_scratch_ints(int T, int E);
+hipError_t launch_moe_route(const float *mu_s, const float *var_s, int T, int E, int k, int *expert,
+                            float *mu_g, float *var_g, float *jcb_g, int *offsets, int *token,
+                            int *slot, int *scratch, hipStream_t stream);
+hipError_t launch_moe_combine_fwd(const float *mu_g, const float *var_g, const float *mu_y,
+                                  const float *var_y, const int *slot, int T, int k, int R, int N,
+                                  float *mu_z, float *var_z, hipStream_t stream);
+hipError_t launch_moe_combine_bwd(const float *mu_g, const float *jcb_g, const float *mu_y,
+                                  const int *expert, const int *slot, const float *dmu,
+                                  const float *dvar, int T, int k, int R, int N, int E,
+                                  float *dmu_y, float *dvar_y, float *dmu_s, float *dvar_s,
+                                  hipStream_t stream);
+hipError_t launch_moe_gather_bwd(const float *dmu_r, const float *dvar_r, const int *slot,
+                                 const float *jcb, const float *res_mu, const float *res_var, int T,
+                                 int k, int R, int K, float *dmu, float *dvar, hipStream_t stream);
+
+// Linear layers grouped by expert (tagi_grouped.hip): rows offsets[e] .. offsets[e+1] of the
+// R rows meet the weights [e][N][K].
+//   FWD: x0,x1 = mu_a,var_a [T or R][K]   y0,y1 = mu_w,var_w    e0,e1 = biases (may be null)
+//   DZ : x0,x1 = innovations [R][N]       y0 = mu_w             e0 = jcb [R][K] (may be null)
+//   DW : x0,x1 = innovations [R][N]       y0 = mu_a [T or R][K] e0 = var_w
+//   bias innovations: x0,x1 = innovations, e0 = var_b
+// rows (may be null): row r reads row rows[r] of the activations (T of them).
+enum GroupedMode { GROUPED_FWD = 0, GROUPED_DZ = 1, GROUPED_DW = 2 };
+struct GroupedParams {
+    const float *x0, *x1, *y0, *y1, *e0, *e1;
+    const int *offsets, *rows;
+    int K, N, E, R, T, act;
+    float *out0, *out1, *out2;
+};
+hipError_t launch_grouped(GroupedMode mode, const GroupedParams &p, hipStream_t stream);
+hipError_t launch_grouped_db(const GroupedParams &p, hipStream_t stream);
+
 // Host-side index tables (tagi_conv_idx.cpp)
 int conv2d_out_size(int kernel, int stride, int wi, int hi, int pad, int pad_type, int *wo,
                     int *ho);

@@ -1,0 +1,526 @@
+// The router of a mixture of experts and what joins its experts' outputs, for Gaussian
+// activations, gfx950: choice of the experts and gates of every token, the plan that
+// orders rows by expert, the gated sum and its backward pass.
+#include <cstdint>
+
+#include "tagi_internal.h"
+
+namespace tagi {
+namespace {
+
+constexpr int TPB = 256;
+
+inline bool aligned16(const void *q) { return (reinterpret_cast<uintptr_t>(q) & 15u) == 0; }
+
+// ---------------------------------------------------------------------------
+// Choice. 2^g_log lanes hold the scores of one token, lane i the experts i, i + 2^g_log,
+// ... (NS of them); top_k rounds of a maximum over (score, lowest index first), each of
+// which takes its winner out. A score of -inf or NaN has the key 0 and is never chosen.
+// The gates are the softmax of the chosen means:
+//   g_j = e_j / S, e_j = exp(s_j - s_0) (s_0 is the largest), S = sum e
+//   dg_j/ds_j = g_j (S - e_j) / S, with S - e_j summed from the other weights, so that a
+//   gate next to one keeps its slope
+// Lane j of the token keeps choice j (top_k <= 64, and <= the lanes where those are fewer).
+// ---------------------------------------------------------------------------
+constexpr int ROUTE_TOKENS = 128;   // tokens of a workgroup of the plan
+constexpr int MASK_WORDS = ROUTE_TOKENS / 32;
+
+__device__ __forceinline__ unsigned order_bits(float s) {
+    if (!(s > -INFINITY)) return 0u;
+    const unsigned u = __float_as_uint(s + 0.f);   // -0 ties with 0
+    return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+__device__ __forceinline__ float from_order_bits(unsigned k) {
+    return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
+}
+
+struct RouteOut {
+    int *expert;              // [T][k]
+    float *mu_g, *var_g, *jcb_g;
+    int *offsets;             // [E + 1]
+    int *token, *slot;        // [T k], [T][k]
+};
+
+// Chooses for the tokens [t0, t1) of a workgroup; every chosen (token, expert) is set in
+// `mask` (LDS, [E][MASK_WORDS], cleared by the caller).
+template <int NS>
+__device__ __forceinline__ void choose(const float *__restrict__ mu_s,
+                                       const float *__restrict__ var_s, int E, int k, int t0,
+                                       int t1, int g_log, const RouteOut &o, unsigned *mask) {
+    const int G = 1 << g_log, gl = threadIdx.x & (G - 1);
+    const int sub = threadIdx.x >> g_log, subs = TPB >> g_log;
+    for (int tb = t0; tb < t1; tb += subs) {
+        const int t = tb + sub;
+        const bool live = t < t1;   // (the shuffles below need every lane)
+        unsigned key[NS];
+#pragma unroll
+        for (int i = 0; i < NS; i++) {
+            const int e = (i << g_log) + gl;
+            key[i] = live && e < E ? order_bits(mu_s[(size_t)t * E + e]) : 0u;
+        }
+        float top = 0.f, w = 0.f, others = 0.f;
+        int chosen = -1;
+        for (int j = 0; j < k; j++) {
+            unsigned best = 0u, at = 0xffffffffu;
+#pragma unroll
+            for (int i = 0; i < NS; i++)
+                if (key[i] > best) {
+                    best = key[i];
+                    at = (unsigned)((i << g_log) + gl);
+                }
+            for (int off = G >> 1; off > 0; off >>= 1) {
+                const unsigned ob = __shfl_xor(best, off, 64), oa = __shfl_xor(at, off, 64);
+                if (ob > best || (ob == best && oa < at)) {
+                    best = ob;
+                    at = oa;
+                }
+            }
+            if (best != 0u) {
+                const float sc = from_order_bits(best);
+                if (j == 0) top = sc;
+                const float e = sc == top ? 1.f : expf(sc - top);   // (inf ties with inf)
+                if (j == gl) {
+                    w = e;
+                    chosen = (int)at;
+                } else {
+                    others += e;
+                }
+#pragma unroll
+                for (int i = 0; i < NS; i++)
+                    if ((unsigned)((i << g_log) + gl) == at) key[i] = 0u;
+            }
+        }
+        if (!live || gl >= k) continue;
+        float g = 0.f, jc = 0.f, vg = 0.f;
+        if (chosen >= 0) {
+            const float sum = w + others;
+            g = w / sum;
+            jc = g * (others / sum);
+            vg = jc * jc * var_s[(size_t)t * E + chosen];
+            const int tl = t - t0;
+            atomicOr(&mask[chosen * MASK_WORDS + (tl >> 5)], 1u << (tl & 31));
+        }
+        const size_t c = (size_t)t * k + gl;
+        o.expert[c] = chosen;
+        o.mu_g[c] = g;
+        o.var_g[c] = vg;
+        o.jcb_g[c] = jc;
+    }
+}
+
+__device__ __forceinline__ int mask_count(const unsigned *mask, int e) {
+    int c = 0;
+#pragma unroll
+    for (int i = 0; i < MASK_WORDS; i++) c += __popc(mask[e * MASK_WORDS + i]);
+    return c;
+}
+
+// Exclusive prefix of v over the workgroup's threads; *total: the sum.
+__device__ __forceinline__ int block_scan(int v, int *s, int *total) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int inc = v;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+        const int u = __shfl_up(inc, off, 64);
+        if (lane >= off) inc += u;
+    }
+    if (lane == 63) s[wave] = inc;
+    __syncthreads();
+    int before = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < TPB / 64; w++) {
+        if (w < wave) before += s[w];
+        all += s[w];
+    }
+    __syncthreads();
+    *total = all;
+    return before + inc - v;
+}
+
+// Offsets of the experts from their row counts. Thread x owns the experts x * per ... of
+// consecutive per = ceil(E / TPB); count(e) gives the total, first(e) the rows of earlier
+// workgroups; base[e] (LDS) becomes the first row of this workgroup's part of expert e.
+template <typename Count, typename First>
+__device__ __forceinline__ int expert_bases(int E, Count count, First first, int *s, int *base,
+                                            int *offsets_out) {
+    const int per = (E + TPB - 1) / TPB;
+    const int e0 = min(E, (int)threadIdx.x * per), e1 = min(E, e0 + per);
+    int mine = 0;
+    for (int e = e0; e < e1; e++) mine += count(e);
+    int total = 0;
+    int at = block_scan(mine, s, &total);
+    for (int e = e0; e < e1; e++) {
+        if (offsets_out != nullptr) offsets_out[e] = at;
+        base[e] = at + first(e);
+        at += count(e);
+    }
+    if (offsets_out != nullptr && threadIdx.x == 0) offsets_out[E] = total;
+    __syncthreads();
+    return total;
+}
+
+// Rows of the choices of the tokens [t0, t1): base[e] + the number of earlier tokens of the
+// workgroup with the same expert.
+__device__ __forceinline__ void place(int k, int t0, int t1, const RouteOut &o,
+                                      const unsigned *mask, const int *base) {
+    for (int c = t0 * k + threadIdx.x; c < t1 * k; c += TPB) {
+        const int e = o.expert[c], t = c / k, tl = t - t0;
+        int row = -1;
+        if (e >= 0) {
+            row = base[e];
+            for (int i = 0; i < (tl >> 5); i++) row += __popc(mask[e * MASK_WORDS + i]);
+            row += __popc(mask[e * MASK_WORDS + (tl >> 5)] & ((1u << (tl & 31)) - 1u));
+            o.token[row] = t;
+        }
+        o.slot[c] = row;
+    }
+}
+
+// LDS: mask [E][MASK_WORDS], base [E]
+extern __shared__ unsigned route_lds[];
+
+// Up to ROUTE_TOKENS tokens: everything in one workgroup.
+template <int NS>
+__global__ __launch_bounds__(TPB) void route_one_kernel(const float *__restrict__ mu_s,
+                                                        const float *__restrict__ var_s, int T,
+                                                        int E, int k, int g_log, RouteOut o) {
+    __shared__ int s[TPB / 64];
+    unsigned *mask = route_lds;
+    int *base = reinterpret_cast<int *>(route_lds + E * MASK_WORDS);
+    for (int i = threadIdx.x; i < E * MASK_WORDS; i += TPB) mask[i] = 0u;
+    __syncthreads();
+    choose<NS>(mu_s, var_s, E, k, 0, T, g_log, o, mask);
+    __syncthreads();
+    const int total = expert_bases(
+        E, [&](int e) { return mask_count(mask, e); }, [](int) { return 0; }, s, base, o.offsets);
+    place(k, 0, T, o, mask, base);
+    for (int r = total + threadIdx.x; r < T * k; r += TPB) o.token[r] = -1;
+}
+
+// counts [blocks][E]: rows of every expert in every workgroup's tokens
+template <int NS>
+__global__ __launch_bounds__(TPB) void route_choose_kernel(const float *__restrict__ mu_s,
+                                                           const float *__restrict__ var_s, int T,
+                                                           int E, int k, int g_log, RouteOut o,
+                                                           int *__restrict__ counts) {
+    unsigned *mask = route_lds;
+    for (int i = threadIdx.x; i < E * MASK_WORDS; i += TPB) mask[i] = 0u;
+    __syncthreads();
+    const int t0 = blockIdx.x * ROUTE_TOKENS;
+    choose<NS>(mu_s, var_s, E, k, t0, min(T, t0 + ROUTE_TOKENS), g_log, o, mask);
+    __syncthreads();
+    for (int e = threadIdx.x; e < E; e += TPB) counts[(size_t)blockIdx.x * E + e] = mask_count(mask, e);
+}
+
+// One wave per expert: counts [blocks][E] become the exclusive sums over the workgroups,
+// totals [E] the sums.
+__global__ __launch_bounds__(64) void route_scan_kernel(int *__restrict__ counts, int blocks,
+                                                        int E, int *__restrict__ totals) {
+    const int e = blockIdx.x, lane = threadIdx.x;
+    int carry = 0;
+    for (int b0 = 0; b0 < blocks; b0 += 64) {
+        const int b = b0 + lane;
+        const int v = b < blocks ? counts[(size_t)b * E + e] : 0;
+        int inc = v;
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) {
+            const int u = __shfl_up(inc, off, 64);
+            if (lane >= off) inc += u;
+        }
+        if (b < blocks) counts[(size_t)b * E + e] = carry + inc - v;
+        carry += __shfl(inc, 63, 64);
+    }
+    if (lane == 0) totals[e] = carry;
+}
+
+__global__ __launch_bounds__(TPB) void route_place_kernel(int T, int E, int k, RouteOut o,
+                                                          const int *__restrict__ counts,
+                                                          const int *__restrict__ totals) {
+    __shared__ int s[TPB / 64];
+    unsigned *mask = route_lds;
+    int *base = reinterpret_cast<int *>(route_lds + E * MASK_WORDS);
+    for (int i = threadIdx.x; i < E * MASK_WORDS; i += TPB) mask[i] = 0u;
+    __syncthreads();
+    const int t0 = blockIdx.x * ROUTE_TOKENS, t1 = min(T, t0 + ROUTE_TOKENS);
+    for (int c = t0 * k + threadIdx.x; c < t1 * k; c += TPB) {
+        const int e = o.expert[c], tl = c / k - t0;
+        if (e >= 0) atomicOr(&mask[e * MASK_WORDS + (tl >> 5)], 1u << (tl & 31));
+    }
+    const int total = expert_bases(
+        E, [&](int e) { return totals[e]; },
+        [&](int e) { return counts[(size_t)blockIdx.x * E + e]; }, s, base,
+        blockIdx.x == 0 ? o.offsets : nullptr);
+    place(k, t0, t1, o, mask, base);
+    for (int r = total + blockIdx.x * TPB + threadIdx.x; r < T * k; r += gridDim.x * TPB)
+        o.token[r] = -1;
+}
+
+// ---------------------------------------------------------------------------
+// The gated sum, W features of one token per thread. A choice without a row (slot < 0, or a
+// slot that is no row) adds nothing.
+//   mu_z = sum_j g y,  var_z = sum_j (g^2 + var_g) var_y + var_g y^2
+// ---------------------------------------------------------------------------
+template <int W>
+__device__ __forceinline__ void load_w(const float *p, float (&v)[W]) {
+    if (W == 4) {
+        const float4 q = *reinterpret_cast<const float4 *>(p);
+        v[0] = q.x;
+        v[1 % W] = q.y;
+        v[2 % W] = q.z;
+        v[3 % W] = q.w;
+    } else {
+        v[0] = p[0];
+    }
+}
+template <int W>
+__device__ __forceinline__ void store_w(float *p, const float (&v)[W]) {
+    if (W == 4)
+        *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1 % W], v[2 % W], v[3 % W]);
+    else
+        p[0] = v[0];
+}
+
+template <int W>
+__global__ __launch_bounds__(TPB) void combine_fwd_kernel(
+    const float *__restrict__ mu_g, const float *__restrict__ var_g,
+    const float *__restrict__ mu_y, const float *__restrict__ var_y, const int *__restrict__ slot,
+    int T, int k, int R, int N, float *__restrict__ mu_z, float *__restrict__ var_z) {
+    const int groups = N / W;
+    const size_t total = (size_t)T * groups, step = (size_t)gridDim.x * TPB;
+    for (size_t i = (size_t)blockIdx.x * TPB + threadIdx.x; i < total; i += step) {
+        const int t = (int)(i / groups);
+        const size_t f = (i - (size_t)t * groups) * W;
+        float om[W], ov[W];
+#pragma unroll
+        for (int c = 0; c < W; c++) om[c] = ov[c] = 0.f;
+        for (int j = 0; j < k; j++) {
+            const size_t at = (size_t)t * k + j;
+            const int r = slot[at];
+            if ((unsigned)r >= (unsigned)R) continue;
+            const float g = mu_g[at], vg = var_g[at], g2 = g * g + vg;
+            float y[W], v[W];
+            load_w<W>(mu_y + (size_t)r * N + f, y);
+            load_w<W>(var_y + (size_t)r * N + f, v);
+#pragma unroll
+            for (int c = 0; c < W; c++) {
+                om[c] += g * y[c];
+                ov[c] += g2 * v[c] + vg * y[c] * y[c];
+            }
+        }
+        store_w<W>(mu_z + (size_t)t * N + f, om);
+        store_w<W>(var_z + (size_t)t * N + f, ov);
+    }
+}
+
+// Backward, THREADS threads per token:
+//   rows    dmu_y = g dmu,  dvar_y = g^2 dvar
+//   scores  dmu_s[e] = jcb_g sum_n y dmu,  dvar_s[e] = jcb_g^2 sum_n y^2 dvar;
+//           zero for the experts that the token did not choose
+template <int THREADS, int W>
+__global__ __launch_bounds__(TPB) void combine_bwd_kernel(
+    const float *__restrict__ mu_g, const float *__restrict__ jcb_g,
+    const float *__restrict__ mu_y, const int *__restrict__ expert, const int *__restrict__ slot,
+    const float *__restrict__ dmu, const float *__restrict__ dvar, int T, int k, int R, int N,
+    int E, float *__restrict__ dmu_y, float *__restrict__ dvar_y, float *__restrict__ dmu_s,
+    float *__restrict__ dvar_s) {
+    __shared__ float s[2][TPB / 64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int x = threadIdx.x % THREADS;
+    const int groups = N / W;
+    // (whole waves leave the loop, and whole workgroups where it holds a barrier)
+    for (long long t = (long long)blockIdx.x * (TPB / THREADS) + threadIdx.x / THREADS; t < T;
+         t += (long long)gridDim.x * (TPB / THREADS)) {
+        for (int e = x; e < E; e += THREADS) {
+            dmu_s[(size_t)t * E + e] = 0.f;
+            dvar_s[(size_t)t * E + e] = 0.f;
+        }
+        for (int j = 0; j < k; j++) {
+            const size_t at = (size_t)t * k + j;
+            const int r = slot[at], e = expert[at];
+            const bool live = (unsigned)r < (unsigned)R;   // the same for all threads of the token
+            float sm = 0.f, sv = 0.f;
+            if (live) {
+                const float g = mu_g[at];
+                for (int q = x; q < groups; q += THREADS) {
+                    float y[W], dm[W], dv[W];
+                    load_w<W>(mu_y + (size_t)r * N + (size_t)q * W, y);
+                    load_w<W>(dmu + (size_t)t * N + (size_t)q * W, dm);
+                    load_w<W>(dvar + (size_t)t * N + (size_t)q * W, dv);
+#pragma unroll
+                    for (int c = 0; c < W; c++) {
+                        sm += y[c] * dm[c];
+                        sv += y[c] * y[c] * dv[c];
+                        dm[c] *= g;
+                        dv[c] *= g * g;
+                    }
+                    store_w<W>(dmu_y + (size_t)r * N + (size_t)q * W, dm);
+                    store_w<W>(dvar_y + (size_t)r * N + (size_t)q * W, dv);
+                }
+            }
+#pragma unroll
+            for (int off = 32; off > 0; off >>= 1) {
+                sm += __shfl_xor(sm, off, 64);
+                sv += __shfl_xor(sv, off, 64);
+            }
+            if (THREADS > 64) {
+                if (lane == 0) {
+                    s[0][wave] = sm;
+                    s[1][wave] = sv;
+                }
+                __syncthreads();
+                sm = (s[0][0] + s[0][1]) + (s[0][2] + s[0][3]);
+                sv = (s[1][0] + s[1][1]) + (s[1][2] + s[1][3]);
+                __syncthreads();
+            }
+            // the thread that cleared the entry adds to it, so the accesses stay in order
+            if (live && (unsigned)e < (unsigned)E && x == e % THREADS) {
+                const float jc = jcb_g[at];
+                dmu_s[(size_t)t * E + e] += jc * sm;
+                dvar_s[(size_t)t * E + e] += jc * jc * sv;
+            }
+        }
+    }
+}
+
+// Rows back to tokens: (sum_j rows[slot] + res) * jcb, jcb^2.
+template <int W>
+__global__ __launch_bounds__(TPB) void gather_bwd_kernel(
+    const float *__restrict__ dmu_r, const float *__restrict__ dvar_r,
+    const int *__restrict__ slot, const float *__restrict__ jcb, const float *res_mu,
+    const float *res_var, int T, int k, int R, int K, float *dmu, float *dvar) {
+    const int groups = K / W;
+    const size_t total = (size_t)T * groups, step = (size_t)gridDim.x * TPB;
+    for (size_t i = (size_t)blockIdx.x * TPB + threadIdx.x; i < total; i += step) {
+        const int t = (int)(i / groups);
+        const size_t f = (i - (size_t)t * groups) * W, at = (size_t)t * K + f;
+        float om[W], ov[W];
+        if (res_mu != nullptr) {
+            load_w<W>(res_mu + at, om);
+            load_w<W>(res_var + at, ov);
+        } else {
+#pragma unroll
+            for (int c = 0; c < W; c++) om[c] = ov[c] = 0.f;
+        }
+        for (int j = 0; j < k; j++) {
+            const int r = slot[(size_t)t * k + j];
+            if ((unsigned)r >= (unsigned)R) continue;
+            float m[W], v[W];
+            load_w<W>(dmu_r + (size_t)r * K + f, m);
+            load_w<W>(dvar_r + (size_t)r * K + f, v);
+#pragma unroll
+            for (int c = 0; c < W; c++) {
+                om[c] += m[c];
+                ov[c] += v[c];
+            }
+        }
+        if (jcb != nullptr) {
+            float jc[W];
+            load_w<W>(jcb + at, jc);
+#pragma unroll
+            for (int c = 0; c < W; c++) {
+                om[c] *= jc[c];
+                ov[c] *= jc[c] * jc[c];
+            }
+        }
+        store_w<W>(dmu + at, om);
+        store_w<W>(dvar + at, ov);
+    }
+}
+
+// one thread per item up to MAX_BLOCKS workgroups (a launch holds fewer than 2^32 threads),
+// which then walk on
+constexpr size_t MAX_BLOCKS = (size_t)1 << 22;
+inline unsigned blocks_for(size_t n) {
+    const size_t b = (n + TPB - 1) / TPB;
+    return (unsigned)(b < MAX_BLOCKS ? b : MAX_BLOCKS);
+}
+inline int route_blocks(int T) { return (T + ROUTE_TOKENS - 1) / ROUTE_TOKENS; }
+
+template <int NS>
+hipError_t route(const float *mu_s, const float *var_s, int T, int E, int k, int g_log,
+                 const RouteOut &o, int *scratch, hipStream_t stream) {
+    const int blocks = route_blocks(T);
+    const unsigned lds_mask = E * MASK_WORDS * 4, lds = lds_mask + E * 4;
+    if (blocks == 1) {
+        hipLaunchKernelGGL(route_one_kernel<NS>, dim3(1), dim3(TPB), lds, stream, mu_s, var_s, T, E,
+                           k, g_log, o);
+        return hipGetLastError();
+    }
+    int *totals = scratch, *counts = scratch + E;
+    hipLaunchKernelGGL(route_choose_kernel<NS>, dim3(blocks), dim3(TPB), lds_mask, stream, mu_s,
+                       var_s, T, E, k, g_log, o, counts);
+    hipLaunchKernelGGL(route_scan_kernel, dim3(E), dim3(64), 0, stream, counts, blocks, E, totals);
+    hipLaunchKernelGGL(route_place_kernel, dim3(blocks), dim3(TPB), lds, stream, T, E, k, o, counts,
+                       totals);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+size_t moe_route_scratch_ints(int T, int E) {
+    return route_blocks(T) > 1 ? ((size_t)route_blocks(T) + 1) * E : 0;
+}
+
+hipError_t launch_moe_route(const float *mu_s, const float *var_s, int T, int E, int k, int *expert,
+                            float *mu_g, float *var_g, float *jcb_g, int *offsets, int *token,
+                            int *slot, int *scratch, hipStream_t stream) {
+    const RouteOut o = {expert, mu_g, var_g, jcb_g, offsets, token, slot};
+    int g_log = 0;
+    while (g_log < 6 && (1 << g_log) < E) g_log++;
+    const int ns = (E + 63) / 64;
+    if (ns <= 1) return route<1>(mu_s, var_s, T, E, k, g_log, o, scratch, stream);
+    if (ns <= 4) return route<4>(mu_s, var_s, T, E, k, g_log, o, scratch, stream);
+    return route<16>(mu_s, var_s, T, E, k, g_log, o, scratch, stream);
+}
+
+hipError_t launch_moe_combine_fwd(const float *mu_g, const float *var_g, const float *mu_y,
+                                  const float *var_y, const int *slot, int T, int k, int R, int N,
+                                  float *mu_z, float *var_z, hipStream_t stream) {
+    if (N % 4 == 0 && aligned16(mu_y) && aligned16(var_y) && aligned16(mu_z) && aligned16(var_z))
+        hipLaunchKernelGGL(combine_fwd_kernel<4>, dim3(blocks_for((size_t)T * (N / 4))), dim3(TPB),
+                           0, stream, mu_g, var_g, mu_y, var_y, slot, T, k, R, N, mu_z, var_z);
+    else
+        hipLaunchKernelGGL(combine_fwd_kernel<1>, dim3(blocks_for((size_t)T * N)), dim3(TPB), 0,
+                           stream, mu_g, var_g, mu_y, var_y, slot, T, k, R, N, mu_z, var_z);
+    return hipGetLastError();
+}
+
+hipError_t launch_moe_combine_bwd(const float *mu_g, const float *jcb_g, const float *mu_y,
+                                  const int *expert, const int *slot, const float *dmu,
+                                  const float *dvar, int T, int k, int R, int N, int E,
+                                  float *dmu_y, float *dvar_y, float *dmu_s, float *dvar_s,
+                                  hipStream_t stream) {
+    const bool vec = N % 4 == 0 && aligned16(mu_y) && aligned16(dmu) && aligned16(dvar) &&
+                     aligned16(dmu_y) && aligned16(dvar_y);
+#define COMBINE_BWD(THREADS, W)                                                                  \
+    hipLaunchKernelGGL((combine_bwd_kernel<THREADS, W>),                                          \
+                       dim3(blocks_for((size_t)T * THREADS)), dim3(TPB), 0, stream,               \
+                       mu_g, jcb_g, mu_y, expert, slot, dmu, dvar, T, k, R, N, E, dmu_y, dvar_y,  \
+                       dmu_s, dvar_s)
+    const bool wide = N > 1024;
+    if (vec && wide)
+        COMBINE_BWD(256, 4);
+    else if (vec)
+        COMBINE_BWD(64, 4);
+    else if (wide)
+        COMBINE_BWD(256, 1);
+    else
+        COMBINE_BWD(64, 1);
+#undef COMBINE_BWD
+    return hipGetLastError();
+}
+
+hipError_t launch_moe_gather_bwd(const float *dmu_r, const float *dvar_r, const int *slot,
+                                 const float *jcb, const float *res_mu, const float *res_var, int T,
+                                 int k, int R, int K, float *dmu, float *dvar, hipStream_t stream) {
+    if (K % 4 == 0 && aligned16(dmu_r) && aligned16(dvar_r) && aligned16(jcb) &&
+        aligned16(res_mu) && aligned16(res_var) && aligned16(dmu) && aligned16(dvar))
+        hipLaunchKernelGGL(gather_bwd_kernel<4>, dim3(blocks_for((size_t)T * (K / 4))), dim3(TPB), 0,
+                           stream, dmu_r, dvar_r, slot, jcb, res_mu, res_var, T, k, R, K, dmu, dvar);
+    else
+        hipLaunchKernelGGL(gather_bwd_kernel<1>, dim3(blocks_for((size_t)T * K)), dim3(TPB), 0,
+                           stream, dmu_r, dvar_r, slot, jcb, res_mu, res_var, T, k, R, K, dmu, dvar);
+    return hipGetLastError();
+}
+
+}  // namespace tagi

@@ -5,6 +5,8 @@ computation is one C-ABI call on raw pointers. Shapes follow the reference:
 weights [N, K], activations [B, K], conv weights [fo, fi*k*k], conv activations
 flattened NCHW.
 """
+import collections
+
 import torch
 
 from . import capi
@@ -338,3 +340,233 @@ def add_shortcut_delta(mu_s, var_s, jcb_s, mu_a, var_a):
     capi.check(capi.lib.tagi_add_shortcut_delta(capi.ptr(mu_s), capi.ptr(var_s), capi.ptr(jcb_s),
                                                 mu_a.numel(), capi.ptr(mu_a), capi.ptr(var_a),
                                                 _stream()))
+
+
+# ---- layer norm, grouped Linear layers, mixture of experts ---------------------------------
+
+
+def _chk_shapes(**named):
+    """named: argument name -> (tensor or None, shape, dtype). Every tensor present has to be
+    a contiguous tensor of that shape and type on the current device."""
+    present = [(name, t, shape, dtype) for name, (t, shape, dtype) in named.items() if t is not None]
+    for name, t, shape, dtype in present:
+        if t.dtype != dtype or not t.is_contiguous():
+            raise ValueError("%s: expected a contiguous %s tensor" % (name, dtype))
+        if tuple(t.shape) != tuple(shape):
+            raise ValueError("%s: expected shape %s, got %s" % (name, tuple(shape), tuple(t.shape)))
+    for name, t, _, _ in present:
+        if not t.is_cuda:
+            raise ValueError("%s: expected a device tensor" % name)
+        if t.device.index != torch.cuda.current_device():
+            raise ValueError("%s is on %s, the current device is cuda:%d"
+                             % (name, t.device, torch.cuda.current_device()))
+
+
+def _pair(a, b, names):
+    if (a is None) != (b is None):
+        raise ValueError("%s and %s come together" % names)
+
+
+_F, _I = torch.float32, torch.int32
+
+
+def _dims(name, t, n):
+    """The n sizes of a tensor argument."""
+    if t.dim() != n:
+        raise ValueError("%s: expected %d dimensions, got %s" % (name, n, tuple(t.shape)))
+    return t.shape
+
+
+def layernorm_fwd(mu_w, var_w, mu_b, var_b, mu_a, var_a, eps=1e-5):
+    """Layer norm over the last dimension of mu_a / var_a [B, n]: (mu_z, var_z, mu_s, var_s),
+    mu_s / var_s [B] the statistics of the rows. mu_b / var_b may be None."""
+    _pair(mu_b, var_b, ("mu_b", "var_b"))
+    B, n = _dims("mu_a", mu_a, 2)
+    _chk_shapes(mu_a=(mu_a, (B, n), _F), var_a=(var_a, (B, n), _F), mu_w=(mu_w, (n,), _F),
+                var_w=(var_w, (n,), _F), mu_b=(mu_b, (n,), _F), var_b=(var_b, (n,), _F))
+    mu_z, var_z = torch.empty_like(mu_a), torch.empty_like(mu_a)
+    mu_s, var_s = torch.empty(B, device=mu_a.device), torch.empty(B, device=mu_a.device)
+    capi.check(capi.lib.tagi_layernorm_fwd(
+        capi.ptr(mu_w), capi.ptr(var_w), capi.ptr(mu_b), capi.ptr(var_b), capi.ptr(mu_a),
+        capi.ptr(var_a), int(mu_b is not None), eps, n, B, capi.ptr(mu_s), capi.ptr(var_s),
+        capi.ptr(mu_z), capi.ptr(var_z), _stream()))
+    return mu_z, var_z, mu_s, var_s
+
+
+def layernorm_bwd(mu_w, var_w, var_b, mu_a, jcb, mu_s, var_s, delta_mu, delta_var, eps=1e-5,
+                  state_update=True, param_update=True):
+    """Returns (dz_mu, dz_var, dw_mu, dw_var, db_mu, db_var); entries not asked for are None.
+    jcb may be None (one everywhere)."""
+    B, n = _dims("delta_mu", delta_mu, 2)
+    _chk_shapes(delta_mu=(delta_mu, (B, n), _F), delta_var=(delta_var, (B, n), _F),
+                mu_w=(mu_w, (n,), _F), var_w=(var_w, (n,), _F), var_b=(var_b, (n,), _F),
+                mu_a=(mu_a, (B, n), _F), jcb=(jcb, (B, n), _F), mu_s=(mu_s, (B,), _F),
+                var_s=(var_s, (B,), _F))
+    dev = delta_mu.device
+    out, scratch = [None] * 6, None
+    if state_update:
+        out[0], out[1] = torch.empty_like(delta_mu), torch.empty_like(delta_mu)
+    if param_update:
+        out[2], out[3] = torch.empty(n, device=dev), torch.empty(n, device=dev)
+        if var_b is not None:
+            out[4], out[5] = torch.empty(n, device=dev), torch.empty(n, device=dev)
+        scratch = torch.empty(capi.layernorm_bwd_scratch(n, B), dtype=torch.uint8, device=dev)
+    capi.check(capi.lib.tagi_layernorm_bwd(
+        capi.ptr(mu_w), capi.ptr(var_w), capi.ptr(var_b), capi.ptr(mu_a), capi.ptr(jcb),
+        capi.ptr(mu_s), capi.ptr(var_s), capi.ptr(delta_mu), capi.ptr(delta_var), eps, n, B,
+        int(var_b is not None), int(state_update), int(param_update), capi.ptr(scratch),
+        *[capi.ptr(t) for t in out], _stream()))
+    return tuple(out)
+
+
+def _grouped_shapes(mu_w, var_w, b, offsets, rows, held, R, K):
+    E, N, _ = _dims("weights", mu_w if mu_w is not None else var_w, 3)
+    _chk_shapes(mu_w=(mu_w, (E, N, K), _F), var_w=(var_w, (E, N, K), _F),
+                offsets=(offsets, (E + 1,), _I), rows=(rows, (R,), _I),
+                **{name: (t, (E, N), _F) for name, t in b.items()},
+                **{name: (t, (t.shape[0] if rows is not None else R, K), _F)
+                   for name, t in held.items()})
+    return E, N
+
+
+def grouped_linear_fwd(mu_w, var_w, mu_b, var_b, mu_a, var_a, offsets, rows=None, out=None):
+    """Linear layers [E, N, K], rows grouped by expert: rows offsets[e] .. offsets[e+1] meet
+    the weights of expert e (offsets: int32 [E+1]). rows (int32 [R]): row r is row rows[r] of
+    mu_a / var_a; without it mu_a / var_a [R, K] hold the rows in order. Returns (mu_z, var_z)
+    [R, N]; rows from offsets[E] on are left as `out` held them (unset without `out`)."""
+    return _grouped_fwd(mu_w, var_w, mu_b, var_b, mu_a, var_a, offsets, rows, None, out)
+
+
+def grouped_linear_fwd_act(mu_w, var_w, mu_b, var_b, mu_a, var_a, offsets, activation, rows=None,
+                           out=None):
+    """grouped_linear_fwd with the following activation ("relu" / "mixture_relu") applied in
+    the kernel's epilogue: returns the activation's (mu_a, var_a, jcb), each [R, N]."""
+    return _grouped_fwd(mu_w, var_w, mu_b, var_b, mu_a, var_a, offsets, rows, activation, out)
+
+
+def _grouped_fwd(mu_w, var_w, mu_b, var_b, mu_a, var_a, offsets, rows, activation, out):
+    _pair(mu_b, var_b, ("mu_b", "var_b"))
+    T, K = _dims("mu_a", mu_a, 2)
+    R = T if rows is None else _dims("rows", rows, 1)[0]
+    if var_a.shape != mu_a.shape:
+        raise ValueError("mu_a and var_a: shapes %s, %s" % (tuple(mu_a.shape), tuple(var_a.shape)))
+    E, N = _grouped_shapes(mu_w, var_w, dict(mu_b=mu_b, var_b=var_b), offsets, rows,
+                           dict(mu_a=mu_a, var_a=var_a), R, K)
+    count = 2 if activation is None else 3
+    if out is None:
+        out = tuple(torch.empty((R, N), device=mu_w.device) for _ in range(count))
+    if len(out) != count:
+        raise ValueError("out: expected %d tensors" % count)
+    _chk_shapes(**{"out[%d]" % i: (t, (R, N), _F) for i, t in enumerate(out)})
+    args = [capi.ptr(t) for t in (mu_w, var_w, mu_b, var_b, mu_a, var_a, offsets, rows)]
+    args += [K, N, E, R, T, int(mu_b is not None)]
+    outs = [capi.ptr(t) for t in out]
+    if activation is None:
+        capi.check(capi.lib.tagi_grouped_linear_fwd(*args, *outs, _stream()))
+    else:
+        capi.check(capi.lib.tagi_grouped_linear_fwd_act(*args, ACTIVATIONS[activation], *outs,
+                                                        _stream()))
+    return tuple(out)
+
+
+def grouped_linear_bwd(mu_w, var_w, var_b, mu_a, jcb, delta_mu, delta_var, offsets, rows=None,
+                       state_update=True, param_update=True, out=None):
+    """All of the backward pass: (dz_mu, dz_var [R, K], dw_mu, dw_var [E, N, K], db_mu, db_var
+    [E, N]); entries not asked for are None. dz is per row, also with `rows` (see
+    moe_gather_bwd); jcb [R, K] may be None (one everywhere). Rows from offsets[E] on are left
+    as out[0] and out[1] held them (unset without `out`)."""
+    R, _ = _dims("delta_mu", delta_mu, 2)
+    T, K = _dims("mu_a", mu_a, 2)
+    E, N = _grouped_shapes(mu_w, var_w, dict(var_b=var_b), offsets, rows, dict(mu_a=mu_a), R, K)
+    _chk_shapes(delta_mu=(delta_mu, (R, N), _F), delta_var=(delta_var, (R, N), _F),
+                jcb=(jcb, (R, K), _F))
+    dev, bias = delta_mu.device, var_b is not None
+    shapes = [(R, K)] * 2 + [(E, N, K)] * 2 + [(E, N)] * 2
+    wanted = [state_update] * 2 + [param_update] * 2 + [param_update and bias] * 2
+    if out is None:
+        out = [torch.empty(s, device=dev) if w else None for s, w in zip(shapes, wanted)]
+    if len(out) != 6 or any(w and t is None for w, t in zip(wanted, out)):
+        raise ValueError("out: six entries, None only where nothing is asked for")
+    _chk_shapes(**{"out[%d]" % i: (t, s, _F) for i, (t, s) in enumerate(zip(out, shapes))})
+    capi.check(capi.lib.tagi_grouped_linear_bwd(
+        *[capi.ptr(t) for t in (mu_w, var_w, var_b, mu_a, jcb, delta_mu, delta_var, offsets, rows)],
+        K, N, E, R, T, int(bias), int(state_update), int(param_update),
+        *[capi.ptr(t) for t in out], _stream()))
+    return tuple(t if w else None for w, t in zip(wanted, out))
+
+
+MoeRoutes = collections.namedtuple("MoeRoutes", "expert mu_g var_g jcb_g offsets token slot")
+
+
+def moe_route(mu_s, var_s, top_k):
+    """The router's choice from its scores [T, E]: the top_k experts of the largest means
+    (ties: lowest index; -inf and NaN are never chosen), their softmax gates, and the rows
+    sorted by expert and then by token. Returns MoeRoutes: expert, mu_g, var_g, jcb_g and slot
+    (the row of the choice) [T, top_k], offsets [E+1], token (of every row) [T*top_k]; -1 in
+    expert, slot and token where there is nothing."""
+    T, E = _dims("mu_s", mu_s, 2)
+    if not 1 <= top_k <= E:
+        raise ValueError("top_k %d: expected 1 to %d" % (top_k, E))
+    _chk_shapes(mu_s=(mu_s, (T, E), _F), var_s=(var_s, (T, E), _F))
+    dev = mu_s.device
+    scratch = torch.empty(capi.moe_route_scratch(T, E), dtype=torch.uint8, device=dev)
+    expert, slot = (torch.empty((T, top_k), dtype=_I, device=dev) for _ in range(2))
+    mu_g, var_g, jcb_g = (torch.empty((T, top_k), device=dev) for _ in range(3))
+    offsets = torch.empty(E + 1, dtype=_I, device=dev)
+    token = torch.empty(T * top_k, dtype=_I, device=dev)
+    capi.check(capi.lib.tagi_moe_route(
+        capi.ptr(mu_s), capi.ptr(var_s), T, E, top_k, capi.ptr(scratch), capi.ptr(expert),
+        capi.ptr(mu_g), capi.ptr(var_g), capi.ptr(jcb_g), capi.ptr(offsets), capi.ptr(token),
+        capi.ptr(slot), _stream()))
+    return MoeRoutes(expert, mu_g, var_g, jcb_g, offsets, token, slot)
+
+
+def moe_combine_fwd(mu_g, var_g, mu_y, var_y, slot):
+    """The gated sum of the experts' outputs mu_y / var_y [R, N]: (mu_z, var_z) [T, N]. A
+    choice whose slot is no row adds nothing."""
+    T, k = _dims("mu_g", mu_g, 2)
+    R, N = _dims("mu_y", mu_y, 2)
+    _chk_shapes(mu_g=(mu_g, (T, k), _F), var_g=(var_g, (T, k), _F), slot=(slot, (T, k), _I),
+                mu_y=(mu_y, (R, N), _F), var_y=(var_y, (R, N), _F))
+    mu_z, var_z = (torch.empty((T, N), device=mu_y.device) for _ in range(2))
+    capi.check(capi.lib.tagi_moe_combine_fwd(
+        capi.ptr(mu_g), capi.ptr(var_g), capi.ptr(mu_y), capi.ptr(var_y), capi.ptr(slot), T, k, R,
+        N, capi.ptr(mu_z), capi.ptr(var_z), _stream()))
+    return mu_z, var_z
+
+
+def moe_combine_bwd(mu_g, jcb_g, mu_y, expert, slot, delta_mu, delta_var, num_experts, out=None):
+    """Backward of moe_combine_fwd: (delta_mu_y, delta_var_y [R, N], delta_mu_s, delta_var_s
+    [T, num_experts]), the innovations of the experts' outputs and of the router's scores.
+    Rows that no choice names are left as `out` (two tensors [R, N]) held them (unset without
+    `out`)."""
+    T, k = _dims("mu_g", mu_g, 2)
+    R, N = _dims("mu_y", mu_y, 2)
+    _chk_shapes(mu_g=(mu_g, (T, k), _F), jcb_g=(jcb_g, (T, k), _F), expert=(expert, (T, k), _I),
+                slot=(slot, (T, k), _I), mu_y=(mu_y, (R, N), _F), delta_mu=(delta_mu, (T, N), _F),
+                delta_var=(delta_var, (T, N), _F))
+    dev = mu_y.device
+    dmu_y, dvar_y = out if out is not None else (torch.empty_like(mu_y), torch.empty_like(mu_y))
+    _chk_shapes(**{"out[0]": (dmu_y, (R, N), _F), "out[1]": (dvar_y, (R, N), _F)})
+    dmu_s, dvar_s = (torch.empty((T, num_experts), device=dev) for _ in range(2))
+    capi.check(capi.lib.tagi_moe_combine_bwd(
+        capi.ptr(mu_g), capi.ptr(jcb_g), capi.ptr(mu_y), capi.ptr(expert), capi.ptr(slot),
+        capi.ptr(delta_mu), capi.ptr(delta_var), T, k, R, N, num_experts, capi.ptr(dmu_y),
+        capi.ptr(dvar_y), capi.ptr(dmu_s), capi.ptr(dvar_s), _stream()))
+    return dmu_y, dvar_y, dmu_s, dvar_s
+
+
+def moe_gather_bwd(delta_mu_r, delta_var_r, slot, jcb=None, res_mu=None, res_var=None):
+    """Row innovations [R, K] back to the tokens: jcb * (sum over the token's rows + res), and
+    jcb^2 for the variances, [T, K]."""
+    _pair(res_mu, res_var, ("res_mu", "res_var"))
+    T, k = _dims("slot", slot, 2)
+    R, K = _dims("delta_mu_r", delta_mu_r, 2)
+    _chk_shapes(slot=(slot, (T, k), _I), delta_mu_r=(delta_mu_r, (R, K), _F),
+                delta_var_r=(delta_var_r, (R, K), _F), jcb=(jcb, (T, K), _F),
+                res_mu=(res_mu, (T, K), _F), res_var=(res_var, (T, K), _F))
+    dmu, dvar = (torch.empty((T, K), device=delta_mu_r.device) for _ in range(2))
+    capi.check(capi.lib.tagi_moe_gather_bwd(
+        capi.ptr(delta_mu_r), capi.ptr(delta_var_r), capi.ptr(slot), capi.ptr(jcb),
+        capi.ptr(res_mu), capi.ptr(res_var), T, k, R, K, capi.ptr(dmu), capi.ptr(dvar), _stream()))
+    return dmu, dvar

@@ -441,6 +441,129 @@ int tagi_batchnorm2d_bwd(const float *mu_w, const float *var_w,
                          float *delta_mu_w, float *delta_var_w,
                          float *delta_mu_b, float *delta_var_b, void *stream);
 
+/* ---- LayerNorm ------------------------------------------------------------------ */
+/* Tensors are [B][n]; parameters are [n], statistics [B]. n >= 2. */
+
+/* Per row: mu_s = mean of mu_a, var_s = (sum of squared deviations + sum of var_a) /
+ * (n - 1); then mu_z = (mu_a - mu_s)/sqrt(var_s + eps) * mu_w (+ mu_b) and var_z likewise
+ * with Gaussian weights, as tagi_batchnorm2d_fwd does per channel. The same in training
+ * and evaluation; mu_s / var_s are what the backward pass needs. Counterpart of the
+ * reference's LayerNorm (src/layernorm_layer.cpp, src/layernorm_layer_cuda.cu). */
+int tagi_layernorm_fwd(const float *mu_w, const float *var_w, const float *mu_b,
+                       const float *var_b, const float *mu_a, const float *var_a,
+                       int bias, float epsilon, int n, int B, float *mu_s,
+                       float *var_s, float *mu_z, float *var_z, void *stream);
+
+/* Bytes of device memory that tagi_layernorm_bwd needs as scratch when param_update != 0
+ * (on the current device). Host only. The caller owns it, so that calls recorded into
+ * several graphs need not share any. */
+int tagi_layernorm_bwd_scratch(int n, int B, size_t *bytes /* host, out */);
+
+/* State innovations (state_update) and parameter innovations (param_update; bias ones
+ * only when bias != 0), the statistics taken as constants:
+ *   delta_mu = t * delta_mu_out, delta_var = t^2 * delta_var_out,
+ *              t = mu_w * jcb / sqrt(var_s + eps)
+ *   delta_mu_w = var_w * sum_b x * delta_mu_out, delta_var_w = var_w^2 * sum_b x^2 *
+ *                delta_var_out, x = (mu_a - mu_s)/sqrt(var_s + eps); biases with x = 1
+ * jcb may be NULL (one everywhere). Sums are taken in a fixed order: the same bits every
+ * call. scratch: tagi_layernorm_bwd_scratch bytes, 16-byte aligned; may be NULL without
+ * param_update. */
+int tagi_layernorm_bwd(const float *mu_w, const float *var_w, const float *var_b,
+                       const float *mu_a, const float *jcb, const float *mu_s,
+                       const float *var_s, const float *delta_mu_out,
+                       const float *delta_var_out, float epsilon, int n, int B,
+                       int bias, int state_update, int param_update,
+                       void *scratch, float *delta_mu, float *delta_var,
+                       float *delta_mu_w, float *delta_var_w, float *delta_mu_b,
+                       float *delta_var_b, void *stream);
+
+/* ---- Linear layers grouped by expert ----------------------------------------------- */
+/* E Linear layers of one shape: weights [E][N][K], biases [E][N]. The R rows are sorted
+ * by expert: rows offsets[e] .. offsets[e+1]-1 (device int[E+1], non-decreasing) belong to
+ * expert e, any of which may have none. Rows from offsets[E] on belong to nobody: they are
+ * not read, and what the outputs hold there is left as it was. With rows != NULL (device
+ * int[R]) row r takes its activations from row rows[r] of the T rows of mu_a / var_a, so a
+ * token that several experts see is stored once; an entry outside 0..T-1 stands for a row
+ * of zeros. Offsets outside 0..R are moved to its ends. E <= 1024 (TAGI_ERR_UNSUPPORTED
+ * beyond). No workspace: calls may be captured and may overlap. No counterpart in the
+ * reference, which has one Linear per layer; the arithmetic of a group is
+ * tagi_linear_fwd's and tagi_linear_bwd's. */
+
+/* mu_z, var_z [R][N] */
+int tagi_grouped_linear_fwd(const float *mu_w, const float *var_w, const float *mu_b,
+                            const float *var_b, const float *mu_a, const float *var_a,
+                            const int *offsets, const int *rows /* may be NULL */,
+                            int K, int N, int E, int R, int T, int bias,
+                            float *mu_z, float *var_z, void *stream);
+
+/* With the activation that follows (TAGI_ACT_*), as tagi_linear_fwd_act. */
+int tagi_grouped_linear_fwd_act(const float *mu_w, const float *var_w, const float *mu_b,
+                                const float *var_b, const float *mu_a, const float *var_a,
+                                const int *offsets, const int *rows /* may be NULL */,
+                                int K, int N, int E, int R, int T, int bias,
+                                int activation, float *mu_out, float *var_out,
+                                float *jcb_out, void *stream);
+
+/* All of the backward pass: with state_update the innovations of every ROW, delta_mu_z /
+ * delta_var_z [R][K] (jcb [R][K], NULL: one everywhere; tagi_moe_gather_bwd adds them up
+ * per token), with param_update those of the weights [E][N][K] and, with bias, of the
+ * biases [E][N]: zeros for an expert without rows. */
+int tagi_grouped_linear_bwd(const float *mu_w, const float *var_w, const float *var_b,
+                            const float *mu_a, const float *jcb /* may be NULL */,
+                            const float *delta_mu, const float *delta_var,
+                            const int *offsets, const int *rows /* may be NULL */,
+                            int K, int N, int E, int R, int T, int bias,
+                            int state_update, int param_update, float *delta_mu_z,
+                            float *delta_var_z, float *delta_mu_w, float *delta_var_w,
+                            float *delta_mu_b, float *delta_var_b, void *stream);
+
+/* ---- mixture of experts --------------------------------------------------------------- */
+/* The router's choice. mu_s / var_s [T][E]: the router layer's outputs. Every token takes
+ * the top_k experts of the largest mean score (ties: the lowest index); a score of -inf or
+ * NaN is never chosen, so a token may end with fewer, and a token whose scores are all -inf
+ * (an empty place of a batch) with none. The gates are the softmax of the chosen means,
+ * linearised for the variance: mu_g = softmax, jcb_g = mu_g (1 - mu_g), var_g = jcb_g^2
+ * var_s. Outputs, [T][top_k] in falling order of the scores:
+ *   expert   the expert, -1 where none was left (its gate, variance and slope are 0)
+ *   slot     its row, -1 where none
+ * and the plan of the rows, sorted by expert and then by token:
+ *   offsets [E+1]     first row of every expert; offsets[E] rows in all
+ *   token [T*top_k]   the token of every row, -1 behind the last
+ * scratch: tagi_moe_route_scratch bytes of device memory, owned by the caller (may be NULL
+ * where that is 0). E <= 1024, top_k <= 64 (TAGI_ERR_UNSUPPORTED beyond), top_k <= E. */
+int tagi_moe_route_scratch(int T, int E, size_t *bytes /* host, out */);
+int tagi_moe_route(const float *mu_s, const float *var_s, int T, int E, int top_k,
+                   void *scratch, int *expert, float *mu_g, float *var_g, float *jcb_g,
+                   int *offsets, int *token, int *slot, void *stream);
+
+/* The gated sum of the chosen experts' outputs (mu_y, var_y [R][N]), gates and outputs
+ * independent Gaussians:
+ *   mu_z = sum_j mu_g mu_y,  var_z = sum_j (mu_g^2 + var_g) var_y + var_g mu_y^2    [T][N]
+ * A choice whose slot is not in 0..R-1 adds nothing; a token without any gets zeros. */
+int tagi_moe_combine_fwd(const float *mu_g, const float *var_g, const float *mu_y,
+                         const float *var_y, const int *slot, int T, int top_k, int R,
+                         int N, float *mu_z, float *var_z, void *stream);
+
+/* Its backward pass: the innovations of the experts' outputs, delta_mu_y = mu_g delta_mu,
+ * delta_var_y = mu_g^2 delta_var at the rows that slot names (each at most once; other
+ * rows are left as they were), and those of the router's scores [T][E]:
+ *   delta_mu_s = jcb_g sum_n mu_y delta_mu,  delta_var_s = jcb_g^2 sum_n mu_y^2 delta_var
+ * for the chosen experts, zero for the others. */
+int tagi_moe_combine_bwd(const float *mu_g, const float *jcb_g, const float *mu_y,
+                         const int *expert, const int *slot, const float *delta_mu,
+                         const float *delta_var, int T, int top_k, int R, int N, int E,
+                         float *delta_mu_y, float *delta_var_y, float *delta_mu_s,
+                         float *delta_var_s, void *stream);
+
+/* Row innovations back to the tokens: delta_mu = jcb (sum_j delta_mu_r[slot] + res_mu),
+ * delta_var = jcb^2 (sum_j delta_var_r[slot] + res_var), [T][K]. res_* (another branch that
+ * starts at the same tokens, as the router) may be NULL, or the outputs themselves; jcb may
+ * be NULL (one everywhere). */
+int tagi_moe_gather_bwd(const float *delta_mu_r, const float *delta_var_r,
+                        const int *slot, const float *jcb, const float *res_mu,
+                        const float *res_var, int T, int top_k, int R, int K,
+                        float *delta_mu, float *delta_var, void *stream);
+
 /* ---- AvgPool2d ---------------------------------------------------------------- */
 
 /* Host tables of a pooling layer, as AvgPool2d::lazy_index_init builds them
