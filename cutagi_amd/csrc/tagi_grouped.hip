@@ -1,6 +1,7 @@
 // Linear layers grouped by expert: row r of expert e (offsets[e] <= r < offsets[e+1])
 // meets the weights [e][N][K]. gfx950.
 #include <cstdint>
+#include <type_traits>
 
 #include "tagi_activation.h"
 #include "tagi_internal.h"
@@ -36,23 +37,23 @@ __device__ __forceinline__ void group_rows(const int *__restrict__ offsets, int 
 // them and write the pieces to LDS; the other four read fragments and issue matrix
 // instructions on 64 x 64 sub-tiles. Every SIMD holds one wave of each kind, so the vector
 // work of the split runs under the matrix instructions without any interleaving in the code,
-// and an element is split once for the four or two waves that read it. Two LDS stages of 16
-// reduction elements, one barrier per stage.
+// and an element is split once for the two waves that read it.
+// The two kinds meet at one barrier per unit, 32 reduction elements of one product (mean;
+// variance, one or two), 48 matrix instructions per wave: while unit u is multiplied, its
+// second half and the first half of unit u + 1 are read from LDS and unit u + 2 is written.
 // ---------------------------------------------------------------------------
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float floatx2 __attribute__((ext_vector_type(2)));
 typedef float floatx16 __attribute__((ext_vector_type(16)));
 
-__device__ __forceinline__ unsigned pack_bf16(float a, float b) {
-    const bf16x2 r = __builtin_convertvector((floatx2){a, b}, bf16x2);
-    return __builtin_bit_cast(unsigned, r);
-}
-// the three bf16 pieces of a and b, packed pairwise
+// The three bf16 pieces of a and b, packed pairwise. (A two-term dot product would take a
+// piece off in one instruction instead of two, but it runs on the matrix pipe and so not
+// beside the matrix instructions of the other wave.)
 __device__ __forceinline__ void split_pair(float a, float b, unsigned (&piece)[3]) {
 #pragma unroll
     for (int s = 0; s < 3; s++) {
-        piece[s] = pack_bf16(a, b);
+        piece[s] = __builtin_bit_cast(unsigned, __builtin_convertvector((floatx2){a, b}, bf16x2));
         if (s < 2) {
             a -= __uint_as_float(piece[s] << 16);
             b -= __uint_as_float(piece[s] & 0xffff0000u);
@@ -61,68 +62,61 @@ __device__ __forceinline__ void split_pair(float a, float b, unsigned (&piece)[3
 }
 
 constexpr int TM = 128;             // rows and columns of a tile
-constexpr int TK = 16;              // reduction elements of a stage
+constexpr int TK = 32;              // reduction elements of a unit
 constexpr int TILE_THREADS = 512;   // 256 that stage, 256 that multiply
-// An LDS plane holds eight reduction elements (16 bytes) of the tile's 128 rows (or columns)
-// for one piece of one operand. The 128 bytes between planes put the two planes of a
-// 16-element stage on different banks when four lanes write one row.
-constexpr int PLANE = TM * 16 + 128;
+// One piece of one operand of a unit: 64 bytes per row (or column) of the tile, four chunks of
+// eight reduction elements, their order turned by the row so that the sixteen lanes of a
+// 16-byte access (one chunk of sixteen rows) and of an 8-byte one (two whole rows) each touch
+// every bank once.
+constexpr int PIECE = TM * TK * 2;
+constexpr int UNIT = 2 * 3 * PIECE;   // rows' pieces, then columns' pieces
+constexpr int RING = 3;
+constexpr int TILE_LDS = RING * UNIT + (MAX_GROUPS + 1) * 4;
+
+__device__ __forceinline__ int chunk_at(int pos, int chunk) {
+    return pos * (TK * 2) + ((chunk ^ ((pos >> 2) & 3)) << 4);
+}
 
 template <int MODE>
 struct TileShape {
-    static constexpr int OPS = MODE == GROUPED_FWD ? 3 : 2;         // operands per side
-    static constexpr int SIDE = OPS * 3 * 2 * PLANE;
-    static constexpr int STAGE = 2 * SIDE;
-    static constexpr int LDS = 2 * STAGE + (MAX_GROUPS + 1) * 4;
+    static constexpr int OPS = MODE == GROUPED_FWD ? 3 : 2;         // products, operands per side
     // reduction contiguous in memory on the row / column side?
     static constexpr bool AK = MODE != GROUPED_DW, BK = MODE == GROUPED_FWD;
 };
 
-// Where row (or column) m of a tile sits in its planes. Operands whose reduction index is
-// the slow one are loaded four neighbouring columns at a time; they go to positions 32 apart,
-// so that neighbouring lanes write neighbouring 16-byte places.
+// Which row (or column) of a tile is at position pos of the LDS. Operands whose reduction
+// index is the slow one are loaded four neighbouring columns at a time; these go to
+// positions 32 apart, so that neighbouring lanes write neighbouring places.
 template <bool KCONTIG>
 __device__ __forceinline__ int row_at(int pos) {
     return KCONTIG ? pos : (pos & 31) * 4 + (pos >> 5);
 }
 
-// Four elements of a row that starts at `base` (16-byte aligned groups), or guarded ones.
-template <bool VEC>
-__device__ __forceinline__ float4 load4(const float *base, int k, int end) {
-    if (VEC) return *reinterpret_cast<const float4 *>(base + min(k, end - 4));
-    float4 v;
-    v.x = base[min(k, end - 1)];
-    v.y = base[min(k + 1, end - 1)];
-    v.z = base[min(k + 2, end - 1)];
-    v.w = base[min(k + 3, end - 1)];
-    return v;
-}
-__device__ __forceinline__ float4 keep4(float4 v, int k, int end) {
-    v.x = k < end ? v.x : 0.f;
-    v.y = k + 1 < end ? v.y : 0.f;
-    v.z = k + 2 < end ? v.z : 0.f;
-    v.w = k + 3 < end ? v.w : 0.f;
-    return v;
-}
-
-__device__ __forceinline__ void stage_barrier() {
+__device__ __forceinline__ void unit_barrier() {
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
-// The operands of one side from the values loaded: FWD rows (mu_a, var_a + mu_a^2, var_a),
-// FWD columns (mu_w, var_w, mu_w^2), innovations (delta_mu, delta_var), DZ / DW columns
-// (w or a, its square).
+// The same for the half that only reads: its reads may cross, because the unit they belong to
+// is overwritten two barriers later, and the registers they fill are used before the next.
+__device__ __forceinline__ void reader_barrier() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+// Operand `o` of one side from the values loaded: FWD rows (mu_a, var_a + mu_a^2, var_a), FWD
+// columns (mu_w, var_w, mu_w^2), innovations (delta_mu, delta_var), DZ / DW columns (w or a,
+// its square).
 template <int MODE, bool ROWS>
-__device__ __forceinline__ void operands(float u, float v, float (&o)[3]) {
-    o[0] = u;
+__device__ __forceinline__ float operand(int o, float u, float v) {
+    if (o == 0) return u;
     if (MODE == GROUPED_FWD) {
-        o[1] = ROWS ? fmaf(u, u, v) : v;
-        o[2] = ROWS ? v : u * u;
-    } else {
-        o[1] = ROWS ? v : u * u;
+        if (o == 1) return ROWS ? fmaf(u, u, v) : v;
+        return ROWS ? v : u * u;
     }
+    return ROWS ? v : u * u;
 }
 
 // A tile of the problem: expert, first row / column, reduction range, and the rows that exist.
@@ -130,163 +124,6 @@ struct Tile {
     int e, m0, c0;      // expert, first output row, first output column
     int m_end, c_end;   // one past the last
     int r0, red;        // DW: first row of the expert; length of the reduction
-};
-
-// Side with its reduction index contiguous: thread u of 128 holds elements 4 (u % 4) .. + 3
-// of the stage for the rows u / 4 + 32 i.
-template <int MODE, bool ROWS, bool VEC>
-struct StageK {
-    const float *p0[4], *p1[4];
-    bool live[4];
-    float4 v0[4], v1[4];
-    int k, red;
-    __device__ __forceinline__ void start(const GroupedParams &p, const Tile &t, int u) {
-        k = (u & 3) * 4;
-        red = t.red;
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int row = (u >> 2) + 32 * i;
-            live[i] = true;
-            size_t at;
-            if (ROWS) {
-                const int m = min(t.m0 + row, t.m_end - 1);
-                int s = m;
-                if (MODE == GROUPED_FWD && p.rows != nullptr) {
-                    s = p.rows[m];
-                    live[i] = (unsigned)s < (unsigned)p.T;
-                    if (!live[i]) s = 0;
-                }
-                at = (size_t)s * t.red;
-            } else {
-                at = ((size_t)t.e * p.N + min(t.c0 + row, t.c_end - 1)) * t.red;
-            }
-            p0[i] = (ROWS ? p.x0 : p.y0) + at;
-            p1[i] = (ROWS ? p.x1 : p.y1) + at;
-        }
-    }
-    __device__ __forceinline__ void load(int stage) {
-        const int at = stage * TK + k;
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            v0[i] = load4<VEC>(p0[i], at, red);
-            v1[i] = load4<VEC>(p1[i], at, red);
-        }
-    }
-    __device__ __forceinline__ void write(char *side, int stage, int u) const {
-        const int at = stage * TK + k;
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const float4 a = keep4(v0[i], live[i] ? at : red, red);
-            const float4 b = keep4(v1[i], live[i] ? at : red, red);
-            float x[4][3];
-            operands<MODE, ROWS>(a.x, b.x, x[0]);
-            operands<MODE, ROWS>(a.y, b.y, x[1]);
-            operands<MODE, ROWS>(a.z, b.z, x[2]);
-            operands<MODE, ROWS>(a.w, b.w, x[3]);
-            char *to = side + ((u & 3) >> 1) * PLANE + ((u >> 2) + 32 * i) * 16 + (u & 1) * 8;
-#pragma unroll
-            for (int o = 0; o < TileShape<MODE>::OPS; o++) {
-                unsigned lo[3], hi[3];
-                split_pair(x[0][o], x[1][o], lo);
-                split_pair(x[2][o], x[3][o], hi);
-#pragma unroll
-                for (int s = 0; s < 3; s++)
-                    *reinterpret_cast<uint2 *>(to + (o * 3 + s) * 2 * PLANE) = make_uint2(lo[s], hi[s]);
-            }
-        }
-    }
-};
-
-// Side with its reduction index slow: thread u of 128 holds the columns 4 c .. + 3 for the
-// reduction elements 4 g .. + 3, g = 2 (u / 64) + u % 2, c = (u % 64) / 2.
-template <int MODE, bool ROWS, bool VEC>
-struct StageM {
-    const float *q0, *q1;     // element (reduction 0, column 0) of the operand
-    int ld, first, red, r0, g;
-    int col, cols;            // column of the thread, columns that exist
-    const int *rows;
-    int tokens;
-    float4 v0[4], v1[4];
-    bool live[4];
-    __device__ __forceinline__ void start(const GroupedParams &p, const Tile &t, int u) {
-        g = 2 * (u >> 6) + (u & 1);
-        red = t.red;
-        r0 = t.r0;
-        rows = nullptr;
-        tokens = 0;
-        if (ROWS) {             // DW: innovations [R][N], columns n
-            ld = p.N;
-            q0 = p.x0 + (size_t)t.r0 * p.N;
-            q1 = p.x1 + (size_t)t.r0 * p.N;
-            first = t.m0;
-            cols = t.m_end;
-        } else {
-            ld = p.K;
-            first = t.c0;
-            cols = t.c_end;
-            if (MODE == GROUPED_DZ) {
-                q0 = p.y0 + (size_t)t.e * p.N * p.K;
-            } else {            // DW: activations [T or R][K]
-                rows = p.rows;
-                tokens = p.T;
-                q0 = p.y0 + (rows == nullptr ? (size_t)t.r0 * p.K : 0);
-            }
-            q1 = q0;
-        }
-        col = first + ((u & 63) >> 1) * 4;
-    }
-    __device__ __forceinline__ void load(int stage) {
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int r = min(stage * TK + 4 * g + i, red - 1);
-            size_t s = (size_t)r;
-            live[i] = true;
-            if (!ROWS && MODE == GROUPED_DW && rows != nullptr) {
-                const int token = rows[r0 + r];
-                live[i] = (unsigned)token < (unsigned)tokens;
-                s = live[i] ? token : 0;
-            }
-            // (columns beyond the last are computed and not stored; they only have to be
-            // addresses that exist)
-            v0[i] = load4<VEC>(q0 + s * ld, col, cols);
-            if (ROWS) v1[i] = load4<VEC>(q1 + s * ld, col, cols);
-        }
-    }
-    __device__ __forceinline__ void write(char *side, int stage, int u) const {
-        const int c = (u & 63) >> 1;
-        float a[4][4], b[4][4];
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const bool in = live[i] && stage * TK + 4 * g + i < red;
-            a[i][0] = in ? v0[i].x : 0.f;
-            a[i][1] = in ? v0[i].y : 0.f;
-            a[i][2] = in ? v0[i].z : 0.f;
-            a[i][3] = in ? v0[i].w : 0.f;
-            if (ROWS) {
-                b[i][0] = in ? v1[i].x : 0.f;
-                b[i][1] = in ? v1[i].y : 0.f;
-                b[i][2] = in ? v1[i].z : 0.f;
-                b[i][3] = in ? v1[i].w : 0.f;
-            }
-        }
-        char *to = side + (g >> 1) * PLANE + c * 16 + (g & 1) * 8;
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            float x[4][3];
-#pragma unroll
-            for (int i = 0; i < 4; i++) operands<MODE, ROWS>(a[i][j], ROWS ? b[i][j] : 0.f, x[i]);
-#pragma unroll
-            for (int o = 0; o < 2; o++) {
-                unsigned lo[3], hi[3];
-                split_pair(x[0][o], x[1][o], lo);
-                split_pair(x[2][o], x[3][o], hi);
-#pragma unroll
-                for (int s = 0; s < 3; s++)
-                    *reinterpret_cast<uint2 *>(to + (o * 3 + s) * 2 * PLANE + j * 32 * 16) =
-                        make_uint2(lo[s], hi[s]);
-            }
-        }
-    }
 };
 
 // The tiles of a workgroup: XCD x (workgroups x, x + 8, ...) takes the x-th eighth of the tile
@@ -341,12 +178,286 @@ struct TileList {
     }
 };
 
+// What the 128 threads that stage one side hold of 32 reduction elements.
+struct Batch {
+    float4 v0[8], v1[8];
+    int left;       // reduction elements from the first of the batch to the end
+    unsigned dead;  // bit i: v[i] belongs to no row and reads as zeros
+};
+
+// Four neighbouring floats at element `off` behind a uniform base. VEC: one 16-byte load,
+// 32-bit offset (launch_grouped sees to the sizes). `last`: the last element that exists.
+template <bool VEC>
+__device__ __forceinline__ float4 load4(const float *base, size_t off, size_t last) {
+    if (VEC)
+        return *reinterpret_cast<const float4 *>(reinterpret_cast<const char *>(base) +
+                                                 (unsigned)((unsigned)off * 4u));
+    float4 v;
+    v.x = base[off];
+    v.y = base[min(off + 1, last)];
+    v.z = base[min(off + 2, last)];
+    v.w = base[min(off + 3, last)];
+    return v;
+}
+
+// Side with its reduction index contiguous: thread u holds the elements 4 (u % 8) .. + 3 of
+// the rows u / 8 + 16 i: eight lanes read a whole 128-byte line.
+template <int MODE, bool ROWS, bool VEC>
+struct SideK {
+    typedef std::conditional_t<VEC, unsigned, size_t> Off;
+    const float *q0, *q1;       // uniform
+    Off row[8];                 // element offset of the thread's rows
+    int source[8];
+    bool fresh, gather;
+    unsigned dead;
+    int k, red;
+    __device__ __forceinline__ void start(const GroupedParams &p, const Tile &t, int u) {
+        k = (u & 7) * 4;
+        red = t.red;
+        fresh = true;
+        gather = ROWS && MODE == GROUPED_FWD && p.rows != nullptr;
+        const size_t first = gather ? 0 : ROWS ? (size_t)t.m0 : (size_t)t.e * p.N + t.c0;
+        q0 = (ROWS ? p.x0 : p.y0) + first * red;
+        q1 = (ROWS ? p.x1 : p.y1) + first * red;
+        const int rows = (ROWS ? t.m_end - t.m0 : t.c_end - t.c0) - 1;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            source[i] = min((u >> 3) + 16 * i, rows);
+            if (gather) source[i] = p.rows[t.m0 + source[i]];
+        }
+    }
+    __device__ __forceinline__ void ahead(const GroupedParams &, int) {}
+    __device__ __forceinline__ void load(const GroupedParams &p, int k0, Batch &b) {
+        if (fresh) {
+            fresh = false;
+            dead = 0u;
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                int s = source[i];
+                if (gather && (unsigned)s >= (unsigned)p.T) {
+                    s = 0;
+                    dead |= 1u << i;
+                }
+                row[i] = (Off)s * (Off)red;
+            }
+        }
+        b.left = red - k0;
+        b.dead = dead;
+        // (never beyond the row's end: what is beyond reads as zeros)
+        const int kk = b.left >= TK ? k : min(k, VEC ? b.left - 4 : b.left - 1);
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            b.v0[i] = load4<VEC>(q0 + k0, row[i] + kk, row[i] + (Off)(b.left - 1));
+            b.v1[i] = load4<VEC>(q1 + k0, row[i] + kk, row[i] + (Off)(b.left - 1));
+        }
+    }
+    // zeros behind the end of the reduction and in rows that are no rows
+    __device__ __forceinline__ void mask(Batch &b) const {
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const int n = (b.dead >> i) & 1u ? 0 : b.left - k;
+            float4 &x = b.v0[i], &y = b.v1[i];
+            x.x = n > 0 ? x.x : 0.f, y.x = n > 0 ? y.x : 0.f;
+            x.y = n > 1 ? x.y : 0.f, y.y = n > 1 ? y.y : 0.f;
+            x.z = n > 2 ? x.z : 0.f, y.z = n > 2 ? y.z : 0.f;
+            x.w = n > 3 ? x.w : 0.f, y.w = n > 3 ? y.w : 0.f;
+        }
+    }
+    template <int O>
+    __device__ __forceinline__ void write(const Batch &b, char *side, int u) const {
+        char *to = side + chunk_at(u >> 3, (u & 7) >> 1) + (u & 1) * 8;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const float4 x = b.v0[i], y = b.v1[i];
+            unsigned lo[3], hi[3];
+            split_pair(operand<MODE, ROWS>(O, x.x, y.x), operand<MODE, ROWS>(O, x.y, y.y), lo);
+            split_pair(operand<MODE, ROWS>(O, x.z, y.z), operand<MODE, ROWS>(O, x.w, y.w), hi);
+#pragma unroll
+            for (int s = 0; s < 3; s++)
+                *reinterpret_cast<uint2 *>(to + s * PIECE + i * 16 * TK * 2) = make_uint2(lo[s], hi[s]);
+        }
+    }
+};
+
+// Side with its reduction index slow: thread u holds the columns 4 (u % 32) .. + 3 of the
+// reduction elements 8 (u / 32) + i: 32 lanes read 512 bytes of one.
+template <int MODE, bool ROWS, bool VEC>
+struct SideM {
+    static constexpr bool GATHER = MODE == GROUPED_DW && !ROWS;
+    const float *q0, *q1;     // element (reduction 0, column 0) of the operand, uniform
+    int ld, red, r0, g, col, cols;
+    bool gather;
+    int source[8];            // gather: the rows that the next batch reads
+    __device__ __forceinline__ void start(const GroupedParams &p, const Tile &t, int u) {
+        g = (u >> 5) * 8;
+        red = t.red;
+        r0 = t.r0;
+        gather = GATHER && p.rows != nullptr;
+        if (ROWS) {             // DW: innovations [R][N], columns n
+            ld = p.N;
+            q0 = p.x0 + (size_t)t.r0 * p.N;
+            q1 = p.x1 + (size_t)t.r0 * p.N;
+            cols = t.m_end;
+            col = t.m0 + (u & 31) * 4;
+        } else {
+            ld = p.K;
+            q0 = p.y0 + (MODE == GROUPED_DZ ? (size_t)t.e * p.N * p.K : gather ? 0 : (size_t)t.r0 * p.K);
+            q1 = q0;
+            cols = t.c_end;
+            col = t.c0 + (u & 31) * 4;
+        }
+        // (columns beyond the last are computed and not stored; they only have to exist)
+        col = min(col, VEC ? cols - 4 : cols - 1);
+    }
+    // the row indices of the batch at k0, on their way while the batch before it is split
+    __device__ __forceinline__ void ahead(const GroupedParams &p, int k0) {
+        if (!GATHER || !gather) return;
+#pragma unroll
+        for (int i = 0; i < 8; i++) source[i] = p.rows[r0 + min(k0 + g + i, red - 1)];
+    }
+    __device__ __forceinline__ void load(const GroupedParams &p, int k0, Batch &b) {
+        typedef std::conditional_t<VEC, unsigned, size_t> Off;
+        b.left = red - k0;
+        b.dead = 0u;
+        if (GATHER && gather) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                int s = source[i];
+                if ((unsigned)s >= (unsigned)p.T) {
+                    s = 0;
+                    b.dead |= 1u << i;
+                }
+                const Off row = (Off)s * (Off)ld;
+                b.v0[i] = load4<VEC>(q0, row + col, row + (Off)(cols - 1));
+            }
+            return;
+        }
+        const float *f0 = q0 + (size_t)k0 * ld, *f1 = q1 + (size_t)k0 * ld;
+        if (b.left >= TK) {
+            const Off row = (Off)g * (Off)ld;
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const size_t up = (size_t)i * ld;
+                b.v0[i] = load4<VEC>(f0 + up, row + col, row + (Off)(cols - 1));
+                if (ROWS) b.v1[i] = load4<VEC>(f1 + up, row + col, row + (Off)(cols - 1));
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const Off row = (Off)min(g + i, b.left - 1) * (Off)ld;
+                b.v0[i] = load4<VEC>(f0, row + col, row + (Off)(cols - 1));
+                if (ROWS) b.v1[i] = load4<VEC>(f1, row + col, row + (Off)(cols - 1));
+            }
+        }
+    }
+    __device__ __forceinline__ void mask(Batch &b) const {
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            if (i >= b.left - g || (b.dead >> i) & 1u) {
+                b.v0[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (ROWS) b.v1[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+    }
+    template <int O>
+    __device__ __forceinline__ void write(const Batch &b, char *side, int u) const {
+        auto at = [&](const float4 &v, int j) { return j == 0 ? v.x : j == 1 ? v.y : j == 2 ? v.z : v.w; };
+        char *to = side + chunk_at(u & 31, u >> 5);
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            unsigned x[4][3];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                auto value = [&](int r) {
+                    return operand<MODE, ROWS>(O, at(b.v0[r], j), ROWS ? at(b.v1[r], j) : 0.f);
+                };
+                split_pair(value(2 * i), value(2 * i + 1), x[i]);
+            }
+#pragma unroll
+            for (int s = 0; s < 3; s++)
+                *reinterpret_cast<uint4 *>(to + s * PIECE + j * 32 * TK * 2) =
+                    make_uint4(x[0][s], x[1][s], x[2][s], x[3][s]);
+        }
+    }
+};
+
+// One of the two staging halves of a workgroup.
+template <int MODE, typename Side>
+struct Stager {
+    const GroupedParams &p;
+    const TileList<MODE> &list;
+    char *lds;
+    int next, step, u;
+    Side side;
+    Tile t;
+    int k0;
+    bool more;
+    int slot;
+
+    // moves to the next batch of the tile, or the first of the next tile that has any
+    __device__ __forceinline__ void advance() {
+        k0 += TK;
+        if (k0 >= t.red) {
+            do {
+                more = list.get(p, next, t);
+                next += step;
+            } while (more && t.red == 0);
+            k0 = 0;
+            if (more) side.start(p, t, u);
+        }
+        if (more) side.ahead(p, k0);
+    }
+    template <int O>
+    __device__ __forceinline__ void units(const Batch &b) {
+        if constexpr (O < TileShape<MODE>::OPS) {
+            side.template write<O>(b, lds + slot * UNIT, u);
+            slot = slot == RING - 1 ? 0 : slot + 1;
+            unit_barrier();
+            units<O + 1>(b);
+        }
+    }
+    __device__ __forceinline__ void put(Batch &b) {
+        if (b.left < TK || b.dead != 0u) side.mask(b);
+        units<0>(b);
+    }
+    __device__ __forceinline__ void run() {
+        Batch a, b;
+        more = true;
+        slot = 0;
+        t.red = 0;
+        k0 = 0;
+        advance();
+        bool held = more;
+        if (held) {
+            side.load(p, k0, a);
+            advance();
+        }
+        while (held) {
+            held = more;
+            if (held) {
+                side.load(p, k0, b);
+                advance();
+            }
+            put(a);
+            if (!held) break;
+            held = more;
+            if (held) {
+                side.load(p, k0, a);
+                advance();
+            }
+            put(b);
+        }
+        // the two barriers by which the multiplying half is behind
+        unit_barrier();
+        unit_barrier();
+    }
+};
+
 template <int MODE, bool VEC>
 __global__ __launch_bounds__(TILE_THREADS) void grouped_tile_kernel(GroupedParams p) {
     extern __shared__ __attribute__((aligned(16))) char tile_lds[];
     typedef TileShape<MODE> Shape;
     const int tid = threadIdx.x, lane = tid & 63;
-    int *prefix = reinterpret_cast<int *>(tile_lds + 2 * Shape::STAGE);
+    int *prefix = reinterpret_cast<int *>(tile_lds + RING * UNIT);
 
     TileList<MODE> list;
     list.prefix = prefix;
@@ -388,47 +499,40 @@ __global__ __launch_bounds__(TILE_THREADS) void grouped_tile_kernel(GroupedParam
     }
     const int first = blockIdx.x >> 3, step = gridDim.x >> 3;
 
-    int buf = 0;
     if (tid < 256) {
         // ---- loads, splits, writes
-        const bool rows_side = tid < 128;
         const int u = tid & 127;
-        auto walk = [&](auto stager, int side) {
-            Tile t;
-            for (int i = first; list.get(p, i, t); i += step) {
-                if (t.red == 0) continue;
-                const int stages = (t.red + TK - 1) / TK;
-                stager.start(p, t, u);
-                stager.load(0);
-                for (int s = 0; s < stages; s++) {
-                    auto now = stager;
-                    if (s + 1 < stages) stager.load(s + 1);
-                    now.write(tile_lds + buf * Shape::STAGE + side * Shape::SIDE, s, u);
-                    buf ^= 1;
-                    stage_barrier();
-                }
-            }
-            // the barrier behind the last stage's matrix work
-            stage_barrier();
-        };
-        if (rows_side) {
-            if constexpr (Shape::AK)
-                walk(StageK<MODE, true, VEC>(), 0);
-            else
-                walk(StageM<MODE, true, VEC>(), 0);
+        if (tid < 128) {
+            typedef std::conditional_t<Shape::AK, SideK<MODE, true, VEC>, SideM<MODE, true, VEC>> Side;
+            Stager<MODE, Side> s{p, list, tile_lds, first, step, u};
+            s.run();
         } else {
-            if constexpr (Shape::BK)
-                walk(StageK<MODE, false, VEC>(), 1);
-            else
-                walk(StageM<MODE, false, VEC>(), 1);
+            typedef std::conditional_t<Shape::BK, SideK<MODE, false, VEC>, SideM<MODE, false, VEC>> Side;
+            Stager<MODE, Side> s{p, list, tile_lds + 3 * PIECE, first, step, u};
+            s.run();
         }
         return;
     }
     // ---- fragments, matrix instructions, results
     const int cw = (tid >> 6) - 4, wm = cw >> 1, wn = cw & 1;
-    const int frag = (lane >> 5) * PLANE + (lane & 31) * 16;
-    const int a_at = frag + wm * 64 * 16, b_at = Shape::SIDE + frag + wn * 64 * 16;
-    stage_barrier();
+    const char *a_base = tile_lds + wm * 64 * TK * 2;
+    const char *b_base = tile_lds + 3 * PIECE + wn * 64 * TK * 2;
+    const int frag[2] = {chunk_at(lane & 31, lane >> 5), chunk_at(lane & 31, 2 + (lane >> 5))};
+    // pieces of the half unit that is multiplied: [piece][sub-tile]
+    bf16x8 a[3][2], b[3][2];
+    auto fetch = [&](bf16x8(&f)[2], const char *base, int slot, int half, int piece) {
+#pragma unroll
+        for (int x = 0; x < 2; x++)
+            f[x] = *reinterpret_cast<const bf16x8 *>(base + slot * UNIT + frag[half] + piece * PIECE + x * 32 * TK * 2);
+    };
+    reader_barrier();
+#pragma unroll
+    for (int q = 0; q < 3; q++) {
+        fetch(a[q], a_base, 0, 0, q);
+        fetch(b[q], b_base, 0, 0, q);
+    }
+    reader_barrier();
+    int slot = 0;
     Tile t;
     for (int i = first; list.get(p, i, t); i += step) {
         floatx16 acc[2][2][2];
@@ -440,31 +544,49 @@ __global__ __launch_bounds__(TILE_THREADS) void grouped_tile_kernel(GroupedParam
                 for (int y = 0; y < 2; y++)
 #pragma unroll
                     for (int v = 0; v < 16; v++) acc[q][x][y][v] = 0.f;
-        const int stages = (t.red + TK - 1) / TK;
-        for (int s = 0; s < stages; s++) {
-            const char *st = tile_lds + buf * Shape::STAGE;
+        for (int k0 = 0; k0 < t.red; k0 += TK) {
 #pragma unroll
             for (int o = 0; o < Shape::OPS; o++) {
-                bf16x8 a[2][3], b[2][3];
+                auto mul = [&](const bf16x8(&x)[2], const bf16x8(&y)[2]) {
 #pragma unroll
-                for (int q = 0; q < 3; q++)
+                    for (int i = 0; i < 2; i++)
+#pragma unroll
+                        for (int j = 0; j < 2; j++)
+                            acc[o > 0][i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+                                x[i], y[j], acc[o > 0][i][j], 0, 0, 0);
+                };
+                const int after = slot == RING - 1 ? 0 : slot + 1;
+#pragma unroll
+                for (int half = 0; half < 2; half++) {
+                    // the small products first; a piece is read anew, for the next half unit, as
+                    // soon as its last product is issued (the high ones are needed to the end)
+                    const int from = half == 0 ? slot : after, other = 1 - half;
+                    bf16x8 ah[2], bh[2];
+                    fetch(ah, a_base, from, other, 0);
+                    fetch(bh, b_base, from, other, 0);
+                    mul(a[2], b[0]);
+                    __builtin_amdgcn_sched_barrier(0);
+                    fetch(a[2], a_base, from, other, 2);
+                    mul(a[0], b[2]);
+                    __builtin_amdgcn_sched_barrier(0);
+                    fetch(b[2], b_base, from, other, 2);
+                    mul(a[1], b[1]);
+                    mul(a[1], b[0]);
+                    __builtin_amdgcn_sched_barrier(0);
+                    fetch(a[1], a_base, from, other, 1);
+                    mul(a[0], b[1]);
+                    __builtin_amdgcn_sched_barrier(0);
+                    fetch(b[1], b_base, from, other, 1);
+                    mul(a[0], b[0]);
 #pragma unroll
                     for (int x = 0; x < 2; x++) {
-                        a[x][q] = *reinterpret_cast<const bf16x8 *>(st + a_at + (o * 3 + q) * 2 * PLANE + x * 32 * 16);
-                        b[x][q] = *reinterpret_cast<const bf16x8 *>(st + b_at + (o * 3 + q) * 2 * PLANE + x * 32 * 16);
+                        a[0][x] = ah[x];
+                        b[0][x] = bh[x];
                     }
-                constexpr int PA[6] = {0, 0, 1, 1, 0, 2}, PB[6] = {0, 1, 0, 1, 2, 0};
-#pragma unroll
-                for (int q = 0; q < 6; q++)
-#pragma unroll
-                    for (int x = 0; x < 2; x++)
-#pragma unroll
-                        for (int y = 0; y < 2; y++)
-                            acc[o > 0][x][y] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-                                a[x][PA[q]], b[y][PB[q]], acc[o > 0][x][y], 0, 0, 0);
+                }
+                slot = after;
+                reader_barrier();
             }
-            buf ^= 1;
-            stage_barrier();
         }
         // register v of lane l: row 8 (v / 4) + 4 (l / 32) + v % 4, column l % 32
         if constexpr (VEC && !Shape::BK) {
@@ -473,27 +595,30 @@ __global__ __launch_bounds__(TILE_THREADS) void grouped_tile_kernel(GroupedParam
             if (c >= t.c_end) continue;
             const size_t base = (MODE == GROUPED_DW ? (size_t)t.e * p.N * p.K : 0) + c;
 #pragma unroll
-            for (int x = 0; x < 2; x++) {
-                float2 f[16];
-                size_t at[16];
+            for (int x = 0; x < 2; x++)
 #pragma unroll
-                for (int v = 0; v < 16; v++) {
-                    const int pos = wm * 64 + x * 32 + 8 * (v >> 2) + 4 * (lane >> 5) + (v & 3);
-                    const int m = t.m0 + row_at<Shape::AK>(pos);
-                    at[v] = base + (size_t)min(m, t.m_end - 1) * p.K;
-                    f[v] = p.e0 != nullptr ? *reinterpret_cast<const float2 *>(p.e0 + at[v])
-                                           : make_float2(1.f, 1.f);
-                }
+                for (int v0 = 0; v0 < 16; v0 += 4) {   // four rows at a time: registers
+                    float2 f[4];
+                    const int pos = wm * 64 + x * 32 + 2 * v0 + 4 * (lane >> 5);
 #pragma unroll
-                for (int v = 0; v < 16; v++) {
-                    const int pos = wm * 64 + x * 32 + 8 * (v >> 2) + 4 * (lane >> 5) + (v & 3);
-                    if (t.m0 + row_at<Shape::AK>(pos) >= t.m_end) continue;
-                    *reinterpret_cast<float2 *>(p.out0 + at[v]) =
-                        make_float2(acc[0][x][0][v] * f[v].x, acc[0][x][1][v] * f[v].y);
-                    *reinterpret_cast<float2 *>(p.out1 + at[v]) = make_float2(
-                        acc[1][x][0][v] * f[v].x * f[v].x, acc[1][x][1][v] * f[v].y * f[v].y);
+                    for (int v = 0; v < 4; v++) {
+                        const int m = min(t.m0 + row_at<Shape::AK>(pos + v), t.m_end - 1);
+                        f[v] = p.e0 != nullptr ? *reinterpret_cast<const float2 *>(p.e0 + base + (size_t)m * p.K)
+                                               : make_float2(1.f, 1.f);
+                    }
+#pragma unroll
+                    for (int v = 0; v < 4; v++) {
+                        const int m = t.m0 + row_at<Shape::AK>(pos + v);
+                        if (m >= t.m_end) continue;
+                        const size_t at = base + (size_t)m * p.K;
+                        *reinterpret_cast<float2 *>(p.out0 + at) =
+                            make_float2(acc[0][x][0][v0 + v] * f[v].x, acc[0][x][1][v0 + v] * f[v].y);
+                        *reinterpret_cast<float2 *>(p.out1 + at) =
+                            make_float2(acc[1][x][0][v0 + v] * f[v].x * f[v].x,
+                                        acc[1][x][1][v0 + v] * f[v].y * f[v].y);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
                 }
-            }
             continue;
         }
 #pragma unroll
@@ -557,14 +682,13 @@ inline bool aligned16(const void *q) { return (reinterpret_cast<uintptr_t>(q) & 
 template <int MODE, bool VEC>
 hipError_t tile_launch(const GroupedParams &p, long long tiles, hipStream_t stream) {
     static PerDeviceOnce once;
-    const int lds = TileShape<MODE>::LDS;
     hipError_t e = allow_dynamic_lds(
-        once, reinterpret_cast<const void *>(&grouped_tile_kernel<MODE, VEC>), lds);
+        once, reinterpret_cast<const void *>(&grouped_tile_kernel<MODE, VEC>), TILE_LDS);
     if (e != hipSuccess) return e;
     // one workgroup per CU at most; every XCD the same number
     const long long most = num_cu() / 8 * 8, want = (tiles + 7) / 8 * 8;
     hipLaunchKernelGGL((grouped_tile_kernel<MODE, VEC>), dim3((unsigned)(want < most ? want : most)),
-                       dim3(TILE_THREADS), lds, stream, p);
+                       dim3(TILE_THREADS), TILE_LDS, stream, p);
     return hipGetLastError();
 }
 
@@ -584,7 +708,10 @@ hipError_t launch_grouped(GroupedMode mode, const GroupedParams &p, hipStream_t 
     const bool vec = p.K % 4 == 0 && (mode == GROUPED_FWD || p.N % 4 == 0) && aligned16(p.x0) &&
                      aligned16(p.x1) && aligned16(p.y0) && (mode != GROUPED_FWD || aligned16(p.y1)) &&
                      (mode == GROUPED_FWD || (aligned16(p.e0) && aligned16(p.out0) && aligned16(p.out1)));
-    return vec ? tile_launch<true>(mode, p, stream) : tile_launch<false>(mode, p, stream);
+    // its 32-bit byte offsets: 128 rows of one operand, or any row where rows are gathered
+    const long long most = 1LL << 30;
+    const bool near = (p.rows == nullptr || (long long)p.T * p.K < most) && 128LL * p.K < most && 128LL * p.N < most;
+    return vec && near ? tile_launch<true>(mode, p, stream) : tile_launch<false>(mode, p, stream);
 }
 
 hipError_t launch_grouped_db(const GroupedParams &p, hipStream_t stream) {
