@@ -23,7 +23,10 @@ hipStream_t as_stream(void *s) { return static_cast<hipStream_t>(s); }
 int grouped_sizes(int K, int N, int E, int R, int T, const int *rows, int columns, bool weights) {
     if (K <= 0 || N <= 0 || E <= 0 || R <= 0 || (rows != nullptr && T <= 0))
         return TAGI_ERR_INVALID_ARG;
-    if (E > MAX_EXPERTS || K > (1 << 30) || N > (1 << 30)) return TAGI_ERR_UNSUPPORTED;
+    if (E > MAX_EXPERTS) return TAGI_ERR_UNSUPPORTED;
+    // element offsets of 32 bits inside a tile's 128 rows, and of any row that is gathered
+    if (K > (1 << 24) || N > (1 << 24)) return TAGI_ERR_UNSUPPORTED;
+    if (rows != nullptr && (long long)T * K > (1LL << 32) - 1) return TAGI_ERR_UNSUPPORTED;
     const double tiles = (columns + 63) / 64 * ((double)R / 64 + E);
     const double weight_tiles = weights ? (double)((K + 63) / 64) * ((N + 63) / 64) * E : 0;
     const double most = (double)(1 << 24) - 1;

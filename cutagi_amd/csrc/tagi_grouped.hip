@@ -185,13 +185,11 @@ struct Batch {
     unsigned dead;  // bit i: v[i] belongs to no row and reads as zeros
 };
 
-// Four neighbouring floats at element `off` behind a uniform base. VEC: one 16-byte load,
-// 32-bit offset (launch_grouped sees to the sizes). `last`: the last element that exists.
+// Four neighbouring floats at element `off` behind a uniform base. VEC: one 16-byte load at a
+// 32-bit byte offset (launch_grouped sees to the sizes). `last`: the last element that exists.
 template <bool VEC>
-__device__ __forceinline__ float4 load4(const float *base, size_t off, size_t last) {
-    if (VEC)
-        return *reinterpret_cast<const float4 *>(reinterpret_cast<const char *>(base) +
-                                                 (unsigned)((unsigned)off * 4u));
+__device__ __forceinline__ float4 load4(const float *base, unsigned off, unsigned last) {
+    if (VEC) return *reinterpret_cast<const float4 *>(reinterpret_cast<const char *>(base) + off * 4u);
     float4 v;
     v.x = base[off];
     v.y = base[min(off + 1, last)];
@@ -204,13 +202,13 @@ __device__ __forceinline__ float4 load4(const float *base, size_t off, size_t la
 // the rows u / 8 + 16 i: eight lanes read a whole 128-byte line.
 template <int MODE, bool ROWS, bool VEC>
 struct SideK {
-    typedef std::conditional_t<VEC, unsigned, size_t> Off;
     const float *q0, *q1;       // uniform
-    Off row[8];                 // element offset of the thread's rows
+    unsigned row[8];            // element offset of the thread's rows
     int source[8];
     bool fresh, gather;
     unsigned dead;
-    int k, red;
+    int k, red, kk;
+    const float *f0, *f1;       // the batch that is loaded
     __device__ __forceinline__ void start(const GroupedParams &p, const Tile &t, int u) {
         k = (u & 7) * 4;
         red = t.red;
@@ -227,7 +225,8 @@ struct SideK {
         }
     }
     __device__ __forceinline__ void ahead(const GroupedParams &, int) {}
-    __device__ __forceinline__ void load(const GroupedParams &p, int k0, Batch &b) {
+    // the batch at k0 is next: addresses
+    __device__ __forceinline__ void begin(const GroupedParams &p, int k0, Batch &b) {
         if (fresh) {
             fresh = false;
             dead = 0u;
@@ -238,18 +237,19 @@ struct SideK {
                     s = 0;
                     dead |= 1u << i;
                 }
-                row[i] = (Off)s * (Off)red;
+                row[i] = (unsigned)s * (unsigned)red;
             }
         }
         b.left = red - k0;
         b.dead = dead;
         // (never beyond the row's end: what is beyond reads as zeros)
-        const int kk = b.left >= TK ? k : min(k, VEC ? b.left - 4 : b.left - 1);
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            b.v0[i] = load4<VEC>(q0 + k0, row[i] + kk, row[i] + (Off)(b.left - 1));
-            b.v1[i] = load4<VEC>(q1 + k0, row[i] + kk, row[i] + (Off)(b.left - 1));
-        }
+        kk = b.left >= TK ? k : min(k, VEC ? b.left - 4 : b.left - 1);
+        f0 = q0 + k0;
+        f1 = q1 + k0;
+    }
+    // its i-th load of array `second`
+    __device__ __forceinline__ void load(Batch &b, int i, bool second) const {
+        (second ? b.v1 : b.v0)[i] = load4<VEC>(second ? f1 : f0, row[i] + kk, row[i] + (b.left - 1));
     }
     // zeros behind the end of the reduction and in rows that are no rows
     __device__ __forceinline__ void mask(Batch &b) const {
@@ -263,11 +263,15 @@ struct SideK {
             x.w = n > 3 ? x.w : 0.f, y.w = n > 3 ? y.w : 0.f;
         }
     }
+    // Operand O of the batch to LDS. The loads of the batch after it go out between the
+    // splits, the first array's under the first operand, the second's under the second: all
+    // at once they would fill the memory pipe's queue and hold the splits up behind it.
     template <int O>
-    __device__ __forceinline__ void write(const Batch &b, char *side, int u) const {
+    __device__ __forceinline__ void write(const Batch &b, char *side, int u, Batch *next) const {
         char *to = side + chunk_at(u >> 3, (u & 7) >> 1) + (u & 1) * 8;
 #pragma unroll
         for (int i = 0; i < 8; i++) {
+            if (O < 2 && next != nullptr) load(*next, i, O == 1);
             const float4 x = b.v0[i], y = b.v1[i];
             unsigned lo[3], hi[3];
             split_pair(operand<MODE, ROWS>(O, x.x, y.x), operand<MODE, ROWS>(O, x.y, y.y), lo);
@@ -288,6 +292,8 @@ struct SideM {
     int ld, red, r0, g, col, cols;
     bool gather;
     int source[8];            // gather: the rows that the next batch reads
+    unsigned row[8];
+    const float *f0, *f1;     // the batch that is loaded
     __device__ __forceinline__ void start(const GroupedParams &p, const Tile &t, int u) {
         g = (u >> 5) * 8;
         red = t.red;
@@ -315,40 +321,29 @@ struct SideM {
 #pragma unroll
         for (int i = 0; i < 8; i++) source[i] = p.rows[r0 + min(k0 + g + i, red - 1)];
     }
-    __device__ __forceinline__ void load(const GroupedParams &p, int k0, Batch &b) {
-        typedef std::conditional_t<VEC, unsigned, size_t> Off;
+    __device__ __forceinline__ void begin(const GroupedParams &p, int k0, Batch &b) {
         b.left = red - k0;
         b.dead = 0u;
-        if (GATHER && gather) {
+        f0 = q0 + (GATHER && gather ? 0 : (size_t)k0 * ld);
+        f1 = q1 + (size_t)k0 * ld;
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                int s = source[i];
+        for (int i = 0; i < 8; i++) {
+            int s = min(g + i, b.left - 1);
+            if (GATHER && gather) {
+                s = source[i];
                 if ((unsigned)s >= (unsigned)p.T) {
                     s = 0;
                     b.dead |= 1u << i;
                 }
-                const Off row = (Off)s * (Off)ld;
-                b.v0[i] = load4<VEC>(q0, row + col, row + (Off)(cols - 1));
             }
-            return;
+            row[i] = (unsigned)s * (unsigned)ld;
         }
-        const float *f0 = q0 + (size_t)k0 * ld, *f1 = q1 + (size_t)k0 * ld;
-        if (b.left >= TK) {
-            const Off row = (Off)g * (Off)ld;
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const size_t up = (size_t)i * ld;
-                b.v0[i] = load4<VEC>(f0 + up, row + col, row + (Off)(cols - 1));
-                if (ROWS) b.v1[i] = load4<VEC>(f1 + up, row + col, row + (Off)(cols - 1));
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const Off row = (Off)min(g + i, b.left - 1) * (Off)ld;
-                b.v0[i] = load4<VEC>(f0, row + col, row + (Off)(cols - 1));
-                if (ROWS) b.v1[i] = load4<VEC>(f1, row + col, row + (Off)(cols - 1));
-            }
-        }
+    }
+    __device__ __forceinline__ void load(Batch &b, int i, bool second) const {
+        if (!second)
+            b.v0[i] = load4<VEC>(f0, row[i] + col, row[i] + (cols - 1));
+        else if (ROWS)
+            b.v1[i] = load4<VEC>(f1, row[i] + col, row[i] + (cols - 1));
     }
     __device__ __forceinline__ void mask(Batch &b) const {
 #pragma unroll
@@ -359,11 +354,15 @@ struct SideM {
             }
     }
     template <int O>
-    __device__ __forceinline__ void write(const Batch &b, char *side, int u) const {
+    __device__ __forceinline__ void write(const Batch &b, char *side, int u, Batch *next) const {
         auto at = [&](const float4 &v, int j) { return j == 0 ? v.x : j == 1 ? v.y : j == 2 ? v.z : v.w; };
         char *to = side + chunk_at(u & 31, u >> 5);
 #pragma unroll
         for (int j = 0; j < 4; j++) {
+            if (next != nullptr) {
+                load(*next, 2 * j, O == 1);
+                load(*next, 2 * j + 1, O == 1);
+            }
             unsigned x[4][3];
 #pragma unroll
             for (int i = 0; i < 4; i++) {
@@ -407,17 +406,25 @@ struct Stager {
         if (more) side.ahead(p, k0);
     }
     template <int O>
-    __device__ __forceinline__ void units(const Batch &b) {
+    __device__ __forceinline__ void units(const Batch &b, Batch *after) {
         if constexpr (O < TileShape<MODE>::OPS) {
-            side.template write<O>(b, lds + slot * UNIT, u);
+            side.template write<O>(b, lds + slot * UNIT, u, after);
             slot = slot == RING - 1 ? 0 : slot + 1;
             unit_barrier();
-            units<O + 1>(b);
+            units<O + 1>(b, after);
         }
     }
-    __device__ __forceinline__ void put(Batch &b) {
+    // batch b to LDS, the batch after it into `after`
+    __device__ __forceinline__ void put(Batch &b, Batch &after) {
         if (b.left < TK || b.dead != 0u) side.mask(b);
-        units<0>(b);
+        if (more) {
+            side.begin(p, k0, after);
+            advance();
+            units<0>(b, &after);
+        } else {
+            after.left = 0;
+            units<0>(b, nullptr);
+        }
     }
     __device__ __forceinline__ void run() {
         Batch a, b;
@@ -426,25 +433,20 @@ struct Stager {
         t.red = 0;
         k0 = 0;
         advance();
-        bool held = more;
-        if (held) {
-            side.load(p, k0, a);
+        if (more) {
+            side.begin(p, k0, a);
             advance();
-        }
-        while (held) {
-            held = more;
-            if (held) {
-                side.load(p, k0, b);
-                advance();
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                side.load(a, i, false);
+                side.load(a, i, true);
             }
-            put(a);
-            if (!held) break;
-            held = more;
-            if (held) {
-                side.load(p, k0, a);
-                advance();
+            while (true) {
+                put(a, b);
+                if (b.left == 0) break;
+                put(b, a);
+                if (a.left == 0) break;
             }
-            put(b);
         }
         // the two barriers by which the multiplying half is behind
         unit_barrier();
@@ -710,7 +712,8 @@ hipError_t launch_grouped(GroupedMode mode, const GroupedParams &p, hipStream_t 
                      (mode == GROUPED_FWD || (aligned16(p.e0) && aligned16(p.out0) && aligned16(p.out1)));
     // its 32-bit byte offsets: 128 rows of one operand, or any row where rows are gathered
     const long long most = 1LL << 30;
-    const bool near = (p.rows == nullptr || (long long)p.T * p.K < most) && 128LL * p.K < most && 128LL * p.N < most;
+    const bool near = (p.rows == nullptr || (long long)p.T * p.K < most) && 128LL * p.K < most &&
+                      128LL * p.N < most;
     return vec && near ? tile_launch<true>(mode, p, stream) : tile_launch<false>(mode, p, stream);
 }
 

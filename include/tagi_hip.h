@@ -484,8 +484,8 @@ int tagi_layernorm_bwd(const float *mu_w, const float *var_w, const float *var_b
  * not read, and what the outputs hold there is left as it was. With rows != NULL (device
  * int[R]) row r takes its activations from row rows[r] of the T rows of mu_a / var_a, so a
  * token that several experts see is stored once; an entry outside 0..T-1 stands for a row
- * of zeros. Offsets outside 0..R are moved to its ends. E <= 1024 (TAGI_ERR_UNSUPPORTED
- * beyond). No workspace: calls may be captured and may overlap. No counterpart in the
+ * of zeros. Offsets outside 0..R are moved to its ends. E <= 1024, K and N <= 2^24, with
+ * rows T K < 2^32 (TAGI_ERR_UNSUPPORTED beyond). No workspace: calls may be captured and may overlap. No counterpart in the
  * reference, which has one Linear per layer; the arithmetic of a group is
  * tagi_linear_fwd's and tagi_linear_bwd's. */
 
