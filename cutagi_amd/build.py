@@ -15,7 +15,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libtagi_hip.so")
 SOURCES = ["tagi_gemm.hip", "tagi_gemv.hip", "tagi_gemv16.hip", "tagi_small.hip", "tagi_elementwise.hip",
            "tagi_conv2d.hip", "tagi_layers.hip", "tagi_conv_idx.cpp", "tagi_layernorm.hip",
-           "tagi_moe.hip", "tagi_grouped.hip", "tagi_capi.hip", "tagi_capi_moe.hip"]
+           "tagi_moe.hip", "tagi_grouped.hip", "tagi_grouped_rows.hip", "tagi_capi.hip", "tagi_capi_moe.hip"]
 # packed fp32 VALU ops are kept off for gfx950 (device pass only; the host pass
 # does not know the feature and says so)
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC",

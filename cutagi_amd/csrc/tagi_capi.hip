@@ -351,6 +351,7 @@ int tagi_hip_tune(const char *key, int value) {
     else if (!strcmp(key, "linear.gemv16.whole_lines")) g_gemv16_fwd_whole_lines = value;
     else if (!strcmp(key, "linear.stream_min_weights")) g_tune.stream_min_weights = value;
     else if (!strcmp(key, "linear.small")) g_tune.small = value;
+    else if (!strcmp(key, "grouped.rows")) g_grouped_rows = value;
     else return TAGI_ERR_INVALID_ARG;
     return TAGI_OK;
 }

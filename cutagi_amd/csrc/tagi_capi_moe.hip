@@ -149,11 +149,8 @@ int tagi_grouped_linear_bwd(const float *mu_w, const float *var_w, const float *
     }
     if (param_update) {
         p.y0 = mu_a, p.e0 = var_w, p.out0 = delta_mu_w, p.out1 = delta_var_w;
+        if (bias) p.e1 = var_b, p.db0 = delta_mu_b, p.db1 = delta_var_b;
         TAGI_TRY(launch_grouped(GROUPED_DW, p, as_stream(stream)));
-        if (bias) {
-            p.e0 = var_b, p.out0 = delta_mu_b, p.out1 = delta_var_b;
-            TAGI_TRY(launch_grouped_db(p, as_stream(stream)));
-        }
     }
     return TAGI_OK;
 }

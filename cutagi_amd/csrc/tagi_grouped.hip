@@ -4,20 +4,17 @@
 #include <type_traits>
 
 #include "tagi_activation.h"
+#include "tagi_grouped.h"
 #include "tagi_internal.h"
 
 namespace tagi {
+
+int g_grouped_rows = -1;
+
 namespace {
 
 constexpr int TPB = 256;
 constexpr int MAX_GROUPS = 1024;
-
-// Rows [first, end) of expert e, whatever the offsets hold: inside 0..R, never negative.
-__device__ __forceinline__ void group_rows(const int *__restrict__ offsets, int e, int R, int &first,
-                                           int &end) {
-    first = min(max(offsets[e], 0), R);
-    end = min(max(offsets[e + 1], first), R);
-}
 
 // ---------------------------------------------------------------------------
 // Tiled kernel. fp32 products on the bf16 matrix instructions.
@@ -653,29 +650,43 @@ __global__ __launch_bounds__(TILE_THREADS) void grouped_tile_kernel(GroupedParam
     }
 }
 
-// Bias innovations of one expert's 64 columns: four waves take every fourth row.
-__global__ __launch_bounds__(TPB) void grouped_db_kernel(GroupedParams p) {
-    __shared__ float s[2][TPB];
+// Bias innovations of one expert's 64 columns: sixteen waves take every sixteenth row, four of
+// them in flight each; their sums are joined in wave order.
+constexpr int DB_WAVES = 16;
+__global__ __launch_bounds__(DB_WAVES * 64) void grouped_db_kernel(GroupedParams p) {
+    __shared__ float s[2][DB_WAVES][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int n = blockIdx.x * 64 + lane, e = blockIdx.y;
+    const int blocks = (p.N + 63) / 64, e = blockIdx.x / blocks;
+    const int n = (blockIdx.x - e * blocks) * 64 + lane, at_n = min(n, p.N - 1);
     int first, end;
     group_rows(p.offsets, e, p.R, first, end);
-    float m = 0.f, v = 0.f;
-    if (n < p.N)
-        for (int r = first + wave; r < end; r += 4) {
-            m += p.x0[(size_t)r * p.N + n];
-            v += p.x1[(size_t)r * p.N + n];
+    float m[4] = {0.f, 0.f, 0.f, 0.f}, v[4] = {0.f, 0.f, 0.f, 0.f};
+    int r = first + wave;
+    for (; r + 3 * DB_WAVES < end; r += 4 * DB_WAVES)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const size_t at = (size_t)(r + i * DB_WAVES) * p.N + at_n;
+            m[i] += p.x0[at];
+            v[i] += p.x1[at];
         }
-    s[0][threadIdx.x] = m;
-    s[1][threadIdx.x] = v;
+    for (; r < end; r += DB_WAVES) {
+        m[0] += p.x0[(size_t)r * p.N + at_n];
+        v[0] += p.x1[(size_t)r * p.N + at_n];
+    }
+    s[0][wave][lane] = (m[0] + m[1]) + (m[2] + m[3]);
+    s[1][wave][lane] = (v[0] + v[1]) + (v[2] + v[3]);
     __syncthreads();
     if (wave != 0 || n >= p.N) return;
-    m = (s[0][lane] + s[0][64 + lane]) + (s[0][128 + lane] + s[0][192 + lane]);
-    v = (s[1][lane] + s[1][64 + lane]) + (s[1][128 + lane] + s[1][192 + lane]);
+    float sm = 0.f, sv = 0.f;
+#pragma unroll
+    for (int w = 0; w < DB_WAVES; w++) {
+        sm += s[0][w][lane];
+        sv += s[1][w][lane];
+    }
     const size_t at = (size_t)e * p.N + n;
-    const float vb = p.e0[at];
-    p.out0[at] = vb * m;
-    p.out1[at] = vb * vb * v;
+    const float vb = p.e1[at];
+    p.db0[at] = vb * sm;
+    p.db1[at] = vb * vb * sv;
 }
 
 inline int ceil_div(int a, int b) { return (a + b - 1) / b; }
@@ -710,15 +721,18 @@ hipError_t launch_grouped(GroupedMode mode, const GroupedParams &p, hipStream_t 
     const bool vec = p.K % 4 == 0 && (mode == GROUPED_FWD || p.N % 4 == 0) && aligned16(p.x0) &&
                      aligned16(p.x1) && aligned16(p.y0) && (mode != GROUPED_FWD || aligned16(p.y1)) &&
                      (mode == GROUPED_FWD || (aligned16(p.e0) && aligned16(p.out0) && aligned16(p.out1)));
+    // (its grid: one workgroup per sixteen outputs of every expert)
+    const bool few = (long long)p.R <= 16LL * p.E && (long long)p.N * p.E < (1LL << 26);
+    if (g_grouped_rows >= 0 ? g_grouped_rows != 0 : few)
+        return launch_grouped_rows(mode, p, vec, stream);
     // its 32-bit byte offsets: 128 rows of one operand, or any row where rows are gathered
     const long long most = 1LL << 30;
     const bool near = (p.rows == nullptr || (long long)p.T * p.K < most) && 128LL * p.K < most &&
                       128LL * p.N < most;
-    return vec && near ? tile_launch<true>(mode, p, stream) : tile_launch<false>(mode, p, stream);
-}
-
-hipError_t launch_grouped_db(const GroupedParams &p, hipStream_t stream) {
-    hipLaunchKernelGGL(grouped_db_kernel, dim3(ceil_div(p.N, 64), p.E), dim3(TPB), 0, stream, p);
+    hipError_t e = vec && near ? tile_launch<true>(mode, p, stream) : tile_launch<false>(mode, p, stream);
+    if (e != hipSuccess || mode != GROUPED_DW || p.db0 == nullptr) return e;
+    hipLaunchKernelGGL(grouped_db_kernel, dim3((unsigned)ceil_div(p.N, 64) * p.E), dim3(DB_WAVES * 64), 0,
+                       stream, p);
     return hipGetLastError();
 }
 

@@ -1,0 +1,401 @@
+// Linear layers grouped by expert where an expert has few rows (a decoding step, a small
+// batch): bound by the weights, which are streamed once per 16 (or 32) rows. gfx950.
+//
+// Products on v_mfma_f32_16x16x4_f32, exact fp32 products and sums: A[i][s] from lane 16 s + i,
+// B[s][j] from lane 16 s + j, D[4 (l / 16) + v][l % 16] in register v of lane l. The weights
+// come straight from memory in the operand's layout, the few rows of activations or
+// innovations from L1 / L2; eight waves share the reduction of an output block and are joined
+// through LDS in wave order.
+#include <cstdint>
+
+#include "tagi_activation.h"
+#include "tagi_grouped.h"
+#include "tagi_internal.h"
+
+namespace tagi {
+namespace {
+
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+
+constexpr int WAVES = 8, TPB = WAVES * 64;
+
+__device__ __forceinline__ floatx4 mfma(float a, float b, floatx4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
+}
+// Four elements at k of a row of `end`; zeros behind it.
+template <bool VEC>
+__device__ __forceinline__ floatx4 load4(const float *row, int k, int end) {
+    floatx4 v;
+    if (VEC) {
+        v = *reinterpret_cast<const floatx4 *>(row + min(k, end - 4));
+        const float f = k < end ? 1.f : 0.f;
+        if (f == 0.f) v = (floatx4){0.f, 0.f, 0.f, 0.f};
+    } else {
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            const float x = row[min(k + t, end - 1)];
+            v[t] = k + t < end ? x : 0.f;
+        }
+    }
+    return v;
+}
+
+// ---------------------------------------------------------------------------
+// Forward, 16 outputs n of one expert. Lane (i = l % 16, s = l / 16) holds the weights
+// [n0 + i][k + 4 s .. + 3] and row i's activations at the same k; component t of both meets in
+// MFMA t. A wave takes every eighth 32-element piece (a 128-byte line of each weight row) and
+// has the next piece's loads in flight while it multiplies.
+// ---------------------------------------------------------------------------
+template <int NG, bool VEC>
+struct FwdPiece {
+    floatx4 w0[2], w1[2], a0[NG][2], a1[NG][2];
+};
+
+template <int NG, bool VEC>
+__device__ __forceinline__ void fwd_rows(const GroupedParams &p, int e, int n0, int r0, int end,
+                                         float (*s)[16][64]) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int i = lane & 15, q = (lane >> 4) * 4, K = p.K;
+    const size_t w_at = ((size_t)e * p.N + min(n0 + i, p.N - 1)) * K;
+    const float *w0 = p.y0 + w_at, *w1 = p.y1 + w_at;
+    const float *a0[NG], *a1[NG];
+    bool live[NG];
+#pragma unroll
+    for (int g = 0; g < NG; g++) {
+        int r = min(r0 + 16 * g + i, end - 1);
+        live[g] = true;
+        if (p.rows != nullptr) {
+            r = p.rows[r];
+            live[g] = (unsigned)r < (unsigned)p.T;
+            if (!live[g]) r = 0;
+        }
+        a0[g] = p.x0 + (size_t)r * K;
+        a1[g] = p.x1 + (size_t)r * K;
+    }
+    floatx4 acc0[NG], acc1[NG];
+#pragma unroll
+    for (int g = 0; g < NG; g++) acc0[g] = acc1[g] = (floatx4){0.f, 0.f, 0.f, 0.f};
+    auto load = [&](FwdPiece<NG, VEC> &f, int kb) {
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const int k = kb + 16 * h + q;
+            f.w0[h] = load4<VEC>(w0, k, K);
+            f.w1[h] = load4<VEC>(w1, k, K);
+#pragma unroll
+            for (int g = 0; g < NG; g++) {
+                f.a0[g][h] = load4<VEC>(a0[g], k, K);
+                f.a1[g][h] = load4<VEC>(a1[g], k, K);
+            }
+        }
+    };
+    auto use = [&](const FwdPiece<NG, VEC> &f) {
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int t = 0; t < 4; t++) {
+                const float w = f.w0[h][t], v = f.w1[h][t], w2 = w * w;
+#pragma unroll
+                for (int g = 0; g < NG; g++) {
+                    const float m = live[g] ? f.a0[g][h][t] : 0.f, u = live[g] ? f.a1[g][h][t] : 0.f;
+                    acc0[g] = mfma(w, m, acc0[g]);
+                    acc1[g] = mfma(v, fmaf(m, m, u), acc1[g]);
+                    acc1[g] = mfma(w2, u, acc1[g]);
+                }
+            }
+    };
+    FwdPiece<NG, VEC> x, y;
+    const int step = 32 * WAVES;
+    int kb = 32 * wave;
+    if (kb < K) load(x, kb);
+    for (; kb < K; kb += 2 * step) {
+        if (kb + step < K) load(y, kb + step);
+        use(x);
+        if (kb + step >= K) break;
+        if (kb + 2 * step < K) load(x, kb + 2 * step);
+        use(y);
+    }
+    // join: s[wave][8 g + 4 a + v][lane]
+#pragma unroll
+    for (int g = 0; g < NG; g++)
+#pragma unroll
+        for (int v = 0; v < 4; v++) {
+            s[wave][8 * g + v][lane] = acc0[g][v];
+            s[wave][8 * g + 4 + v][lane] = acc1[g][v];
+        }
+    __syncthreads();
+    // thread: output n0 + x of row j of group g
+    if (tid < 256 * NG) {
+        const int g = tid >> 8, j = (tid >> 4) & 15, x16 = tid & 15;
+        const int l = (x16 >> 2) * 16 + j, v = x16 & 3;
+        float m = 0.f, u = 0.f;
+#pragma unroll
+        for (int w = 0; w < WAVES; w++) {
+            m += s[w][8 * g + v][l];
+            u += s[w][8 * g + 4 + v][l];
+        }
+        const int r = r0 + 16 * g + j, n = n0 + x16;
+        if (r < end && n < p.N) {
+            if (p.e0 != nullptr) {
+                m += p.e0[(size_t)e * p.N + n];
+                u += p.e1[(size_t)e * p.N + n];
+            }
+            store_activated(p.act, m, u, (size_t)r * p.N + n, p.out0, p.out1, p.out2);
+        }
+    }
+    __syncthreads();
+}
+
+template <bool VEC>
+__global__ __launch_bounds__(TPB) void rows_fwd_kernel(GroupedParams p) {
+    __shared__ float s[WAVES][16][64];
+    const int blocks = (p.N + 15) / 16;
+    const int e = blockIdx.x / blocks, n0 = (blockIdx.x - e * blocks) * 16;
+    int first, end;
+    group_rows(p.offsets, e, p.R, first, end);
+    for (int r = first; r < end; r += 32) {
+        if (end - r > 16)
+            fwd_rows<2, VEC>(p, e, n0, r, end, s);
+        else
+            fwd_rows<1, VEC>(p, e, n0, r, end, s);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// State backward, 64 inputs k of one expert. Lane (i, s) holds mu_w[n + 4 s + u][k0 + 4 i .. + 3]
+// for u = 0..3 (a load covers four weight rows of 256 bytes) and row i's innovations at
+// n + 4 s .. + 3: component t of step u meets component u of the innovations in an MFMA of
+// its own sum, D[i][j] = output k0 + 4 i + t of row j.
+// ---------------------------------------------------------------------------
+template <int NG>
+struct DzPiece {
+    floatx4 w[4], d0[NG], d1[NG];
+};
+
+template <int NG, bool VEC>
+__device__ __forceinline__ void dz_rows(const GroupedParams &p, int e, int k0, int r0, int end,
+                                        float (*s)[16][65]) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int i = lane & 15, q = (lane >> 4) * 4, K = p.K, N = p.N;
+    const float *w = p.y0 + (size_t)e * N * K;
+    const int k = k0 + 4 * i;
+    const float *d0[NG], *d1[NG];
+#pragma unroll
+    for (int g = 0; g < NG; g++) {
+        const size_t r = (size_t)min(r0 + 16 * g + i, end - 1) * N;
+        d0[g] = p.x0 + r;
+        d1[g] = p.x1 + r;
+    }
+    floatx4 acc0[NG][4], acc1[NG][4];
+#pragma unroll
+    for (int g = 0; g < NG; g++)
+#pragma unroll
+        for (int t = 0; t < 4; t++) acc0[g][t] = acc1[g][t] = (floatx4){0.f, 0.f, 0.f, 0.f};
+    auto load = [&](DzPiece<NG> &f, int nb) {
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            const int n = nb + q + u;
+            f.w[u] = load4<VEC>(w + (size_t)min(n, N - 1) * K, k, K);
+            if (n >= N) f.w[u] = (floatx4){0.f, 0.f, 0.f, 0.f};
+        }
+#pragma unroll
+        for (int g = 0; g < NG; g++) {
+            f.d0[g] = load4<VEC>(d0[g], nb + q, N);
+            f.d1[g] = load4<VEC>(d1[g], nb + q, N);
+        }
+    };
+    auto use = [&](const DzPiece<NG> &f) {
+#pragma unroll
+        for (int u = 0; u < 4; u++)
+#pragma unroll
+            for (int t = 0; t < 4; t++) {
+                const float x = f.w[u][t], x2 = x * x;
+#pragma unroll
+                for (int g = 0; g < NG; g++) {
+                    acc0[g][t] = mfma(x, f.d0[g][u], acc0[g][t]);
+                    acc1[g][t] = mfma(x2, f.d1[g][u], acc1[g][t]);
+                }
+            }
+    };
+    DzPiece<NG> x, y;
+    const int step = 16 * WAVES;
+    int nb = 16 * wave;
+    if (nb < N) load(x, nb);
+    for (; nb < N; nb += 2 * step) {
+        if (nb + step < N) load(y, nb + step);
+        use(x);
+        if (nb + step >= N) break;
+        if (nb + 2 * step < N) load(x, nb + 2 * step);
+        use(y);
+    }
+#pragma unroll
+    for (int g = 0; g < NG; g++) {
+        float sum[2][2];
+#pragma unroll
+        for (int a = 0; a < 2; a++) {
+            __syncthreads();
+#pragma unroll
+            for (int t = 0; t < 4; t++)
+#pragma unroll
+                for (int v = 0; v < 4; v++) s[wave][4 * t + v][lane] = (a == 0 ? acc0 : acc1)[g][t][v];
+            __syncthreads();
+            // thread: input k0 + tid % 64 of the rows tid / 64 and 8 + tid / 64
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const int c = tid & 63, j = (tid >> 6) + 8 * h;
+                const int l = (c >> 4) * 16 + j, x16 = 4 * (c & 3) + ((c >> 2) & 3);
+                float m = 0.f;
+#pragma unroll
+                for (int w8 = 0; w8 < WAVES; w8++) m += s[w8][x16][l];
+                sum[a][h] = m;
+            }
+        }
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const int c = k0 + (tid & 63), r = r0 + 16 * g + (tid >> 6) + 8 * h;
+            if (r < end && c < K) {
+                const size_t at = (size_t)r * K + c;
+                const float f = p.e0 != nullptr ? p.e0[at] : 1.f;
+                p.out0[at] = sum[0][h] * f;
+                p.out1[at] = sum[1][h] * f * f;
+            }
+        }
+    }
+    __syncthreads();
+}
+
+template <bool VEC>
+__global__ __launch_bounds__(TPB) void rows_dz_kernel(GroupedParams p) {
+    __shared__ float s[WAVES][16][65];
+    const int blocks = (p.K + 63) / 64;
+    const int e = blockIdx.x / blocks, k0 = (blockIdx.x - e * blocks) * 64;
+    int first, end;
+    group_rows(p.offsets, e, p.R, first, end);
+    for (int r = first; r < end; r += 32) {
+        if (end - r > 16)
+            dz_rows<2, VEC>(p, e, k0, r, end, s);
+        else
+            dz_rows<1, VEC>(p, e, k0, r, end, s);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Weight (and bias) backward: a wave owns eight rows n by 256 columns k of one expert's
+// weights, four columns per lane, and adds the outer products of the expert's rows four at a
+// time; the innovations of a row are the same for the whole wave. Twelve bytes move per
+// weight, two multiplications-and-additions per row of the batch: bound by memory up to some
+// tens of rows.
+// ---------------------------------------------------------------------------
+constexpr int DW_ROWS = 8, DW_COLS = 256, DW_WAVES = 4;
+
+template <bool VEC>
+__global__ __launch_bounds__(DW_WAVES * 64) void rows_dw_kernel(GroupedParams p) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int K = p.K, N = p.N;
+    const int col_blocks = (K + DW_COLS - 1) / DW_COLS;
+    const int row_blocks = (N + DW_ROWS * DW_WAVES - 1) / (DW_ROWS * DW_WAVES);
+    const int kb = blockIdx.x % col_blocks, rest = blockIdx.x / col_blocks;
+    const int e = rest / row_blocks;
+    const int n0 = (rest - e * row_blocks) * DW_ROWS * DW_WAVES + wave * DW_ROWS;
+    const int k = kb * DW_COLS + lane * 4;
+    int first, end;
+    group_rows(p.offsets, e, p.R, first, end);
+    if (n0 >= N) return;
+    const int rows_n = min(DW_ROWS, N - n0);
+    const float *__restrict__ d0 = p.x0, *__restrict__ d1 = p.x1;
+    if (p.db0 != nullptr && kb == 0 && lane < rows_n) {
+        float m = 0.f, v = 0.f;
+        for (int r = first; r < end; r++) {
+            m += d0[(size_t)r * N + n0 + lane];
+            v += d1[(size_t)r * N + n0 + lane];
+        }
+        const size_t at = (size_t)e * N + n0 + lane;
+        const float vb = p.e1[at];
+        p.db0[at] = vb * m;
+        p.db1[at] = vb * vb * v;
+    }
+    if (k >= K) return;
+    floatx4 acc0[DW_ROWS], acc1[DW_ROWS];
+#pragma unroll
+    for (int n = 0; n < DW_ROWS; n++) acc0[n] = acc1[n] = (floatx4){0.f, 0.f, 0.f, 0.f};
+    for (int r = first; r < end; r += 4) {
+        floatx4 a[4], a2[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            int s = min(r + j, end - 1);
+            bool live = r + j < end;
+            if (p.rows != nullptr) {
+                s = p.rows[s];
+                live = live && (unsigned)s < (unsigned)p.T;
+                if (!live) s = 0;
+            }
+            a[j] = load4<VEC>(p.y0 + (size_t)s * K, k, K);
+            if (!live) a[j] = (floatx4){0.f, 0.f, 0.f, 0.f};
+            a2[j] = a[j] * a[j];
+        }
+#pragma unroll
+        for (int n = 0; n < DW_ROWS; n++) {
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const size_t at = (size_t)min(r + j, end - 1) * N + min(n0 + n, N - 1);
+                const bool live = r + j < end;
+                const float m = live ? d0[at] : 0.f, v = live ? d1[at] : 0.f;
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    acc0[n][c] = fmaf(m, a[j][c], acc0[n][c]);
+                    acc1[n][c] = fmaf(v, a2[j][c], acc1[n][c]);
+                }
+            }
+        }
+    }
+    for (int n = 0; n < rows_n; n++) {
+        const size_t at = ((size_t)e * N + n0 + n) * K + k;
+        floatx4 x = acc0[0], y = acc1[0];
+#pragma unroll
+        for (int i = 1; i < DW_ROWS; i++)
+            if (i == n) {
+                x = acc0[i];
+                y = acc1[i];
+            }
+        if (VEC) {
+            const floatx4 w = *reinterpret_cast<const floatx4 *>(p.e0 + at);
+            *reinterpret_cast<floatx4 *>(p.out0 + at) = x * w;
+            *reinterpret_cast<floatx4 *>(p.out1 + at) = y * w * w;
+        } else {
+#pragma unroll
+            for (int c = 0; c < 4; c++)
+                if (k + c < K) {
+                    const float w = p.e0[at + c];
+                    p.out0[at + c] = x[c] * w;
+                    p.out1[at + c] = y[c] * w * w;
+                }
+        }
+    }
+}
+
+}  // namespace
+
+hipError_t launch_grouped_rows(GroupedMode mode, const GroupedParams &p, bool vec, hipStream_t stream) {
+    if (mode == GROUPED_FWD) {
+        const dim3 grid((unsigned)((p.N + 15) / 16) * p.E);
+        if (vec)
+            hipLaunchKernelGGL(rows_fwd_kernel<true>, grid, dim3(TPB), 0, stream, p);
+        else
+            hipLaunchKernelGGL(rows_fwd_kernel<false>, grid, dim3(TPB), 0, stream, p);
+    } else if (mode == GROUPED_DZ) {
+        const dim3 grid((unsigned)((p.K + 63) / 64) * p.E);
+        if (vec)
+            hipLaunchKernelGGL(rows_dz_kernel<true>, grid, dim3(TPB), 0, stream, p);
+        else
+            hipLaunchKernelGGL(rows_dz_kernel<false>, grid, dim3(TPB), 0, stream, p);
+    } else {
+        const int rows = DW_ROWS * DW_WAVES;
+        const dim3 grid((unsigned)((p.K + DW_COLS - 1) / DW_COLS) * ((p.N + rows - 1) / rows) * p.E);
+        if (vec)
+            hipLaunchKernelGGL(rows_dw_kernel<true>, grid, dim3(DW_WAVES * 64), 0, stream, p);
+        else
+            hipLaunchKernelGGL(rows_dw_kernel<false>, grid, dim3(DW_WAVES * 64), 0, stream, p);
+    }
+    return hipGetLastError();
+}
+
+}  // namespace tagi

@@ -341,18 +341,21 @@ hipError_t launch_moe_gather_bwd(const float *dmu_r, const float *dvar_r, const 
 // R rows meet the weights [e][N][K].
 //   FWD: x0,x1 = mu_a,var_a [T or R][K]   y0,y1 = mu_w,var_w    e0,e1 = biases (may be null)
 //   DZ : x0,x1 = innovations [R][N]       y0 = mu_w             e0 = jcb [R][K] (may be null)
-//   DW : x0,x1 = innovations [R][N]       y0 = mu_a [T or R][K] e0 = var_w
-//   bias innovations: x0,x1 = innovations, e0 = var_b
+//   DW : x0,x1 = innovations [R][N]       y0 = mu_a [T or R][K] e0 = var_w, e1 = var_b;
+//        db0,db1: the bias innovations, in the same call (may be null)
 // rows (may be null): row r reads row rows[r] of the activations (T of them).
 enum GroupedMode { GROUPED_FWD = 0, GROUPED_DZ = 1, GROUPED_DW = 2 };
 struct GroupedParams {
     const float *x0, *x1, *y0, *y1, *e0, *e1;
     const int *offsets, *rows;
     int K, N, E, R, T, act;
-    float *out0, *out1, *out2;
+    float *out0, *out1, *out2, *db0, *db1;
 };
+// 0 / 1: always the tiled kernels / always those for few rows (tuning knob); -1: by size
+extern int g_grouped_rows;
 hipError_t launch_grouped(GroupedMode mode, const GroupedParams &p, hipStream_t stream);
-hipError_t launch_grouped_db(const GroupedParams &p, hipStream_t stream);
+// the kernels for few rows per expert (tagi_grouped_rows.hip)
+hipError_t launch_grouped_rows(GroupedMode mode, const GroupedParams &p, bool vec, hipStream_t stream);
 
 // Host-side index tables (tagi_conv_idx.cpp)
 int conv2d_out_size(int kernel, int stride, int wi, int hi, int pad, int pad_type, int *wo,

@@ -39,7 +39,9 @@ extern "C" {
  * all four phases in one workgroup and its pair-wise fold, weight backward - which leaves
  * those layers on the table-driven kernels; "conv2d.bwd_pair": 0 gives the state and the
  * weight backward of tagi_conv2d_bwd launches of their own). "batchnorm.fused_train": 0
- * gives tagi_batchnorm2d_fwd_train a launch of its own for the merge of the statistics. */
+ * gives tagi_batchnorm2d_fwd_train a launch of its own for the merge of the statistics.
+ * "grouped.rows": 1 sends every grouped Linear call to the kernels for few rows per expert,
+ * 0 to the tiled ones, < 0 by size. */
 int tagi_hip_tune(const char *key /* host */, int value);
 
 #ifdef __cplusplus

@@ -19,6 +19,16 @@ def _host(t):
     return t.cpu().numpy()
 
 
+@pytest.fixture(params=["by_size", "few_rows", "tiled"])
+def kernel_choice(request):
+    """Calls with few rows per expert go to kernels of their own; "few_rows" and "tiled" send
+    every call to the ones or the others, so that the small shapes reach both."""
+    from cutagi_amd import capi
+    capi.tune("grouped.rows", {"by_size": -1, "few_rows": 1, "tiled": 0}[request.param])
+    yield request.param
+    capi.tune("grouped.rows", -1)
+
+
 # (rows of the experts, K, N, tokens or None, rows behind the last group)
 GROUPS = [
     ([1], 1, 1, None, 0),
@@ -42,7 +52,7 @@ GUARD = 12345.0
 
 @pytest.mark.parametrize("bias", [True, False])
 @pytest.mark.parametrize("sizes,K,N,tokens,tail", GROUPS)
-def test_grouped_linear(sizes, K, N, tokens, tail, bias):
+def test_grouped_linear(kernel_choice, sizes, K, N, tokens, tail, bias):
     import torch
     import cutagi_amd.functional as F
     d = C.grouped_inputs(sizes, K, N, seed=K + N, tokens=tokens, tail=tail)
@@ -75,7 +85,7 @@ def test_grouped_linear(sizes, K, N, tokens, tail, bias):
 
 @pytest.mark.parametrize("sizes,K,N,tokens", [([5, 0, 20], 96, 64, None), ([70, 130], 132, 260, 40),
                                               ([2, 1], 256, 128, 2)])
-def test_parts_and_the_same_bits_every_call(sizes, K, N, tokens):
+def test_parts_and_the_same_bits_every_call(kernel_choice, sizes, K, N, tokens):
     import torch
     import cutagi_amd.functional as F
     t = _dev(C.grouped_inputs(sizes, K, N, seed=1, tokens=tokens))
@@ -93,7 +103,7 @@ def test_parts_and_the_same_bits_every_call(sizes, K, N, tokens):
 
 @pytest.mark.parametrize("activation", ["relu", "mixture_relu"])
 @pytest.mark.parametrize("sizes,K,N", [([3, 0, 2], 64, 40), ([90, 40], 72, 130)])
-def test_fused_activation_is_the_activation_of_the_layer(activation, sizes, K, N):
+def test_fused_activation_is_the_activation_of_the_layer(kernel_choice, activation, sizes, K, N):
     import torch
     import cutagi_amd.functional as F
     t = _dev(C.grouped_inputs(sizes, K, N, seed=2, tokens=11))
@@ -109,7 +119,7 @@ def test_fused_activation_is_the_activation_of_the_layer(activation, sizes, K, N
 
 
 @pytest.mark.parametrize("sizes,K,N", [([5, 9], 64, 32), ([100, 31], 128, 132), ([140, 150], 260, 256)])
-def test_arrays_that_are_not_16_byte_aligned(sizes, K, N):
+def test_arrays_that_are_not_16_byte_aligned(kernel_choice, sizes, K, N):
     import torch
     import cutagi_amd.functional as F
     d = C.grouped_inputs(sizes, K, N, seed=4, tokens=30)
@@ -130,7 +140,7 @@ def test_arrays_that_are_not_16_byte_aligned(sizes, K, N):
         C.check(_host(g), *C.grouped_bwd(d)[name], name)
 
 
-def test_indices_outside_the_arrays_read_nothing():
+def test_indices_outside_the_arrays_read_nothing(kernel_choice):
     """Row indices that are no token stand for rows of zeros, offsets beyond the rows are
     moved to their end."""
     import torch
@@ -150,7 +160,7 @@ def test_indices_outside_the_arrays_read_nothing():
         C.check(_host(g), *C.grouped_bwd(d)[name], name)
 
 
-def test_one_group_is_the_linear_layer():
+def test_one_group_is_the_linear_layer(kernel_choice):
     """E = 1 against the ungrouped entry points (each is within its own bound of the exact
     result, so they are within twice that of one another)."""
     import cutagi_amd.functional as F
@@ -169,7 +179,7 @@ def test_one_group_is_the_linear_layer():
         C.check(_host(g).reshape(_host(r).shape), _host(r), bound.reshape(_host(r).shape), name)
 
 
-def test_innovations_against_differences():
+def test_innovations_against_differences(kernel_choice):
     """mu_z is linear in mu_a and in mu_w: <mu_z(a + v) - mu_z(a), delta_mu> = <v, delta_mu_z>
     without a Jacobian, and the same for the weights with delta_mu_w / var_w. Inputs in a few
     bits, so that the differences are exact."""
