@@ -721,8 +721,12 @@ hipError_t launch_grouped(GroupedMode mode, const GroupedParams &p, hipStream_t 
     const bool vec = p.K % 4 == 0 && (mode == GROUPED_FWD || p.N % 4 == 0) && aligned16(p.x0) &&
                      aligned16(p.x1) && aligned16(p.y0) && (mode != GROUPED_FWD || aligned16(p.y1)) &&
                      (mode == GROUPED_FWD || (aligned16(p.e0) && aligned16(p.out0) && aligned16(p.out1)));
-    // (its grid: one workgroup per sixteen outputs of every expert)
-    const bool few = (long long)p.R <= 16LL * p.E && (long long)p.N * p.E < (1LL << 26);
+    // Few rows per expert on average: the weights are what takes the time. At 32 rows (256 rows,
+    // 8 experts of 2048 x 2048) streaming against tiles: forward 150 / 130 us, state backward
+    // 65 / 180 us, weight backward 218 / 194 us; at 4 rows (16 experts) streaming wins all
+    // three. (The streaming grid: one workgroup per sixteen outputs of every expert.)
+    const bool few = (long long)p.R <= (mode == GROUPED_DZ ? 32LL : 16LL) * p.E &&
+                     (long long)p.N * p.E < (1LL << 26);
     if (g_grouped_rows >= 0 ? g_grouped_rows != 0 : few)
         return launch_grouped_rows(mode, p, vec, stream);
     // its 32-bit byte offsets: 128 rows of one operand, or any row where rows are gathered

@@ -4,7 +4,7 @@
 // Products on v_mfma_f32_16x16x4_f32, exact fp32 products and sums: A[i][s] from lane 16 s + i,
 // B[s][j] from lane 16 s + j, D[4 (l / 16) + v][l % 16] in register v of lane l. The weights
 // come straight from memory in the operand's layout, the few rows of activations or
-// innovations from L1 / L2; eight waves share the reduction of an output block and are joined
+// innovations from L1 / L2; the waves of a workgroup share the reduction of an output block and are joined
 // through LDS in wave order.
 #include <cstdint>
 
@@ -16,8 +16,6 @@ namespace tagi {
 namespace {
 
 typedef float floatx4 __attribute__((ext_vector_type(4)));
-
-constexpr int WAVES = 8, TPB = WAVES * 64;
 
 __device__ __forceinline__ floatx4 mfma(float a, float b, floatx4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
@@ -43,7 +41,7 @@ __device__ __forceinline__ floatx4 load4(const float *row, int k, int end) {
 // ---------------------------------------------------------------------------
 // Forward, 16 outputs n of one expert. Lane (i = l % 16, s = l / 16) holds the weights
 // [n0 + i][k + 4 s .. + 3] and row i's activations at the same k; component t of both meets in
-// MFMA t. A wave takes every eighth 32-element piece (a 128-byte line of each weight row) and
+// MFMA t. A wave takes every WAVES-th 32-element piece (a 128-byte line of each weight row) and
 // has the next piece's loads in flight while it multiplies.
 // ---------------------------------------------------------------------------
 template <int NG, bool VEC>
@@ -51,13 +49,25 @@ struct FwdPiece {
     floatx4 w0[2], w1[2], a0[NG][2], a1[NG][2];
 };
 
-template <int NG, bool VEC>
+template <int WAVES, int NG, bool VEC>
 __device__ __forceinline__ void fwd_rows(const GroupedParams &p, int e, int n0, int r0, int end,
-                                         float (*s)[16][64]) {
+                                         float (*s)[8 * NG][64]) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int i = lane & 15, q = (lane >> 4) * 4, K = p.K;
     const size_t w_at = ((size_t)e * p.N + min(n0 + i, p.N - 1)) * K;
     const float *w0 = p.y0 + w_at, *w1 = p.y1 + w_at;
+    // the first weights are on their way before the row indices are known
+    FwdPiece<NG, VEC> x, y;
+    const int step = 32 * WAVES;
+    int kb = 32 * wave;
+    auto load_w = [&](FwdPiece<NG, VEC> &f, int kb) {
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            f.w0[h] = load4<VEC>(w0, kb + 16 * h + q, K);
+            f.w1[h] = load4<VEC>(w1, kb + 16 * h + q, K);
+        }
+    };
+    if (kb < K) load_w(x, kb);
     const float *a0[NG], *a1[NG];
     bool live[NG];
 #pragma unroll
@@ -75,18 +85,18 @@ __device__ __forceinline__ void fwd_rows(const GroupedParams &p, int e, int n0, 
     floatx4 acc0[NG], acc1[NG];
 #pragma unroll
     for (int g = 0; g < NG; g++) acc0[g] = acc1[g] = (floatx4){0.f, 0.f, 0.f, 0.f};
-    auto load = [&](FwdPiece<NG, VEC> &f, int kb) {
+    auto load_a = [&](FwdPiece<NG, VEC> &f, int kb) {
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            const int k = kb + 16 * h + q;
-            f.w0[h] = load4<VEC>(w0, k, K);
-            f.w1[h] = load4<VEC>(w1, k, K);
+        for (int h = 0; h < 2; h++)
 #pragma unroll
             for (int g = 0; g < NG; g++) {
-                f.a0[g][h] = load4<VEC>(a0[g], k, K);
-                f.a1[g][h] = load4<VEC>(a1[g], k, K);
+                f.a0[g][h] = load4<VEC>(a0[g], kb + 16 * h + q, K);
+                f.a1[g][h] = load4<VEC>(a1[g], kb + 16 * h + q, K);
             }
-        }
+    };
+    auto load = [&](FwdPiece<NG, VEC> &f, int kb) {
+        load_w(f, kb);
+        load_a(f, kb);
     };
     auto use = [&](const FwdPiece<NG, VEC> &f) {
 #pragma unroll
@@ -103,10 +113,7 @@ __device__ __forceinline__ void fwd_rows(const GroupedParams &p, int e, int n0, 
                 }
             }
     };
-    FwdPiece<NG, VEC> x, y;
-    const int step = 32 * WAVES;
-    int kb = 32 * wave;
-    if (kb < K) load(x, kb);
+    if (kb < K) load_a(x, kb);
     for (; kb < K; kb += 2 * step) {
         if (kb + step < K) load(y, kb + step);
         use(x);
@@ -124,8 +131,9 @@ __device__ __forceinline__ void fwd_rows(const GroupedParams &p, int e, int n0, 
         }
     __syncthreads();
     // thread: output n0 + x of row j of group g
-    if (tid < 256 * NG) {
-        const int g = tid >> 8, j = (tid >> 4) & 15, x16 = tid & 15;
+#pragma unroll
+    for (int at = tid; at < 256 * NG; at += WAVES * 64) {
+        const int g = at >> 8, j = (at >> 4) & 15, x16 = at & 15;
         const int l = (x16 >> 2) * 16 + j, v = x16 & 3;
         float m = 0.f, u = 0.f;
 #pragma unroll
@@ -145,19 +153,14 @@ __device__ __forceinline__ void fwd_rows(const GroupedParams &p, int e, int n0, 
     __syncthreads();
 }
 
-template <bool VEC>
-__global__ __launch_bounds__(TPB) void rows_fwd_kernel(GroupedParams p) {
-    __shared__ float s[WAVES][16][64];
+template <int WAVES, int NG, bool VEC>
+__global__ __launch_bounds__(WAVES * 64, NG == 1 && VEC ? 4 : 2) void rows_fwd_kernel(GroupedParams p) {
+    __shared__ float s[WAVES][8 * NG][64];
     const int blocks = (p.N + 15) / 16;
     const int e = blockIdx.x / blocks, n0 = (blockIdx.x - e * blocks) * 16;
     int first, end;
     group_rows(p.offsets, e, p.R, first, end);
-    for (int r = first; r < end; r += 32) {
-        if (end - r > 16)
-            fwd_rows<2, VEC>(p, e, n0, r, end, s);
-        else
-            fwd_rows<1, VEC>(p, e, n0, r, end, s);
-    }
+    for (int r = first; r < end; r += 16 * NG) fwd_rows<WAVES, NG, VEC>(p, e, n0, r, end, s);
 }
 
 // ---------------------------------------------------------------------------
@@ -166,6 +169,8 @@ __global__ __launch_bounds__(TPB) void rows_fwd_kernel(GroupedParams p) {
 // n + 4 s .. + 3: component t of step u meets component u of the innovations in an MFMA of
 // its own sum, D[i][j] = output k0 + 4 i + t of row j.
 // ---------------------------------------------------------------------------
+constexpr int DZ_WAVES = 8;
+
 template <int NG>
 struct DzPiece {
     floatx4 w[4], d0[NG], d1[NG];
@@ -217,7 +222,7 @@ __device__ __forceinline__ void dz_rows(const GroupedParams &p, int e, int k0, i
             }
     };
     DzPiece<NG> x, y;
-    const int step = 16 * WAVES;
+    const int step = 16 * DZ_WAVES;
     int nb = 16 * wave;
     if (nb < N) load(x, nb);
     for (; nb < N; nb += 2 * step) {
@@ -227,9 +232,10 @@ __device__ __forceinline__ void dz_rows(const GroupedParams &p, int e, int k0, i
         if (nb + 2 * step < N) load(x, nb + 2 * step);
         use(y);
     }
+    constexpr int STEPS = 1024 / (DZ_WAVES * 64);   // outputs of a thread: 16 rows by 64 inputs
 #pragma unroll
     for (int g = 0; g < NG; g++) {
-        float sum[2][2];
+        float sum[2][STEPS];
 #pragma unroll
         for (int a = 0; a < 2; a++) {
             __syncthreads();
@@ -238,20 +244,19 @@ __device__ __forceinline__ void dz_rows(const GroupedParams &p, int e, int k0, i
 #pragma unroll
                 for (int v = 0; v < 4; v++) s[wave][4 * t + v][lane] = (a == 0 ? acc0 : acc1)[g][t][v];
             __syncthreads();
-            // thread: input k0 + tid % 64 of the rows tid / 64 and 8 + tid / 64
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                const int c = tid & 63, j = (tid >> 6) + 8 * h;
+            for (int h = 0; h < STEPS; h++) {
+                const int c = tid & 63, j = (tid >> 6) + DZ_WAVES * h;
                 const int l = (c >> 4) * 16 + j, x16 = 4 * (c & 3) + ((c >> 2) & 3);
                 float m = 0.f;
 #pragma unroll
-                for (int w8 = 0; w8 < WAVES; w8++) m += s[w8][x16][l];
+                for (int w8 = 0; w8 < DZ_WAVES; w8++) m += s[w8][x16][l];
                 sum[a][h] = m;
             }
         }
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            const int c = k0 + (tid & 63), r = r0 + 16 * g + (tid >> 6) + 8 * h;
+        for (int h = 0; h < STEPS; h++) {
+            const int c = k0 + (tid & 63), r = r0 + 16 * g + (tid >> 6) + DZ_WAVES * h;
             if (r < end && c < K) {
                 const size_t at = (size_t)r * K + c;
                 const float f = p.e0 != nullptr ? p.e0[at] : 1.f;
@@ -263,19 +268,14 @@ __device__ __forceinline__ void dz_rows(const GroupedParams &p, int e, int k0, i
     __syncthreads();
 }
 
-template <bool VEC>
-__global__ __launch_bounds__(TPB) void rows_dz_kernel(GroupedParams p) {
-    __shared__ float s[WAVES][16][65];
+template <int NG, bool VEC>
+__global__ __launch_bounds__(DZ_WAVES * 64, NG == 1 && VEC ? 4 : 2) void rows_dz_kernel(GroupedParams p) {
+    __shared__ float s[DZ_WAVES][16][65];
     const int blocks = (p.K + 63) / 64;
     const int e = blockIdx.x / blocks, k0 = (blockIdx.x - e * blocks) * 64;
     int first, end;
     group_rows(p.offsets, e, p.R, first, end);
-    for (int r = first; r < end; r += 32) {
-        if (end - r > 16)
-            dz_rows<2, VEC>(p, e, k0, r, end, s);
-        else
-            dz_rows<1, VEC>(p, e, k0, r, end, s);
-    }
+    for (int r = first; r < end; r += 16 * NG) dz_rows<NG, VEC>(p, e, k0, r, end, s);
 }
 
 // ---------------------------------------------------------------------------
@@ -372,21 +372,47 @@ __global__ __launch_bounds__(DW_WAVES * 64) void rows_dw_kernel(GroupedParams p)
     }
 }
 
+template <int WAVES, int NG, bool VEC>
+void rows_fwd(const GroupedParams &p, unsigned grid, hipStream_t stream) {
+    hipLaunchKernelGGL((rows_fwd_kernel<WAVES, NG, VEC>), dim3(grid), dim3(WAVES * 64), 0, stream, p);
+}
+template <int NG, bool VEC>
+void rows_dz(const GroupedParams &p, unsigned grid, hipStream_t stream) {
+    hipLaunchKernelGGL((rows_dz_kernel<NG, VEC>), dim3(grid), dim3(DZ_WAVES * 64), 0, stream, p);
+}
+
 }  // namespace
 
 hipError_t launch_grouped_rows(GroupedMode mode, const GroupedParams &p, bool vec, hipStream_t stream) {
+    // two groups of sixteen rows share a pass over the weights where experts have more than
+    // eight rows on average; one group leaves registers for twice the waves
+    const bool one = (long long)p.R <= 8LL * p.E;
+    // experts that can have rows
+    const long long used = p.E < p.R ? p.E : p.R;
     if (mode == GROUPED_FWD) {
-        const dim3 grid((unsigned)((p.N + 15) / 16) * p.E);
-        if (vec)
-            hipLaunchKernelGGL(rows_fwd_kernel<true>, grid, dim3(TPB), 0, stream, p);
+        const unsigned blocks = (p.N + 15) / 16, grid = blocks * p.E;
+        // Waves that share a block: many blocks fill the chip with few waves each, which
+        // spend less of their time starting and joining. 4 / 8 / 16 waves: 216 / 231 / 266 us
+        // at 16 x 256 blocks of 2048, 73 / 61 / 69 at 2 x 256 of 4096, 43 / 30 / 26 at 2 x 64.
+        const long long working = used * blocks;
+        if (!vec)
+            one ? rows_fwd<8, 1, false>(p, grid, stream) : rows_fwd<8, 2, false>(p, grid, stream);
+        else if (!one)
+            rows_fwd<8, 2, true>(p, grid, stream);
+        else if (working > 1024)
+            rows_fwd<4, 1, true>(p, grid, stream);
+        else if (working > 256)
+            rows_fwd<8, 1, true>(p, grid, stream);
         else
-            hipLaunchKernelGGL(rows_fwd_kernel<false>, grid, dim3(TPB), 0, stream, p);
+            rows_fwd<16, 1, true>(p, grid, stream);
     } else if (mode == GROUPED_DZ) {
-        const dim3 grid((unsigned)((p.K + 63) / 64) * p.E);
-        if (vec)
-            hipLaunchKernelGGL(rows_dz_kernel<true>, grid, dim3(TPB), 0, stream, p);
+        const unsigned blocks = (p.K + 63) / 64, grid = blocks * p.E;
+        if (!vec)
+            one ? rows_dz<1, false>(p, grid, stream) : rows_dz<2, false>(p, grid, stream);
+        else if (!one)
+            rows_dz<2, true>(p, grid, stream);
         else
-            hipLaunchKernelGGL(rows_dz_kernel<false>, grid, dim3(TPB), 0, stream, p);
+            rows_dz<1, true>(p, grid, stream);
     } else {
         const int rows = DW_ROWS * DW_WAVES;
         const dim3 grid((unsigned)((p.K + DW_COLS - 1) / DW_COLS) * ((p.N + rows - 1) / rows) * p.E);
