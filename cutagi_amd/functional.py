@@ -343,11 +343,24 @@ def add_shortcut_delta(mu_s, var_s, jcb_s, mu_a, var_a):
 
 
 # ---- layer norm, grouped Linear layers, mixture of experts ---------------------------------
+# Calls for single tokens are bound by the host, so these keep to a few allocations each and
+# name what is wrong with an argument only once something is.
+
+_F, _I = torch.float32, torch.int32
 
 
-def _chk_shapes(**named):
-    """named: argument name -> (tensor or None, shape, dtype). Every tensor present has to be
-    a contiguous tensor of that shape and type on the current device."""
+def _fits(device, dtype, shape, *tensors):
+    """Whether every tensor (None: absent) is a contiguous one of this device, type and shape."""
+    for t in tensors:
+        if t is not None and (t.dtype is not dtype or t.shape != shape or not t.is_contiguous()
+                              or t.get_device() != device):
+            return False
+    return True
+
+
+def _explain(**named):
+    """Raises for the first argument, name -> (tensor or None, shape, dtype), that is not a
+    contiguous tensor of that shape and type on the current device."""
     present = [(name, t, shape, dtype) for name, (t, shape, dtype) in named.items() if t is not None]
     for name, t, shape, dtype in present:
         if t.dtype != dtype or not t.is_contiguous():
@@ -360,14 +373,26 @@ def _chk_shapes(**named):
         if t.device.index != torch.cuda.current_device():
             raise ValueError("%s is on %s, the current device is cuda:%d"
                              % (name, t.device, torch.cuda.current_device()))
+    raise ValueError("arguments on more than one device")
+
+
+def _device(t):
+    """Index of the current device for calls that start from tensor t (-2 for a host tensor:
+    nothing fits it)."""
+    return torch._C._cuda_getDevice() if t.is_cuda else -2
+
+
+def _raw_stream(device):
+    return torch._C._cuda_getCurrentRawStream(device)
+
+
+def _at(t):
+    return None if t is None else t.data_ptr()
 
 
 def _pair(a, b, names):
     if (a is None) != (b is None):
         raise ValueError("%s and %s come together" % names)
-
-
-_F, _I = torch.float32, torch.int32
 
 
 def _dims(name, t, n):
@@ -377,19 +402,26 @@ def _dims(name, t, n):
     return t.shape
 
 
+def _new(like, count, *shape):
+    """`count` new fp32 tensors of a shape, from one allocation."""
+    return like.new_empty((count,) + shape, dtype=_F).unbind(0)
+
+
 def layernorm_fwd(mu_w, var_w, mu_b, var_b, mu_a, var_a, eps=1e-5):
     """Layer norm over the last dimension of mu_a / var_a [B, n]: (mu_z, var_z, mu_s, var_s),
     mu_s / var_s [B] the statistics of the rows. mu_b / var_b may be None."""
     _pair(mu_b, var_b, ("mu_b", "var_b"))
     B, n = _dims("mu_a", mu_a, 2)
-    _chk_shapes(mu_a=(mu_a, (B, n), _F), var_a=(var_a, (B, n), _F), mu_w=(mu_w, (n,), _F),
-                var_w=(var_w, (n,), _F), mu_b=(mu_b, (n,), _F), var_b=(var_b, (n,), _F))
-    mu_z, var_z = torch.empty_like(mu_a), torch.empty_like(mu_a)
-    mu_s, var_s = torch.empty(B, device=mu_a.device), torch.empty(B, device=mu_a.device)
+    dev = _device(mu_a)
+    if not (_fits(dev, _F, (B, n), mu_a, var_a) and _fits(dev, _F, (n,), mu_w, var_w, mu_b, var_b)):
+        _explain(mu_a=(mu_a, (B, n), _F), var_a=(var_a, (B, n), _F), mu_w=(mu_w, (n,), _F),
+                 var_w=(var_w, (n,), _F), mu_b=(mu_b, (n,), _F), var_b=(var_b, (n,), _F))
+    mu_z, var_z = _new(mu_a, 2, B, n)
+    mu_s, var_s = _new(mu_a, 2, B)
     capi.check(capi.lib.tagi_layernorm_fwd(
-        capi.ptr(mu_w), capi.ptr(var_w), capi.ptr(mu_b), capi.ptr(var_b), capi.ptr(mu_a),
-        capi.ptr(var_a), int(mu_b is not None), eps, n, B, capi.ptr(mu_s), capi.ptr(var_s),
-        capi.ptr(mu_z), capi.ptr(var_z), _stream()))
+        mu_w.data_ptr(), var_w.data_ptr(), _at(mu_b), _at(var_b), mu_a.data_ptr(),
+        var_a.data_ptr(), int(mu_b is not None), eps, n, B, mu_s.data_ptr(), var_s.data_ptr(),
+        mu_z.data_ptr(), var_z.data_ptr(), _raw_stream(dev)))
     return mu_z, var_z, mu_s, var_s
 
 
@@ -398,35 +430,26 @@ def layernorm_bwd(mu_w, var_w, var_b, mu_a, jcb, mu_s, var_s, delta_mu, delta_va
     """Returns (dz_mu, dz_var, dw_mu, dw_var, db_mu, db_var); entries not asked for are None.
     jcb may be None (one everywhere)."""
     B, n = _dims("delta_mu", delta_mu, 2)
-    _chk_shapes(delta_mu=(delta_mu, (B, n), _F), delta_var=(delta_var, (B, n), _F),
-                mu_w=(mu_w, (n,), _F), var_w=(var_w, (n,), _F), var_b=(var_b, (n,), _F),
-                mu_a=(mu_a, (B, n), _F), jcb=(jcb, (B, n), _F), mu_s=(mu_s, (B,), _F),
-                var_s=(var_s, (B,), _F))
-    dev = delta_mu.device
+    dev = _device(delta_mu)
+    if not (_fits(dev, _F, (B, n), delta_mu, delta_var, mu_a, jcb) and
+            _fits(dev, _F, (n,), mu_w, var_w, var_b) and _fits(dev, _F, (B,), mu_s, var_s)):
+        _explain(delta_mu=(delta_mu, (B, n), _F), delta_var=(delta_var, (B, n), _F),
+                 mu_w=(mu_w, (n,), _F), var_w=(var_w, (n,), _F), var_b=(var_b, (n,), _F),
+                 mu_a=(mu_a, (B, n), _F), jcb=(jcb, (B, n), _F), mu_s=(mu_s, (B,), _F),
+                 var_s=(var_s, (B,), _F))
     out, scratch = [None] * 6, None
     if state_update:
-        out[0], out[1] = torch.empty_like(delta_mu), torch.empty_like(delta_mu)
+        out[:2] = _new(delta_mu, 2, B, n)
     if param_update:
-        out[2], out[3] = torch.empty(n, device=dev), torch.empty(n, device=dev)
-        if var_b is not None:
-            out[4], out[5] = torch.empty(n, device=dev), torch.empty(n, device=dev)
-        scratch = torch.empty(capi.layernorm_bwd_scratch(n, B), dtype=torch.uint8, device=dev)
+        count = 2 if var_b is None else 4
+        out[2:2 + count] = _new(delta_mu, count, n)
+        scratch = delta_mu.new_empty(capi.layernorm_bwd_scratch(n, B), dtype=torch.uint8)
     capi.check(capi.lib.tagi_layernorm_bwd(
-        capi.ptr(mu_w), capi.ptr(var_w), capi.ptr(var_b), capi.ptr(mu_a), capi.ptr(jcb),
-        capi.ptr(mu_s), capi.ptr(var_s), capi.ptr(delta_mu), capi.ptr(delta_var), eps, n, B,
-        int(var_b is not None), int(state_update), int(param_update), capi.ptr(scratch),
-        *[capi.ptr(t) for t in out], _stream()))
+        mu_w.data_ptr(), var_w.data_ptr(), _at(var_b), mu_a.data_ptr(), _at(jcb), mu_s.data_ptr(),
+        var_s.data_ptr(), delta_mu.data_ptr(), delta_var.data_ptr(), eps, n, B,
+        int(var_b is not None), int(state_update), int(param_update), _at(scratch),
+        *[_at(t) for t in out], _raw_stream(dev)))
     return tuple(out)
-
-
-def _grouped_shapes(mu_w, var_w, b, offsets, rows, held, R, K):
-    E, N, _ = _dims("weights", mu_w if mu_w is not None else var_w, 3)
-    _chk_shapes(mu_w=(mu_w, (E, N, K), _F), var_w=(var_w, (E, N, K), _F),
-                offsets=(offsets, (E + 1,), _I), rows=(rows, (R,), _I),
-                **{name: (t, (E, N), _F) for name, t in b.items()},
-                **{name: (t, (t.shape[0] if rows is not None else R, K), _F)
-                   for name, t in held.items()})
-    return E, N
 
 
 def grouped_linear_fwd(mu_w, var_w, mu_b, var_b, mu_a, var_a, offsets, rows=None, out=None):
@@ -441,31 +464,35 @@ def grouped_linear_fwd_act(mu_w, var_w, mu_b, var_b, mu_a, var_a, offsets, activ
                            out=None):
     """grouped_linear_fwd with the following activation ("relu" / "mixture_relu") applied in
     the kernel's epilogue: returns the activation's (mu_a, var_a, jcb), each [R, N]."""
-    return _grouped_fwd(mu_w, var_w, mu_b, var_b, mu_a, var_a, offsets, rows, activation, out)
+    return _grouped_fwd(mu_w, var_w, mu_b, var_b, mu_a, var_a, offsets, rows, ACTIVATIONS[activation],
+                        out)
 
 
 def _grouped_fwd(mu_w, var_w, mu_b, var_b, mu_a, var_a, offsets, rows, activation, out):
     _pair(mu_b, var_b, ("mu_b", "var_b"))
     T, K = _dims("mu_a", mu_a, 2)
     R = T if rows is None else _dims("rows", rows, 1)[0]
-    if var_a.shape != mu_a.shape:
-        raise ValueError("mu_a and var_a: shapes %s, %s" % (tuple(mu_a.shape), tuple(var_a.shape)))
-    E, N = _grouped_shapes(mu_w, var_w, dict(mu_b=mu_b, var_b=var_b), offsets, rows,
-                           dict(mu_a=mu_a, var_a=var_a), R, K)
+    E, N, _ = _dims("mu_w", mu_w, 3)
+    dev = _device(mu_a)
     count = 2 if activation is None else 3
-    if out is None:
-        out = tuple(torch.empty((R, N), device=mu_w.device) for _ in range(count))
-    if len(out) != count:
+    if out is not None and len(out) != count:
         raise ValueError("out: expected %d tensors" % count)
-    _chk_shapes(**{"out[%d]" % i: (t, (R, N), _F) for i, t in enumerate(out)})
-    args = [capi.ptr(t) for t in (mu_w, var_w, mu_b, var_b, mu_a, var_a, offsets, rows)]
-    args += [K, N, E, R, T, int(mu_b is not None)]
-    outs = [capi.ptr(t) for t in out]
+    if not (_fits(dev, _F, (E, N, K), mu_w, var_w) and _fits(dev, _F, (E, N), mu_b, var_b) and
+            _fits(dev, _F, (T, K), mu_a, var_a) and _fits(dev, _I, (E + 1,), offsets) and
+            _fits(dev, _I, (R,), rows) and _fits(dev, _F, (R, N), *(out or ()))):
+        _explain(mu_w=(mu_w, (E, N, K), _F), var_w=(var_w, (E, N, K), _F), mu_b=(mu_b, (E, N), _F),
+                 var_b=(var_b, (E, N), _F), mu_a=(mu_a, (T, K), _F), var_a=(var_a, (T, K), _F),
+                 offsets=(offsets, (E + 1,), _I), rows=(rows, (R,), _I),
+                 **{"out[%d]" % i: (t, (R, N), _F) for i, t in enumerate(out or ())})
+    if out is None:
+        out = _new(mu_w, count, R, N)
+    args = (mu_w.data_ptr(), var_w.data_ptr(), _at(mu_b), _at(var_b), mu_a.data_ptr(),
+            var_a.data_ptr(), offsets.data_ptr(), _at(rows), K, N, E, R, T, int(mu_b is not None))
+    outs = [t.data_ptr() for t in out]
     if activation is None:
-        capi.check(capi.lib.tagi_grouped_linear_fwd(*args, *outs, _stream()))
+        capi.check(capi.lib.tagi_grouped_linear_fwd(*args, *outs, _raw_stream(dev)))
     else:
-        capi.check(capi.lib.tagi_grouped_linear_fwd_act(*args, ACTIVATIONS[activation], *outs,
-                                                        _stream()))
+        capi.check(capi.lib.tagi_grouped_linear_fwd_act(*args, activation, *outs, _raw_stream(dev)))
     return tuple(out)
 
 
@@ -477,21 +504,32 @@ def grouped_linear_bwd(mu_w, var_w, var_b, mu_a, jcb, delta_mu, delta_var, offse
     as out[0] and out[1] held them (unset without `out`)."""
     R, _ = _dims("delta_mu", delta_mu, 2)
     T, K = _dims("mu_a", mu_a, 2)
-    E, N = _grouped_shapes(mu_w, var_w, dict(var_b=var_b), offsets, rows, dict(mu_a=mu_a), R, K)
-    _chk_shapes(delta_mu=(delta_mu, (R, N), _F), delta_var=(delta_var, (R, N), _F),
-                jcb=(jcb, (R, K), _F))
-    dev, bias = delta_mu.device, var_b is not None
+    E, N, _ = _dims("mu_w", mu_w, 3)
+    dev, bias = _device(delta_mu), var_b is not None
+    held = T if rows is not None else R
     shapes = [(R, K)] * 2 + [(E, N, K)] * 2 + [(E, N)] * 2
     wanted = [state_update] * 2 + [param_update] * 2 + [param_update and bias] * 2
-    if out is None:
-        out = [torch.empty(s, device=dev) if w else None for s, w in zip(shapes, wanted)]
-    if len(out) != 6 or any(w and t is None for w, t in zip(wanted, out)):
+    if out is not None and (len(out) != 6 or any(w and t is None for w, t in zip(wanted, out))):
         raise ValueError("out: six entries, None only where nothing is asked for")
-    _chk_shapes(**{"out[%d]" % i: (t, s, _F) for i, (t, s) in enumerate(zip(out, shapes))})
+    if not (_fits(dev, _F, (E, N, K), mu_w, var_w) and _fits(dev, _F, (E, N), var_b) and
+            _fits(dev, _F, (held, K), mu_a) and _fits(dev, _I, (E + 1,), offsets) and
+            _fits(dev, _I, (R,), rows) and _fits(dev, _F, (R, N), delta_mu, delta_var) and
+            _fits(dev, _F, (R, K), jcb) and
+            all(_fits(dev, _F, s, t) for s, t in zip(shapes, out or ()))):
+        _explain(mu_w=(mu_w, (E, N, K), _F), var_w=(var_w, (E, N, K), _F), var_b=(var_b, (E, N), _F),
+                 mu_a=(mu_a, (held, K), _F), offsets=(offsets, (E + 1,), _I), rows=(rows, (R,), _I),
+                 delta_mu=(delta_mu, (R, N), _F), delta_var=(delta_var, (R, N), _F),
+                 jcb=(jcb, (R, K), _F),
+                 **{"out[%d]" % i: (t, s, _F) for i, (t, s) in enumerate(zip(out or (), shapes))})
+    if out is None:
+        out = [None] * 6
+        for i in (0, 2, 4):
+            if wanted[i]:
+                out[i:i + 2] = _new(delta_mu, 2, *shapes[i])
     capi.check(capi.lib.tagi_grouped_linear_bwd(
-        *[capi.ptr(t) for t in (mu_w, var_w, var_b, mu_a, jcb, delta_mu, delta_var, offsets, rows)],
-        K, N, E, R, T, int(bias), int(state_update), int(param_update),
-        *[capi.ptr(t) for t in out], _stream()))
+        mu_w.data_ptr(), var_w.data_ptr(), _at(var_b), mu_a.data_ptr(), _at(jcb),
+        delta_mu.data_ptr(), delta_var.data_ptr(), offsets.data_ptr(), _at(rows), K, N, E, R, T,
+        int(bias), int(state_update), int(param_update), *[_at(t) for t in out], _raw_stream(dev)))
     return tuple(t if w else None for w, t in zip(wanted, out))
 
 
@@ -507,17 +545,21 @@ def moe_route(mu_s, var_s, top_k):
     T, E = _dims("mu_s", mu_s, 2)
     if not 1 <= top_k <= E:
         raise ValueError("top_k %d: expected 1 to %d" % (top_k, E))
-    _chk_shapes(mu_s=(mu_s, (T, E), _F), var_s=(var_s, (T, E), _F))
-    dev = mu_s.device
-    scratch = torch.empty(capi.moe_route_scratch(T, E), dtype=torch.uint8, device=dev)
-    expert, slot = (torch.empty((T, top_k), dtype=_I, device=dev) for _ in range(2))
-    mu_g, var_g, jcb_g = (torch.empty((T, top_k), device=dev) for _ in range(3))
-    offsets = torch.empty(E + 1, dtype=_I, device=dev)
-    token = torch.empty(T * top_k, dtype=_I, device=dev)
+    dev = _device(mu_s)
+    if not _fits(dev, _F, (T, E), mu_s, var_s):
+        _explain(mu_s=(mu_s, (T, E), _F), var_s=(var_s, (T, E), _F))
+    size = capi.moe_route_scratch(T, E)
+    scratch = mu_s.new_empty(size, dtype=torch.uint8) if size else None
+    mu_g, var_g, jcb_g = _new(mu_s, 3, T, top_k)
+    # expert, slot, token, then offsets
+    n = T * top_k
+    whole = mu_s.new_empty(3 * n + E + 1, dtype=_I)
+    expert, slot, token, offsets = whole.split((n, n, n, E + 1))
+    expert, slot = expert.view(T, top_k), slot.view(T, top_k)
+    at = whole.data_ptr()
     capi.check(capi.lib.tagi_moe_route(
-        capi.ptr(mu_s), capi.ptr(var_s), T, E, top_k, capi.ptr(scratch), capi.ptr(expert),
-        capi.ptr(mu_g), capi.ptr(var_g), capi.ptr(jcb_g), capi.ptr(offsets), capi.ptr(token),
-        capi.ptr(slot), _stream()))
+        mu_s.data_ptr(), var_s.data_ptr(), T, E, top_k, _at(scratch), at, mu_g.data_ptr(),
+        var_g.data_ptr(), jcb_g.data_ptr(), at + 12 * n, at + 8 * n, at + 4 * n, _raw_stream(dev)))
     return MoeRoutes(expert, mu_g, var_g, jcb_g, offsets, token, slot)
 
 
@@ -526,12 +568,15 @@ def moe_combine_fwd(mu_g, var_g, mu_y, var_y, slot):
     choice whose slot is no row adds nothing."""
     T, k = _dims("mu_g", mu_g, 2)
     R, N = _dims("mu_y", mu_y, 2)
-    _chk_shapes(mu_g=(mu_g, (T, k), _F), var_g=(var_g, (T, k), _F), slot=(slot, (T, k), _I),
-                mu_y=(mu_y, (R, N), _F), var_y=(var_y, (R, N), _F))
-    mu_z, var_z = (torch.empty((T, N), device=mu_y.device) for _ in range(2))
+    dev = _device(mu_y)
+    if not (_fits(dev, _F, (T, k), mu_g, var_g) and _fits(dev, _I, (T, k), slot) and
+            _fits(dev, _F, (R, N), mu_y, var_y)):
+        _explain(mu_g=(mu_g, (T, k), _F), var_g=(var_g, (T, k), _F), slot=(slot, (T, k), _I),
+                 mu_y=(mu_y, (R, N), _F), var_y=(var_y, (R, N), _F))
+    mu_z, var_z = _new(mu_y, 2, T, N)
     capi.check(capi.lib.tagi_moe_combine_fwd(
-        capi.ptr(mu_g), capi.ptr(var_g), capi.ptr(mu_y), capi.ptr(var_y), capi.ptr(slot), T, k, R,
-        N, capi.ptr(mu_z), capi.ptr(var_z), _stream()))
+        mu_g.data_ptr(), var_g.data_ptr(), mu_y.data_ptr(), var_y.data_ptr(), slot.data_ptr(), T, k,
+        R, N, mu_z.data_ptr(), var_z.data_ptr(), _raw_stream(dev)))
     return mu_z, var_z
 
 
@@ -542,17 +587,21 @@ def moe_combine_bwd(mu_g, jcb_g, mu_y, expert, slot, delta_mu, delta_var, num_ex
     `out`)."""
     T, k = _dims("mu_g", mu_g, 2)
     R, N = _dims("mu_y", mu_y, 2)
-    _chk_shapes(mu_g=(mu_g, (T, k), _F), jcb_g=(jcb_g, (T, k), _F), expert=(expert, (T, k), _I),
-                slot=(slot, (T, k), _I), mu_y=(mu_y, (R, N), _F), delta_mu=(delta_mu, (T, N), _F),
-                delta_var=(delta_var, (T, N), _F))
-    dev = mu_y.device
-    dmu_y, dvar_y = out if out is not None else (torch.empty_like(mu_y), torch.empty_like(mu_y))
-    _chk_shapes(**{"out[0]": (dmu_y, (R, N), _F), "out[1]": (dvar_y, (R, N), _F)})
-    dmu_s, dvar_s = (torch.empty((T, num_experts), device=dev) for _ in range(2))
+    dev = _device(mu_y)
+    if out is not None and len(out) != 2:
+        raise ValueError("out: expected 2 tensors")
+    if not (_fits(dev, _F, (T, k), mu_g, jcb_g) and _fits(dev, _I, (T, k), expert, slot) and
+            _fits(dev, _F, (R, N), mu_y, *(out or ())) and _fits(dev, _F, (T, N), delta_mu, delta_var)):
+        _explain(mu_g=(mu_g, (T, k), _F), jcb_g=(jcb_g, (T, k), _F), expert=(expert, (T, k), _I),
+                 slot=(slot, (T, k), _I), mu_y=(mu_y, (R, N), _F), delta_mu=(delta_mu, (T, N), _F),
+                 delta_var=(delta_var, (T, N), _F),
+                 **{"out[%d]" % i: (t, (R, N), _F) for i, t in enumerate(out or ())})
+    dmu_y, dvar_y = out if out is not None else _new(mu_y, 2, R, N)
+    dmu_s, dvar_s = _new(mu_y, 2, T, num_experts)
     capi.check(capi.lib.tagi_moe_combine_bwd(
-        capi.ptr(mu_g), capi.ptr(jcb_g), capi.ptr(mu_y), capi.ptr(expert), capi.ptr(slot),
-        capi.ptr(delta_mu), capi.ptr(delta_var), T, k, R, N, num_experts, capi.ptr(dmu_y),
-        capi.ptr(dvar_y), capi.ptr(dmu_s), capi.ptr(dvar_s), _stream()))
+        mu_g.data_ptr(), jcb_g.data_ptr(), mu_y.data_ptr(), expert.data_ptr(), slot.data_ptr(),
+        delta_mu.data_ptr(), delta_var.data_ptr(), T, k, R, N, num_experts, dmu_y.data_ptr(),
+        dvar_y.data_ptr(), dmu_s.data_ptr(), dvar_s.data_ptr(), _raw_stream(dev)))
     return dmu_y, dvar_y, dmu_s, dvar_s
 
 
@@ -562,11 +611,14 @@ def moe_gather_bwd(delta_mu_r, delta_var_r, slot, jcb=None, res_mu=None, res_var
     _pair(res_mu, res_var, ("res_mu", "res_var"))
     T, k = _dims("slot", slot, 2)
     R, K = _dims("delta_mu_r", delta_mu_r, 2)
-    _chk_shapes(slot=(slot, (T, k), _I), delta_mu_r=(delta_mu_r, (R, K), _F),
-                delta_var_r=(delta_var_r, (R, K), _F), jcb=(jcb, (T, K), _F),
-                res_mu=(res_mu, (T, K), _F), res_var=(res_var, (T, K), _F))
-    dmu, dvar = (torch.empty((T, K), device=delta_mu_r.device) for _ in range(2))
+    dev = _device(delta_mu_r)
+    if not (_fits(dev, _I, (T, k), slot) and _fits(dev, _F, (R, K), delta_mu_r, delta_var_r) and
+            _fits(dev, _F, (T, K), jcb, res_mu, res_var)):
+        _explain(slot=(slot, (T, k), _I), delta_mu_r=(delta_mu_r, (R, K), _F),
+                 delta_var_r=(delta_var_r, (R, K), _F), jcb=(jcb, (T, K), _F),
+                 res_mu=(res_mu, (T, K), _F), res_var=(res_var, (T, K), _F))
+    dmu, dvar = _new(delta_mu_r, 2, T, K)
     capi.check(capi.lib.tagi_moe_gather_bwd(
-        capi.ptr(delta_mu_r), capi.ptr(delta_var_r), capi.ptr(slot), capi.ptr(jcb),
-        capi.ptr(res_mu), capi.ptr(res_var), T, k, R, K, capi.ptr(dmu), capi.ptr(dvar), _stream()))
+        delta_mu_r.data_ptr(), delta_var_r.data_ptr(), slot.data_ptr(), _at(jcb), _at(res_mu),
+        _at(res_var), T, k, R, K, dmu.data_ptr(), dvar.data_ptr(), _raw_stream(dev)))
     return dmu, dvar

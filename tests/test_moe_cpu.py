@@ -117,8 +117,8 @@ def test_tensor_calls_refuse():
     no("offsets: expected shape", F.grouped_linear_fwd, W, W, None, None, f(5, 8), f(5, 8), i(3))
     no("offsets: expected a contiguous", F.grouped_linear_fwd, W, W, None, None, f(5, 8), f(5, 8), i(4).long())
     no("mu_w: expected shape", F.grouped_linear_fwd, W, W, None, None, f(5, 9), f(5, 9), i(4))
-    no("mu_a and var_a", F.grouped_linear_fwd, W, W, None, None, f(5, 8), f(4, 8), i(4))
-    no("weights: expected 3 dim", F.grouped_linear_fwd, W[0], W[0], None, None, f(5, 8), f(5, 8), i(4))
+    no("var_a: expected shape", F.grouped_linear_fwd, W, W, None, None, f(5, 8), f(4, 8), i(4))
+    no("mu_w: expected 3 dim", F.grouped_linear_fwd, W[0], W[0], None, None, f(5, 8), f(5, 8), i(4))
     no("rows: expected 1 dim", F.grouped_linear_fwd, W, W, None, None, f(5, 8), f(5, 8), i(4), rows=i(2, 2))
     no("come together", F.grouped_linear_fwd, W, W, f(3, 4), None, f(5, 8), f(5, 8), i(4))
     no("device tensor", F.grouped_linear_fwd, W, W, None, None, f(5, 8), f(5, 8), i(4))
