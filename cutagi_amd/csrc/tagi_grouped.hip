@@ -222,7 +222,8 @@ struct SideK {
         }
     }
     __device__ __forceinline__ void ahead(const GroupedParams &, int) {}
-    // the batch at k0 is next: addresses
+    // The batch at k0 is next: everything that its loads need. (They go out after start() may
+    // have moved this side on to the next tile.)
     __device__ __forceinline__ void begin(const GroupedParams &p, int k0, Batch &b) {
         if (fresh) {
             fresh = false;
@@ -289,8 +290,9 @@ struct SideM {
     int ld, red, r0, g, col, cols;
     bool gather;
     int source[8];            // gather: the rows that the next batch reads
-    unsigned row[8];
-    const float *f0, *f1;     // the batch that is loaded
+    unsigned row[8];          // the batch that is loaded: the thread's elements in its rows,
+    unsigned last[VEC ? 1 : 8];   // the rows' last elements
+    const float *f0, *f1;
     __device__ __forceinline__ void start(const GroupedParams &p, const Tile &t, int u) {
         g = (u >> 5) * 8;
         red = t.red;
@@ -333,14 +335,15 @@ struct SideM {
                     b.dead |= 1u << i;
                 }
             }
-            row[i] = (unsigned)s * (unsigned)ld;
+            row[i] = (unsigned)s * (unsigned)ld + (unsigned)col;
+            if (!VEC) last[i] = (unsigned)s * (unsigned)ld + (unsigned)(cols - 1);
         }
     }
     __device__ __forceinline__ void load(Batch &b, int i, bool second) const {
         if (!second)
-            b.v0[i] = load4<VEC>(f0, row[i] + col, row[i] + (cols - 1));
+            b.v0[i] = load4<VEC>(f0, row[i], last[VEC ? 0 : i]);
         else if (ROWS)
-            b.v1[i] = load4<VEC>(f1, row[i] + col, row[i] + (cols - 1));
+            b.v1[i] = load4<VEC>(f1, row[i], last[VEC ? 0 : i]);
     }
     __device__ __forceinline__ void mask(Batch &b) const {
 #pragma unroll

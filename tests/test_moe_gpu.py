@@ -46,6 +46,10 @@ GROUPS = [
     ([1] * 40, 64, 64, 7, 0),
     ([9, 0, 12, 4] * 5, 72, 68, 30, 6),
     ([512, 600], 256, 256, None, 0),
+    # more tiles than workgroups: every pass has workgroups that walk several
+    ([130, 700, 0, 450], 4100, 72, 300, 5),
+    ([130, 700, 0, 450], 72, 4100, None, 5),
+    ([33, 90, 40], 1300, 1284, 100, 0),
 ]
 GUARD = 12345.0
 
