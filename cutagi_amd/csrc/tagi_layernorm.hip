@@ -10,6 +10,7 @@
 #include <cstdint>
 
 #include "tagi_internal.h"
+#include "tagi_stream.h"
 
 namespace tagi {
 namespace {
@@ -38,26 +39,6 @@ __device__ __forceinline__ void row_sum(float (&v)[NV], float (*s)[TPB / 64]) {
     __syncthreads();
 }
 
-template <int W>
-__device__ __forceinline__ void load_w(const float *p, float (&v)[W]) {
-    if (W == 4) {
-        const float4 q = *reinterpret_cast<const float4 *>(p);
-        v[0] = q.x;
-        v[1 % W] = q.y;
-        v[2 % W] = q.z;
-        v[3 % W] = q.w;
-    } else {
-        v[0] = p[0];
-    }
-}
-template <int W>
-__device__ __forceinline__ void store_w(float *p, const float (&v)[W]) {
-    if (W == 4)
-        *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1 % W], v[2 % W], v[3 % W]);
-    else
-        p[0] = v[0];
-}
-
 // ---------------------------------------------------------------------------
 // Forward. THREADS threads hold one row, PER groups of W features each (W = 4 where rows
 // are whole 16-byte groups, else 1); PER == 0: a row of any length, read three times.
@@ -67,7 +48,7 @@ __global__ __launch_bounds__(TPB) void ln_fwd_kernel(
     const float *__restrict__ mu_w, const float *__restrict__ var_w,
     const float *__restrict__ mu_b, const float *__restrict__ var_b,
     const float *__restrict__ mu_a, const float *__restrict__ var_a, float epsilon, int n, int B,
-    float *__restrict__ mu_s, float *__restrict__ var_s, float *__restrict__ mu_z,
+    bool past_cache, float *__restrict__ mu_s, float *__restrict__ var_s, float *__restrict__ mu_z,
     float *__restrict__ var_z) {
     __shared__ float s[2][TPB / 64];
     const int t = threadIdx.x % THREADS;
@@ -158,8 +139,8 @@ __global__ __launch_bounds__(TPB) void ln_fwd_kernel(
                     ov[c] += vw[c];
                 }
             }
-            store_w<W>(mu_z + (size_t)b * n + f, om);
-            store_w<W>(var_z + (size_t)b * n + f, ov);
+            store_w<W>(mu_z + (size_t)b * n + f, om, past_cache);
+            store_w<W>(var_z + (size_t)b * n + f, ov, past_cache);
         };
         if (PER > 0) {
 #pragma unroll
@@ -188,7 +169,7 @@ __global__ __launch_bounds__(TPB) void ln_bwd_kernel(
     const float *__restrict__ mu_w, const float *__restrict__ mu_a, const float *__restrict__ jcb,
     const float *__restrict__ mu_s, const float *__restrict__ var_s,
     const float *__restrict__ dmu_out, const float *__restrict__ dvar_out, float epsilon, int n,
-    int B, int rows_per_chunk, int cw_log, int state_update, int param_update,
+    int B, int rows_per_chunk, int cw_log, int state_update, int param_update, bool past_cache,
     float *__restrict__ dmu, float *__restrict__ dvar, float *__restrict__ part) {
     __shared__ float s[4][W][TPB];
     const int cw = 1 << cw_log;
@@ -224,8 +205,8 @@ __global__ __launch_bounds__(TPB) void ln_bwd_kernel(
                     om[c] = t[c] * dm[c];
                     ov[c] = t[c] * dv[c] * t[c];
                 }
-                store_w<W>(dmu + at, om);
-                store_w<W>(dvar + at, ov);
+                store_w<W>(dmu + at, om, past_cache);
+                store_w<W>(dvar + at, ov, past_cache);
             }
             if (param_update) {
                 float x[W];
@@ -264,28 +245,33 @@ __global__ __launch_bounds__(TPB) void ln_bwd_kernel(
     }
 }
 
-// The chunks of 64 columns: four waves take every fourth chunk, their sums are joined in
+// The chunks of 64 columns: sixteen waves take every sixteenth chunk, their sums are joined in
 // wave order.
-__global__ __launch_bounds__(TPB) void ln_bwd_final_kernel(
+constexpr int FINAL_WAVES = 16;
+__global__ __launch_bounds__(FINAL_WAVES * 64) void ln_bwd_final_kernel(
     const float *__restrict__ part, const float *__restrict__ var_w,
     const float *__restrict__ var_b, int n, int chunks, float *__restrict__ dmu_w,
     float *__restrict__ dvar_w, float *__restrict__ dmu_b, float *__restrict__ dvar_b) {
-    __shared__ float s[4][TPB];
+    __shared__ float s[4][FINAL_WAVES][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int c = blockIdx.x * 64 + lane;
     float v[4] = {0.f, 0.f, 0.f, 0.f};
     if (c < n)
-        for (int q = wave; q < chunks; q += 4) {
+        for (int q = wave; q < chunks; q += FINAL_WAVES) {
             const float *o = part + (size_t)q * 4 * n + c;
 #pragma unroll
             for (int k = 0; k < 4; k++) v[k] += o[(size_t)k * n];
         }
 #pragma unroll
-    for (int k = 0; k < 4; k++) s[k][threadIdx.x] = v[k];
+    for (int k = 0; k < 4; k++) s[k][wave][lane] = v[k];
     __syncthreads();
     if (wave != 0 || c >= n) return;
 #pragma unroll
-    for (int k = 0; k < 4; k++) v[k] = (s[k][lane] + s[k][64 + lane]) + (s[k][128 + lane] + s[k][192 + lane]);
+    for (int k = 0; k < 4; k++) {
+        v[k] = 0.f;
+#pragma unroll
+        for (int w = 0; w < FINAL_WAVES; w++) v[k] += s[k][w][lane];
+    }
     const float vw = var_w[c];
     dmu_w[c] = vw * v[0];
     dvar_w[c] = vw * vw * v[1];
@@ -301,7 +287,9 @@ __global__ __launch_bounds__(TPB) void ln_bwd_final_kernel(
 // is a multiple of four; unaligned arrays then take the one-column form with the same chunks.
 int ln_rows_per_chunk(int n, int B) {
     const long long col_blocks = (n + 255) / 256;
-    long long chunks = (8LL * num_cu() + col_blocks - 1) / col_blocks;
+    // four workgroups per CU (16384 x 4096, forward and backward: 2 / 3 / 4 / 8 / 16 per CU take
+    // 540 / 497 / 493 / 517 / 508 us; more of them also leave more partial sums)
+    long long chunks = (4LL * num_cu() + col_blocks - 1) / col_blocks;
     long long rows = (B + chunks - 1) / chunks;
     if (rows < 16) rows = 16;
     return (int)rows;
@@ -314,8 +302,8 @@ hipError_t fwd(const float *mu_w, const float *var_w, const float *mu_b, const f
     // (a launch holds fewer than 2^32 threads; beyond that the workgroups walk on)
     const long long rows = TPB / THREADS, blocks = (B + rows - 1) / rows;
     const unsigned grid = (unsigned)(blocks < (1 << 22) ? blocks : 1 << 22);
-    hipLaunchKernelGGL((ln_fwd_kernel<THREADS, PER, W>), dim3(grid), dim3(TPB), 0, stream, mu_w, var_w, mu_b, var_b, mu_a, var_a, epsilon, n, B, mu_s, var_s,
-                       mu_z, var_z);
+    hipLaunchKernelGGL((ln_fwd_kernel<THREADS, PER, W>), dim3(grid), dim3(TPB), 0, stream, mu_w, var_w, mu_b, var_b, mu_a, var_a, epsilon, n, B,
+                       goes_past_cache((size_t)2 * B * n), mu_s, var_s, mu_z, var_z);
     return hipGetLastError();
 }
 
@@ -336,15 +324,20 @@ hipError_t launch_layernorm_fwd(const float *mu_w, const float *var_w, const flo
 #define LN_FWD(T, P, W)                                                                          \
     return fwd<T, P, W>(mu_w, var_w, mu_b, var_b, mu_a, var_a, epsilon, n, B, mu_s, var_s, mu_z, \
                         var_z, stream)
+    // One wave per row up to 1024 features, unless the rows would not fill the chip that way
+    // (four waves for every SIMD): then a workgroup each.
+    const bool many = B >= 16 * num_cu();
     if (vec) {
         if (n <= 256) LN_FWD(64, 1, 4);
-        if (n <= 1024) LN_FWD(64, 4, 4);
+        if (n <= 1024 && many) LN_FWD(64, 4, 4);
+        if (n <= 1024) LN_FWD(256, 1, 4);
         if (n <= 4096) LN_FWD(256, 4, 4);
         if (n <= 8192) LN_FWD(256, 8, 4);
         LN_FWD(256, 0, 4);
     }
     if (n <= 256) LN_FWD(64, 4, 1);
-    if (n <= 1024) LN_FWD(64, 16, 1);
+    if (n <= 1024 && many) LN_FWD(64, 16, 1);
+    if (n <= 1024) LN_FWD(256, 4, 1);
     if (n <= 4096) LN_FWD(256, 16, 1);
     if (n <= 8192) LN_FWD(256, 32, 1);
     LN_FWD(256, 0, 1);
@@ -360,6 +353,7 @@ hipError_t launch_layernorm_bwd(const float *mu_w, const float *var_w, const flo
     const bool vec = n % 4 == 0 && aligned16(mu_w) && aligned16(dmu_out) && aligned16(dvar_out) &&
                      (!state_update || (aligned16(jcb) && aligned16(dmu) && aligned16(dvar))) &&
                      (!param_update || aligned16(mu_a));
+    const bool past_cache = goes_past_cache((size_t)2 * B * n);
     const int rows = ln_rows_per_chunk(n, B);
     const int chunks = (B + rows - 1) / rows, groups = vec ? n / 4 : n;
     int cw_log = 0;
@@ -368,14 +362,15 @@ hipError_t launch_layernorm_bwd(const float *mu_w, const float *var_w, const flo
     if (vec)
         hipLaunchKernelGGL(ln_bwd_kernel<4>, grid, dim3(TPB), 0, stream, mu_w, mu_a, jcb, mu_s,
                            var_s, dmu_out, dvar_out, epsilon, n, B, rows, cw_log, state_update,
-                           param_update, dmu, dvar, scratch);
+                           param_update, past_cache, dmu, dvar, scratch);
     else
         hipLaunchKernelGGL(ln_bwd_kernel<1>, grid, dim3(TPB), 0, stream, mu_w, mu_a, jcb, mu_s,
                            var_s, dmu_out, dvar_out, epsilon, n, B, rows, cw_log, state_update,
-                           param_update, dmu, dvar, scratch);
+                           param_update, past_cache, dmu, dvar, scratch);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || !param_update) return e;
-    hipLaunchKernelGGL(ln_bwd_final_kernel, dim3((n + 63) / 64), dim3(TPB), 0, stream, scratch,
+    hipLaunchKernelGGL(ln_bwd_final_kernel, dim3((n + 63) / 64), dim3(FINAL_WAVES * 64), 0, stream,
+                       scratch,
                        var_w, var_b, n, chunks, dmu_w, dvar_w, dmu_b, dvar_b);
     return hipGetLastError();
 }

@@ -4,6 +4,7 @@
 #include <cstdint>
 
 #include "tagi_internal.h"
+#include "tagi_stream.h"
 
 namespace tagi {
 namespace {
@@ -13,17 +14,20 @@ constexpr int TPB = 256;
 inline bool aligned16(const void *q) { return (reinterpret_cast<uintptr_t>(q) & 15u) == 0; }
 
 // ---------------------------------------------------------------------------
-// Choice. 2^g_log lanes hold the scores of one token, lane i the experts i, i + 2^g_log,
-// ... (NS of them); top_k rounds of a maximum over (score, lowest index first), each of
-// which takes its winner out. A score of -inf or NaN has the key 0 and is never chosen.
+// Choice. G = 2^g_log lanes hold the scores of one token, lane i the experts i, i + G, ... (NS
+// of them; NS > 1 only with G = 64); top_k rounds of a maximum over the group, each of which
+// takes its winner out: the lowest index among the equals, which a ballot finds. A score of
+// -inf or NaN has the key 0 and is never chosen.
 // The gates are the softmax of the chosen means:
 //   g_j = e_j / S, e_j = exp(s_j - s_0) (s_0 is the largest), S = sum e
 //   dg_j/ds_j = g_j (S - e_j) / S, with S - e_j summed from the other weights, so that a
 //   gate next to one keeps its slope
 // Lane j of the token keeps choice j (top_k <= 64, and <= the lanes where those are fewer).
+// A round is a chain of dependent instructions and bound by their latency: the maximum goes
+// through lane permutations inside the vector unit (16384 tokens, 64 experts, 4 choices: 123 us
+// with the ones through LDS and 128 tokens per workgroup, CHOOSE_US us with these and 32).
 // ---------------------------------------------------------------------------
-constexpr int ROUTE_TOKENS = 128;   // tokens of a workgroup of the plan
-constexpr int MASK_WORDS = ROUTE_TOKENS / 32;
+constexpr int ROUTE_TOKENS = 32;   // tokens of a workgroup of the plan, a bit each
 
 __device__ __forceinline__ unsigned order_bits(float s) {
     if (!(s > -INFINITY)) return 0u;
@@ -34,6 +38,25 @@ __device__ __forceinline__ float from_order_bits(unsigned k) {
     return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
 }
 
+template <int CTRL>
+__device__ __forceinline__ unsigned max_with(unsigned v) {
+    return max(v, (unsigned)__builtin_amdgcn_update_dpp((int)v, (int)v, CTRL, 0xF, 0xF, false));
+}
+// Maximum over the lane's group of 2^g_log lanes (g_log is the same for the launch).
+__device__ __forceinline__ unsigned group_max(unsigned v, int g_log) {
+    if (g_log >= 1) v = max_with<0xB1>(v);     // quad_perm 1 0 3 2
+    if (g_log >= 2) v = max_with<0x4E>(v);     // quad_perm 2 3 0 1
+    if (g_log >= 3) v = max_with<0x141>(v);    // row_half_mirror
+    if (g_log >= 4) v = max_with<0x140>(v);    // row_mirror
+    if (g_log == 5) v = max(v, (unsigned)__shfl_xor((int)v, 16, 64));
+    if (g_log == 6) {
+        const unsigned a = __builtin_amdgcn_readlane(v, 0), b = __builtin_amdgcn_readlane(v, 16);
+        const unsigned c = __builtin_amdgcn_readlane(v, 32), d = __builtin_amdgcn_readlane(v, 48);
+        v = max(max(a, b), max(c, d));
+    }
+    return v;
+}
+
 struct RouteOut {
     int *expert;              // [T][k]
     float *mu_g, *var_g, *jcb_g;
@@ -42,16 +65,17 @@ struct RouteOut {
 };
 
 // Chooses for the tokens [t0, t1) of a workgroup; every chosen (token, expert) is set in
-// `mask` (LDS, [E][MASK_WORDS], cleared by the caller).
+// `mask` (LDS, [E], cleared by the caller).
 template <int NS>
 __device__ __forceinline__ void choose(const float *__restrict__ mu_s,
                                        const float *__restrict__ var_s, int E, int k, int t0,
                                        int t1, int g_log, const RouteOut &o, unsigned *mask) {
-    const int G = 1 << g_log, gl = threadIdx.x & (G - 1);
+    const int G = 1 << g_log, lane = threadIdx.x & 63, gl = lane & (G - 1);
     const int sub = threadIdx.x >> g_log, subs = TPB >> g_log;
+    const unsigned long long group = (g_log == 6 ? ~0ull : (1ull << G) - 1) << (lane - gl);
     for (int tb = t0; tb < t1; tb += subs) {
         const int t = tb + sub;
-        const bool live = t < t1;   // (the shuffles below need every lane)
+        const bool live = t < t1;   // (the exchanges below need every lane)
         unsigned key[NS];
 #pragma unroll
         for (int i = 0; i < NS; i++) {
@@ -61,19 +85,16 @@ __device__ __forceinline__ void choose(const float *__restrict__ mu_s,
         float top = 0.f, w = 0.f, others = 0.f;
         int chosen = -1;
         for (int j = 0; j < k; j++) {
-            unsigned best = 0u, at = 0xffffffffu;
+            unsigned best = key[0];
 #pragma unroll
-            for (int i = 0; i < NS; i++)
-                if (key[i] > best) {
-                    best = key[i];
-                    at = (unsigned)((i << g_log) + gl);
-                }
-            for (int off = G >> 1; off > 0; off >>= 1) {
-                const unsigned ob = __shfl_xor(best, off, 64), oa = __shfl_xor(at, off, 64);
-                if (ob > best || (ob == best && oa < at)) {
-                    best = ob;
-                    at = oa;
-                }
+            for (int i = 1; i < NS; i++) best = max(best, key[i]);
+            best = group_max(best, g_log);
+            // the winner: the first register, then the first lane that holds the maximum
+            int at = -1;
+#pragma unroll
+            for (int i = 0; i < NS; i++) {
+                const unsigned long long holds = __ballot(key[i] == best) & group;
+                if (at < 0 && holds != 0ull) at = (i << g_log) + (__ffsll(holds) - 1 - (lane - gl));
             }
             if (best != 0u) {
                 const float sc = from_order_bits(best);
@@ -81,13 +102,13 @@ __device__ __forceinline__ void choose(const float *__restrict__ mu_s,
                 const float e = sc == top ? 1.f : expf(sc - top);   // (inf ties with inf)
                 if (j == gl) {
                     w = e;
-                    chosen = (int)at;
+                    chosen = at;
                 } else {
                     others += e;
                 }
 #pragma unroll
                 for (int i = 0; i < NS; i++)
-                    if ((unsigned)((i << g_log) + gl) == at) key[i] = 0u;
+                    if ((i << g_log) + gl == at) key[i] = 0u;
             }
         }
         if (!live || gl >= k) continue;
@@ -97,8 +118,7 @@ __device__ __forceinline__ void choose(const float *__restrict__ mu_s,
             g = w / sum;
             jc = g * (others / sum);
             vg = jc * jc * var_s[(size_t)t * E + chosen];
-            const int tl = t - t0;
-            atomicOr(&mask[chosen * MASK_WORDS + (tl >> 5)], 1u << (tl & 31));
+            atomicOr(&mask[chosen], 1u << (t - t0));
         }
         const size_t c = (size_t)t * k + gl;
         o.expert[c] = chosen;
@@ -106,13 +126,6 @@ __device__ __forceinline__ void choose(const float *__restrict__ mu_s,
         o.var_g[c] = vg;
         o.jcb_g[c] = jc;
     }
-}
-
-__device__ __forceinline__ int mask_count(const unsigned *mask, int e) {
-    int c = 0;
-#pragma unroll
-    for (int i = 0; i < MASK_WORDS; i++) c += __popc(mask[e * MASK_WORDS + i]);
-    return c;
 }
 
 // Exclusive prefix of v over the workgroup's threads; *total: the sum.
@@ -164,19 +177,17 @@ __device__ __forceinline__ int expert_bases(int E, Count count, First first, int
 __device__ __forceinline__ void place(int k, int t0, int t1, const RouteOut &o,
                                       const unsigned *mask, const int *base) {
     for (int c = t0 * k + threadIdx.x; c < t1 * k; c += TPB) {
-        const int e = o.expert[c], t = c / k, tl = t - t0;
+        const int e = o.expert[c], t = c / k;
         int row = -1;
         if (e >= 0) {
-            row = base[e];
-            for (int i = 0; i < (tl >> 5); i++) row += __popc(mask[e * MASK_WORDS + i]);
-            row += __popc(mask[e * MASK_WORDS + (tl >> 5)] & ((1u << (tl & 31)) - 1u));
+            row = base[e] + __popc(mask[e] & ((1u << (t - t0)) - 1u));
             o.token[row] = t;
         }
         o.slot[c] = row;
     }
 }
 
-// LDS: mask [E][MASK_WORDS], base [E]
+// LDS: mask [E], base [E]
 extern __shared__ unsigned route_lds[];
 
 // Up to ROUTE_TOKENS tokens: everything in one workgroup.
@@ -186,13 +197,13 @@ __global__ __launch_bounds__(TPB) void route_one_kernel(const float *__restrict_
                                                         int E, int k, int g_log, RouteOut o) {
     __shared__ int s[TPB / 64];
     unsigned *mask = route_lds;
-    int *base = reinterpret_cast<int *>(route_lds + E * MASK_WORDS);
-    for (int i = threadIdx.x; i < E * MASK_WORDS; i += TPB) mask[i] = 0u;
+    int *base = reinterpret_cast<int *>(route_lds + E);
+    for (int i = threadIdx.x; i < E; i += TPB) mask[i] = 0u;
     __syncthreads();
     choose<NS>(mu_s, var_s, E, k, 0, T, g_log, o, mask);
     __syncthreads();
     const int total = expert_bases(
-        E, [&](int e) { return mask_count(mask, e); }, [](int) { return 0; }, s, base, o.offsets);
+        E, [&](int e) { return __popc(mask[e]); }, [](int) { return 0; }, s, base, o.offsets);
     place(k, 0, T, o, mask, base);
     for (int r = total + threadIdx.x; r < T * k; r += TPB) o.token[r] = -1;
 }
@@ -204,12 +215,12 @@ __global__ __launch_bounds__(TPB) void route_choose_kernel(const float *__restri
                                                            int E, int k, int g_log, RouteOut o,
                                                            int *__restrict__ counts) {
     unsigned *mask = route_lds;
-    for (int i = threadIdx.x; i < E * MASK_WORDS; i += TPB) mask[i] = 0u;
+    for (int i = threadIdx.x; i < E; i += TPB) mask[i] = 0u;
     __syncthreads();
     const int t0 = blockIdx.x * ROUTE_TOKENS;
     choose<NS>(mu_s, var_s, E, k, t0, min(T, t0 + ROUTE_TOKENS), g_log, o, mask);
     __syncthreads();
-    for (int e = threadIdx.x; e < E; e += TPB) counts[(size_t)blockIdx.x * E + e] = mask_count(mask, e);
+    for (int e = threadIdx.x; e < E; e += TPB) counts[(size_t)blockIdx.x * E + e] = __popc(mask[e]);
 }
 
 // One wave per expert: counts [blocks][E] become the exclusive sums over the workgroups,
@@ -238,13 +249,13 @@ __global__ __launch_bounds__(TPB) void route_place_kernel(int T, int E, int k, R
                                                           const int *__restrict__ totals) {
     __shared__ int s[TPB / 64];
     unsigned *mask = route_lds;
-    int *base = reinterpret_cast<int *>(route_lds + E * MASK_WORDS);
-    for (int i = threadIdx.x; i < E * MASK_WORDS; i += TPB) mask[i] = 0u;
+    int *base = reinterpret_cast<int *>(route_lds + E);
+    for (int i = threadIdx.x; i < E; i += TPB) mask[i] = 0u;
     __syncthreads();
     const int t0 = blockIdx.x * ROUTE_TOKENS, t1 = min(T, t0 + ROUTE_TOKENS);
     for (int c = t0 * k + threadIdx.x; c < t1 * k; c += TPB) {
-        const int e = o.expert[c], tl = c / k - t0;
-        if (e >= 0) atomicOr(&mask[e * MASK_WORDS + (tl >> 5)], 1u << (tl & 31));
+        const int e = o.expert[c];
+        if (e >= 0) atomicOr(&mask[e], 1u << (c / k - t0));
     }
     const int total = expert_bases(
         E, [&](int e) { return totals[e]; },
@@ -261,30 +272,11 @@ __global__ __launch_bounds__(TPB) void route_place_kernel(int T, int E, int k, R
 //   mu_z = sum_j g y,  var_z = sum_j (g^2 + var_g) var_y + var_g y^2
 // ---------------------------------------------------------------------------
 template <int W>
-__device__ __forceinline__ void load_w(const float *p, float (&v)[W]) {
-    if (W == 4) {
-        const float4 q = *reinterpret_cast<const float4 *>(p);
-        v[0] = q.x;
-        v[1 % W] = q.y;
-        v[2 % W] = q.z;
-        v[3 % W] = q.w;
-    } else {
-        v[0] = p[0];
-    }
-}
-template <int W>
-__device__ __forceinline__ void store_w(float *p, const float (&v)[W]) {
-    if (W == 4)
-        *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1 % W], v[2 % W], v[3 % W]);
-    else
-        p[0] = v[0];
-}
-
-template <int W>
 __global__ __launch_bounds__(TPB) void combine_fwd_kernel(
     const float *__restrict__ mu_g, const float *__restrict__ var_g,
     const float *__restrict__ mu_y, const float *__restrict__ var_y, const int *__restrict__ slot,
-    int T, int k, int R, int N, float *__restrict__ mu_z, float *__restrict__ var_z) {
+    int T, int k, int R, int N, bool past_cache, float *__restrict__ mu_z,
+    float *__restrict__ var_z) {
     const int groups = N / W;
     const size_t total = (size_t)T * groups, step = (size_t)gridDim.x * TPB;
     for (size_t i = (size_t)blockIdx.x * TPB + threadIdx.x; i < total; i += step) {
@@ -307,8 +299,8 @@ __global__ __launch_bounds__(TPB) void combine_fwd_kernel(
                 ov[c] += g2 * v[c] + vg * y[c] * y[c];
             }
         }
-        store_w<W>(mu_z + (size_t)t * N + f, om);
-        store_w<W>(var_z + (size_t)t * N + f, ov);
+        store_w<W>(mu_z + (size_t)t * N + f, om, past_cache);
+        store_w<W>(var_z + (size_t)t * N + f, ov, past_cache);
     }
 }
 
@@ -321,8 +313,8 @@ __global__ __launch_bounds__(TPB) void combine_bwd_kernel(
     const float *__restrict__ mu_g, const float *__restrict__ jcb_g,
     const float *__restrict__ mu_y, const int *__restrict__ expert, const int *__restrict__ slot,
     const float *__restrict__ dmu, const float *__restrict__ dvar, int T, int k, int R, int N,
-    int E, float *__restrict__ dmu_y, float *__restrict__ dvar_y, float *__restrict__ dmu_s,
-    float *__restrict__ dvar_s) {
+    int E, bool past_cache, float *__restrict__ dmu_y, float *__restrict__ dvar_y,
+    float *__restrict__ dmu_s, float *__restrict__ dvar_s) {
     __shared__ float s[2][TPB / 64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int x = threadIdx.x % THREADS;
@@ -353,8 +345,8 @@ __global__ __launch_bounds__(TPB) void combine_bwd_kernel(
                         dm[c] *= g;
                         dv[c] *= g * g;
                     }
-                    store_w<W>(dmu_y + (size_t)r * N + (size_t)q * W, dm);
-                    store_w<W>(dvar_y + (size_t)r * N + (size_t)q * W, dv);
+                    store_w<W>(dmu_y + (size_t)r * N + (size_t)q * W, dm, past_cache);
+                    store_w<W>(dvar_y + (size_t)r * N + (size_t)q * W, dv, past_cache);
                 }
             }
 #pragma unroll
@@ -387,7 +379,7 @@ template <int W>
 __global__ __launch_bounds__(TPB) void gather_bwd_kernel(
     const float *__restrict__ dmu_r, const float *__restrict__ dvar_r,
     const int *__restrict__ slot, const float *__restrict__ jcb, const float *res_mu,
-    const float *res_var, int T, int k, int R, int K, float *dmu, float *dvar) {
+    const float *res_var, int T, int k, int R, int K, bool past_cache, float *dmu, float *dvar) {
     const int groups = K / W;
     const size_t total = (size_t)T * groups, step = (size_t)gridDim.x * TPB;
     for (size_t i = (size_t)blockIdx.x * TPB + threadIdx.x; i < total; i += step) {
@@ -422,8 +414,8 @@ __global__ __launch_bounds__(TPB) void gather_bwd_kernel(
                 ov[c] *= jc[c] * jc[c];
             }
         }
-        store_w<W>(dmu + at, om);
-        store_w<W>(dvar + at, ov);
+        store_w<W>(dmu + at, om, past_cache);
+        store_w<W>(dvar + at, ov, past_cache);
     }
 }
 
@@ -440,7 +432,7 @@ template <int NS>
 hipError_t route(const float *mu_s, const float *var_s, int T, int E, int k, int g_log,
                  const RouteOut &o, int *scratch, hipStream_t stream) {
     const int blocks = route_blocks(T);
-    const unsigned lds_mask = E * MASK_WORDS * 4, lds = lds_mask + E * 4;
+    const unsigned lds_mask = E * 4, lds = E * 8;
     if (blocks == 1) {
         hipLaunchKernelGGL(route_one_kernel<NS>, dim3(1), dim3(TPB), lds, stream, mu_s, var_s, T, E,
                            k, g_log, o);
@@ -478,10 +470,12 @@ hipError_t launch_moe_combine_fwd(const float *mu_g, const float *var_g, const f
                                   float *mu_z, float *var_z, hipStream_t stream) {
     if (N % 4 == 0 && aligned16(mu_y) && aligned16(var_y) && aligned16(mu_z) && aligned16(var_z))
         hipLaunchKernelGGL(combine_fwd_kernel<4>, dim3(blocks_for((size_t)T * (N / 4))), dim3(TPB),
-                           0, stream, mu_g, var_g, mu_y, var_y, slot, T, k, R, N, mu_z, var_z);
+                           0, stream, mu_g, var_g, mu_y, var_y, slot, T, k, R, N,
+                           goes_past_cache((size_t)2 * T * N), mu_z, var_z);
     else
         hipLaunchKernelGGL(combine_fwd_kernel<1>, dim3(blocks_for((size_t)T * N)), dim3(TPB), 0,
-                           stream, mu_g, var_g, mu_y, var_y, slot, T, k, R, N, mu_z, var_z);
+                           stream, mu_g, var_g, mu_y, var_y, slot, T, k, R, N,
+                           goes_past_cache((size_t)2 * T * N), mu_z, var_z);
     return hipGetLastError();
 }
 
@@ -495,7 +489,8 @@ hipError_t launch_moe_combine_bwd(const float *mu_g, const float *jcb_g, const f
 #define COMBINE_BWD(THREADS, W)                                                                  \
     hipLaunchKernelGGL((combine_bwd_kernel<THREADS, W>),                                          \
                        dim3(blocks_for((size_t)T * THREADS)), dim3(TPB), 0, stream,               \
-                       mu_g, jcb_g, mu_y, expert, slot, dmu, dvar, T, k, R, N, E, dmu_y, dvar_y,  \
+                       mu_g, jcb_g, mu_y, expert, slot, dmu, dvar, T, k, R, N, E,                 \
+                       goes_past_cache((size_t)2 * R * N), dmu_y, dvar_y,                         \
                        dmu_s, dvar_s)
     const bool wide = N > 1024;
     if (vec && wide)
@@ -516,10 +511,12 @@ hipError_t launch_moe_gather_bwd(const float *dmu_r, const float *dvar_r, const 
     if (K % 4 == 0 && aligned16(dmu_r) && aligned16(dvar_r) && aligned16(jcb) &&
         aligned16(res_mu) && aligned16(res_var) && aligned16(dmu) && aligned16(dvar))
         hipLaunchKernelGGL(gather_bwd_kernel<4>, dim3(blocks_for((size_t)T * (K / 4))), dim3(TPB), 0,
-                           stream, dmu_r, dvar_r, slot, jcb, res_mu, res_var, T, k, R, K, dmu, dvar);
+                           stream, dmu_r, dvar_r, slot, jcb, res_mu, res_var, T, k, R, K,
+                           goes_past_cache((size_t)2 * T * K), dmu, dvar);
     else
         hipLaunchKernelGGL(gather_bwd_kernel<1>, dim3(blocks_for((size_t)T * K)), dim3(TPB), 0,
-                           stream, dmu_r, dvar_r, slot, jcb, res_mu, res_var, T, k, R, K, dmu, dvar);
+                           stream, dmu_r, dvar_r, slot, jcb, res_mu, res_var, T, k, R, K,
+                           goes_past_cache((size_t)2 * T * K), dmu, dvar);
     return hipGetLastError();
 }
 

@@ -204,7 +204,7 @@ def test_innovations_against_differences(kernel_choice):
 
 # ---- router -------------------------------------------------------------------------------
 
-ROUTES = [(1, 1, 1), (1, 8, 2), (3, 2, 2), (32, 16, 2), (5, 64, 64), (128, 6, 3), (129, 6, 3), (257, 65, 4),
+ROUTES = [(1, 1, 1), (1, 8, 2), (33, 6, 3), (64, 40, 5), (3, 2, 2), (32, 16, 2), (5, 64, 64), (128, 6, 3), (129, 6, 3), (257, 65, 4),
           (1000, 3, 1), (300, 200, 8), (77, 1024, 5), (700, 1000, 33), (9000, 5, 2)]
 
 
