@@ -11,4 +11,8 @@ __device__ __forceinline__ void group_rows(const int *__restrict__ offsets, int 
     end = min(max(offsets[e + 1], first), R);
 }
 
+// Vectors of floats at any float's address: the memory instructions need four bytes only.
+typedef float float4_any __attribute__((ext_vector_type(4), aligned(4)));
+typedef float float2_any __attribute__((ext_vector_type(2), aligned(4)));
+
 }  // namespace tagi

@@ -177,48 +177,55 @@ struct TileList {
 
 // What the 128 threads that stage one side hold of 32 reduction elements.
 struct Batch {
-    float4 v0[8], v1[8];
+    float4_any v0[8], v1[8];
     int left;       // reduction elements from the first of the batch to the end
+    int shift;      // columns by which the loads were moved to end with their row
     unsigned dead;  // bit i: v[i] belongs to no row and reads as zeros
 };
 
-// Four neighbouring floats at element `off` behind a uniform base. VEC: one 16-byte load at a
-// 32-bit byte offset (launch_grouped sees to the sizes). `last`: the last element that exists.
-template <bool VEC>
-__device__ __forceinline__ float4 load4(const float *base, unsigned off, unsigned last) {
-    if (VEC) return *reinterpret_cast<const float4 *>(reinterpret_cast<const char *>(base) + off * 4u);
-    float4 v;
-    v.x = base[off];
-    v.y = base[min(off + 1, last)];
-    v.z = base[min(off + 2, last)];
-    v.w = base[min(off + 3, last)];
-    return v;
+// Four neighbouring floats at element `off` behind a uniform base, at a 32-bit byte offset
+// (launch_grouped sees to the sizes) or, FAR, a 64-bit one.
+template <bool FAR>
+__device__ __forceinline__ float4_any load4(const float *base, unsigned off) {
+    if (FAR) return *reinterpret_cast<const float4_any *>(base + off);
+    return *reinterpret_cast<const float4_any *>(reinterpret_cast<const char *>(base) + off * 4u);
+}
+// v moved by n elements to the front, zeros behind them (0 <= n <= 4)
+__device__ __forceinline__ float4_any to_front(float4_any v, int n) {
+    const bool one = n & 1, two = n & 2, all = n & 4;
+    v = one ? (float4_any){v[1], v[2], v[3], 0.f} : v;
+    v = two ? (float4_any){v[2], v[3], 0.f, 0.f} : v;
+    return all ? (float4_any){0.f, 0.f, 0.f, 0.f} : v;
 }
 
 // Side with its reduction index contiguous: thread u holds the elements 4 (u % 8) .. + 3 of
-// the rows u / 8 + 16 i: eight lanes read a whole 128-byte line.
-template <int MODE, bool ROWS, bool VEC>
+// the rows u / 8 + 16 i: eight lanes read a whole 128-byte line. At the end of a reduction
+// that is no multiple of four the loads are moved to end with their row, and what they bring
+// is moved back before the split.
+template <int MODE, bool ROWS, bool FAR>
 struct SideK {
     const float *q0, *q1;       // uniform
+    static constexpr bool GATHER = ROWS && MODE == GROUPED_FWD;
     unsigned row[8];            // element offset of the thread's rows
-    int source[8];
+    int source[GATHER ? 8 : 1]; // gather: the rows of the next tile
     bool fresh, gather;
     unsigned dead;
-    int k, red, kk;
+    int k, red, at, first_row, last_row;
     const float *f0, *f1;       // the batch that is loaded
     __device__ __forceinline__ void start(const GroupedParams &p, const Tile &t, int u) {
         k = (u & 7) * 4;
         red = t.red;
         fresh = true;
-        gather = ROWS && MODE == GROUPED_FWD && p.rows != nullptr;
+        gather = GATHER && p.rows != nullptr;
         const size_t first = gather ? 0 : ROWS ? (size_t)t.m0 : (size_t)t.e * p.N + t.c0;
         q0 = (ROWS ? p.x0 : p.y0) + first * red;
         q1 = (ROWS ? p.x1 : p.y1) + first * red;
-        const int rows = (ROWS ? t.m_end - t.m0 : t.c_end - t.c0) - 1;
+        first_row = u >> 3;
+        last_row = (ROWS ? t.m_end - t.m0 : t.c_end - t.c0) - 1;
+        if constexpr (GATHER) {
+            if (gather)
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            source[i] = min((u >> 3) + 16 * i, rows);
-            if (gather) source[i] = p.rows[t.m0 + source[i]];
+                for (int i = 0; i < 8; i++) source[i] = p.rows[t.m0 + min(first_row + 16 * i, last_row)];
         }
     }
     __device__ __forceinline__ void ahead(const GroupedParams &, int) {}
@@ -230,35 +237,36 @@ struct SideK {
             dead = 0u;
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                int s = source[i];
-                if (gather && (unsigned)s >= (unsigned)p.T) {
-                    s = 0;
-                    dead |= 1u << i;
+                int s = min(first_row + 16 * i, last_row);
+                if constexpr (GATHER) {
+                    if (gather) s = source[i];
+                    if (gather && (unsigned)s >= (unsigned)p.T) {
+                        s = 0;
+                        dead |= 1u << i;
+                    }
                 }
                 row[i] = (unsigned)s * (unsigned)red;
             }
         }
         b.left = red - k0;
+        b.shift = 0;
         b.dead = dead;
-        // (never beyond the row's end: what is beyond reads as zeros)
-        kk = b.left >= TK ? k : min(k, VEC ? b.left - 4 : b.left - 1);
-        f0 = q0 + k0;
-        f1 = q1 + k0;
+        const bool whole = b.left >= TK;
+        at = whole ? k : min(k0 + k, red - 4);
+        f0 = q0 + (whole ? k0 : 0);
+        f1 = q1 + (whole ? k0 : 0);
     }
     // its i-th load of array `second`
     __device__ __forceinline__ void load(Batch &b, int i, bool second) const {
-        (second ? b.v1 : b.v0)[i] = load4<VEC>(second ? f1 : f0, row[i] + kk, row[i] + (b.left - 1));
+        (second ? b.v1 : b.v0)[i] = load4<FAR>(second ? f1 : f0, row[i] + at);
     }
     // zeros behind the end of the reduction and in rows that are no rows
     __device__ __forceinline__ void mask(Batch &b) const {
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            const int n = (b.dead >> i) & 1u ? 0 : b.left - k;
-            float4 &x = b.v0[i], &y = b.v1[i];
-            x.x = n > 0 ? x.x : 0.f, y.x = n > 0 ? y.x : 0.f;
-            x.y = n > 1 ? x.y : 0.f, y.y = n > 1 ? y.y : 0.f;
-            x.z = n > 2 ? x.z : 0.f, y.z = n > 2 ? y.z : 0.f;
-            x.w = n > 3 ? x.w : 0.f, y.w = n > 3 ? y.w : 0.f;
+            const int over = (b.dead >> i) & 1u ? 4 : min(max(4 - (b.left - k), 0), 4);
+            b.v0[i] = to_front(b.v0[i], over);
+            b.v1[i] = to_front(b.v1[i], over);
         }
     }
     // Operand O of the batch to LDS. The loads of the batch after it go out between the
@@ -270,10 +278,10 @@ struct SideK {
 #pragma unroll
         for (int i = 0; i < 8; i++) {
             if (O < 2 && next != nullptr) load(*next, i, O == 1);
-            const float4 x = b.v0[i], y = b.v1[i];
+            const float4_any x = b.v0[i], y = b.v1[i];
             unsigned lo[3], hi[3];
-            split_pair(operand<MODE, ROWS>(O, x.x, y.x), operand<MODE, ROWS>(O, x.y, y.y), lo);
-            split_pair(operand<MODE, ROWS>(O, x.z, y.z), operand<MODE, ROWS>(O, x.w, y.w), hi);
+            split_pair(operand<MODE, ROWS>(O, x[0], y[0]), operand<MODE, ROWS>(O, x[1], y[1]), lo);
+            split_pair(operand<MODE, ROWS>(O, x[2], y[2]), operand<MODE, ROWS>(O, x[3], y[3]), hi);
 #pragma unroll
             for (int s = 0; s < 3; s++)
                 *reinterpret_cast<uint2 *>(to + s * PIECE + i * 16 * TK * 2) = make_uint2(lo[s], hi[s]);
@@ -283,15 +291,14 @@ struct SideK {
 
 // Side with its reduction index slow: thread u holds the columns 4 (u % 32) .. + 3 of the
 // reduction elements 8 (u / 32) + i: 32 lanes read 512 bytes of one.
-template <int MODE, bool ROWS, bool VEC>
+template <int MODE, bool ROWS, bool FAR>
 struct SideM {
     static constexpr bool GATHER = MODE == GROUPED_DW && !ROWS;
     const float *q0, *q1;     // element (reduction 0, column 0) of the operand, uniform
-    int ld, red, r0, g, col, cols;
+    int ld, red, r0, g, col, shift;
     bool gather;
     int source[8];            // gather: the rows that the next batch reads
-    unsigned row[8];          // the batch that is loaded: the thread's elements in its rows,
-    unsigned last[VEC ? 1 : 8];   // the rows' last elements
+    unsigned row[8];          // the batch that is loaded: the thread's elements in its rows
     const float *f0, *f1;
     __device__ __forceinline__ void start(const GroupedParams &p, const Tile &t, int u) {
         g = (u >> 5) * 8;
@@ -302,17 +309,15 @@ struct SideM {
             ld = p.N;
             q0 = p.x0 + (size_t)t.r0 * p.N;
             q1 = p.x1 + (size_t)t.r0 * p.N;
-            cols = t.m_end;
-            col = t.m0 + (u & 31) * 4;
         } else {
             ld = p.K;
             q0 = p.y0 + (MODE == GROUPED_DZ ? (size_t)t.e * p.N * p.K : gather ? 0 : (size_t)t.r0 * p.K);
             q1 = q0;
-            cols = t.c_end;
-            col = t.c0 + (u & 31) * 4;
         }
         // (columns beyond the last are computed and not stored; they only have to exist)
-        col = min(col, VEC ? cols - 4 : cols - 1);
+        const int want = (ROWS ? t.m0 : t.c0) + (u & 31) * 4;
+        col = min(want, ld - 4);
+        shift = want - col;
     }
     // the row indices of the batch at k0, on their way while the batch before it is split
     __device__ __forceinline__ void ahead(const GroupedParams &p, int k0) {
@@ -322,6 +327,7 @@ struct SideM {
     }
     __device__ __forceinline__ void begin(const GroupedParams &p, int k0, Batch &b) {
         b.left = red - k0;
+        b.shift = shift;
         b.dead = 0u;
         f0 = q0 + (GATHER && gather ? 0 : (size_t)k0 * ld);
         f1 = q1 + (size_t)k0 * ld;
@@ -336,26 +342,24 @@ struct SideM {
                 }
             }
             row[i] = (unsigned)s * (unsigned)ld + (unsigned)col;
-            if (!VEC) last[i] = (unsigned)s * (unsigned)ld + (unsigned)(cols - 1);
         }
     }
     __device__ __forceinline__ void load(Batch &b, int i, bool second) const {
         if (!second)
-            b.v0[i] = load4<VEC>(f0, row[i], last[VEC ? 0 : i]);
+            b.v0[i] = load4<FAR>(f0, row[i]);
         else if (ROWS)
-            b.v1[i] = load4<VEC>(f1, row[i], last[VEC ? 0 : i]);
+            b.v1[i] = load4<FAR>(f1, row[i]);
     }
     __device__ __forceinline__ void mask(Batch &b) const {
 #pragma unroll
-        for (int i = 0; i < 8; i++)
-            if (i >= b.left - g || (b.dead >> i) & 1u) {
-                b.v0[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (ROWS) b.v1[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-            }
+        for (int i = 0; i < 8; i++) {
+            const int over = i >= b.left - g || (b.dead >> i) & 1u ? 4 : min(b.shift, 4);
+            b.v0[i] = to_front(b.v0[i], over);
+            if (ROWS) b.v1[i] = to_front(b.v1[i], over);
+        }
     }
     template <int O>
     __device__ __forceinline__ void write(const Batch &b, char *side, int u, Batch *next) const {
-        auto at = [&](const float4 &v, int j) { return j == 0 ? v.x : j == 1 ? v.y : j == 2 ? v.z : v.w; };
         char *to = side + chunk_at(u & 31, u >> 5);
 #pragma unroll
         for (int j = 0; j < 4; j++) {
@@ -366,9 +370,7 @@ struct SideM {
             unsigned x[4][3];
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                auto value = [&](int r) {
-                    return operand<MODE, ROWS>(O, at(b.v0[r], j), ROWS ? at(b.v1[r], j) : 0.f);
-                };
+                auto value = [&](int r) { return operand<MODE, ROWS>(O, b.v0[r][j], ROWS ? b.v1[r][j] : 0.f); };
                 split_pair(value(2 * i), value(2 * i + 1), x[i]);
             }
 #pragma unroll
@@ -416,7 +418,7 @@ struct Stager {
     }
     // batch b to LDS, the batch after it into `after`
     __device__ __forceinline__ void put(Batch &b, Batch &after) {
-        if (b.left < TK || b.dead != 0u) side.mask(b);
+        if (b.left < TK || b.dead != 0u || b.shift != 0) side.mask(b);
         if (more) {
             side.begin(p, k0, after);
             advance();
@@ -454,7 +456,7 @@ struct Stager {
     }
 };
 
-template <int MODE, bool VEC>
+template <int MODE, bool FAR>
 __global__ __launch_bounds__(TILE_THREADS) void grouped_tile_kernel(GroupedParams p) {
     extern __shared__ __attribute__((aligned(16))) char tile_lds[];
     typedef TileShape<MODE> Shape;
@@ -505,11 +507,11 @@ __global__ __launch_bounds__(TILE_THREADS) void grouped_tile_kernel(GroupedParam
         // ---- loads, splits, writes
         const int u = tid & 127;
         if (tid < 128) {
-            typedef std::conditional_t<Shape::AK, SideK<MODE, true, VEC>, SideM<MODE, true, VEC>> Side;
+            typedef std::conditional_t<Shape::AK, SideK<MODE, true, FAR>, SideM<MODE, true, FAR>> Side;
             Stager<MODE, Side> s{p, list, tile_lds, first, step, u};
             s.run();
         } else {
-            typedef std::conditional_t<Shape::BK, SideK<MODE, false, VEC>, SideM<MODE, false, VEC>> Side;
+            typedef std::conditional_t<Shape::BK, SideK<MODE, false, FAR>, SideM<MODE, false, FAR>> Side;
             Stager<MODE, Side> s{p, list, tile_lds + 3 * PIECE, first, step, u};
             s.run();
         }
@@ -591,65 +593,64 @@ __global__ __launch_bounds__(TILE_THREADS) void grouped_tile_kernel(GroupedParam
             }
         }
         // register v of lane l: row 8 (v / 4) + 4 (l / 32) + v % 4, column l % 32
-        if constexpr (VEC && !Shape::BK) {
+        if constexpr (!Shape::BK) {
             // the two column sub-tiles hold neighbouring columns
             const int c = t.c0 + row_at<false>(wn * 64 + (lane & 31));
             if (c >= t.c_end) continue;
+            const bool both = c + 1 < t.c_end;
             const size_t base = (MODE == GROUPED_DW ? (size_t)t.e * p.N * p.K : 0) + c;
 #pragma unroll
             for (int x = 0; x < 2; x++)
 #pragma unroll
                 for (int v0 = 0; v0 < 16; v0 += 4) {   // four rows at a time: registers
-                    float2 f[4];
+                    float2_any f[4];
                     const int pos = wm * 64 + x * 32 + 2 * v0 + 4 * (lane >> 5);
 #pragma unroll
                     for (int v = 0; v < 4; v++) {
                         const int m = min(t.m0 + row_at<Shape::AK>(pos + v), t.m_end - 1);
-                        f[v] = p.e0 != nullptr ? *reinterpret_cast<const float2 *>(p.e0 + base + (size_t)m * p.K)
-                                               : make_float2(1.f, 1.f);
+                        const float *e = p.e0 + base + (size_t)m * p.K;
+                        f[v] = p.e0 == nullptr ? (float2_any){1.f, 1.f}
+                               : both          ? *reinterpret_cast<const float2_any *>(e)
+                                               : (float2_any){e[0], 1.f};
                     }
 #pragma unroll
                     for (int v = 0; v < 4; v++) {
                         const int m = t.m0 + row_at<Shape::AK>(pos + v);
                         if (m >= t.m_end) continue;
                         const size_t at = base + (size_t)m * p.K;
-                        *reinterpret_cast<float2 *>(p.out0 + at) =
-                            make_float2(acc[0][x][0][v0 + v] * f[v].x, acc[0][x][1][v0 + v] * f[v].y);
-                        *reinterpret_cast<float2 *>(p.out1 + at) =
-                            make_float2(acc[1][x][0][v0 + v] * f[v].x * f[v].x,
-                                        acc[1][x][1][v0 + v] * f[v].y * f[v].y);
+                        const float2_any s0 = (float2_any){acc[0][x][0][v0 + v], acc[0][x][1][v0 + v]} * f[v];
+                        const float2_any s1 = (float2_any){acc[1][x][0][v0 + v], acc[1][x][1][v0 + v]} * f[v] * f[v];
+                        if (both) {
+                            *reinterpret_cast<float2_any *>(p.out0 + at) = s0;
+                            *reinterpret_cast<float2_any *>(p.out1 + at) = s1;
+                        } else {
+                            p.out0[at] = s0[0];
+                            p.out1[at] = s1[0];
+                        }
                     }
                     __builtin_amdgcn_sched_barrier(0);
                 }
-            continue;
-        }
+        } else {
 #pragma unroll
-        for (int x = 0; x < 2; x++)
+            for (int x = 0; x < 2; x++)
 #pragma unroll
-            for (int y = 0; y < 2; y++) {
-                const int c = t.c0 + row_at<Shape::BK>(wn * 64 + y * 32 + (lane & 31));
-                if (c >= t.c_end) continue;
-                float b0 = 0.f, b1 = 0.f;
-                if (MODE == GROUPED_FWD && p.e0 != nullptr) {
-                    b0 = p.e0[(size_t)t.e * p.N + c];
-                    b1 = p.e1[(size_t)t.e * p.N + c];
-                }
+                for (int y = 0; y < 2; y++) {
+                    const int c = t.c0 + wn * 64 + y * 32 + (lane & 31);
+                    if (c >= t.c_end) continue;
+                    float b0 = 0.f, b1 = 0.f;
+                    if (p.e0 != nullptr) {
+                        b0 = p.e0[(size_t)t.e * p.N + c];
+                        b1 = p.e1[(size_t)t.e * p.N + c];
+                    }
 #pragma unroll
-                for (int v = 0; v < 16; v++) {
-                    const int pos = wm * 64 + x * 32 + 8 * (v >> 2) + 4 * (lane >> 5) + (v & 3);
-                    const int m = t.m0 + row_at<Shape::AK>(pos);
-                    if (m >= t.m_end) continue;
-                    const float s0 = acc[0][x][y][v], s1 = acc[1][x][y][v];
-                    if (MODE == GROUPED_FWD) {
-                        store_activated(p.act, s0 + b0, s1 + b1, (size_t)m * p.N + c, p.out0, p.out1, p.out2);
-                    } else {
-                        const size_t at = (MODE == GROUPED_DW ? (size_t)t.e * p.N * p.K : 0) + (size_t)m * p.K + c;
-                        const float f = p.e0 != nullptr ? p.e0[at] : 1.f;
-                        p.out0[at] = s0 * f;
-                        p.out1[at] = s1 * f * f;
+                    for (int v = 0; v < 16; v++) {
+                        const int m = t.m0 + wm * 64 + x * 32 + 8 * (v >> 2) + 4 * (lane >> 5) + (v & 3);
+                        if (m >= t.m_end) continue;
+                        store_activated(p.act, acc[0][x][y][v] + b0, acc[1][x][y][v] + b1,
+                                        (size_t)m * p.N + c, p.out0, p.out1, p.out2);
                     }
                 }
-            }
+        }
     }
 }
 
@@ -693,51 +694,50 @@ __global__ __launch_bounds__(DB_WAVES * 64) void grouped_db_kernel(GroupedParams
 }
 
 inline int ceil_div(int a, int b) { return (a + b - 1) / b; }
-inline bool aligned16(const void *q) { return (reinterpret_cast<uintptr_t>(q) & 15u) == 0; }
 
-template <int MODE, bool VEC>
+template <int MODE, bool FAR>
 hipError_t tile_launch(const GroupedParams &p, long long tiles, hipStream_t stream) {
     static PerDeviceOnce once;
     hipError_t e = allow_dynamic_lds(
-        once, reinterpret_cast<const void *>(&grouped_tile_kernel<MODE, VEC>), TILE_LDS);
+        once, reinterpret_cast<const void *>(&grouped_tile_kernel<MODE, FAR>), TILE_LDS);
     if (e != hipSuccess) return e;
     // one workgroup per CU at most; every XCD the same number
     const long long most = num_cu() / 8 * 8, want = (tiles + 7) / 8 * 8;
-    hipLaunchKernelGGL((grouped_tile_kernel<MODE, VEC>), dim3((unsigned)(want < most ? want : most)),
+    hipLaunchKernelGGL((grouped_tile_kernel<MODE, FAR>), dim3((unsigned)(want < most ? want : most)),
                        dim3(TILE_THREADS), TILE_LDS, stream, p);
     return hipGetLastError();
-}
-
-template <bool VEC>
-hipError_t tile_launch(GroupedMode mode, const GroupedParams &p, hipStream_t stream) {
-    // row tiles over all groups: every group ends with at most one part tile
-    const long long row_tiles = p.R / TM + (p.E < p.R ? p.E : p.R);
-    if (mode == GROUPED_FWD) return tile_launch<GROUPED_FWD, VEC>(p, row_tiles * ceil_div(p.N, TM), stream);
-    if (mode == GROUPED_DZ) return tile_launch<GROUPED_DZ, VEC>(p, row_tiles * ceil_div(p.K, TM), stream);
-    return tile_launch<GROUPED_DW, VEC>(p, (long long)ceil_div(p.K, TM) * ceil_div(p.N, TM) * p.E, stream);
 }
 
 }  // namespace
 
 hipError_t launch_grouped(GroupedMode mode, const GroupedParams &p, hipStream_t stream) {
-    // 16-byte loads: every row of every operand starts on 16 bytes
-    const bool vec = p.K % 4 == 0 && (mode == GROUPED_FWD || p.N % 4 == 0) && aligned16(p.x0) &&
-                     aligned16(p.x1) && aligned16(p.y0) && (mode != GROUPED_FWD || aligned16(p.y1)) &&
-                     (mode == GROUPED_FWD || (aligned16(p.e0) && aligned16(p.out0) && aligned16(p.out1)));
+    // 16-byte loads are moved to stay inside their row, so a row holds four elements at least
+    const bool vec = p.K >= 4 && p.N >= 4;
     // Few rows per expert on average: the weights are what takes the time. At 32 rows (256 rows,
     // 8 experts of 2048 x 2048) streaming against tiles: forward 150 / 130 us, state backward
     // 65 / 180 us, weight backward 218 / 194 us; at 4 rows (16 experts) streaming wins all
     // three. (The streaming grid: one workgroup per sixteen outputs of every expert.)
     const bool few = (long long)p.R <= (mode == GROUPED_DZ ? 32LL : 16LL) * p.E &&
                      (long long)p.N * p.E < (1LL << 26);
-    if (g_grouped_rows >= 0 ? g_grouped_rows != 0 : few)
+    if (!vec || (g_grouped_rows >= 0 ? g_grouped_rows != 0 : few))
         return launch_grouped_rows(mode, p, vec, stream);
-    // its 32-bit byte offsets: 128 rows of one operand, or any row where rows are gathered
-    const long long most = 1LL << 30;
-    const bool near = (p.rows == nullptr || (long long)p.T * p.K < most) && 128LL * p.K < most &&
-                      128LL * p.N < most;
-    hipError_t e = vec && near ? tile_launch<true>(mode, p, stream) : tile_launch<false>(mode, p, stream);
-    if (e != hipSuccess || mode != GROUPED_DW || p.db0 == nullptr) return e;
+    // row tiles over all groups: every group ends with at most one part tile
+    const long long row_tiles = p.R / TM + (p.E < p.R ? p.E : p.R);
+    // byte offsets from a tile's first row fit 32 bits (K, N <= 2^22), those of gathered rows
+    // while the activations have fewer than 2^30 elements
+    const bool far = (p.rows != nullptr && (long long)p.T * p.K >= (1LL << 30)) || p.K > (1 << 22) || p.N > (1 << 22);
+    hipError_t e;
+    if (mode == GROUPED_FWD) {
+        const long long tiles = row_tiles * ceil_div(p.N, TM);
+        return far ? tile_launch<GROUPED_FWD, true>(p, tiles, stream) : tile_launch<GROUPED_FWD, false>(p, tiles, stream);
+    }
+    if (mode == GROUPED_DZ) {
+        const long long tiles = row_tiles * ceil_div(p.K, TM);
+        return far ? tile_launch<GROUPED_DZ, true>(p, tiles, stream) : tile_launch<GROUPED_DZ, false>(p, tiles, stream);
+    }
+    const long long tiles = (long long)ceil_div(p.K, TM) * ceil_div(p.N, TM) * p.E;
+    e = far ? tile_launch<GROUPED_DW, true>(p, tiles, stream) : tile_launch<GROUPED_DW, false>(p, tiles, stream);
+    if (e != hipSuccess || p.db0 == nullptr) return e;
     hipLaunchKernelGGL(grouped_db_kernel, dim3((unsigned)ceil_div(p.N, 64) * p.E), dim3(DB_WAVES * 64), 0,
                        stream, p);
     return hipGetLastError();

@@ -20,21 +20,31 @@ typedef float floatx4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ floatx4 mfma(float a, float b, floatx4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
 }
-// Four elements at k of a row of `end`; zeros behind it.
+// Four elements at k of a row of `end`, to be passed through settle() where k + 4 > end. VEC:
+// the row has four at least, and a load that would leave it is moved to end with it.
 template <bool VEC>
 __device__ __forceinline__ floatx4 load4(const float *row, int k, int end) {
-    floatx4 v;
     if (VEC) {
-        v = *reinterpret_cast<const floatx4 *>(row + min(k, end - 4));
-        const float f = k < end ? 1.f : 0.f;
-        if (f == 0.f) v = (floatx4){0.f, 0.f, 0.f, 0.f};
-    } else {
-#pragma unroll
-        for (int t = 0; t < 4; t++) {
-            const float x = row[min(k + t, end - 1)];
-            v[t] = k + t < end ? x : 0.f;
-        }
+        const float4_any q = *reinterpret_cast<const float4_any *>(row + min(k, end - 4));
+        return (floatx4){q[0], q[1], q[2], q[3]};
     }
+    floatx4 v;
+#pragma unroll
+    for (int t = 0; t < 4; t++) v[t] = row[min(k + t, end - 1)];
+    return v;
+}
+// What load4 brought, moved back, with zeros behind the end. (Apart from the load, so that
+// loads in flight are not waited for.)
+template <bool VEC>
+__device__ __forceinline__ floatx4 settle(floatx4 v, int k, int end) {
+    if (VEC) {
+        const int n = min(max(k + 4 - end, 0), 4);
+        v = n & 1 ? (floatx4){v[1], v[2], v[3], 0.f} : v;
+        v = n & 2 ? (floatx4){v[2], v[3], 0.f, 0.f} : v;
+        return n & 4 ? (floatx4){0.f, 0.f, 0.f, 0.f} : v;
+    }
+#pragma unroll
+    for (int t = 0; t < 4; t++) v[t] = k + t < end ? v[t] : 0.f;
     return v;
 }
 
@@ -98,7 +108,20 @@ __device__ __forceinline__ void fwd_rows(const GroupedParams &p, int e, int n0, 
         load_w(f, kb);
         load_a(f, kb);
     };
-    auto use = [&](const FwdPiece<NG, VEC> &f) {
+    auto use = [&](FwdPiece<NG, VEC> &f, int kb) {
+        if (kb + 32 > K) {
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const int k = kb + 16 * h + q;
+                f.w0[h] = settle<VEC>(f.w0[h], k, K);
+                f.w1[h] = settle<VEC>(f.w1[h], k, K);
+#pragma unroll
+                for (int g = 0; g < NG; g++) {
+                    f.a0[g][h] = settle<VEC>(f.a0[g][h], k, K);
+                    f.a1[g][h] = settle<VEC>(f.a1[g][h], k, K);
+                }
+            }
+        }
 #pragma unroll
         for (int h = 0; h < 2; h++)
 #pragma unroll
@@ -116,10 +139,10 @@ __device__ __forceinline__ void fwd_rows(const GroupedParams &p, int e, int n0, 
     if (kb < K) load_a(x, kb);
     for (; kb < K; kb += 2 * step) {
         if (kb + step < K) load(y, kb + step);
-        use(x);
+        use(x, kb);
         if (kb + step >= K) break;
         if (kb + 2 * step < K) load(x, kb + 2 * step);
-        use(y);
+        use(y, kb + step);
     }
     // join: s[wave][8 g + 4 a + v][lane]
 #pragma unroll
@@ -200,7 +223,6 @@ __device__ __forceinline__ void dz_rows(const GroupedParams &p, int e, int k0, i
         for (int u = 0; u < 4; u++) {
             const int n = nb + q + u;
             f.w[u] = load4<VEC>(w + (size_t)min(n, N - 1) * K, k, K);
-            if (n >= N) f.w[u] = (floatx4){0.f, 0.f, 0.f, 0.f};
         }
 #pragma unroll
         for (int g = 0; g < NG; g++) {
@@ -208,7 +230,20 @@ __device__ __forceinline__ void dz_rows(const GroupedParams &p, int e, int k0, i
             f.d1[g] = load4<VEC>(d1[g], nb + q, N);
         }
     };
-    auto use = [&](const DzPiece<NG> &f) {
+    const bool edge = k0 + 64 > K;
+    auto use = [&](DzPiece<NG> &f, int nb) {
+        if (edge || nb + 16 > N) {
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                f.w[u] = settle<VEC>(f.w[u], k, K);
+                if (nb + q + u >= N) f.w[u] = (floatx4){0.f, 0.f, 0.f, 0.f};
+            }
+#pragma unroll
+            for (int g = 0; g < NG; g++) {
+                f.d0[g] = settle<VEC>(f.d0[g], nb + q, N);
+                f.d1[g] = settle<VEC>(f.d1[g], nb + q, N);
+            }
+        }
 #pragma unroll
         for (int u = 0; u < 4; u++)
 #pragma unroll
@@ -227,10 +262,10 @@ __device__ __forceinline__ void dz_rows(const GroupedParams &p, int e, int k0, i
     if (nb < N) load(x, nb);
     for (; nb < N; nb += 2 * step) {
         if (nb + step < N) load(y, nb + step);
-        use(x);
+        use(x, nb);
         if (nb + step >= N) break;
         if (nb + 2 * step < N) load(x, nb + 2 * step);
-        use(y);
+        use(y, nb + step);
     }
     constexpr int STEPS = 1024 / (DZ_WAVES * 64);   // outputs of a thread: 16 rows by 64 inputs
 #pragma unroll
@@ -328,7 +363,7 @@ __global__ __launch_bounds__(DW_WAVES * 64) void rows_dw_kernel(GroupedParams p)
                 live = live && (unsigned)s < (unsigned)p.T;
                 if (!live) s = 0;
             }
-            a[j] = load4<VEC>(p.y0 + (size_t)s * K, k, K);
+            a[j] = settle<VEC>(load4<VEC>(p.y0 + (size_t)s * K, k, K), k, K);
             if (!live) a[j] = (floatx4){0.f, 0.f, 0.f, 0.f};
             a2[j] = a[j] * a[j];
         }
@@ -356,10 +391,16 @@ __global__ __launch_bounds__(DW_WAVES * 64) void rows_dw_kernel(GroupedParams p)
                 x = acc0[i];
                 y = acc1[i];
             }
-        if (VEC) {
-            const floatx4 w = *reinterpret_cast<const floatx4 *>(p.e0 + at);
-            *reinterpret_cast<floatx4 *>(p.out0 + at) = x * w;
-            *reinterpret_cast<floatx4 *>(p.out1 + at) = y * w * w;
+        if (k + 4 <= K) {
+            const float4_any w = *reinterpret_cast<const float4_any *>(p.e0 + at);
+            float4_any m, v;
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                m[c] = x[c] * w[c];
+                v[c] = y[c] * w[c] * w[c];
+            }
+            *reinterpret_cast<float4_any *>(p.out0 + at) = m;
+            *reinterpret_cast<float4_any *>(p.out1 + at) = v;
         } else {
 #pragma unroll
             for (int c = 0; c < 4; c++)
