@@ -708,18 +708,44 @@ hipError_t tile_launch(const GroupedParams &p, long long tiles, hipStream_t stre
     return hipGetLastError();
 }
 
+// Which kernels a call goes to. Up to sixteen rows per expert on average the weights are what
+// takes the time, and the kernels for few rows read them once (64 rows, 16 experts of 2048 ->
+// 4096: 202 against 497 us). Beyond that those also win where the tiles are too few for the
+// chip, because their groups of 32 rows by 16 (forward) or 64 (state backward) outputs are
+// many more. Their time in us is about 8 + 3.3e-6 (1.6e-6) per group, N and K; that of the
+// tiles 12 + 2.6 (1.75) per round of tiles and 32 reduction elements. Measured, few rows / tiles:
+//   forward         777 rows,  6 experts,  301 ->  415   24 /  46 us
+//                   512        8          1024 -> 1024   78 / 103
+//                   256        4          2048 ->  512   51 / 183
+//                  2048        8           512 ->  512   87 /  63
+//                  1024        8          2048 -> 2048  495 / 227
+//   state backward  777        6           301 ->  415   16 /  44
+//                  2048        8           512 ->  512   43 /  41
+//                  1024        8          2048 -> 2048  200 / 142
+// The weight backward has as many tiles as the weights: few rows only (777 rows: 104 / 29 us).
+bool streams(GroupedMode mode, const GroupedParams &p) {
+    // (its grid: one workgroup per sixteen outputs of every group of rows)
+    const long long used = p.E < p.R ? p.E : p.R;
+    const long long cols = mode == GROUPED_FWD ? p.N : p.K, red = mode == GROUPED_FWD ? p.K : p.N;
+    if (cols * (p.R / 16 + used) >= 1LL << 26) return false;
+    if ((long long)p.R <= 16LL * p.E) return true;
+    if (mode == GROUPED_DW) return false;
+    // (tiles as they come: a part tile for most experts)
+    const long long row_tiles = p.R / TM + used / 2;
+    const long long tiles = (row_tiles > used ? row_tiles : used) * ceil_div((int)cols, TM);
+    const long long rounds = (tiles + num_cu() - 1) / num_cu();
+    const double groups = p.R / 32 + 0.5 * used;
+    const double rows_us = 8 + (mode == GROUPED_FWD ? 3.3e-6 : 1.6e-6) * groups * p.N * p.K;
+    const double tile_us = 12 + (mode == GROUPED_FWD ? 2.6 : 1.75) * rounds * ((red + TK - 1) / TK);
+    return rows_us < tile_us;
+}
+
 }  // namespace
 
 hipError_t launch_grouped(GroupedMode mode, const GroupedParams &p, hipStream_t stream) {
     // 16-byte loads are moved to stay inside their row, so a row holds four elements at least
     const bool vec = p.K >= 4 && p.N >= 4;
-    // Few rows per expert on average: the weights are what takes the time. At 32 rows (256 rows,
-    // 8 experts of 2048 x 2048) streaming against tiles: forward 150 / 130 us, state backward
-    // 65 / 180 us, weight backward 218 / 194 us; at 4 rows (16 experts) streaming wins all
-    // three. (The streaming grid: one workgroup per sixteen outputs of every expert.)
-    const bool few = (long long)p.R <= (mode == GROUPED_DZ ? 32LL : 16LL) * p.E &&
-                     (long long)p.N * p.E < (1LL << 26);
-    if (!vec || (g_grouped_rows >= 0 ? g_grouped_rows != 0 : few))
+    if (!vec || (g_grouped_rows >= 0 ? g_grouped_rows != 0 : streams(mode, p)))
         return launch_grouped_rows(mode, p, vec, stream);
     // row tiles over all groups: every group ends with at most one part tile
     const long long row_tiles = p.R / TM + (p.E < p.R ? p.E : p.R);

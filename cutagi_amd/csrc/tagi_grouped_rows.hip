@@ -179,11 +179,10 @@ __device__ __forceinline__ void fwd_rows(const GroupedParams &p, int e, int n0, 
 template <int WAVES, int NG, bool VEC>
 __global__ __launch_bounds__(WAVES * 64, NG == 1 && VEC ? 4 : 2) void rows_fwd_kernel(GroupedParams p) {
     __shared__ float s[WAVES][8 * NG][64];
-    const int blocks = (p.N + 15) / 16;
-    const int e = blockIdx.x / blocks, n0 = (blockIdx.x - e * blocks) * 16;
-    int first, end;
-    group_rows(p.offsets, e, p.R, first, end);
-    for (int r = first; r < end; r += 16 * NG) fwd_rows<WAVES, NG, VEC>(p, e, n0, r, end, s);
+    const int blocks = (p.N + 15) / 16, slot = blockIdx.x / blocks, n0 = (blockIdx.x - slot * blocks) * 16;
+    int r0, end;
+    const int e = find_rows(p.offsets, p.E, p.R, 16 * NG, slot, r0, end);
+    if (e >= 0) fwd_rows<WAVES, NG, VEC>(p, e, n0, r0, end, s);
 }
 
 // ---------------------------------------------------------------------------
@@ -306,11 +305,10 @@ __device__ __forceinline__ void dz_rows(const GroupedParams &p, int e, int k0, i
 template <int NG, bool VEC>
 __global__ __launch_bounds__(DZ_WAVES * 64, NG == 1 && VEC ? 4 : 2) void rows_dz_kernel(GroupedParams p) {
     __shared__ float s[DZ_WAVES][16][65];
-    const int blocks = (p.K + 63) / 64;
-    const int e = blockIdx.x / blocks, k0 = (blockIdx.x - e * blocks) * 64;
-    int first, end;
-    group_rows(p.offsets, e, p.R, first, end);
-    for (int r = first; r < end; r += 16 * NG) dz_rows<NG, VEC>(p, e, k0, r, end, s);
+    const int blocks = (p.K + 63) / 64, slot = blockIdx.x / blocks, k0 = (blockIdx.x - slot * blocks) * 64;
+    int r0, end;
+    const int e = find_rows(p.offsets, p.E, p.R, 16 * NG, slot, r0, end);
+    if (e >= 0) dz_rows<NG, VEC>(p, e, k0, r0, end, s);
 }
 
 // ---------------------------------------------------------------------------
@@ -428,18 +426,19 @@ hipError_t launch_grouped_rows(GroupedMode mode, const GroupedParams &p, bool ve
     // two groups of sixteen rows share a pass over the weights where experts have more than
     // eight rows on average; one group leaves registers for twice the waves
     const bool one = (long long)p.R <= 8LL * p.E;
-    // experts that can have rows
-    const long long used = p.E < p.R ? p.E : p.R;
+    // groups of rows at most, experts that can have rows
+    const int used = p.E < p.R ? p.E : p.R;
+    const unsigned slots = p.R / (one ? 16 : 32) + used;
     if (mode == GROUPED_FWD) {
-        const unsigned blocks = (p.N + 15) / 16, grid = blocks * p.E;
+        const unsigned blocks = (p.N + 15) / 16, grid = blocks * slots;
         // Waves that share a block: many blocks fill the chip with few waves each, which
         // spend less of their time starting and joining. 4 / 8 / 16 waves: 216 / 231 / 266 us
         // at 16 x 256 blocks of 2048, 73 / 61 / 69 at 2 x 256 of 4096, 43 / 30 / 26 at 2 x 64.
-        const long long working = used * blocks;
+        const long long working = (long long)used * blocks;
         if (!vec)
             one ? rows_fwd<8, 1, false>(p, grid, stream) : rows_fwd<8, 2, false>(p, grid, stream);
-        else if (!one)
-            rows_fwd<8, 2, true>(p, grid, stream);
+        else if (!one)   // (a wave needs some 32-element pieces to be worth its join)
+            p.K > 512 ? rows_fwd<8, 2, true>(p, grid, stream) : rows_fwd<4, 2, true>(p, grid, stream);
         else if (working > 1024)
             rows_fwd<4, 1, true>(p, grid, stream);
         else if (working > 256)
@@ -447,7 +446,7 @@ hipError_t launch_grouped_rows(GroupedMode mode, const GroupedParams &p, bool ve
         else
             rows_fwd<16, 1, true>(p, grid, stream);
     } else if (mode == GROUPED_DZ) {
-        const unsigned blocks = (p.K + 63) / 64, grid = blocks * p.E;
+        const unsigned blocks = (p.K + 63) / 64, grid = blocks * slots;
         if (!vec)
             one ? rows_dz<1, false>(p, grid, stream) : rows_dz<2, false>(p, grid, stream);
         else if (!one)
