@@ -9,6 +9,7 @@
 
 #include "../../include/tagi_hip.h"
 #include "blocks.h"
+#include "experts.h"
 #include "sequential.h"
 
 namespace py = pybind11;
@@ -155,6 +156,23 @@ PYBIND11_MODULE(cutagi, m) {
         .def("init_weight_bias", &BatchNorm2d::init_weight_bias);
     py::class_<BatchNorm2dHip, BaseLayer, std::shared_ptr<BatchNorm2dHip>>(m, "BatchNorm2dCuda")
         .def("get_norm_mean_var", &BatchNorm2dHip::get_norm_mean_var);
+    py::class_<LayerNorm, BaseLayer, std::shared_ptr<LayerNorm>>(m, "LayerNorm")
+        .def(py::init<const std::vector<int> &, float, bool, float, float>(),
+             py::arg("normalized_shape"), py::arg("eps") = 1e-5f, py::arg("bias") = true,
+             py::arg("gain_weight") = 1.0f, py::arg("gain_bias") = 1.0f)
+        .def("init_weight_bias", &LayerNorm::init_weight_bias);
+    py::class_<LayerNormHip, BaseLayer, std::shared_ptr<LayerNormHip>>(m, "LayerNormCuda");
+    py::class_<MixtureOfExperts, BaseLayer, std::shared_ptr<MixtureOfExperts>>(m, "MixtureOfExperts")
+        .def(py::init<size_t, size_t, size_t, int, int, const std::string &, bool, float, float,
+                      std::string>(),
+             py::arg("input_size"), py::arg("hidden_size"), py::arg("output_size"),
+             py::arg("num_experts"), py::arg("top_k"), py::arg("activation") = "relu",
+             py::arg("bias") = true, py::arg("gain_weight") = 1.0f, py::arg("gain_bias") = 1.0f,
+             py::arg("method") = "He")
+        .def("init_weight_bias", &MixtureOfExperts::init_weight_bias);
+    py::class_<MixtureOfExpertsHip, BaseLayer, std::shared_ptr<MixtureOfExpertsHip>>(
+        m, "MixtureOfExpertsCuda")
+        .def("get_expert_choices", &MixtureOfExpertsHip::get_expert_choices);
     py::class_<AvgPool2d, BaseLayer, std::shared_ptr<AvgPool2d>>(m, "AvgPool2d")
         .def(py::init<size_t, int, int, int, int>(), py::arg("kernel_size"),
              py::arg("stride") = -1, py::arg("padding") = 0, py::arg("padding_type") = 0,

@@ -568,6 +568,8 @@ void LayerBlock::compute_input_output_size(const InitArgs &args) {
     out_width = layers.back()->out_width;
     input_size = in_width * in_width * in_channels;
     output_size = out_width * out_height * out_channels;
+    // no image comes in (a block behind a Linear layer): the features of its layers
+    if (input_size == 0) this->add_layers();
 }
 
 void LayerBlock::save(std::ofstream &file) {
@@ -694,6 +696,10 @@ void ResNetBlock::compute_input_output_size(const InitArgs &args) {
     out_width = main_block->out_width;
     input_size = in_width * in_width * in_channels;
     output_size = out_width * out_height * out_channels;
+    if (input_size == 0) {   // no image comes in: the features of the main block
+        input_size = main_block->input_size;
+        output_size = main_block->output_size;
+    }
     if (shortcut && shortcut->output_size != output_size)
         LOG(LogLevel::ERROR, "ResNetBlock: shortcut output " +
                                  std::to_string(shortcut->output_size) + " vs main block output " +

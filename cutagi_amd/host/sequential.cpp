@@ -340,6 +340,9 @@ void Sequential::prepare_buffers(int batch_size) {
     if (batch_size != this->z_buffer_block_size) {
         this->z_buffer_size = batch_size * (this->z_buffer_size / this->z_buffer_block_size);
         this->z_buffer_block_size = batch_size;
+        // Growing frees these buffers, and what the layers and the library hold for a batch:
+        // what was recorded refers to them, even where new ones come to lie in their place.
+        if ((size_t)this->z_buffer_size > this->input_z_buffer->size) this->clear_graphs();
         this->input_z_buffer->set_size(this->z_buffer_size, batch_size);
         this->output_z_buffer->set_size(this->z_buffer_size, batch_size);
         // a model first run in eval mode has no delta buffers yet: they are created

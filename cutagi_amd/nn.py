@@ -13,7 +13,7 @@ arithmetic; every call goes to the C++ host classes, which call the HIP library.
 softmax encoding, class probabilities, error rate).
 
 Not here, because they are outside the Linear / Conv2d path: the other layer
-families of pytagi.nn (LSTM, attention, normalisations other than BatchNorm2d,
+families of pytagi.nn (LSTM, attention, normalisations other than BatchNorm2d and LayerNorm,
 max pooling, further activations), DDP and ``OutputUpdater.update_heteros``.
 """
 import math
@@ -96,6 +96,29 @@ class BatchNorm2d(BaseLayer):
                  gain_bias=1.0):
         self._cpp_backend = cutagi.BatchNorm2d(num_features, eps, momentum, bias, gain_weight,
                                                gain_bias)
+
+
+class LayerNorm(BaseLayer):
+    """Normalisation over the features of each sample (reference: pytagi/nn/layer_norm.py).
+    normalized_shape: the number of features, or a list whose product it is."""
+
+    def __init__(self, normalized_shape, eps=1e-5, bias=True, gain_weight=1.0, gain_bias=1.0):
+        shape = [normalized_shape] if np.isscalar(normalized_shape) else list(normalized_shape)
+        self._cpp_backend = cutagi.LayerNorm([int(n) for n in shape], eps, bias, gain_weight, gain_bias)
+
+
+class MixtureOfExperts(BaseLayer):
+    """A router that sends every sample to ``top_k`` of ``num_experts`` perceptrons
+    (input -> hidden, activation, hidden -> output) and adds their outputs up, weighted by the
+    softmax of its scores. No counterpart in the reference. activation: "relu" or
+    "mixture_relu". With top_k = 1 the one gate is 1 whatever the score, so the router's
+    weights do not move."""
+
+    def __init__(self, input_size, hidden_size, output_size, num_experts, top_k, activation="relu",
+                 bias=True, gain_weight=1.0, gain_bias=1.0, init_method="He"):
+        self._cpp_backend = cutagi.MixtureOfExperts(input_size, hidden_size, output_size, num_experts,
+                                                    top_k, activation, bias, gain_weight, gain_bias,
+                                                    init_method)
 
 
 class AvgPool2d(BaseLayer):

@@ -1,0 +1,205 @@
+"""LayerNorm and MixtureOfExperts as layers of a Sequential: the same bits as the tensor-level
+calls they are made of (which have their own tests against 64 bits), through forward,
+backward, parameter step, replayed graphs, blocks and checkpoints."""
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+N_IN, HIDDEN, N_OUT, EXPERTS, TOP_K = 24, 40, 12, 5, 2
+
+
+def _net(cutagi, activation="relu", bias=True, seed=0, first=True):
+    cutagi.manual_seed(seed)
+    layers = [cutagi.Linear(16, N_IN), cutagi.MixtureReLU()] if first else []
+    layers += [cutagi.LayerNorm([N_IN], 1e-5, bias),
+               cutagi.MixtureOfExperts(N_IN, HIDDEN, N_OUT, EXPERTS, TOP_K, activation, bias)]
+    net = cutagi.Sequential(layers)
+    net.to_device("cuda")
+    return net
+
+
+def _params(net, name):
+    import torch
+    return [torch.tensor(x, dtype=torch.float32, device="cuda") if len(x) else None
+            for x in net.state_dict()[name]]
+
+
+def _split(p, bias):
+    """(mu_w, var_w, mu_b, var_b) of the router, the first and the second expert layers."""
+    E, K, H, N = EXPERTS, N_IN, HIDDEN, N_OUT
+    ends = [0, E * K, E * K + E * H * K, E * K + E * H * K + E * N * H]
+    bends = [0, E, E + E * H, E + E * H + E * N]
+    shapes = [(E, K), (E, H, K), (E, N, H)]
+    bshapes = [(E,), (E, H), (E, N)]
+    out = []
+    for i in range(3):
+        w = [x[ends[i]:ends[i + 1]].reshape(shapes[i]) for x in p[:2]]
+        b = [x[bends[i]:bends[i + 1]].reshape(bshapes[i]) if bias else None for x in p[2:]]
+        out.append([t.clone() if t is not None else None for t in w + b])
+    return out
+
+
+@pytest.mark.parametrize("activation", ["relu", "mixture_relu"])
+@pytest.mark.parametrize("bias", [True, False])
+@pytest.mark.parametrize("batch", [1, 7, 300])
+def test_layers_are_their_calls(batch, bias, activation):
+    import torch
+    import cutagi_amd.functional as F
+    from cutagi_amd import capi, cutagi
+    rng = np.random.default_rng(batch)
+    f = np.float32
+    net = _net(cutagi, activation, bias, first=False)
+    net.input_state_update = True
+    x, v = rng.standard_normal((batch, N_IN)).astype(f), rng.uniform(0.01, 0.2, (batch, N_IN)).astype(f)
+    dmu, dvar = (0.1 * rng.standard_normal((batch, N_OUT))).astype(f), (-rng.uniform(0, 0.01, (batch, N_OUT))).astype(f)
+    names = ("LayerNormCuda.0", "MixtureOfExpertsCuda.1")
+    norm, moe = (_params(net, n) for n in names)
+    net.forward(x, v)
+    got = net.get_outputs()
+    choices = np.array(net.layers[1].get_expert_choices()).reshape(batch, TOP_K)
+    pad = np.zeros(net.input_delta_z_buffer.size - dmu.size, f)      # the buffer's whole length
+    net.set_delta_z(np.concatenate([dmu.ravel(), pad]), np.concatenate([dvar.ravel(), pad]))
+    net.backward()
+    net.delta_z_to_host()
+    back = [net.output_delta_z_buffer.delta_mu, net.output_delta_z_buffer.delta_var]
+    net.step()
+
+    t = lambda a: torch.from_numpy(a).cuda()
+    z, vz, m, s = F.layernorm_fwd(*norm, t(x), t(v), 1e-5)
+    router, up, down = _split(moe, bias)
+    scores = F.linear_fwd(*router, z, vz)
+    r = F.moe_route(*scores, TOP_K)
+    h, vh, jh = F.grouped_linear_fwd_act(*up, z, vz, r.offsets, activation, rows=r.token)
+    y, vy = F.grouped_linear_fwd(*down, h, vh, r.offsets)
+    out = F.moe_combine_fwd(r.mu_g, r.var_g, y, vy, r.slot)
+    for g, w in zip(got, out):
+        assert np.array_equal(np.asarray(g).ravel(), w.cpu().numpy().ravel())
+    assert np.array_equal(choices, r.expert.cpu().numpy())
+
+    dy, dvy, ds, dvs = F.moe_combine_bwd(r.mu_g, r.jcb_g, y, r.expert, r.slot, t(dmu), t(dvar), EXPERTS)
+    gd = F.grouped_linear_bwd(down[0], down[1], down[3], h, jh, dy, dvy, r.offsets)
+    gu = F.grouped_linear_bwd(up[0], up[1], up[3], z, None, gd[0], gd[1], r.offsets, rows=r.token)
+    gr = F.linear_bwd(router[0], router[1], router[3], z, torch.ones_like(z), ds, dvs)
+    dz = F.moe_gather_bwd(gu[0], gu[1], r.slot, None, gr[0], gr[1])
+    gn = F.layernorm_bwd(norm[0], norm[1], norm[3], t(x), None, m, s, *dz, 1e-5)
+    for g, w in zip(back, gn[:2]):
+        assert np.array_equal(np.asarray(g)[:batch * N_IN], w.cpu().numpy().ravel())
+
+    # the step: every parameter through the same capped update
+    cap = capi.cap_factor(batch)
+    flat = lambda parts: torch.cat([p.reshape(-1) for p in parts])
+    deltas = [flat([a[i] for a in (gr, gu, gd)]) for i in (2, 3)]
+    if bias:
+        deltas += [flat([a[i] for a in (gr, gu, gd)]) for i in (4, 5)]
+    for name, p, d in ((names[0], norm, list(gn[2:])), (names[1], moe, deltas)):
+        F.param_update(d[0].contiguous(), d[1].contiguous(), cap, p[0], p[1])
+        if bias:
+            F.param_update(d[2].contiguous(), d[3].contiguous(), cap, p[2], p[3])
+        for a, b in zip(_params(net, name), p):
+            if a is not None:
+                assert torch.equal(a, b), name
+
+
+def _train(net, cutagi, xs, ys):
+    updater = cutagi.OutputUpdater(net.device)
+    trace = []
+    for x, y in zip(xs, ys):
+        net.forward(x)
+        trace.append([a.copy() for a in net.get_outputs()])
+        updater.update(net.output_z_buffer, y, np.full(y.size, 0.5, np.float32), net.input_delta_z_buffer)
+        net.backward()
+        net.step()
+    return trace, net.state_dict()
+
+
+def test_replay_gives_the_eager_bits():
+    from cutagi_amd import cutagi
+    rng = np.random.default_rng(0)
+    sizes = [32] * 5 + [9] * 4 + [64] * 4 + [32] * 2
+    xs = [rng.standard_normal((b, 16)).astype(np.float32) for b in sizes]
+    ys = [rng.standard_normal(b * N_OUT).astype(np.float32) for b in sizes]
+    eager, p0 = _train(_net(cutagi), cutagi, xs, ys)
+    net = _net(cutagi)
+    net.enable_graphs(True)
+    replay, p1 = _train(net, cutagi, xs, ys)
+    captured = net.graphs_captured()
+    net.enable_graphs(False)
+    for i, (a, b) in enumerate(zip(eager, replay)):
+        assert all(np.array_equal(u, w) for u, w in zip(a, b)), "outputs differ at step %d" % i
+    assert p0 == p1 and captured >= 2
+    assert all(np.all(np.isfinite(u)) for a in eager for u in a)
+
+
+def test_residual_block_and_evaluation_mode():
+    """x + experts(norm(x)): the block adds the shortcut forward and its innovations back."""
+    from cutagi_amd import cutagi
+    rng = np.random.default_rng(1)
+    cutagi.manual_seed(3)
+    block = cutagi.LayerBlock([cutagi.LayerNorm([16]), cutagi.MixtureOfExperts(16, 24, 16, 4, 2)])
+    net = cutagi.Sequential([cutagi.Linear(8, 16), cutagi.ResNetBlock(block), cutagi.Linear(16, 3)])
+    net.to_device("cuda")
+    xs = [rng.standard_normal((10, 8)).astype(np.float32) for _ in range(4)]
+    ys = [rng.standard_normal(30).astype(np.float32) for _ in range(4)]
+    trace, _ = _train(net, cutagi, xs, ys)
+    assert all(np.all(np.isfinite(u)) for a in trace for u in a)
+    # against the layers one by one, with the sum in between
+    net.eval()
+    net.forward(xs[0])
+    got = [np.asarray(a) for a in net.get_outputs()]
+    import torch
+    import cutagi_amd.functional as F
+    sd = net.state_dict()
+    p = lambda n: [torch.tensor(a, dtype=torch.float32, device="cuda") for a in sd[n]]
+    keys = {k.split(".")[0] + "." + k.rsplit(".", 1)[-1]: k for k in sd}
+    lin0, lin2 = sorted(k for k in sd if k.startswith("Linear"))
+    ln = next(k for k in sd if "LayerNorm" in k)
+    me = next(k for k in sd if "MixtureOfExperts" in k)
+    a = torch.from_numpy(xs[0]).cuda()
+    w = p(lin0)
+    h = F.linear_fwd(w[0].reshape(16, 8), w[1].reshape(16, 8), w[2], w[3], a, torch.zeros_like(a))
+    z = F.layernorm_fwd(*p(ln), *h, 1e-5)
+    q = p(me)
+    E, K, H, N = 4, 16, 24, 16
+    part = lambda x, a, n, s: x[a:a + n].reshape(s).clone()
+    wr = [part(x, 0, E * K, (E, K)) for x in q[:2]] + [part(x, 0, E, (E,)) for x in q[2:]]
+    wu = [part(x, E * K, E * H * K, (E, H, K)) for x in q[:2]] + [part(x, E, E * H, (E, H)) for x in q[2:]]
+    wd = [part(x, E * K + E * H * K, E * N * H, (E, N, H)) for x in q[:2]] + [part(x, E + E * H, E * N, (E, N)) for x in q[2:]]
+    r = F.moe_route(*F.linear_fwd(*wr, z[0], z[1]), 2)
+    u = F.grouped_linear_fwd_act(*wu, z[0], z[1], r.offsets, "relu", rows=r.token)
+    y = F.grouped_linear_fwd(*wd, u[0], u[1], r.offsets)
+    c = F.moe_combine_fwd(r.mu_g, r.var_g, *y, r.slot)
+    w = p(lin2)
+    want = F.linear_fwd(w[0].reshape(3, 16), w[1].reshape(3, 16), w[2], w[3], c[0] + h[0], c[1] + h[1])
+    for g, x in zip(got, want):
+        assert np.array_equal(g.ravel(), x.cpu().numpy().ravel()), keys
+
+
+def test_checkpoints(tmp_path):
+    from cutagi_amd import cutagi
+    net, other = _net(cutagi, seed=0), _net(cutagi, seed=1)
+    x = np.random.default_rng(0).standard_normal((5, 16)).astype(np.float32)
+    net.forward(x)
+    want = [a.copy() for a in net.get_outputs()]
+    other.forward(x)
+    assert not np.array_equal(want[0], other.get_outputs()[0])
+    net.save(str(tmp_path / "net.bin"))
+    other.load(str(tmp_path / "net.bin"))
+    assert net.state_dict() == other.state_dict()
+    other.forward(x)
+    assert all(np.array_equal(a, b) for a, b in zip(want, other.get_outputs()))
+    third = _net(cutagi, seed=2)
+    third.load_state_dict(net.state_dict())
+    third.forward(x)
+    assert all(np.array_equal(a, b) for a, b in zip(want, third.get_outputs()))
+
+
+def test_refusals():
+    from cutagi_amd import cutagi
+    net = _net(cutagi, first=False)
+    with pytest.raises(RuntimeError, match="mismatch"):
+        net.forward(np.zeros((2, N_IN + 1), np.float32))
+    bad = cutagi.Sequential([cutagi.Linear(4, 6), cutagi.LayerNorm([8])])
+    bad.to_device("cuda")
+    with pytest.raises(RuntimeError, match="mismatch"):
+        bad.forward(np.zeros((2, 4), np.float32))

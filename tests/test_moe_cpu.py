@@ -132,3 +132,26 @@ def test_tensor_calls_refuse():
     no("expert: expected shape", F.moe_combine_bwd, f(4, 2), f(4, 2), f(8, 3), i(4, 3), i(4, 2), f(4, 3), f(4, 3), 4)
     no("come together", F.moe_gather_bwd, f(8, 3), f(8, 3), i(4, 2), None, f(4, 3), None)
 
+
+
+def test_layer_descriptions():
+    """The host layers without a GPU: sizes, parameters, refusals, no CPU compute path."""
+    import numpy as np
+    from cutagi_amd import cutagi, nn
+    cutagi.manual_seed(0)
+    net = nn.Sequential(nn.LayerNorm([4, 2]), nn.MixtureOfExperts(8, 16, 4, 3, 2), nn.LayerNorm(4, bias=False))
+    assert net.get_layer_stack_info().split() == ["LayerNorm()", "MixtureOfExperts(8,16,4,3,2)", "LayerNorm()"]
+    sizes = {k: [len(x) for x in v] for k, v in net.state_dict().items()}
+    w, b = 3 * 8 + 3 * 16 * 8 + 3 * 4 * 16, 3 + 3 * 16 + 3 * 4
+    assert sizes == {"LayerNorm.0": [8] * 4, "MixtureOfExperts.1": [w, w, b, b], "LayerNorm.2": [4, 4, 0, 0]}
+    mu_w, var_w = net.state_dict()["MixtureOfExperts.1"][:2]
+    assert np.allclose(var_w[:24 + 384], 1 / 8) and np.allclose(var_w[24 + 384:], 1 / 16)   # He, by part
+    assert net.state_dict()["LayerNorm.0"][0] == [1.0] * 8
+    for make in (lambda: nn.LayerNorm(1), lambda: nn.LayerNorm([]), lambda: nn.LayerNorm([4, 0]),
+                 lambda: nn.MixtureOfExperts(8, 16, 4, 3, 4), lambda: nn.MixtureOfExperts(8, 16, 4, 3, 0),
+                 lambda: nn.MixtureOfExperts(0, 16, 4, 3, 2), lambda: nn.MixtureOfExperts(8, 16, 4, 2000, 2),
+                 lambda: nn.MixtureOfExperts(8, 16, 4, 3, 2, "tanh")):
+        with pytest.raises(RuntimeError):
+            make()
+    with pytest.raises(RuntimeError, match="GPU only"):
+        net.forward(np.zeros((2, 8), np.float32))
