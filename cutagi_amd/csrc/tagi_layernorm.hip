@@ -7,8 +7,6 @@
 // Backward: the state innovations are element by element; the parameter innovations are
 // sums over the rows, taken in two steps (row chunks, then the chunks in index order: the
 // same bits every run, no atomics).
-#include <cstdint>
-
 #include "tagi_internal.h"
 #include "tagi_stream.h"
 
@@ -16,8 +14,6 @@ namespace tagi {
 namespace {
 
 constexpr int TPB = 256;
-
-inline bool aligned16(const void *q) { return (reinterpret_cast<uintptr_t>(q) & 15u) == 0; }
 
 // Sums over the THREADS (64 or 256) threads that share a row; every thread gets the result.
 template <int THREADS, int NV>
@@ -40,10 +36,10 @@ __device__ __forceinline__ void row_sum(float (&v)[NV], float (*s)[TPB / 64]) {
 }
 
 // ---------------------------------------------------------------------------
-// Forward. THREADS threads hold one row, PER groups of W features each (W = 4 where rows
-// are whole 16-byte groups, else 1); PER == 0: a row of any length, read three times.
+// Forward. THREADS threads hold one row, PER groups of four features each; PER == 0: a row of
+// any length, read three times.
 // ---------------------------------------------------------------------------
-template <int THREADS, int PER, int W>
+template <int THREADS, int PER>
 __global__ __launch_bounds__(TPB) void ln_fwd_kernel(
     const float *__restrict__ mu_w, const float *__restrict__ var_w,
     const float *__restrict__ mu_b, const float *__restrict__ var_b,
@@ -52,63 +48,52 @@ __global__ __launch_bounds__(TPB) void ln_fwd_kernel(
     float *__restrict__ var_z) {
     __shared__ float s[2][TPB / 64];
     const int t = threadIdx.x % THREADS;
+    const int groups = (n + 3) / 4;
+    constexpr int HELD = PER > 0 ? PER : 1;
     // (whole waves leave the loop, and whole workgroups where it holds a barrier)
     for (long long b = (long long)blockIdx.x * (TPB / THREADS) + threadIdx.x / THREADS; b < B;
          b += (long long)gridDim.x * (TPB / THREADS)) {
         const float *a = mu_a + (size_t)b * n, *q = var_a + (size_t)b * n;
-        const int groups = n / W;
-        constexpr int HELD = PER > 0 ? PER : 1;
-        float m[HELD][W], v[HELD][W];
+        float m[HELD][4], v[HELD][4];
 
         float sum[2] = {0.f, 0.f};
+        auto add = [&](const float (&mi)[4], const float (&vi)[4]) {
+            sum[0] += (mi[0] + mi[1]) + (mi[2] + mi[3]);
+            sum[1] += (vi[0] + vi[1]) + (vi[2] + vi[3]);
+        };
         if (PER > 0) {
 #pragma unroll
             for (int i = 0; i < HELD; i++) {
-                const int g = i * THREADS + t;
-                if (g < groups) {
-                    load_w<W>(a + (size_t)g * W, m[i]);
-                    load_w<W>(q + (size_t)g * W, v[i]);
-                } else {
-#pragma unroll
-                    for (int c = 0; c < W; c++) m[i][c] = v[i][c] = 0.f;
-                }
+                const int g = i * THREADS + t, valid = in_group(g, n);
+                load_group(a + (size_t)g * 4, valid, m[i]);
+                load_group(q + (size_t)g * 4, valid, v[i]);
             }
 #pragma unroll
-            for (int i = 0; i < HELD; i++)
-#pragma unroll
-                for (int c = 0; c < W; c++) {
-                    sum[0] += m[i][c];
-                    sum[1] += v[i][c];
-                }
+            for (int i = 0; i < HELD; i++) add(m[i], v[i]);
         } else {
             for (int g = t; g < groups; g += THREADS) {
-                load_w<W>(a + (size_t)g * W, m[0]);
-                load_w<W>(q + (size_t)g * W, v[0]);
-#pragma unroll
-                for (int c = 0; c < W; c++) {
-                    sum[0] += m[0][c];
-                    sum[1] += v[0][c];
-                }
+                load_group(a + (size_t)g * 4, in_group(g, n), m[0]);
+                load_group(q + (size_t)g * 4, in_group(g, n), v[0]);
+                add(m[0], v[0]);
             }
         }
         row_sum<THREADS, 2>(sum, s);
         const float mean = sum[0] / n;
         float dev[1] = {0.f};
+        auto deviate = [&](const float (&mi)[4], int valid) {
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                const float d = c < valid ? mi[c] - mean : 0.f;
+                dev[0] += d * d;
+            }
+        };
         if (PER > 0) {
 #pragma unroll
-            for (int i = 0; i < HELD; i++) {
-                const bool live = i * THREADS + t < groups;
-#pragma unroll
-                for (int c = 0; c < W; c++) {
-                    const float d = live ? m[i][c] - mean : 0.f;
-                    dev[0] += d * d;
-                }
-            }
+            for (int i = 0; i < HELD; i++) deviate(m[i], in_group(i * THREADS + t, n));
         } else {
             for (int g = t; g < groups; g += THREADS) {
-                load_w<W>(a + (size_t)g * W, m[0]);
-#pragma unroll
-                for (int c = 0; c < W; c++) dev[0] += (m[0][c] - mean) * (m[0][c] - mean);
+                load_group(a + (size_t)g * 4, in_group(g, n), m[0]);
+                deviate(m[0], in_group(g, n));
             }
         }
         row_sum<THREADS, 1>(dev, s);
@@ -119,28 +104,29 @@ __global__ __launch_bounds__(TPB) void ln_fwd_kernel(
         }
         const float inv = 1.0f / sqrtf(var + epsilon);
         const bool bias = mu_b != nullptr;
-        auto one = [&](int g, float (&mi)[W], float (&vi)[W]) {
-            const size_t f = (size_t)g * W;
-            float mw[W], vw[W], om[W], ov[W];
-            load_w<W>(mu_w + f, mw);
-            load_w<W>(var_w + f, vw);
+        auto one = [&](int g, const float (&mi)[4], const float (&vi)[4]) {
+            const size_t f = (size_t)g * 4;
+            const int valid = in_group(g, n);
+            float mw[4], vw[4], om[4], ov[4];
+            load_group(mu_w + f, valid, mw);
+            load_group(var_w + f, valid, vw);
 #pragma unroll
-            for (int c = 0; c < W; c++) {
+            for (int c = 0; c < 4; c++) {
                 const float x = inv * (mi[c] - mean);
                 om[c] = x * mw[c];
                 ov[c] = inv * inv * vi[c] * (mw[c] * mw[c] + vw[c]) + vw[c] * x * x;
             }
             if (bias) {
-                load_w<W>(mu_b + f, mw);
-                load_w<W>(var_b + f, vw);
+                load_group(mu_b + f, valid, mw);
+                load_group(var_b + f, valid, vw);
 #pragma unroll
-                for (int c = 0; c < W; c++) {
+                for (int c = 0; c < 4; c++) {
                     om[c] += mw[c];
                     ov[c] += vw[c];
                 }
             }
-            store_w<W>(mu_z + (size_t)b * n + f, om, past_cache);
-            store_w<W>(var_z + (size_t)b * n + f, ov, past_cache);
+            store_group(mu_z + (size_t)b * n + f, valid, om, past_cache);
+            store_group(var_z + (size_t)b * n + f, valid, ov, past_cache);
         };
         if (PER > 0) {
 #pragma unroll
@@ -150,8 +136,8 @@ __global__ __launch_bounds__(TPB) void ln_fwd_kernel(
             }
         } else {
             for (int g = t; g < groups; g += THREADS) {
-                load_w<W>(a + (size_t)g * W, m[0]);
-                load_w<W>(q + (size_t)g * W, v[0]);
+                load_group(a + (size_t)g * 4, in_group(g, n), m[0]);
+                load_group(q + (size_t)g * 4, in_group(g, n), v[0]);
                 one(g, m[0], v[0]);
             }
         }
@@ -159,61 +145,59 @@ __global__ __launch_bounds__(TPB) void ln_fwd_kernel(
 }
 
 // ---------------------------------------------------------------------------
-// Backward of one (block of columns, chunk of rows). 2^cw_log threads hold neighbouring
-// groups of W columns, the other bits of the thread index are rows. A thread keeps its
-// columns' four sums over the rows it walks; the row threads are joined through LDS.
-// part: [chunk][4][n].
+// Backward of one (block of columns, chunk of rows). 2^cw_log threads (up to a wave) hold
+// neighbouring groups of four columns, the other bits of the thread index are rows. A thread
+// keeps its columns' four sums over the rows it walks; the row threads of a wave are joined by
+// lane exchanges, the waves through LDS. part: [chunk][4][n].
 // ---------------------------------------------------------------------------
-template <int W>
 __global__ __launch_bounds__(TPB) void ln_bwd_kernel(
     const float *__restrict__ mu_w, const float *__restrict__ mu_a, const float *__restrict__ jcb,
     const float *__restrict__ mu_s, const float *__restrict__ var_s,
     const float *__restrict__ dmu_out, const float *__restrict__ dvar_out, float epsilon, int n,
     int B, int rows_per_chunk, int cw_log, int state_update, int param_update, bool past_cache,
     float *__restrict__ dmu, float *__restrict__ dvar, float *__restrict__ part) {
-    __shared__ float s[4][W][TPB];
-    const int cw = 1 << cw_log;
+    __shared__ float s[TPB / 64][16][64];
+    const int cw = 1 << cw_log, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int ct = threadIdx.x & (cw - 1), rt = threadIdx.x >> cw_log, row_step = TPB >> cw_log;
-    const int g = blockIdx.x * cw + ct;
-    const bool live = g < n / W;
-    const size_t f = (size_t)(live ? g : 0) * W;
+    const int g = blockIdx.x * cw + ct, valid = in_group(g, n);
+    const size_t f = (size_t)g * 4;
     const int b_lo = blockIdx.y * rows_per_chunk, b_hi = min(B, b_lo + rows_per_chunk);
-    float mw[W], acc[4][W];
-    load_w<W>(mu_w + f, mw);
+    float mw[4], acc[4][4];
+    load_group(mu_w + f, valid, mw);
 #pragma unroll
     for (int k = 0; k < 4; k++)
 #pragma unroll
-        for (int c = 0; c < W; c++) acc[k][c] = 0.f;
-    if (live) {
+        for (int c = 0; c < 4; c++) acc[k][c] = 0.f;
+    if (valid > 0) {
         for (int b = b_lo + rt; b < b_hi; b += row_step) {
             const size_t at = (size_t)b * n + f;
-            float dm[W], dv[W];
-            load_w<W>(dmu_out + at, dm);
-            load_w<W>(dvar_out + at, dv);
+            float dm[4], dv[4];
+            load_group(dmu_out + at, valid, dm);
+            load_group(dvar_out + at, valid, dv);
             const float inv = 1.0f / sqrtf(var_s[b] + epsilon);
             if (state_update) {
-                float t[W], om[W], ov[W];
+                float t[4], om[4], ov[4];
                 if (jcb != nullptr) {
-                    load_w<W>(jcb + at, t);
+                    load_group(jcb + at, valid, t);
                 } else {
 #pragma unroll
-                    for (int c = 0; c < W; c++) t[c] = 1.f;
+                    for (int c = 0; c < 4; c++) t[c] = 1.f;
                 }
 #pragma unroll
-                for (int c = 0; c < W; c++) {
+                for (int c = 0; c < 4; c++) {
                     t[c] *= inv * mw[c];
                     om[c] = t[c] * dm[c];
                     ov[c] = t[c] * dv[c] * t[c];
                 }
-                store_w<W>(dmu + at, om, past_cache);
-                store_w<W>(dvar + at, ov, past_cache);
+                store_group(dmu + at, valid, om, past_cache);
+                store_group(dvar + at, valid, ov, past_cache);
             }
             if (param_update) {
-                float x[W];
-                load_w<W>(mu_a + at, x);
+                float x[4];
+                load_group(mu_a + at, valid, x);
                 const float mean = mu_s[b];
 #pragma unroll
-                for (int c = 0; c < W; c++) {
+                for (int c = 0; c < 4; c++) {
                     x[c] = inv * (x[c] - mean);
                     acc[0][c] += x[c] * dm[c];
                     acc[1][c] += x[c] * x[c] * dv[c];
@@ -224,48 +208,52 @@ __global__ __launch_bounds__(TPB) void ln_bwd_kernel(
         }
     }
     if (!param_update) return;
+    for (int off = 32; off >= cw; off >>= 1)
 #pragma unroll
-    for (int k = 0; k < 4; k++)
+        for (int k = 0; k < 4; k++)
 #pragma unroll
-        for (int c = 0; c < W; c++) s[k][c][threadIdx.x] = acc[k][c];
+            for (int c = 0; c < 4; c++) acc[k][c] += __shfl_xor(acc[k][c], off, 64);
+    if (lane < cw)
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+#pragma unroll
+            for (int c = 0; c < 4; c++) s[wave][4 * k + c][lane] = acc[k][c];
     __syncthreads();
-    if (rt == 0 && live) {
-        float *o = part + (size_t)blockIdx.y * 4 * n + f;
+    // thread: sum k of column group ct (256 threads: four sums of 64 groups)
+    for (int i = threadIdx.x; i < 4 * cw; i += TPB) {
+        const int k = i >> cw_log, at = i & (cw - 1), have = in_group(blockIdx.x * cw + at, n);
+        float v[4];
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-            float v[W];
-#pragma unroll
-            for (int c = 0; c < W; c++) {
-                v[c] = 0.f;
-                for (int r = 0; r < row_step; r++) v[c] += s[k][c][(r << cw_log) + ct];
-            }
-#pragma unroll
-            for (int c = 0; c < W; c++) o[(size_t)k * n + c] = v[c];
-        }
+        for (int c = 0; c < 4; c++)
+            v[c] = (s[0][4 * k + c][at] + s[1][4 * k + c][at]) + (s[2][4 * k + c][at] + s[3][4 * k + c][at]);
+        store_group(part + ((size_t)blockIdx.y * 4 + k) * n + (size_t)(blockIdx.x * cw + at) * 4, have, v, false);
     }
 }
 
-// The chunks of 64 columns: sixteen waves take every sixteenth chunk, their sums are joined in
-// wave order.
+// The chunks of 2^cw_log (up to 64) columns: the other bits of the thread index share out the
+// chunks; their sums are joined like the row threads' above.
 constexpr int FINAL_WAVES = 16;
 __global__ __launch_bounds__(FINAL_WAVES * 64) void ln_bwd_final_kernel(
     const float *__restrict__ part, const float *__restrict__ var_w,
-    const float *__restrict__ var_b, int n, int chunks, float *__restrict__ dmu_w,
+    const float *__restrict__ var_b, int n, int chunks, int cw_log, float *__restrict__ dmu_w,
     float *__restrict__ dvar_w, float *__restrict__ dmu_b, float *__restrict__ dvar_b) {
     __shared__ float s[4][FINAL_WAVES][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int c = blockIdx.x * 64 + lane;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, cw = 1 << cw_log;
+    const int c = blockIdx.x * cw + (threadIdx.x & (cw - 1));
     float v[4] = {0.f, 0.f, 0.f, 0.f};
     if (c < n)
-        for (int q = wave; q < chunks; q += FINAL_WAVES) {
+        for (int q = threadIdx.x >> cw_log; q < chunks; q += (FINAL_WAVES * 64) >> cw_log) {
             const float *o = part + (size_t)q * 4 * n + c;
 #pragma unroll
             for (int k = 0; k < 4; k++) v[k] += o[(size_t)k * n];
         }
+    for (int off = 32; off >= cw; off >>= 1)
+#pragma unroll
+        for (int k = 0; k < 4; k++) v[k] += __shfl_xor(v[k], off, 64);
 #pragma unroll
     for (int k = 0; k < 4; k++) s[k][wave][lane] = v[k];
     __syncthreads();
-    if (wave != 0 || c >= n) return;
+    if (threadIdx.x >= cw || c >= n) return;
 #pragma unroll
     for (int k = 0; k < 4; k++) {
         v[k] = 0.f;
@@ -282,28 +270,33 @@ __global__ __launch_bounds__(FINAL_WAVES * 64) void ln_bwd_final_kernel(
     }
 }
 
-// Launch shape of the backward pass: columns per workgroup and rows per chunk, from n and B
-// alone, so that the scratch size does not depend on the pointers. `groups` is n / 4 where n
-// is a multiple of four; unaligned arrays then take the one-column form with the same chunks.
+// Threads that hold neighbouring groups of columns, and rows per chunk: from n and B alone.
+int ln_cw_log(int n) {
+    int l = 0;
+    while (l < 6 && (1 << l) < (n + 3) / 4) l++;
+    return l;
+}
 int ln_rows_per_chunk(int n, int B) {
-    const long long col_blocks = (n + 255) / 256;
     // four workgroups per CU (16384 x 4096, forward and backward: 2 / 3 / 4 / 8 / 16 per CU take
-    // 540 / 497 / 493 / 517 / 508 us; more of them also leave more partial sums)
-    long long chunks = (4LL * num_cu() + col_blocks - 1) / col_blocks;
-    long long rows = (B + chunks - 1) / chunks;
-    if (rows < 16) rows = 16;
-    return (int)rows;
+    // 540 / 497 / 493 / 517 / 508 us; more of them also leave more partial sums), but four rows
+    // for every row thread (sixteen in all at least)
+    const int cw = 1 << ln_cw_log(n);
+    const long long col_blocks = ((n + 3) / 4 + cw - 1) / cw;
+    const long long chunks = (4LL * num_cu() + col_blocks - 1) / col_blocks;
+    const long long rows = (B + chunks - 1) / chunks, least = 4 * (TPB / cw);
+    return (int)(rows > least ? rows : least);
 }
 
-template <int THREADS, int PER, int W>
+template <int THREADS, int PER>
 hipError_t fwd(const float *mu_w, const float *var_w, const float *mu_b, const float *var_b,
                const float *mu_a, const float *var_a, float epsilon, int n, int B, float *mu_s,
                float *var_s, float *mu_z, float *var_z, hipStream_t stream) {
     // (a launch holds fewer than 2^32 threads; beyond that the workgroups walk on)
     const long long rows = TPB / THREADS, blocks = (B + rows - 1) / rows;
     const unsigned grid = (unsigned)(blocks < (1 << 22) ? blocks : 1 << 22);
-    hipLaunchKernelGGL((ln_fwd_kernel<THREADS, PER, W>), dim3(grid), dim3(TPB), 0, stream, mu_w, var_w, mu_b, var_b, mu_a, var_a, epsilon, n, B,
-                       goes_past_cache((size_t)2 * B * n), mu_s, var_s, mu_z, var_z);
+    hipLaunchKernelGGL((ln_fwd_kernel<THREADS, PER>), dim3(grid), dim3(TPB), 0, stream, mu_w, var_w,
+                       mu_b, var_b, mu_a, var_a, epsilon, n, B, goes_past_cache((size_t)2 * B * n),
+                       mu_s, var_s, mu_z, var_z);
     return hipGetLastError();
 }
 
@@ -318,30 +311,16 @@ hipError_t launch_layernorm_fwd(const float *mu_w, const float *var_w, const flo
                                 const float *var_b, const float *mu_a, const float *var_a,
                                 float epsilon, int n, int B, float *mu_s, float *var_s,
                                 float *mu_z, float *var_z, hipStream_t stream) {
-    const bool vec = n % 4 == 0 && aligned16(mu_w) && aligned16(var_w) && aligned16(mu_b) &&
-                     aligned16(var_b) && aligned16(mu_a) && aligned16(var_a) && aligned16(mu_z) &&
-                     aligned16(var_z);
-#define LN_FWD(T, P, W)                                                                          \
-    return fwd<T, P, W>(mu_w, var_w, mu_b, var_b, mu_a, var_a, epsilon, n, B, mu_s, var_s, mu_z, \
-                        var_z, stream)
     // One wave per row up to 1024 features, unless the rows would not fill the chip that way
     // (four waves for every SIMD): then a workgroup each.
     const bool many = B >= 16 * num_cu();
-    if (vec) {
-        if (n <= 256) LN_FWD(64, 1, 4);
-        if (n <= 1024 && many) LN_FWD(64, 4, 4);
-        if (n <= 1024) LN_FWD(256, 1, 4);
-        if (n <= 4096) LN_FWD(256, 4, 4);
-        if (n <= 8192) LN_FWD(256, 8, 4);
-        LN_FWD(256, 0, 4);
-    }
-    if (n <= 256) LN_FWD(64, 4, 1);
-    if (n <= 1024 && many) LN_FWD(64, 16, 1);
-    if (n <= 1024) LN_FWD(256, 4, 1);
-    if (n <= 4096) LN_FWD(256, 16, 1);
-    if (n <= 8192) LN_FWD(256, 32, 1);
-    LN_FWD(256, 0, 1);
-#undef LN_FWD
+    auto *run = n <= 256            ? fwd<64, 1>
+                : n <= 1024 && many ? fwd<64, 4>
+                : n <= 1024         ? fwd<256, 1>
+                : n <= 4096         ? fwd<256, 4>
+                : n <= 8192         ? fwd<256, 8>
+                                    : fwd<256, 0>;
+    return run(mu_w, var_w, mu_b, var_b, mu_a, var_a, epsilon, n, B, mu_s, var_s, mu_z, var_z, stream);
 }
 
 hipError_t launch_layernorm_bwd(const float *mu_w, const float *var_w, const float *var_b,
@@ -350,28 +329,18 @@ hipError_t launch_layernorm_bwd(const float *mu_w, const float *var_w, const flo
                                 float epsilon, int n, int B, int state_update, int param_update,
                                 float *scratch, float *dmu, float *dvar, float *dmu_w,
                                 float *dvar_w, float *dmu_b, float *dvar_b, hipStream_t stream) {
-    const bool vec = n % 4 == 0 && aligned16(mu_w) && aligned16(dmu_out) && aligned16(dvar_out) &&
-                     (!state_update || (aligned16(jcb) && aligned16(dmu) && aligned16(dvar))) &&
-                     (!param_update || aligned16(mu_a));
-    const bool past_cache = goes_past_cache((size_t)2 * B * n);
-    const int rows = ln_rows_per_chunk(n, B);
-    const int chunks = (B + rows - 1) / rows, groups = vec ? n / 4 : n;
-    int cw_log = 0;
-    while (cw_log < 6 && (1 << cw_log) < groups) cw_log++;
+    const int rows = ln_rows_per_chunk(n, B), cw_log = ln_cw_log(n);
+    const int chunks = (B + rows - 1) / rows, groups = (n + 3) / 4;
     const dim3 grid((groups + (1 << cw_log) - 1) >> cw_log, chunks);
-    if (vec)
-        hipLaunchKernelGGL(ln_bwd_kernel<4>, grid, dim3(TPB), 0, stream, mu_w, mu_a, jcb, mu_s,
-                           var_s, dmu_out, dvar_out, epsilon, n, B, rows, cw_log, state_update,
-                           param_update, past_cache, dmu, dvar, scratch);
-    else
-        hipLaunchKernelGGL(ln_bwd_kernel<1>, grid, dim3(TPB), 0, stream, mu_w, mu_a, jcb, mu_s,
-                           var_s, dmu_out, dvar_out, epsilon, n, B, rows, cw_log, state_update,
-                           param_update, past_cache, dmu, dvar, scratch);
+    hipLaunchKernelGGL(ln_bwd_kernel, grid, dim3(TPB), 0, stream, mu_w, mu_a, jcb, mu_s, var_s, dmu_out,
+                       dvar_out, epsilon, n, B, rows, cw_log, state_update, param_update,
+                       goes_past_cache((size_t)2 * B * n), dmu, dvar, scratch);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || !param_update) return e;
-    hipLaunchKernelGGL(ln_bwd_final_kernel, dim3((n + 63) / 64), dim3(FINAL_WAVES * 64), 0, stream,
-                       scratch,
-                       var_w, var_b, n, chunks, dmu_w, dvar_w, dmu_b, dvar_b);
+    int f_log = 0;
+    while (f_log < 6 && (1 << f_log) < n) f_log++;
+    hipLaunchKernelGGL(ln_bwd_final_kernel, dim3((n + (1 << f_log) - 1) >> f_log), dim3(FINAL_WAVES * 64), 0,
+                       stream, scratch, var_w, var_b, n, chunks, f_log, dmu_w, dvar_w, dmu_b, dvar_b);
     return hipGetLastError();
 }
 

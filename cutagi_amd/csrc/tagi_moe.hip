@@ -1,8 +1,6 @@
 // The router of a mixture of experts and what joins its experts' outputs, for Gaussian
 // activations, gfx950: choice of the experts and gates of every token, the plan that
 // orders rows by expert, the gated sum and its backward pass.
-#include <cstdint>
-
 #include "tagi_internal.h"
 #include "tagi_stream.h"
 
@@ -10,8 +8,6 @@ namespace tagi {
 namespace {
 
 constexpr int TPB = 256;
-
-inline bool aligned16(const void *q) { return (reinterpret_cast<uintptr_t>(q) & 15u) == 0; }
 
 // ---------------------------------------------------------------------------
 // Choice. G = 2^g_log lanes hold the scores of one token, lane i the experts i, i + G, ... (NS
@@ -267,40 +263,40 @@ __global__ __launch_bounds__(TPB) void route_place_kernel(int T, int E, int k, R
 }
 
 // ---------------------------------------------------------------------------
-// The gated sum, W features of one token per thread. A choice without a row (slot < 0, or a
+// The gated sum, four features of one token per thread. A choice without a row (slot < 0, or a
 // slot that is no row) adds nothing.
 //   mu_z = sum_j g y,  var_z = sum_j (g^2 + var_g) var_y + var_g y^2
 // ---------------------------------------------------------------------------
-template <int W>
 __global__ __launch_bounds__(TPB) void combine_fwd_kernel(
     const float *__restrict__ mu_g, const float *__restrict__ var_g,
     const float *__restrict__ mu_y, const float *__restrict__ var_y, const int *__restrict__ slot,
     int T, int k, int R, int N, bool past_cache, float *__restrict__ mu_z,
     float *__restrict__ var_z) {
-    const int groups = N / W;
+    const int groups = (N + 3) / 4;
     const size_t total = (size_t)T * groups, step = (size_t)gridDim.x * TPB;
     for (size_t i = (size_t)blockIdx.x * TPB + threadIdx.x; i < total; i += step) {
         const int t = (int)(i / groups);
-        const size_t f = (i - (size_t)t * groups) * W;
-        float om[W], ov[W];
+        const int g = (int)(i - (size_t)t * groups), valid = in_group(g, N);
+        const size_t f = (size_t)g * 4;
+        float om[4], ov[4];
 #pragma unroll
-        for (int c = 0; c < W; c++) om[c] = ov[c] = 0.f;
+        for (int c = 0; c < 4; c++) om[c] = ov[c] = 0.f;
         for (int j = 0; j < k; j++) {
             const size_t at = (size_t)t * k + j;
             const int r = slot[at];
             if ((unsigned)r >= (unsigned)R) continue;
-            const float g = mu_g[at], vg = var_g[at], g2 = g * g + vg;
-            float y[W], v[W];
-            load_w<W>(mu_y + (size_t)r * N + f, y);
-            load_w<W>(var_y + (size_t)r * N + f, v);
+            const float gate = mu_g[at], vg = var_g[at], g2 = gate * gate + vg;
+            float y[4], v[4];
+            load_group(mu_y + (size_t)r * N + f, valid, y);
+            load_group(var_y + (size_t)r * N + f, valid, v);
 #pragma unroll
-            for (int c = 0; c < W; c++) {
-                om[c] += g * y[c];
+            for (int c = 0; c < 4; c++) {
+                om[c] += gate * y[c];
                 ov[c] += g2 * v[c] + vg * y[c] * y[c];
             }
         }
-        store_w<W>(mu_z + (size_t)t * N + f, om, past_cache);
-        store_w<W>(var_z + (size_t)t * N + f, ov, past_cache);
+        store_group(mu_z + (size_t)t * N + f, valid, om, past_cache);
+        store_group(var_z + (size_t)t * N + f, valid, ov, past_cache);
     }
 }
 
@@ -308,7 +304,7 @@ __global__ __launch_bounds__(TPB) void combine_fwd_kernel(
 //   rows    dmu_y = g dmu,  dvar_y = g^2 dvar
 //   scores  dmu_s[e] = jcb_g sum_n y dmu,  dvar_s[e] = jcb_g^2 sum_n y^2 dvar;
 //           zero for the experts that the token did not choose
-template <int THREADS, int W>
+template <int THREADS>
 __global__ __launch_bounds__(TPB) void combine_bwd_kernel(
     const float *__restrict__ mu_g, const float *__restrict__ jcb_g,
     const float *__restrict__ mu_y, const int *__restrict__ expert, const int *__restrict__ slot,
@@ -318,7 +314,7 @@ __global__ __launch_bounds__(TPB) void combine_bwd_kernel(
     __shared__ float s[2][TPB / 64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int x = threadIdx.x % THREADS;
-    const int groups = N / W;
+    const int groups = (N + 3) / 4;
     // (whole waves leave the loop, and whole workgroups where it holds a barrier)
     for (long long t = (long long)blockIdx.x * (TPB / THREADS) + threadIdx.x / THREADS; t < T;
          t += (long long)gridDim.x * (TPB / THREADS)) {
@@ -334,19 +330,20 @@ __global__ __launch_bounds__(TPB) void combine_bwd_kernel(
             if (live) {
                 const float g = mu_g[at];
                 for (int q = x; q < groups; q += THREADS) {
-                    float y[W], dm[W], dv[W];
-                    load_w<W>(mu_y + (size_t)r * N + (size_t)q * W, y);
-                    load_w<W>(dmu + (size_t)t * N + (size_t)q * W, dm);
-                    load_w<W>(dvar + (size_t)t * N + (size_t)q * W, dv);
+                    const int valid = in_group(q, N);
+                    float y[4], dm[4], dv[4];
+                    load_group(mu_y + (size_t)r * N + (size_t)q * 4, valid, y);
+                    load_group(dmu + (size_t)t * N + (size_t)q * 4, valid, dm);
+                    load_group(dvar + (size_t)t * N + (size_t)q * 4, valid, dv);
 #pragma unroll
-                    for (int c = 0; c < W; c++) {
+                    for (int c = 0; c < 4; c++) {
                         sm += y[c] * dm[c];
                         sv += y[c] * y[c] * dv[c];
                         dm[c] *= g;
                         dv[c] *= g * g;
                     }
-                    store_w<W>(dmu_y + (size_t)r * N + (size_t)q * W, dm, past_cache);
-                    store_w<W>(dvar_y + (size_t)r * N + (size_t)q * W, dv, past_cache);
+                    store_group(dmu_y + (size_t)r * N + (size_t)q * 4, valid, dm, past_cache);
+                    store_group(dvar_y + (size_t)r * N + (size_t)q * 4, valid, dv, past_cache);
                 }
             }
 #pragma unroll
@@ -375,47 +372,47 @@ __global__ __launch_bounds__(TPB) void combine_bwd_kernel(
 }
 
 // Rows back to tokens: (sum_j rows[slot] + res) * jcb, jcb^2.
-template <int W>
 __global__ __launch_bounds__(TPB) void gather_bwd_kernel(
     const float *__restrict__ dmu_r, const float *__restrict__ dvar_r,
     const int *__restrict__ slot, const float *__restrict__ jcb, const float *res_mu,
     const float *res_var, int T, int k, int R, int K, bool past_cache, float *dmu, float *dvar) {
-    const int groups = K / W;
+    const int groups = (K + 3) / 4;
     const size_t total = (size_t)T * groups, step = (size_t)gridDim.x * TPB;
     for (size_t i = (size_t)blockIdx.x * TPB + threadIdx.x; i < total; i += step) {
         const int t = (int)(i / groups);
-        const size_t f = (i - (size_t)t * groups) * W, at = (size_t)t * K + f;
-        float om[W], ov[W];
+        const int g = (int)(i - (size_t)t * groups), valid = in_group(g, K);
+        const size_t f = (size_t)g * 4, at = (size_t)t * K + f;
+        float om[4], ov[4];
         if (res_mu != nullptr) {
-            load_w<W>(res_mu + at, om);
-            load_w<W>(res_var + at, ov);
+            load_group(res_mu + at, valid, om);
+            load_group(res_var + at, valid, ov);
         } else {
 #pragma unroll
-            for (int c = 0; c < W; c++) om[c] = ov[c] = 0.f;
+            for (int c = 0; c < 4; c++) om[c] = ov[c] = 0.f;
         }
         for (int j = 0; j < k; j++) {
             const int r = slot[(size_t)t * k + j];
             if ((unsigned)r >= (unsigned)R) continue;
-            float m[W], v[W];
-            load_w<W>(dmu_r + (size_t)r * K + f, m);
-            load_w<W>(dvar_r + (size_t)r * K + f, v);
+            float m[4], v[4];
+            load_group(dmu_r + (size_t)r * K + f, valid, m);
+            load_group(dvar_r + (size_t)r * K + f, valid, v);
 #pragma unroll
-            for (int c = 0; c < W; c++) {
+            for (int c = 0; c < 4; c++) {
                 om[c] += m[c];
                 ov[c] += v[c];
             }
         }
         if (jcb != nullptr) {
-            float jc[W];
-            load_w<W>(jcb + at, jc);
+            float jc[4];
+            load_group(jcb + at, valid, jc);
 #pragma unroll
-            for (int c = 0; c < W; c++) {
+            for (int c = 0; c < 4; c++) {
                 om[c] *= jc[c];
                 ov[c] *= jc[c] * jc[c];
             }
         }
-        store_w<W>(dmu + at, om, past_cache);
-        store_w<W>(dvar + at, ov, past_cache);
+        store_group(dmu + at, valid, om, past_cache);
+        store_group(dvar + at, valid, ov, past_cache);
     }
 }
 
@@ -468,14 +465,9 @@ hipError_t launch_moe_route(const float *mu_s, const float *var_s, int T, int E,
 hipError_t launch_moe_combine_fwd(const float *mu_g, const float *var_g, const float *mu_y,
                                   const float *var_y, const int *slot, int T, int k, int R, int N,
                                   float *mu_z, float *var_z, hipStream_t stream) {
-    if (N % 4 == 0 && aligned16(mu_y) && aligned16(var_y) && aligned16(mu_z) && aligned16(var_z))
-        hipLaunchKernelGGL(combine_fwd_kernel<4>, dim3(blocks_for((size_t)T * (N / 4))), dim3(TPB),
-                           0, stream, mu_g, var_g, mu_y, var_y, slot, T, k, R, N,
-                           goes_past_cache((size_t)2 * T * N), mu_z, var_z);
-    else
-        hipLaunchKernelGGL(combine_fwd_kernel<1>, dim3(blocks_for((size_t)T * N)), dim3(TPB), 0,
-                           stream, mu_g, var_g, mu_y, var_y, slot, T, k, R, N,
-                           goes_past_cache((size_t)2 * T * N), mu_z, var_z);
+    hipLaunchKernelGGL(combine_fwd_kernel, dim3(blocks_for((size_t)T * ((N + 3) / 4))), dim3(TPB), 0,
+                       stream, mu_g, var_g, mu_y, var_y, slot, T, k, R, N,
+                       goes_past_cache((size_t)2 * T * N), mu_z, var_z);
     return hipGetLastError();
 }
 
@@ -484,39 +476,25 @@ hipError_t launch_moe_combine_bwd(const float *mu_g, const float *jcb_g, const f
                                   const float *dvar, int T, int k, int R, int N, int E,
                                   float *dmu_y, float *dvar_y, float *dmu_s, float *dvar_s,
                                   hipStream_t stream) {
-    const bool vec = N % 4 == 0 && aligned16(mu_y) && aligned16(dmu) && aligned16(dvar) &&
-                     aligned16(dmu_y) && aligned16(dvar_y);
-#define COMBINE_BWD(THREADS, W)                                                                  \
-    hipLaunchKernelGGL((combine_bwd_kernel<THREADS, W>),                                          \
-                       dim3(blocks_for((size_t)T * THREADS)), dim3(TPB), 0, stream,               \
-                       mu_g, jcb_g, mu_y, expert, slot, dmu, dvar, T, k, R, N, E,                 \
-                       goes_past_cache((size_t)2 * R * N), dmu_y, dvar_y,                         \
-                       dmu_s, dvar_s)
-    const bool wide = N > 1024;
-    if (vec && wide)
-        COMBINE_BWD(256, 4);
-    else if (vec)
-        COMBINE_BWD(64, 4);
-    else if (wide)
-        COMBINE_BWD(256, 1);
+    const bool past_cache = goes_past_cache((size_t)2 * R * N);
+    // a wave per token up to 1024 features, a workgroup beyond
+    if (N > 1024)
+        hipLaunchKernelGGL(combine_bwd_kernel<256>, dim3(blocks_for((size_t)T * 256)), dim3(TPB), 0, stream,
+                           mu_g, jcb_g, mu_y, expert, slot, dmu, dvar, T, k, R, N, E, past_cache, dmu_y,
+                           dvar_y, dmu_s, dvar_s);
     else
-        COMBINE_BWD(64, 1);
-#undef COMBINE_BWD
+        hipLaunchKernelGGL(combine_bwd_kernel<64>, dim3(blocks_for((size_t)T * 64)), dim3(TPB), 0, stream,
+                           mu_g, jcb_g, mu_y, expert, slot, dmu, dvar, T, k, R, N, E, past_cache, dmu_y,
+                           dvar_y, dmu_s, dvar_s);
     return hipGetLastError();
 }
 
 hipError_t launch_moe_gather_bwd(const float *dmu_r, const float *dvar_r, const int *slot,
                                  const float *jcb, const float *res_mu, const float *res_var, int T,
                                  int k, int R, int K, float *dmu, float *dvar, hipStream_t stream) {
-    if (K % 4 == 0 && aligned16(dmu_r) && aligned16(dvar_r) && aligned16(jcb) &&
-        aligned16(res_mu) && aligned16(res_var) && aligned16(dmu) && aligned16(dvar))
-        hipLaunchKernelGGL(gather_bwd_kernel<4>, dim3(blocks_for((size_t)T * (K / 4))), dim3(TPB), 0,
-                           stream, dmu_r, dvar_r, slot, jcb, res_mu, res_var, T, k, R, K,
-                           goes_past_cache((size_t)2 * T * K), dmu, dvar);
-    else
-        hipLaunchKernelGGL(gather_bwd_kernel<1>, dim3(blocks_for((size_t)T * K)), dim3(TPB), 0,
-                           stream, dmu_r, dvar_r, slot, jcb, res_mu, res_var, T, k, R, K,
-                           goes_past_cache((size_t)2 * T * K), dmu, dvar);
+    hipLaunchKernelGGL(gather_bwd_kernel, dim3(blocks_for((size_t)T * ((K + 3) / 4))), dim3(TPB), 0,
+                       stream, dmu_r, dvar_r, slot, jcb, res_mu, res_var, T, k, R, K,
+                       goes_past_cache((size_t)2 * T * K), dmu, dvar);
     return hipGetLastError();
 }
 

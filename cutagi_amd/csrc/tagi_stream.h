@@ -1,34 +1,41 @@
-// Loads and stores of W neighbouring floats (one 16-byte access for W = 4), for the kernels
-// that pass over their arrays once.
+// Loads and stores of four neighbouring floats at any float's address, for the kernels that
+// pass over the rows of their arrays once: a row of any length is groups of four and one part
+// group.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stddef.h>
 
 namespace tagi {
 
-typedef float stream_floatx4 __attribute__((ext_vector_type(4)));
+// (the memory instructions need four bytes only)
+typedef float stream4 __attribute__((ext_vector_type(4), aligned(4)));
 
-template <int W>
-__device__ __forceinline__ void load_w(const float *p, float (&v)[W]) {
-    if (W == 4) {
-        const stream_floatx4 q = *reinterpret_cast<const stream_floatx4 *>(p);
+// Elements 4 g .. 4 g + 3 that a row of n has: 0 to 4.
+__device__ __forceinline__ int in_group(int g, int n) { return min(max(n - 4 * g, 0), 4); }
+
+// `valid` floats from p on, zeros behind them
+__device__ __forceinline__ void load_group(const float *p, int valid, float (&v)[4]) {
+    if (valid == 4) {
+        const stream4 q = *reinterpret_cast<const stream4 *>(p);
 #pragma unroll
-        for (int c = 0; c < W; c++) v[c] = q[c];
+        for (int c = 0; c < 4; c++) v[c] = q[c];
     } else {
-        v[0] = p[0];
+#pragma unroll
+        for (int c = 0; c < 4; c++) v[c] = c < valid ? p[c] : 0.f;
     }
 }
 // past_cache: a streaming store
-template <int W>
-__device__ __forceinline__ void store_w(float *p, const float (&v)[W], bool past_cache) {
-    if (W == 4) {
-        const stream_floatx4 q = {v[0], v[1 % W], v[2 % W], v[3 % W]};
+__device__ __forceinline__ void store_group(float *p, int valid, const float (&v)[4], bool past_cache) {
+    if (valid == 4) {
+        const stream4 q = {v[0], v[1], v[2], v[3]};
         if (past_cache)
-            __builtin_nontemporal_store(q, reinterpret_cast<stream_floatx4 *>(p));
+            __builtin_nontemporal_store(q, reinterpret_cast<stream4 *>(p));
         else
-            *reinterpret_cast<stream_floatx4 *>(p) = q;
+            *reinterpret_cast<stream4 *>(p) = q;
     } else {
-        p[0] = v[0];
+#pragma unroll
+        for (int c = 0; c < 3; c++)
+            if (c < valid) p[c] = v[c];
     }
 }
 // Outputs that the 256 MB memory-side cache cannot hold for whoever reads them next go past

@@ -11,7 +11,7 @@ EPS = 1e-5
 # registers and one beyond, with and without whole 16-byte groups
 SHAPES = [(1, 2), (3, 3), (5, 13), (2, 64), (129, 65), (1, 1024), (67, 1000), (33, 1023), (4, 2048),
           (3, 4095), (2, 4096), (3, 4100), (2, 8191), (2, 8192), (2, 8196), (3, 9001), (1000, 7),
-          (4099, 24), (2051, 260)]
+          (4099, 24), (2051, 260), (9001, 4), (70001, 2), (5000, 1001)]
 
 
 def _dev(d):
