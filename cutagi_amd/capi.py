@@ -70,9 +70,10 @@ SIGNATURES = {
     "tagi_layernorm_fwd": (_i, [_vp] * 6 + [_i, _f, _i, _i] + [_vp] * 5),
     "tagi_layernorm_bwd_scratch": (_i, [_i, _i, _szp]),
     "tagi_layernorm_bwd": (_i, [_vp] * 9 + [_f] + [_i] * 5 + [_vp] * 8),
-    "tagi_grouped_linear_fwd": (_i, [_vp] * 8 + [_i] * 6 + [_vp] * 3),
-    "tagi_grouped_linear_fwd_act": (_i, [_vp] * 8 + [_i] * 7 + [_vp] * 4),
-    "tagi_grouped_linear_bwd": (_i, [_vp] * 9 + [_i] * 8 + [_vp] * 7),
+    "tagi_grouped_linear_scratch": (_i, [_i] * 4 + [_szp]),
+    "tagi_grouped_linear_fwd": (_i, [_vp] * 8 + [_i] * 6 + [_vp] * 4),
+    "tagi_grouped_linear_fwd_act": (_i, [_vp] * 8 + [_i] * 7 + [_vp] * 5),
+    "tagi_grouped_linear_bwd": (_i, [_vp] * 9 + [_i] * 8 + [_vp] * 8),
     "tagi_moe_route_scratch": (_i, [_i, _i, _szp]),
     "tagi_moe_route": (_i, [_vp] * 2 + [_i] * 3 + [_vp] * 9),
     "tagi_moe_combine_fwd": (_i, [_vp] * 5 + [_i] * 4 + [_vp] * 3),
@@ -161,6 +162,13 @@ def layernorm_bwd_scratch(n, B):
     """Bytes of scratch that tagi_layernorm_bwd needs for the parameter innovations."""
     size = ctypes.c_size_t(0)
     check(lib.tagi_layernorm_bwd_scratch(n, B, ctypes.byref(size)))
+    return size.value
+
+
+def grouped_linear_scratch(K, N, E, R):
+    """Bytes of scratch that the grouped Linear calls need."""
+    size = ctypes.c_size_t(0)
+    check(lib.tagi_grouped_linear_scratch(K, N, E, R, ctypes.byref(size)))
     return size.value
 
 

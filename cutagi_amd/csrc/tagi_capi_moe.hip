@@ -38,20 +38,28 @@ int moe_sizes(int T, int k, int R, int N) {
     return (long long)T * k > MAX_INT ? TAGI_ERR_UNSUPPORTED : TAGI_OK;
 }
 
+// whether the scratch that a call needs is there
+bool grouped_scratch_ok(int K, int N, int E, int R, const void *scratch) {
+    return scratch != nullptr ? (reinterpret_cast<size_t>(scratch) & 15u) == 0
+                              : grouped_scratch_floats(K, N, E, R) == 0;
+}
+
 int grouped_fwd(const float *mu_w, const float *var_w, const float *mu_b, const float *var_b,
                 const float *mu_a, const float *var_a, const int *offsets, const int *rows, int K,
-                int N, int E, int R, int T, int bias, int act, float *out0, float *out1, float *out2,
-                void *stream) {
+                int N, int E, int R, int T, int bias, int act, void *scratch, float *out0, float *out1,
+                float *out2, void *stream) {
     if (!mu_w || !var_w || !mu_a || !var_a || !offsets || !out0 || !out1) return TAGI_ERR_INVALID_ARG;
     if (bias && (!mu_b || !var_b)) return TAGI_ERR_INVALID_ARG;
     const int rc = grouped_sizes(K, N, E, R, T, rows, N, false);
     if (rc != TAGI_OK) return rc;
+    if (!grouped_scratch_ok(K, N, E, R, scratch)) return TAGI_ERR_INVALID_ARG;
     GroupedParams p = {};
     p.x0 = mu_a, p.x1 = var_a, p.y0 = mu_w, p.y1 = var_w;
     p.e0 = bias ? mu_b : nullptr, p.e1 = bias ? var_b : nullptr;
     p.offsets = offsets, p.rows = rows;
     p.K = K, p.N = N, p.E = E, p.R = R, p.T = T, p.act = act;
     p.out0 = out0, p.out1 = out1, p.out2 = out2;
+    p.scratch = static_cast<float *>(scratch);
     TAGI_TRY(launch_grouped(GROUPED_FWD, p, as_stream(stream)));
     return TAGI_OK;
 }
@@ -104,33 +112,41 @@ int tagi_layernorm_bwd(const float *mu_w, const float *var_w, const float *var_b
     return TAGI_OK;
 }
 
+int tagi_grouped_linear_scratch(int K, int N, int E, int R, size_t *bytes) {
+    if (bytes == nullptr) return TAGI_ERR_INVALID_ARG;
+    const int rc = grouped_sizes(K, N, E, R, 0, nullptr, N, false);
+    if (rc != TAGI_OK) return rc;
+    *bytes = grouped_scratch_floats(K, N, E, R) * sizeof(float);
+    return TAGI_OK;
+}
+
 int tagi_grouped_linear_fwd(const float *mu_w, const float *var_w, const float *mu_b,
                             const float *var_b, const float *mu_a, const float *var_a,
                             const int *offsets, const int *rows, int K, int N, int E, int R, int T,
-                            int bias, float *mu_z, float *var_z, void *stream) {
+                            int bias, void *scratch, float *mu_z, float *var_z, void *stream) {
     return grouped_fwd(mu_w, var_w, mu_b, var_b, mu_a, var_a, offsets, rows, K, N, E, R, T, bias, 0,
-                       mu_z, var_z, nullptr, stream);
+                       scratch, mu_z, var_z, nullptr, stream);
 }
 
 int tagi_grouped_linear_fwd_act(const float *mu_w, const float *var_w, const float *mu_b,
                                 const float *var_b, const float *mu_a, const float *var_a,
                                 const int *offsets, const int *rows, int K, int N, int E, int R,
-                                int T, int bias, int activation, float *mu_out, float *var_out,
-                                float *jcb_out, void *stream) {
+                                int T, int bias, int activation, void *scratch, float *mu_out,
+                                float *var_out, float *jcb_out, void *stream) {
     if (activation != TAGI_ACT_RELU && activation != TAGI_ACT_MIXTURE_RELU)
         return TAGI_ERR_INVALID_ARG;
     if (!jcb_out) return TAGI_ERR_INVALID_ARG;
     return grouped_fwd(mu_w, var_w, mu_b, var_b, mu_a, var_a, offsets, rows, K, N, E, R, T, bias,
-                       activation, mu_out, var_out, jcb_out, stream);
+                       activation, scratch, mu_out, var_out, jcb_out, stream);
 }
 
 int tagi_grouped_linear_bwd(const float *mu_w, const float *var_w, const float *var_b,
                             const float *mu_a, const float *jcb, const float *delta_mu,
                             const float *delta_var, const int *offsets, const int *rows, int K,
                             int N, int E, int R, int T, int bias, int state_update,
-                            int param_update, float *delta_mu_z, float *delta_var_z,
-                            float *delta_mu_w, float *delta_var_w, float *delta_mu_b,
-                            float *delta_var_b, void *stream) {
+                            int param_update, void *scratch, float *delta_mu_z,
+                            float *delta_var_z, float *delta_mu_w, float *delta_var_w,
+                            float *delta_mu_b, float *delta_var_b, void *stream) {
     if (!delta_mu || !delta_var || !offsets) return TAGI_ERR_INVALID_ARG;
     if (state_update && (!mu_w || !delta_mu_z || !delta_var_z)) return TAGI_ERR_INVALID_ARG;
     if (param_update && (!var_w || !mu_a || !delta_mu_w || !delta_var_w))
@@ -139,7 +155,9 @@ int tagi_grouped_linear_bwd(const float *mu_w, const float *var_w, const float *
         return TAGI_ERR_INVALID_ARG;
     const int rc = grouped_sizes(K, N, E, R, T, rows, K, param_update != 0);
     if (rc != TAGI_OK) return rc;
+    if (!grouped_scratch_ok(K, N, E, R, scratch)) return TAGI_ERR_INVALID_ARG;
     GroupedParams p = {};
+    p.scratch = static_cast<float *>(scratch);
     p.x0 = delta_mu, p.x1 = delta_var;
     p.offsets = offsets, p.rows = rows;
     p.K = K, p.N = N, p.E = E, p.R = R, p.T = T;

@@ -1,11 +1,13 @@
 // Linear layers grouped by expert: row r of expert e (offsets[e] <= r < offsets[e+1])
 // meets the weights [e][N][K]. gfx950.
+#include <algorithm>
 #include <cstdint>
 #include <type_traits>
 
 #include "tagi_activation.h"
 #include "tagi_grouped.h"
 #include "tagi_internal.h"
+#include "tagi_stream.h"
 
 namespace tagi {
 
@@ -120,7 +122,8 @@ __device__ __forceinline__ float operand(int o, float u, float v) {
 struct Tile {
     int e, m0, c0;      // expert, first output row, first output column
     int m_end, c_end;   // one past the last
-    int r0, red;        // DW: first row of the expert; length of the reduction
+    int r0, red;        // first element of the reduction (DW: row), their number
+    int part;           // which part of a divided reduction
 };
 
 // The tiles of a workgroup: XCD x (workgroups x, x + 8, ...) takes the x-th eighth of the tile
@@ -129,17 +132,29 @@ struct Tile {
 //            of an XCD share rows and columns in its L2
 //   DW: the same eighth of every expert's tiles, whatever its number of rows; an eighth of
 //            all experts' tiles in order where an expert has too few to divide
+// A divided reduction has all tiles once per part; the parts are whole units.
 template <int MODE>
 struct TileList {
     int tiles_m, tiles_c, lo, count;   // this XCD's part of the list
-    int per;                           // DW: tiles of it per expert, 0: a part of all tiles in order
+    int per;                           // DW: tiles of it per expert and part, 0: of all in order
     const int *prefix;                 // row tiles before every group (LDS)
+    // the part-th of p.splits parts of a reduction
+    static __device__ __forceinline__ void divide(const GroupedParams &p, Tile &t) {
+        if (p.splits == 1) return;
+        const int units = (t.red + TK - 1) / TK;
+        const int lo = (int)((long long)units * t.part / p.splits) * TK;
+        const int hi = (int)((long long)units * (t.part + 1) / p.splits) * TK;
+        t.red = min(hi, t.red) - lo;
+        t.r0 += lo;
+    }
     __device__ __forceinline__ bool get(const GroupedParams &p, int i, Tile &t) const {
         if (i >= count) return false;
         if (MODE == GROUPED_DW) {
             const int n = tiles_m * tiles_c;
             const int flat = lo + i;
-            t.e = per > 0 ? i / per : flat / n;
+            const int each = per > 0 ? i / per : flat / n;
+            t.e = each % p.E;
+            t.part = each / p.E;
             const int at = per > 0 ? lo + i % per : flat % n;
             t.m0 = at % tiles_m * TM;
             t.c0 = at / tiles_m * TM;
@@ -148,9 +163,11 @@ struct TileList {
             int end;
             group_rows(p.offsets, t.e, p.R, t.r0, end);
             t.red = end - t.r0;
+            divide(p, t);
             return true;
         }
-        const int at = lo + i;
+        t.part = (lo + i) / (tiles_m * tiles_c);
+        const int at = lo + i - t.part * tiles_m * tiles_c;
         const int band = at / (8 * tiles_c), in = at - band * 8 * tiles_c;
         const int height = min(8, tiles_m - band * 8);
         const int rt = band * 8 + in % height;
@@ -171,6 +188,7 @@ struct TileList {
         t.c_end = MODE == GROUPED_FWD ? p.N : p.K;
         t.r0 = 0;
         t.red = MODE == GROUPED_FWD ? p.K : p.N;
+        divide(p, t);
         return true;
     }
 };
@@ -218,8 +236,9 @@ struct SideK {
         fresh = true;
         gather = GATHER && p.rows != nullptr;
         const size_t first = gather ? 0 : ROWS ? (size_t)t.m0 : (size_t)t.e * p.N + t.c0;
-        q0 = (ROWS ? p.x0 : p.y0) + first * red;
-        q1 = (ROWS ? p.x1 : p.y1) + first * red;
+        const size_t from = first * (MODE == GROUPED_FWD ? p.K : p.N) + t.r0;
+        q0 = (ROWS ? p.x0 : p.y0) + from;
+        q1 = (ROWS ? p.x1 : p.y1) + from;
         first_row = u >> 3;
         last_row = (ROWS ? t.m_end - t.m0 : t.c_end - t.c0) - 1;
         if constexpr (GATHER) {
@@ -245,7 +264,7 @@ struct SideK {
                         dead |= 1u << i;
                     }
                 }
-                row[i] = (unsigned)s * (unsigned)red;
+                row[i] = (unsigned)s * (unsigned)(MODE == GROUPED_FWD ? p.K : p.N);
             }
         }
         b.left = red - k0;
@@ -311,7 +330,8 @@ struct SideM {
             q1 = p.x1 + (size_t)t.r0 * p.N;
         } else {
             ld = p.K;
-            q0 = p.y0 + (MODE == GROUPED_DZ ? (size_t)t.e * p.N * p.K : gather ? 0 : (size_t)t.r0 * p.K);
+            const size_t before = MODE == GROUPED_DZ ? (size_t)t.e * p.N + t.r0 : gather ? 0 : (size_t)t.r0;
+            q0 = p.y0 + before * p.K;
             q1 = q0;
         }
         // (columns beyond the last are computed and not stored; they only have to exist)
@@ -470,11 +490,11 @@ __global__ __launch_bounds__(TILE_THREADS) void grouped_tile_kernel(GroupedParam
         list.tiles_m = (p.N + TM - 1) / TM;
         const int n = list.tiles_m * list.tiles_c, x = blockIdx.x & 7;
         const bool shared = n >= 64;
-        const long long part = shared ? n : (long long)n * p.E;
+        const long long part = shared ? n : (long long)n * p.E * p.splits;
         list.lo = (int)(part * x / 8);
         list.count = (int)(part * (x + 1) / 8) - list.lo;
         list.per = shared ? list.count : 0;
-        if (shared) list.count *= p.E;
+        if (shared) list.count *= p.E * p.splits;
     } else {
         // one wave sums the row tiles of the groups
         if (tid < 64) {
@@ -497,7 +517,7 @@ __global__ __launch_bounds__(TILE_THREADS) void grouped_tile_kernel(GroupedParam
         }
         __syncthreads();
         list.tiles_m = prefix[p.E];
-        const long long total = (long long)list.tiles_m * list.tiles_c;
+        const long long total = (long long)list.tiles_m * list.tiles_c * p.splits;
         list.lo = (int)(total * (blockIdx.x & 7) / 8);
         list.count = (int)(total * ((blockIdx.x & 7) + 1) / 8) - list.lo;
     }
@@ -592,6 +612,7 @@ __global__ __launch_bounds__(TILE_THREADS) void grouped_tile_kernel(GroupedParam
                 reader_barrier();
             }
         }
+        float *out0 = p.out0 + t.part * p.part, *out1 = p.out1 + t.part * p.part;
         // register v of lane l: row 8 (v / 4) + 4 (l / 32) + v % 4, column l % 32
         if constexpr (!Shape::BK) {
             // the two column sub-tiles hold neighbouring columns
@@ -621,11 +642,11 @@ __global__ __launch_bounds__(TILE_THREADS) void grouped_tile_kernel(GroupedParam
                         const float2_any s0 = (float2_any){acc[0][x][0][v0 + v], acc[0][x][1][v0 + v]} * f[v];
                         const float2_any s1 = (float2_any){acc[1][x][0][v0 + v], acc[1][x][1][v0 + v]} * f[v] * f[v];
                         if (both) {
-                            *reinterpret_cast<float2_any *>(p.out0 + at) = s0;
-                            *reinterpret_cast<float2_any *>(p.out1 + at) = s1;
+                            *reinterpret_cast<float2_any *>(out0 + at) = s0;
+                            *reinterpret_cast<float2_any *>(out1 + at) = s1;
                         } else {
-                            p.out0[at] = s0[0];
-                            p.out1[at] = s1[0];
+                            out0[at] = s0[0];
+                            out1[at] = s1[0];
                         }
                     }
                     __builtin_amdgcn_sched_barrier(0);
@@ -647,45 +668,129 @@ __global__ __launch_bounds__(TILE_THREADS) void grouped_tile_kernel(GroupedParam
                         const int m = t.m0 + wm * 64 + x * 32 + 8 * (v >> 2) + 4 * (lane >> 5) + (v & 3);
                         if (m >= t.m_end) continue;
                         store_activated(p.act, acc[0][x][y][v] + b0, acc[1][x][y][v] + b1,
-                                        (size_t)m * p.N + c, p.out0, p.out1, p.out2);
+                                        (size_t)m * p.N + c, out0, out1, p.out2);
                     }
                 }
         }
     }
 }
 
-// Bias innovations of one expert's 64 columns: sixteen waves take every sixteenth row, four of
-// them in flight each; their sums are joined in wave order.
-constexpr int DB_WAVES = 16;
-__global__ __launch_bounds__(DB_WAVES * 64) void grouped_db_kernel(GroupedParams p) {
-    __shared__ float s[2][DB_WAVES][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int blocks = (p.N + 63) / 64, e = blockIdx.x / blocks;
-    const int n = (blockIdx.x - e * blocks) * 64 + lane, at_n = min(n, p.N - 1);
+// The parts of a divided reduction, in order, and what the tile kernel would have done with
+// their sums (p.x0, p.x1: the parts' outputs).
+constexpr int JOIN_ROWS = 8;
+template <int MODE>
+__global__ __launch_bounds__(TPB) void grouped_join_kernel(GroupedParams p) {
+    auto join = [&](size_t at, int valid, float (&m)[4], float (&v)[4]) {
+#pragma unroll
+        for (int c = 0; c < 4; c++) m[c] = v[c] = 0.f;
+#pragma unroll 4
+        for (int s = 0; s < p.splits; s++) {
+            float x[4], y[4];
+            load_group(p.x0 + s * p.part + at, valid, x);
+            load_group(p.x1 + s * p.part + at, valid, y);
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                m[c] += x[c];
+                v[c] += y[c];
+            }
+        }
+    };
+    auto scaled = [&](size_t at, int valid) {
+        float m[4], v[4], f[4] = {1.f, 1.f, 1.f, 1.f};
+        join(at, valid, m, v);
+        if (p.e0 != nullptr) load_group(p.e0 + at, valid, f);
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            m[c] *= f[c];
+            v[c] *= f[c] * f[c];
+        }
+        store_group(p.out0 + at, valid, m, false);
+        store_group(p.out1 + at, valid, v, false);
+    };
+    if (MODE == GROUPED_DW) {
+        const size_t groups = (p.part + 3) / 4;
+        for (size_t i = (size_t)blockIdx.x * TPB + threadIdx.x; i < groups; i += (size_t)gridDim.x * TPB)
+            scaled(4 * i, (int)min((size_t)4, p.part - 4 * i));
+        return;
+    }
+    // blockIdx.x: up to eight rows of one expert, the threads share their groups of four columns
+    int r0, end;
+    const int e = find_rows(p.offsets, p.E, p.R, JOIN_ROWS, blockIdx.x, r0, end);
+    if (e < 0) return;
+    const int cols = MODE == GROUPED_FWD ? p.N : p.K, groups = (cols + 3) / 4;
+    const int i = blockIdx.y * TPB + threadIdx.x, r = r0 + i / groups, g = i % groups;
+    if (i / groups >= JOIN_ROWS || r >= end) return;
+    const int valid = in_group(g, cols);
+    const size_t at = (size_t)r * cols + 4 * g;
+    if (MODE == GROUPED_DZ) {
+        scaled(at, valid);
+        return;
+    }
+    float m[4], v[4], b0[4] = {0.f, 0.f, 0.f, 0.f}, b1[4] = {0.f, 0.f, 0.f, 0.f};
+    join(at, valid, m, v);
+    if (p.e0 != nullptr) {
+        load_group(p.e0 + (size_t)e * p.N + 4 * g, valid, b0);
+        load_group(p.e1 + (size_t)e * p.N + 4 * g, valid, b1);
+    }
+#pragma unroll
+    for (int c = 0; c < 4; c++)
+        if (c < valid) store_activated(p.act, m[c] + b0[c], v[c] + b1[c], at + c, p.out0, p.out1, p.out2);
+}
+
+// Bias innovations of one expert's columns, 2^cw_log (up to sixteen) groups of four of them to
+// a workgroup: the other bits of the thread index are rows, four of them in flight each. The
+// row threads of a wave are joined by lane exchanges, the waves in their order.
+constexpr int DB_WAVES = 16, DB_GROUPS = 16;
+__global__ __launch_bounds__(DB_WAVES * 64) void grouped_db_kernel(GroupedParams p, int cw_log) {
+    __shared__ float s[2][DB_WAVES][DB_GROUPS * 4];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, cw = 1 << cw_log;
+    const int blocks = ((p.N + 3) / 4 + cw - 1) >> cw_log, e = blockIdx.x / blocks;
+    const int g = (blockIdx.x - e * blocks) * cw + (threadIdx.x & (cw - 1)), valid = in_group(g, p.N);
     int first, end;
     group_rows(p.offsets, e, p.R, first, end);
-    float m[4] = {0.f, 0.f, 0.f, 0.f}, v[4] = {0.f, 0.f, 0.f, 0.f};
-    int r = first + wave;
-    for (; r + 3 * DB_WAVES < end; r += 4 * DB_WAVES)
+    float m[4][4], v[4][4];
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const size_t at = (size_t)(r + i * DB_WAVES) * p.N + at_n;
-            m[i] += p.x0[at];
-            v[i] += p.x1[at];
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int c = 0; c < 4; c++) m[i][c] = v[i][c] = 0.f;
+    const int step = (DB_WAVES * 64) >> cw_log;
+    auto add = [&](int r, int i) {
+        float x[4], y[4];
+        load_group(p.x0 + (size_t)r * p.N + 4 * g, valid, x);
+        load_group(p.x1 + (size_t)r * p.N + 4 * g, valid, y);
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            m[i][c] += x[c];
+            v[i][c] += y[c];
         }
-    for (; r < end; r += DB_WAVES) {
-        m[0] += p.x0[(size_t)r * p.N + at_n];
-        v[0] += p.x1[(size_t)r * p.N + at_n];
+    };
+    if (valid > 0) {
+        long long r = first + (threadIdx.x >> cw_log);
+        for (; r + 3 * step < end; r += 4 * step)
+#pragma unroll
+            for (int i = 0; i < 4; i++) add((int)r + i * step, i);
+        for (; r < end; r += step) add((int)r, 0);
     }
-    s[0][wave][lane] = (m[0] + m[1]) + (m[2] + m[3]);
-    s[1][wave][lane] = (v[0] + v[1]) + (v[2] + v[3]);
+#pragma unroll
+    for (int c = 0; c < 4; c++) {
+        float sm = (m[0][c] + m[1][c]) + (m[2][c] + m[3][c]), sv = (v[0][c] + v[1][c]) + (v[2][c] + v[3][c]);
+        for (int off = 32; off >= cw; off >>= 1) {
+            sm += __shfl_xor(sm, off, 64);
+            sv += __shfl_xor(sv, off, 64);
+        }
+        if (lane < cw) {
+            s[0][wave][4 * lane + c] = sm;
+            s[1][wave][4 * lane + c] = sv;
+        }
+    }
     __syncthreads();
-    if (wave != 0 || n >= p.N) return;
+    const int n = (blockIdx.x - e * blocks) * cw * 4 + threadIdx.x;
+    if (threadIdx.x >= 4 * cw || n >= p.N) return;
     float sm = 0.f, sv = 0.f;
 #pragma unroll
     for (int w = 0; w < DB_WAVES; w++) {
-        sm += s[0][w][lane];
-        sv += s[1][w][lane];
+        sm += s[0][w][threadIdx.x];
+        sv += s[1][w][threadIdx.x];
     }
     const size_t at = (size_t)e * p.N + n;
     const float vb = p.e1[at];
@@ -708,6 +813,36 @@ hipError_t tile_launch(const GroupedParams &p, long long tiles, hipStream_t stre
     return hipGetLastError();
 }
 
+// How a call runs on the tiles: parts of the reduction, and the time in us that this is
+// expected to take.
+struct TilePlan {
+    long long tiles;
+    int splits;
+    double us;
+};
+constexpr int MAX_SPLITS = 16;
+
+TilePlan plan_tiles(GroupedMode mode, int K, int N, int E, int R) {
+    const long long used = E < R ? E : R;
+    const long long cols = mode == GROUPED_FWD ? N : K;
+    // (tiles as they come: a part tile for most experts)
+    const long long row_tiles = std::max(R / TM + used / 2, used);
+    const long long tiles = mode == GROUPED_DW ? (long long)ceil_div(K, TM) * ceil_div(N, TM) * E
+                                               : row_tiles * ceil_div((int)cols, TM);
+    const double out = mode == GROUPED_DW ? (double)E * N * K : (double)R * cols;
+    const int red = mode == GROUPED_FWD ? K : mode == GROUPED_DZ ? N : (int)(R / used);
+    const int units = ceil_div(red, TK);
+    const double unit_us = mode == GROUPED_FWD ? 2.6 : 1.75;
+    const double room = (double)grouped_scratch_floats(K, N, E, R);
+    TilePlan best = {tiles, 1, 12 + unit_us * ((tiles + num_cu() - 1) / num_cu()) * units};
+    // four units to a part at least; the parts are written and read once more
+    for (int s = 2; s <= MAX_SPLITS && tiles * s <= num_cu() && units / s >= 4 && 2 * out * s <= room; s++) {
+        const double us = 18 + unit_us * ceil_div(units, s) + 16 * out * s / 4e6;
+        if (us < best.us) best = {tiles, s, us};
+    }
+    return best;
+}
+
 // Which kernels a call goes to. Up to sixteen rows per expert on average the weights are what
 // takes the time, and the kernels for few rows read them once (64 rows, 16 experts of 2048 ->
 // 4096: 202 against 497 us). Beyond that those also win where the tiles are too few for the
@@ -726,46 +861,73 @@ hipError_t tile_launch(const GroupedParams &p, long long tiles, hipStream_t stre
 bool streams(GroupedMode mode, const GroupedParams &p) {
     // (its grid: one workgroup per sixteen outputs of every group of rows)
     const long long used = p.E < p.R ? p.E : p.R;
-    const long long cols = mode == GROUPED_FWD ? p.N : p.K, red = mode == GROUPED_FWD ? p.K : p.N;
+    const long long cols = mode == GROUPED_FWD ? p.N : p.K;
     if (cols * (p.R / 16 + used) >= 1LL << 26) return false;
     if ((long long)p.R <= 16LL * p.E) return true;
     if (mode == GROUPED_DW) return false;
-    // (tiles as they come: a part tile for most experts)
-    const long long row_tiles = p.R / TM + used / 2;
-    const long long tiles = (row_tiles > used ? row_tiles : used) * ceil_div((int)cols, TM);
-    const long long rounds = (tiles + num_cu() - 1) / num_cu();
     const double groups = p.R / 32 + 0.5 * used;
     const double rows_us = 8 + (mode == GROUPED_FWD ? 3.3e-6 : 1.6e-6) * groups * p.N * p.K;
-    const double tile_us = 12 + (mode == GROUPED_FWD ? 2.6 : 1.75) * rounds * ((red + TK - 1) / TK);
-    return rows_us < tile_us;
+    return rows_us < plan_tiles(mode, p.K, p.N, p.E, p.R).us;
 }
 
 }  // namespace
 
-hipError_t launch_grouped(GroupedMode mode, const GroupedParams &p, hipStream_t stream) {
+size_t grouped_scratch_floats(int K, int N, int E, int R) {
+    // the few-rows kernels need none
+    if (K < 4 || N < 4 || (g_grouped_rows < 0 ? (long long)R <= 16LL * E : g_grouped_rows != 0)) return 0;
+    // parts of two outputs: no more parts of tiles than CUs, MAX_SPLITS parts
+    const double outputs = std::max((double)R * std::max(K, N), (double)E * K * N);
+    return (size_t)(2 * std::min((double)num_cu() * TM * TM, MAX_SPLITS * outputs));
+}
+
+hipError_t launch_grouped(GroupedMode mode, const GroupedParams &params, hipStream_t stream) {
+    GroupedParams p = params;
     // 16-byte loads are moved to stay inside their row, so a row holds four elements at least
     const bool vec = p.K >= 4 && p.N >= 4;
     if (!vec || (g_grouped_rows >= 0 ? g_grouped_rows != 0 : streams(mode, p)))
         return launch_grouped_rows(mode, p, vec, stream);
-    // row tiles over all groups: every group ends with at most one part tile
-    const long long row_tiles = p.R / TM + (p.E < p.R ? p.E : p.R);
+    const TilePlan plan = plan_tiles(mode, p.K, p.N, p.E, p.R);
+    const int cols = mode == GROUPED_FWD ? p.N : p.K;
+    p.splits = plan.splits;
+    p.part = 0;
+    GroupedParams join = p;
+    if (p.splits > 1) {
+        join.part = p.part = mode == GROUPED_DW ? (size_t)p.E * p.N * p.K : (size_t)p.R * cols;
+        join.x0 = p.out0 = p.scratch;
+        join.x1 = p.out1 = p.scratch + p.splits * p.part;
+        p.e0 = nullptr;
+        p.act = ACT_NONE;
+    }
     // byte offsets from a tile's first row fit 32 bits (K, N <= 2^22), those of gathered rows
     // while the activations have fewer than 2^30 elements
     const bool far = (p.rows != nullptr && (long long)p.T * p.K >= (1LL << 30)) || p.K > (1 << 22) || p.N > (1 << 22);
+    // row tiles over all groups: every group ends with at most one part tile
+    const long long row_tiles = p.R / TM + (p.E < p.R ? p.E : p.R);
+    const long long tiles = p.splits * (mode == GROUPED_DW ? plan.tiles : row_tiles * ceil_div(cols, TM));
     hipError_t e;
-    if (mode == GROUPED_FWD) {
-        const long long tiles = row_tiles * ceil_div(p.N, TM);
-        return far ? tile_launch<GROUPED_FWD, true>(p, tiles, stream) : tile_launch<GROUPED_FWD, false>(p, tiles, stream);
+    if (mode == GROUPED_FWD)
+        e = far ? tile_launch<GROUPED_FWD, true>(p, tiles, stream) : tile_launch<GROUPED_FWD, false>(p, tiles, stream);
+    else if (mode == GROUPED_DZ)
+        e = far ? tile_launch<GROUPED_DZ, true>(p, tiles, stream) : tile_launch<GROUPED_DZ, false>(p, tiles, stream);
+    else
+        e = far ? tile_launch<GROUPED_DW, true>(p, tiles, stream) : tile_launch<GROUPED_DW, false>(p, tiles, stream);
+    if (e != hipSuccess) return e;
+    if (p.splits > 1) {
+        const dim3 grid(p.R / JOIN_ROWS + (p.E < p.R ? p.E : p.R), ceil_div(JOIN_ROWS * ((cols + 3) / 4), TPB));
+        const dim3 flat((unsigned)std::min<size_t>((join.part / 4 + TPB) / TPB, 4 * num_cu()));
+        if (mode == GROUPED_FWD)
+            hipLaunchKernelGGL(grouped_join_kernel<GROUPED_FWD>, grid, dim3(TPB), 0, stream, join);
+        else if (mode == GROUPED_DZ)
+            hipLaunchKernelGGL(grouped_join_kernel<GROUPED_DZ>, grid, dim3(TPB), 0, stream, join);
+        else
+            hipLaunchKernelGGL(grouped_join_kernel<GROUPED_DW>, flat, dim3(TPB), 0, stream, join);
+        e = hipGetLastError();
     }
-    if (mode == GROUPED_DZ) {
-        const long long tiles = row_tiles * ceil_div(p.K, TM);
-        return far ? tile_launch<GROUPED_DZ, true>(p, tiles, stream) : tile_launch<GROUPED_DZ, false>(p, tiles, stream);
-    }
-    const long long tiles = (long long)ceil_div(p.K, TM) * ceil_div(p.N, TM) * p.E;
-    e = far ? tile_launch<GROUPED_DW, true>(p, tiles, stream) : tile_launch<GROUPED_DW, false>(p, tiles, stream);
-    if (e != hipSuccess || p.db0 == nullptr) return e;
-    hipLaunchKernelGGL(grouped_db_kernel, dim3((unsigned)ceil_div(p.N, 64) * p.E), dim3(DB_WAVES * 64), 0,
-                       stream, p);
+    if (e != hipSuccess || mode != GROUPED_DW || p.db0 == nullptr) return e;
+    int cw_log = 0;
+    while ((1 << cw_log) < DB_GROUPS && (4 << cw_log) < p.N) cw_log++;
+    hipLaunchKernelGGL(grouped_db_kernel, dim3((unsigned)ceil_div(ceil_div(p.N, 4), 1 << cw_log) * p.E),
+                       dim3(DB_WAVES * 64), 0, stream, p, cw_log);
     return hipGetLastError();
 }
 

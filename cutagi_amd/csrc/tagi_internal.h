@@ -350,7 +350,12 @@ struct GroupedParams {
     const int *offsets, *rows;
     int K, N, E, R, T, act;
     float *out0, *out1, *out2, *db0, *db1;
+    float *scratch;   // grouped_scratch_floats of them
+    int splits;       // set by launch_grouped: parts of the reduction,
+    size_t part;      // floats of one part's output
 };
+// never more for fewer rows
+size_t grouped_scratch_floats(int K, int N, int E, int R);
 // 0 / 1: always the tiled kernels / always those for few rows (tuning knob); -1: by size
 extern int g_grouped_rows;
 hipError_t launch_grouped(GroupedMode mode, const GroupedParams &p, hipStream_t stream);

@@ -468,6 +468,11 @@ def grouped_linear_fwd_act(mu_w, var_w, mu_b, var_b, mu_a, var_a, offsets, activ
                         out)
 
 
+def _grouped_scratch(like, K, N, E, R):
+    size = capi.grouped_linear_scratch(K, N, E, R)
+    return like.new_empty(size, dtype=torch.uint8) if size else None
+
+
 def _grouped_fwd(mu_w, var_w, mu_b, var_b, mu_a, var_a, offsets, rows, activation, out):
     _pair(mu_b, var_b, ("mu_b", "var_b"))
     T, K = _dims("mu_a", mu_a, 2)
@@ -488,7 +493,8 @@ def _grouped_fwd(mu_w, var_w, mu_b, var_b, mu_a, var_a, offsets, rows, activatio
         out = _new(mu_w, count, R, N)
     args = (mu_w.data_ptr(), var_w.data_ptr(), _at(mu_b), _at(var_b), mu_a.data_ptr(),
             var_a.data_ptr(), offsets.data_ptr(), _at(rows), K, N, E, R, T, int(mu_b is not None))
-    outs = [t.data_ptr() for t in out]
+    scratch = _grouped_scratch(mu_w, K, N, E, R)
+    outs = [_at(scratch)] + [t.data_ptr() for t in out]
     if activation is None:
         capi.check(capi.lib.tagi_grouped_linear_fwd(*args, *outs, _raw_stream(dev)))
     else:
@@ -526,10 +532,12 @@ def grouped_linear_bwd(mu_w, var_w, var_b, mu_a, jcb, delta_mu, delta_var, offse
         for i in (0, 2, 4):
             if wanted[i]:
                 out[i:i + 2] = _new(delta_mu, 2, *shapes[i])
+    scratch = _grouped_scratch(mu_w, K, N, E, R)
     capi.check(capi.lib.tagi_grouped_linear_bwd(
         mu_w.data_ptr(), var_w.data_ptr(), _at(var_b), mu_a.data_ptr(), _at(jcb),
         delta_mu.data_ptr(), delta_var.data_ptr(), offsets.data_ptr(), _at(rows), K, N, E, R, T,
-        int(bias), int(state_update), int(param_update), *[_at(t) for t in out], _raw_stream(dev)))
+        int(bias), int(state_update), int(param_update), _at(scratch), *[_at(t) for t in out],
+        _raw_stream(dev)))
     return tuple(t if w else None for w, t in zip(wanted, out))
 
 

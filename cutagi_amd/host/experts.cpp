@@ -1,6 +1,7 @@
 // LayerNorm and MixtureOfExperts: see experts.h.
 #include "experts.h"
 
+#include <algorithm>
 #include <cmath>
 
 #include "../../include/tagi_hip.h"
@@ -244,7 +245,7 @@ struct MixtureOfExpertsHip::Work {
     float *dmu_y, *dvar_y;                  // [T k][output]
     float *dmu_h, *dvar_h;                  // [T k][hidden]
     float *dmu_x, *dvar_x;                  // [T k][input]
-    void *scratch;                          // of the router
+    void *scratch;                          // of one call at a time
     size_t bytes;
 };
 
@@ -265,8 +266,12 @@ MixtureOfExpertsHip::Work MixtureOfExpertsHip::work(int batch) const {
     take(w.dmu_y, R * sizes.output), take(w.dvar_y, R * sizes.output);
     take(w.dmu_h, R * sizes.hidden), take(w.dvar_h, R * sizes.hidden);
     take(w.dmu_x, R * sizes.input), take(w.dvar_x, R * sizes.input);
-    size_t scratch = 0;
+    const int K = (int)sizes.input, H = (int)sizes.hidden, N = (int)sizes.output;
+    size_t scratch = 0, up = 0, down = 0;
     TAGI_OK_OR_THROW(tagi_moe_route_scratch(batch, sizes.experts, &scratch));
+    TAGI_OK_OR_THROW(tagi_grouped_linear_scratch(K, H, sizes.experts, (int)R, &up));
+    TAGI_OK_OR_THROW(tagi_grouped_linear_scratch(H, N, sizes.experts, (int)R, &down));
+    scratch = std::max(scratch, std::max(up, down));
     char *s = nullptr;
     take(s, (scratch + 3) / 4);
     w.scratch = s;
@@ -310,10 +315,11 @@ void MixtureOfExpertsHip::forward(BaseHiddenStates &input_states, BaseHiddenStat
                                     w.jcb_g, w.offsets, w.token, w.slot, stream));
     TAGI_OK_OR_THROW(tagi_grouped_linear_fwd_act(
         d_mu_w + up, d_var_w + up, b(d_mu_b, up_b), b(d_var_b, up_b), in->d_mu_a, in->d_var_a,
-        w.offsets, w.token, K, H, E, R, T, has_b, sizes.activation, w.mu_h, w.var_h, w.jcb_h, stream));
+        w.offsets, w.token, K, H, E, R, T, has_b, sizes.activation, w.scratch, w.mu_h, w.var_h,
+        w.jcb_h, stream));
     TAGI_OK_OR_THROW(tagi_grouped_linear_fwd(
         d_mu_w + down, d_var_w + down, b(d_mu_b, down_b), b(d_var_b, down_b), w.mu_h, w.var_h,
-        w.offsets, nullptr, H, N, E, R, R, has_b, w.mu_y, w.var_y, stream));
+        w.offsets, nullptr, H, N, E, R, R, has_b, w.scratch, w.mu_y, w.var_y, stream));
     TAGI_OK_OR_THROW(tagi_moe_combine_fwd(w.mu_g, w.var_g, w.mu_y, w.var_y, w.slot, T, k, R, N,
                                           out->d_mu_a, out->d_var_a, stream));
     last_batch = T;
@@ -351,12 +357,12 @@ void MixtureOfExpertsHip::backward(BaseDeltaStates &input_delta_states,
                                           w.dvar_s, stream));
     TAGI_OK_OR_THROW(tagi_grouped_linear_bwd(
         d_mu_w + down, d_var_w + down, b(d_var_b, down_b), w.mu_h, w.jcb_h, w.dmu_y, w.dvar_y, w.offsets,
-        nullptr, H, N, E, R, R, has_b, 1, params, w.dmu_h, w.dvar_h, d_delta_mu_w + down,
+        nullptr, H, N, E, R, R, has_b, 1, params, w.scratch, w.dmu_h, w.dvar_h, d_delta_mu_w + down,
         d_delta_var_w + down, b(d_delta_mu_b, down_b), b(d_delta_var_b, down_b), stream));
     if (states || params)
         TAGI_OK_OR_THROW(tagi_grouped_linear_bwd(
             d_mu_w + up, d_var_w + up, b(d_var_b, up_b), bwd->d_mu_a, nullptr, w.dmu_h, w.dvar_h,
-            w.offsets, w.token, K, H, E, R, T, has_b, states, params, w.dmu_x, w.dvar_x,
+            w.offsets, w.token, K, H, E, R, T, has_b, states, params, w.scratch, w.dmu_x, w.dvar_x,
             d_delta_mu_w + up, d_delta_var_w + up, b(d_delta_mu_b, up_b), b(d_delta_var_b, up_b), stream));
     // the router's share of the state innovations, not yet times the Jacobian, then both
     TAGI_OK_OR_THROW(tagi_linear_bwd(

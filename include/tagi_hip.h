@@ -485,15 +485,21 @@ int tagi_layernorm_bwd(const float *mu_w, const float *var_w, const float *var_b
  * int[R]) row r takes its activations from row rows[r] of the T rows of mu_a / var_a, so a
  * token that several experts see is stored once; an entry outside 0..T-1 stands for a row
  * of zeros. Offsets outside 0..R are moved to its ends. E <= 1024, K and N <= 2^24, with
- * rows T K < 2^32 (TAGI_ERR_UNSUPPORTED beyond). No workspace: calls may be captured and may overlap. No counterpart in the
- * reference, which has one Linear per layer; the arithmetic of a group is
+ * rows T K < 2^32 (TAGI_ERR_UNSUPPORTED beyond). The same bits every call. No counterpart in
+ * the reference, which has one Linear per layer; the arithmetic of a group is
  * tagi_linear_fwd's and tagi_linear_bwd's. */
+
+/* Bytes of device memory that any of the calls below needs as scratch at these sizes (on the
+ * current device; may be 0, and is never more for fewer rows). Host only. The caller owns it,
+ * 16-byte aligned; calls may be captured, and may overlap unless they share it. */
+int tagi_grouped_linear_scratch(int K, int N, int E, int R, size_t *bytes /* host, out */);
 
 /* mu_z, var_z [R][N] */
 int tagi_grouped_linear_fwd(const float *mu_w, const float *var_w, const float *mu_b,
                             const float *var_b, const float *mu_a, const float *var_a,
                             const int *offsets, const int *rows /* may be NULL */,
                             int K, int N, int E, int R, int T, int bias,
+                            void *scratch /* may be NULL where that is 0 */,
                             float *mu_z, float *var_z, void *stream);
 
 /* With the activation that follows (TAGI_ACT_*), as tagi_linear_fwd_act. */
@@ -501,8 +507,8 @@ int tagi_grouped_linear_fwd_act(const float *mu_w, const float *var_w, const flo
                                 const float *var_b, const float *mu_a, const float *var_a,
                                 const int *offsets, const int *rows /* may be NULL */,
                                 int K, int N, int E, int R, int T, int bias,
-                                int activation, float *mu_out, float *var_out,
-                                float *jcb_out, void *stream);
+                                int activation, void *scratch, float *mu_out,
+                                float *var_out, float *jcb_out, void *stream);
 
 /* All of the backward pass: with state_update the innovations of every ROW, delta_mu_z /
  * delta_var_z [R][K] (jcb [R][K], NULL: one everywhere; tagi_moe_gather_bwd adds them up
@@ -513,9 +519,10 @@ int tagi_grouped_linear_bwd(const float *mu_w, const float *var_w, const float *
                             const float *delta_mu, const float *delta_var,
                             const int *offsets, const int *rows /* may be NULL */,
                             int K, int N, int E, int R, int T, int bias,
-                            int state_update, int param_update, float *delta_mu_z,
-                            float *delta_var_z, float *delta_mu_w, float *delta_var_w,
-                            float *delta_mu_b, float *delta_var_b, void *stream);
+                            int state_update, int param_update, void *scratch,
+                            float *delta_mu_z, float *delta_var_z, float *delta_mu_w,
+                            float *delta_var_w, float *delta_mu_b, float *delta_var_b,
+                            void *stream);
 
 /* ---- mixture of experts --------------------------------------------------------------- */
 /* The router's choice. mu_s / var_s [T][E]: the router layer's outputs. Every token takes

@@ -39,26 +39,52 @@ def test_layernorm_refuses():
 
 def test_grouped_linear_refuses():
     capi, L = _lib()
-    fwd = [one] * 8 + [8, 8, 4, 16, 16, 1] + [one] * 2 + [None]
-    for i in [0, 1, 2, 3, 4, 5, 6, 14, 15]:
+    fwd = [one] * 8 + [8, 8, 4, 16, 16, 1] + [one] * 3 + [None]
+    for i in [0, 1, 2, 3, 4, 5, 6, 15, 16]:
         assert L.tagi_grouped_linear_fwd(*_without(fwd, i)) == capi.ERR_INVALID_ARG
     for i in [8, 9, 10, 11, 12]:
         for bad in (0, -3):
             assert L.tagi_grouped_linear_fwd(*_without(fwd, i, bad)) == capi.ERR_INVALID_ARG
     assert L.tagi_grouped_linear_fwd(*_without(fwd, 10, 1025)) == capi.ERR_UNSUPPORTED
-    act = [one] * 8 + [8, 8, 4, 16, 16, 1, 1] + [one] * 3 + [None]
+    act = [one] * 8 + [8, 8, 4, 16, 16, 1, 1] + [one] * 4 + [None]
     for bad in (0, 3, -1):
         assert L.tagi_grouped_linear_fwd_act(*_without(act, 14, bad)) == capi.ERR_INVALID_ARG
-    assert L.tagi_grouped_linear_fwd_act(*_without(act, 17)) == capi.ERR_INVALID_ARG
-    bwd = [one] * 9 + [8, 8, 4, 16, 16, 1, 1, 1] + [one] * 6 + [None]
-    for i in [0, 1, 2, 3, 5, 6, 7] + list(range(17, 23)):
+    assert L.tagi_grouped_linear_fwd_act(*_without(act, 18)) == capi.ERR_INVALID_ARG
+    bwd = [one] * 9 + [8, 8, 4, 16, 16, 1, 1, 1] + [one] * 7 + [None]
+    for i in [0, 1, 2, 3, 5, 6, 7] + list(range(18, 24)):
         assert L.tagi_grouped_linear_bwd(*_without(bwd, i)) == capi.ERR_INVALID_ARG
     assert L.tagi_grouped_linear_bwd(*_without(bwd, 11, 2000)) == capi.ERR_UNSUPPORTED
     # more tiles than a launch holds
-    huge = [one] * 8 + [1 << 30, 1 << 30, 1024, 16, 16, 1] + [one] * 2 + [None]
+    huge = [one] * 8 + [1 << 30, 1 << 30, 1024, 16, 16, 1] + [one] * 3 + [None]
     assert L.tagi_grouped_linear_fwd(*huge) == capi.ERR_UNSUPPORTED
-    huge = [one] * 9 + [1 << 30, 1 << 30, 1024, 16, 16, 1, 0, 1] + [one] * 6 + [None]
+    huge = [one] * 9 + [1 << 30, 1 << 30, 1024, 16, 16, 1, 0, 1] + [one] * 7 + [None]
     assert L.tagi_grouped_linear_bwd(*huge) == capi.ERR_UNSUPPORTED
+    # scratch that is needed and missing, or not 16-byte aligned
+    size = capi.grouped_linear_scratch(256, 128, 4, 400)
+    assert size > 0
+    for scratch in (None, odd):
+        call = _without(_without(fwd, 11, 400), 14, scratch)
+        assert L.tagi_grouped_linear_fwd(*call) == capi.ERR_INVALID_ARG
+        call = _without(_without(bwd, 12, 400), 17, scratch)
+        assert L.tagi_grouped_linear_bwd(*call) == capi.ERR_INVALID_ARG
+
+
+def test_grouped_linear_scratch():
+    capi, L = _lib()
+    size = ctypes.c_size_t(0)
+    for bad in ((0, 8, 4, 16), (8, -1, 4, 16), (8, 8, 0, 16), (8, 8, 4, 0)):
+        assert L.tagi_grouped_linear_scratch(*bad, ctypes.byref(size)) == capi.ERR_INVALID_ARG
+    assert L.tagi_grouped_linear_scratch(8, 8, 4, 16, None) == capi.ERR_INVALID_ARG
+    assert L.tagi_grouped_linear_scratch(8, 8, 1025, 16, ctypes.byref(size)) == capi.ERR_UNSUPPORTED
+    assert capi.grouped_linear_scratch(4096, 4096, 8, 8) == 0
+    # what is held for a batch does for every smaller one
+    for K, N, E in ((64, 48, 4), (2048, 4096, 8), (3, 100, 2), (515, 20, 2), (4100, 300, 1)):
+        held = 0
+        for R in list(range(1, 300)) + [1000, 4096, 8192, 100000, 1 << 20]:
+            now = capi.grouped_linear_scratch(K, N, E, R)
+            assert now >= held
+            held = now
+    assert held < 1 << 26
 
 
 def test_router_refuses():

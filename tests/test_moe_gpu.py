@@ -50,6 +50,12 @@ GROUPS = [
     ([130, 700, 0, 450], 4100, 72, 300, 5),
     ([130, 700, 0, 450], 72, 4100, None, 5),
     ([33, 90, 40], 1300, 1284, 100, 0),
+    # long reductions of few tiles, taken in parts: of every pass, and parts of no rows
+    ([700, 0, 300, 5], 523, 20, None, 3),
+    ([40, 0, 200, 31], 2051, 37, 90, 0),
+    ([150, 90], 70, 2050, None, 7),
+    ([3000, 130], 36, 132, 77, 0),
+    ([0, 1500, 0], 129, 6, 2, 100),
 ]
 GUARD = 12345.0
 
@@ -88,7 +94,7 @@ def test_grouped_linear(kernel_choice, sizes, K, N, tokens, tail, bias):
 
 
 @pytest.mark.parametrize("sizes,K,N,tokens", [([5, 0, 20], 96, 64, None), ([70, 130], 132, 260, 40),
-                                              ([2, 1], 256, 128, 2)])
+                                              ([2, 1], 256, 128, 2), ([300, 0, 90], 600, 130, 70)])
 def test_parts_and_the_same_bits_every_call(kernel_choice, sizes, K, N, tokens):
     import torch
     import cutagi_amd.functional as F
@@ -106,7 +112,7 @@ def test_parts_and_the_same_bits_every_call(kernel_choice, sizes, K, N, tokens):
 
 
 @pytest.mark.parametrize("activation", ["relu", "mixture_relu"])
-@pytest.mark.parametrize("sizes,K,N", [([3, 0, 2], 64, 40), ([90, 40], 72, 130)])
+@pytest.mark.parametrize("sizes,K,N", [([3, 0, 2], 64, 40), ([90, 40], 72, 130), ([90, 0, 41], 777, 66)])
 def test_fused_activation_is_the_activation_of_the_layer(kernel_choice, activation, sizes, K, N):
     import torch
     import cutagi_amd.functional as F
@@ -122,7 +128,8 @@ def test_fused_activation_is_the_activation_of_the_layer(kernel_choice, activati
         C.check(_host(g), _host(w), 16 * C.U * _host(scale), name)
 
 
-@pytest.mark.parametrize("sizes,K,N", [([5, 9], 64, 32), ([100, 31], 128, 132), ([140, 150], 260, 256)])
+@pytest.mark.parametrize("sizes,K,N", [([5, 9], 64, 32), ([100, 31], 128, 132), ([140, 150], 260, 256),
+                                       ([300, 270], 520, 518)])
 def test_arrays_that_are_not_16_byte_aligned(kernel_choice, sizes, K, N):
     import torch
     import cutagi_amd.functional as F
