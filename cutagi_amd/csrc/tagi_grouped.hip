@@ -7,7 +7,6 @@
 #include "tagi_activation.h"
 #include "tagi_grouped.h"
 #include "tagi_internal.h"
-#include "tagi_stream.h"
 
 namespace tagi {
 
@@ -675,66 +674,52 @@ __global__ __launch_bounds__(TILE_THREADS) void grouped_tile_kernel(GroupedParam
     }
 }
 
+// The kernels below take four columns to a thread; the last four of a row start at its end less
+// four, so that some columns are taken twice, with the same result.
+__device__ __forceinline__ void add4(float4_any &sum, const float *p) {
+    sum += *reinterpret_cast<const float4_any *>(p);
+}
+
 // The parts of a divided reduction, in order, and what the tile kernel would have done with
 // their sums (p.x0, p.x1: the parts' outputs).
 constexpr int JOIN_ROWS = 8;
 template <int MODE>
 __global__ __launch_bounds__(TPB) void grouped_join_kernel(GroupedParams p) {
-    auto join = [&](size_t at, int valid, float (&m)[4], float (&v)[4]) {
-#pragma unroll
-        for (int c = 0; c < 4; c++) m[c] = v[c] = 0.f;
-#pragma unroll 4
-        for (int s = 0; s < p.splits; s++) {
-            float x[4], y[4];
-            load_group(p.x0 + s * p.part + at, valid, x);
-            load_group(p.x1 + s * p.part + at, valid, y);
-#pragma unroll
-            for (int c = 0; c < 4; c++) {
-                m[c] += x[c];
-                v[c] += y[c];
-            }
-        }
-    };
-    auto scaled = [&](size_t at, int valid) {
-        float m[4], v[4], f[4] = {1.f, 1.f, 1.f, 1.f};
-        join(at, valid, m, v);
-        if (p.e0 != nullptr) load_group(p.e0 + at, valid, f);
-#pragma unroll
-        for (int c = 0; c < 4; c++) {
-            m[c] *= f[c];
-            v[c] *= f[c] * f[c];
-        }
-        store_group(p.out0 + at, valid, m, false);
-        store_group(p.out1 + at, valid, v, false);
-    };
+    size_t at, bias = 0;
     if (MODE == GROUPED_DW) {
-        const size_t groups = (p.part + 3) / 4;
-        for (size_t i = (size_t)blockIdx.x * TPB + threadIdx.x; i < groups; i += (size_t)gridDim.x * TPB)
-            scaled(4 * i, (int)min((size_t)4, p.part - 4 * i));
-        return;
+        const size_t i = 4 * ((size_t)blockIdx.x * TPB + threadIdx.x);
+        if (i >= p.part) return;
+        at = min(i, p.part - 4);
+    } else {
+        // blockIdx.x: up to eight rows of one expert, the threads share their groups of columns
+        int r0, end;
+        const int e = find_rows(p.offsets, p.E, p.R, JOIN_ROWS, blockIdx.x, r0, end);
+        if (e < 0) return;
+        const int cols = MODE == GROUPED_FWD ? p.N : p.K, groups = (cols + 3) / 4;
+        const int i = blockIdx.y * TPB + threadIdx.x, r = r0 + i / groups;
+        if (i / groups >= JOIN_ROWS || r >= end) return;
+        const int c = min(4 * (i % groups), cols - 4);
+        at = (size_t)r * cols + c;
+        bias = (size_t)e * cols + c;
     }
-    // blockIdx.x: up to eight rows of one expert, the threads share their groups of four columns
-    int r0, end;
-    const int e = find_rows(p.offsets, p.E, p.R, JOIN_ROWS, blockIdx.x, r0, end);
-    if (e < 0) return;
-    const int cols = MODE == GROUPED_FWD ? p.N : p.K, groups = (cols + 3) / 4;
-    const int i = blockIdx.y * TPB + threadIdx.x, r = r0 + i / groups, g = i % groups;
-    if (i / groups >= JOIN_ROWS || r >= end) return;
-    const int valid = in_group(g, cols);
-    const size_t at = (size_t)r * cols + 4 * g;
-    if (MODE == GROUPED_DZ) {
-        scaled(at, valid);
-        return;
+    float4_any m = {0.f, 0.f, 0.f, 0.f}, v = {0.f, 0.f, 0.f, 0.f}, f = {1.f, 1.f, 1.f, 1.f};
+    if (MODE != GROUPED_FWD && p.e0 != nullptr) f = *reinterpret_cast<const float4_any *>(p.e0 + at);
+#pragma unroll 4
+    for (int s = 0; s < p.splits; s++) {
+        add4(m, p.x0 + s * p.part + at);
+        add4(v, p.x1 + s * p.part + at);
     }
-    float m[4], v[4], b0[4] = {0.f, 0.f, 0.f, 0.f}, b1[4] = {0.f, 0.f, 0.f, 0.f};
-    join(at, valid, m, v);
-    if (p.e0 != nullptr) {
-        load_group(p.e0 + (size_t)e * p.N + 4 * g, valid, b0);
-        load_group(p.e1 + (size_t)e * p.N + 4 * g, valid, b1);
-    }
+    if (MODE == GROUPED_FWD) {
+        if (p.e0 != nullptr) {
+            add4(m, p.e0 + bias);
+            add4(v, p.e1 + bias);
+        }
 #pragma unroll
-    for (int c = 0; c < 4; c++)
-        if (c < valid) store_activated(p.act, m[c] + b0[c], v[c] + b1[c], at + c, p.out0, p.out1, p.out2);
+        for (int c = 0; c < 4; c++) store_activated(p.act, m[c], v[c], at + c, p.out0, p.out1, p.out2);
+        return;
+    }
+    *reinterpret_cast<float4_any *>(p.out0 + at) = m * f;
+    *reinterpret_cast<float4_any *>(p.out1 + at) = v * f * f;
 }
 
 // Bias innovations of one expert's columns, 2^cw_log (up to sixteen) groups of four of them to
@@ -745,35 +730,31 @@ __global__ __launch_bounds__(DB_WAVES * 64) void grouped_db_kernel(GroupedParams
     __shared__ float s[2][DB_WAVES][DB_GROUPS * 4];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, cw = 1 << cw_log;
     const int blocks = ((p.N + 3) / 4 + cw - 1) >> cw_log, e = blockIdx.x / blocks;
-    const int g = (blockIdx.x - e * blocks) * cw + (threadIdx.x & (cw - 1)), valid = in_group(g, p.N);
+    const int c0 = (blockIdx.x - e * blocks) * cw * 4;
     int first, end;
     group_rows(p.offsets, e, p.R, first, end);
-    float m[4][4], v[4][4];
+    float4_any m[4], v[4];
 #pragma unroll
-    for (int i = 0; i < 4; i++)
-#pragma unroll
-        for (int c = 0; c < 4; c++) m[i][c] = v[i][c] = 0.f;
+    for (int i = 0; i < 4; i++) m[i] = v[i] = (float4_any){0.f, 0.f, 0.f, 0.f};
     const int step = (DB_WAVES * 64) >> cw_log;
-    auto add = [&](int r, int i) {
-        float x[4], y[4];
-        load_group(p.x0 + (size_t)r * p.N + 4 * g, valid, x);
-        load_group(p.x1 + (size_t)r * p.N + 4 * g, valid, y);
+    const size_t col = min(c0 + 4 * ((int)threadIdx.x & (cw - 1)), p.N - 4);
+    const float *x = p.x0 + col, *y = p.x1 + col;
+    long long r = first + (threadIdx.x >> cw_log);
+    for (; r + 3 * step < end; r += 4 * step)
 #pragma unroll
-        for (int c = 0; c < 4; c++) {
-            m[i][c] += x[c];
-            v[i][c] += y[c];
+        for (int i = 0; i < 4; i++) {
+            add4(m[i], x + (r + i * step) * p.N);
+            add4(v[i], y + (r + i * step) * p.N);
         }
-    };
-    if (valid > 0) {
-        long long r = first + (threadIdx.x >> cw_log);
-        for (; r + 3 * step < end; r += 4 * step)
-#pragma unroll
-            for (int i = 0; i < 4; i++) add((int)r + i * step, i);
-        for (; r < end; r += step) add((int)r, 0);
+    for (; r < end; r += step) {
+        add4(m[0], x + r * p.N);
+        add4(v[0], y + r * p.N);
     }
+    m[0] = (m[0] + m[1]) + (m[2] + m[3]);
+    v[0] = (v[0] + v[1]) + (v[2] + v[3]);
 #pragma unroll
     for (int c = 0; c < 4; c++) {
-        float sm = (m[0][c] + m[1][c]) + (m[2][c] + m[3][c]), sv = (v[0][c] + v[1][c]) + (v[2][c] + v[3][c]);
+        float sm = m[0][c], sv = v[0][c];
         for (int off = 32; off >= cw; off >>= 1) {
             sm += __shfl_xor(sm, off, 64);
             sv += __shfl_xor(sv, off, 64);
@@ -784,15 +765,15 @@ __global__ __launch_bounds__(DB_WAVES * 64) void grouped_db_kernel(GroupedParams
         }
     }
     __syncthreads();
-    const int n = (blockIdx.x - e * blocks) * cw * 4 + threadIdx.x;
-    if (threadIdx.x >= 4 * cw || n >= p.N) return;
+    const int t = threadIdx.x, want = c0 + (t & ~3);
+    if (t >= 4 * cw || want >= p.N) return;
     float sm = 0.f, sv = 0.f;
 #pragma unroll
     for (int w = 0; w < DB_WAVES; w++) {
-        sm += s[0][w][threadIdx.x];
-        sv += s[1][w][threadIdx.x];
+        sm += s[0][w][t];
+        sv += s[1][w][t];
     }
-    const size_t at = (size_t)e * p.N + n;
+    const size_t at = (size_t)e * p.N + min(want, p.N - 4) + (t & 3);
     const float vb = p.e1[at];
     p.db0[at] = vb * sm;
     p.db1[at] = vb * vb * sv;
@@ -814,7 +795,9 @@ hipError_t tile_launch(const GroupedParams &p, long long tiles, hipStream_t stre
 }
 
 // How a call runs on the tiles: parts of the reduction, and the time in us that this is
-// expected to take.
+// expected to take. Few tiles of long reductions leave most of the chip idle: taken in parts /
+// in one piece, 8000 rows of 4096 -> 128: forward 158 / 367 us; 6826 rows, 2 experts of 529 ->
+// 20: weight backward 42 / 350 us.
 struct TilePlan {
     long long tiles;
     int splits;
@@ -832,12 +815,13 @@ TilePlan plan_tiles(GroupedMode mode, int K, int N, int E, int R) {
     const double out = mode == GROUPED_DW ? (double)E * N * K : (double)R * cols;
     const int red = mode == GROUPED_FWD ? K : mode == GROUPED_DZ ? N : (int)(R / used);
     const int units = ceil_div(red, TK);
-    const double unit_us = mode == GROUPED_FWD ? 2.6 : 1.75;
+    // (more where an expert's weights pass through one row of tiles only, all from memory)
+    const double unit_us = (mode == GROUPED_FWD ? 2.6 : 1.75) * (mode != GROUPED_DW && row_tiles <= used ? 1.4 : 1);
     const double room = (double)grouped_scratch_floats(K, N, E, R);
     TilePlan best = {tiles, 1, 12 + unit_us * ((tiles + num_cu() - 1) / num_cu()) * units};
     // four units to a part at least; the parts are written and read once more
     for (int s = 2; s <= MAX_SPLITS && tiles * s <= num_cu() && units / s >= 4 && 2 * out * s <= room; s++) {
-        const double us = 18 + unit_us * ceil_div(units, s) + 16 * out * s / 4e6;
+        const double us = 30 + unit_us * ceil_div(units, s) + 16 * out * s / 4e6;
         if (us < best.us) best = {tiles, s, us};
     }
     return best;
@@ -845,19 +829,26 @@ TilePlan plan_tiles(GroupedMode mode, int K, int N, int E, int R) {
 
 // Which kernels a call goes to. Up to sixteen rows per expert on average the weights are what
 // takes the time, and the kernels for few rows read them once (64 rows, 16 experts of 2048 ->
-// 4096: 202 against 497 us). Beyond that those also win where the tiles are too few for the
+// 4096: 180 against 497 us). Beyond that those also win where the tiles are too few for the
 // chip, because their groups of 32 rows by 16 (forward) or 64 (state backward) outputs are
-// many more. Their time in us is about 8 + 3.3e-6 (1.6e-6) per group, N and K; that of the
-// tiles 12 + 2.6 (1.75) per round of tiles and 32 reduction elements. Measured, few rows / tiles:
-//   forward         777 rows,  6 experts,  301 ->  415   24 /  46 us
-//                   512        8          1024 -> 1024   78 / 103
-//                   256        4          2048 ->  512   51 / 183
-//                  2048        8           512 ->  512   87 /  63
-//                  1024        8          2048 -> 2048  495 / 227
+// many more, and where the tiles would be mostly empty. Measured, few rows / tiles, and the
+// two formulas were fitted to these (us):
+//   forward         777 rows,  6 experts,  301 ->  415   15 /  45
+//                   192        8          2048 -> 4096  183 / 260
+//                   256        8          2048 -> 4096  264 / 265
+//                   512        8          2048 -> 4096  440 / 275
+//                   512        8          1024 -> 1024   61 /  57
+//                   256        4          2048 ->  512   49 /  42
+//                  2048        8           512 ->  512   58 /  62
+//                  1024        8          2048 -> 2048  393 / 216
+//                  8000        1          4096 ->  128  421 / 154
 //   state backward  777        6           301 ->  415   16 /  44
-//                  2048        8           512 ->  512   43 /  41
-//                  1024        8          2048 -> 2048  200 / 142
-// The weight backward has as many tiles as the weights: few rows only (777 rows: 104 / 29 us).
+//                   256        8          2048 -> 4096  155 / 177
+//                   512        8          2048 -> 4096  251 / 187
+//                  2048        8           512 ->  512   44 /  41
+//                  1024        8          2048 -> 2048  199 / 141
+//                  6826        2           529 ->   20   46 /  27
+// The weight backward has as many tiles as the weights: few rows only (777 rows: 89 / 31 us).
 bool streams(GroupedMode mode, const GroupedParams &p) {
     // (its grid: one workgroup per sixteen outputs of every group of rows)
     const long long used = p.E < p.R ? p.E : p.R;
@@ -866,7 +857,8 @@ bool streams(GroupedMode mode, const GroupedParams &p) {
     if ((long long)p.R <= 16LL * p.E) return true;
     if (mode == GROUPED_DW) return false;
     const double groups = p.R / 32 + 0.5 * used;
-    const double rows_us = 8 + (mode == GROUPED_FWD ? 3.3e-6 : 1.6e-6) * groups * p.N * p.K;
+    const double rows_us = mode == GROUPED_FWD ? 8 + 2.4e-6 * groups * p.N * p.K
+                                               : 8 + groups * (1.3e-6 * p.N * p.K + 0.02 * ceil_div(p.K, 64));
     return rows_us < plan_tiles(mode, p.K, p.N, p.E, p.R).us;
 }
 
@@ -914,7 +906,7 @@ hipError_t launch_grouped(GroupedMode mode, const GroupedParams &params, hipStre
     if (e != hipSuccess) return e;
     if (p.splits > 1) {
         const dim3 grid(p.R / JOIN_ROWS + (p.E < p.R ? p.E : p.R), ceil_div(JOIN_ROWS * ((cols + 3) / 4), TPB));
-        const dim3 flat((unsigned)std::min<size_t>((join.part / 4 + TPB) / TPB, 4 * num_cu()));
+        const dim3 flat((unsigned)((join.part / 4 + TPB) / TPB));
         if (mode == GROUPED_FWD)
             hipLaunchKernelGGL(grouped_join_kernel<GROUPED_FWD>, grid, dim3(TPB), 0, stream, join);
         else if (mode == GROUPED_DZ)

@@ -186,25 +186,25 @@ __global__ __launch_bounds__(WAVES * 64, NG == 1 && VEC ? 4 : 2) void rows_fwd_k
 }
 
 // ---------------------------------------------------------------------------
-// State backward, 64 inputs k of one expert. Lane (i, s) holds mu_w[n + 4 s + u][k0 + 4 i .. + 3]
-// for u = 0..3 (a load covers four weight rows of 256 bytes) and row i's innovations at
-// n + 4 s .. + 3: component t of step u meets component u of the innovations in an MFMA of
-// its own sum, D[i][j] = output k0 + 4 i + t of row j.
+// State backward, 16 C inputs k of one expert (C = 4, or 1 where few inputs and rows would leave
+// most of the chip idle). Lane (i, s) holds mu_w[n + 4 s + u][k0 + C i .. + C - 1] for u = 0..3
+// (C = 4: a load covers four weight rows of 256 bytes) and row i's innovations at n + 4 s .. + 3:
+// component t of step u meets component u of the innovations in an MFMA of its own sum,
+// D[i][j] = output k0 + C i + t of row j.
 // ---------------------------------------------------------------------------
-constexpr int DZ_WAVES = 8;
-
-template <int NG>
+template <int NG, int C>
 struct DzPiece {
-    floatx4 w[4], d0[NG], d1[NG];
+    float w[4][C];
+    floatx4 d0[NG], d1[NG];
 };
 
-template <int NG, bool VEC>
+template <int WAVES, int NG, int C, bool VEC>
 __device__ __forceinline__ void dz_rows(const GroupedParams &p, int e, int k0, int r0, int end,
-                                        float (*s)[16][65]) {
+                                        float (*s)[4 * C][65]) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int i = lane & 15, q = (lane >> 4) * 4, K = p.K, N = p.N;
     const float *w = p.y0 + (size_t)e * N * K;
-    const int k = k0 + 4 * i;
+    const int k = k0 + C * i;
     const float *d0[NG], *d1[NG];
 #pragma unroll
     for (int g = 0; g < NG; g++) {
@@ -212,16 +212,22 @@ __device__ __forceinline__ void dz_rows(const GroupedParams &p, int e, int k0, i
         d0[g] = p.x0 + r;
         d1[g] = p.x1 + r;
     }
-    floatx4 acc0[NG][4], acc1[NG][4];
+    floatx4 acc0[NG][C], acc1[NG][C];
 #pragma unroll
     for (int g = 0; g < NG; g++)
 #pragma unroll
-        for (int t = 0; t < 4; t++) acc0[g][t] = acc1[g][t] = (floatx4){0.f, 0.f, 0.f, 0.f};
-    auto load = [&](DzPiece<NG> &f, int nb) {
+        for (int t = 0; t < C; t++) acc0[g][t] = acc1[g][t] = (floatx4){0.f, 0.f, 0.f, 0.f};
+    auto load = [&](DzPiece<NG, C> &f, int nb) {
 #pragma unroll
         for (int u = 0; u < 4; u++) {
-            const int n = nb + q + u;
-            f.w[u] = load4<VEC>(w + (size_t)min(n, N - 1) * K, k, K);
+            const float *row = w + (size_t)min(nb + q + u, N - 1) * K;
+            if constexpr (C == 4) {
+                const floatx4 x = load4<VEC>(row, k, K);
+#pragma unroll
+                for (int t = 0; t < C; t++) f.w[u][t] = x[t];
+            } else {
+                f.w[u][0] = row[min(k, K - 1)];   // (columns beyond the last are not stored)
+            }
         }
 #pragma unroll
         for (int g = 0; g < NG; g++) {
@@ -229,13 +235,19 @@ __device__ __forceinline__ void dz_rows(const GroupedParams &p, int e, int k0, i
             f.d1[g] = load4<VEC>(d1[g], nb + q, N);
         }
     };
-    const bool edge = k0 + 64 > K;
-    auto use = [&](DzPiece<NG> &f, int nb) {
+    const bool edge = C == 4 && k0 + 64 > K;
+    auto use = [&](DzPiece<NG, C> &f, int nb) {
         if (edge || nb + 16 > N) {
 #pragma unroll
             for (int u = 0; u < 4; u++) {
-                f.w[u] = settle<VEC>(f.w[u], k, K);
-                if (nb + q + u >= N) f.w[u] = (floatx4){0.f, 0.f, 0.f, 0.f};
+                if constexpr (C == 4) {
+                    const floatx4 x = settle<VEC>((floatx4){f.w[u][0], f.w[u][1], f.w[u][2], f.w[u][3]}, k, K);
+#pragma unroll
+                    for (int t = 0; t < C; t++) f.w[u][t] = x[t];
+                }
+#pragma unroll
+                for (int t = 0; t < C; t++)
+                    if (nb + q + u >= N) f.w[u][t] = 0.f;
             }
 #pragma unroll
             for (int g = 0; g < NG; g++) {
@@ -246,7 +258,7 @@ __device__ __forceinline__ void dz_rows(const GroupedParams &p, int e, int k0, i
 #pragma unroll
         for (int u = 0; u < 4; u++)
 #pragma unroll
-            for (int t = 0; t < 4; t++) {
+            for (int t = 0; t < C; t++) {
                 const float x = f.w[u][t], x2 = x * x;
 #pragma unroll
                 for (int g = 0; g < NG; g++) {
@@ -255,8 +267,8 @@ __device__ __forceinline__ void dz_rows(const GroupedParams &p, int e, int k0, i
                 }
             }
     };
-    DzPiece<NG> x, y;
-    const int step = 16 * DZ_WAVES;
+    DzPiece<NG, C> x, y;
+    const int step = 16 * WAVES;
     int nb = 16 * wave;
     if (nb < N) load(x, nb);
     for (; nb < N; nb += 2 * step) {
@@ -266,7 +278,8 @@ __device__ __forceinline__ void dz_rows(const GroupedParams &p, int e, int k0, i
         if (nb + 2 * step < N) load(x, nb + 2 * step);
         use(y, nb + step);
     }
-    constexpr int STEPS = 1024 / (DZ_WAVES * 64);   // outputs of a thread: 16 rows by 64 inputs
+    constexpr int COLS = 16 * C, THREADS = WAVES * 64;
+    constexpr int STEPS = (16 * COLS + THREADS - 1) / THREADS;   // outputs of a thread
 #pragma unroll
     for (int g = 0; g < NG; g++) {
         float sum[2][STEPS];
@@ -274,24 +287,24 @@ __device__ __forceinline__ void dz_rows(const GroupedParams &p, int e, int k0, i
         for (int a = 0; a < 2; a++) {
             __syncthreads();
 #pragma unroll
-            for (int t = 0; t < 4; t++)
+            for (int t = 0; t < C; t++)
 #pragma unroll
                 for (int v = 0; v < 4; v++) s[wave][4 * t + v][lane] = (a == 0 ? acc0 : acc1)[g][t][v];
             __syncthreads();
 #pragma unroll
             for (int h = 0; h < STEPS; h++) {
-                const int c = tid & 63, j = (tid >> 6) + DZ_WAVES * h;
-                const int l = (c >> 4) * 16 + j, x16 = 4 * (c & 3) + ((c >> 2) & 3);
+                const int c = tid % COLS, j = (tid / COLS + THREADS / COLS * h) & 15, at = c / C;
+                const int l = (at >> 2) * 16 + j, x = 4 * (c % C) + (at & 3);
                 float m = 0.f;
 #pragma unroll
-                for (int w8 = 0; w8 < DZ_WAVES; w8++) m += s[w8][x16][l];
+                for (int w = 0; w < WAVES; w++) m += s[w][x][l];
                 sum[a][h] = m;
             }
         }
 #pragma unroll
         for (int h = 0; h < STEPS; h++) {
-            const int c = k0 + (tid & 63), r = r0 + 16 * g + (tid >> 6) + DZ_WAVES * h;
-            if (r < end && c < K) {
+            const int c = k0 + tid % COLS, j = tid / COLS + THREADS / COLS * h, r = r0 + 16 * g + j;
+            if (j < 16 && r < end && c < K) {
                 const size_t at = (size_t)r * K + c;
                 const float f = p.e0 != nullptr ? p.e0[at] : 1.f;
                 p.out0[at] = sum[0][h] * f;
@@ -302,13 +315,14 @@ __device__ __forceinline__ void dz_rows(const GroupedParams &p, int e, int k0, i
     __syncthreads();
 }
 
-template <int NG, bool VEC>
-__global__ __launch_bounds__(DZ_WAVES * 64, NG == 1 && VEC ? 4 : 2) void rows_dz_kernel(GroupedParams p) {
-    __shared__ float s[DZ_WAVES][16][65];
-    const int blocks = (p.K + 63) / 64, slot = blockIdx.x / blocks, k0 = (blockIdx.x - slot * blocks) * 64;
+template <int WAVES, int NG, int C, bool VEC>
+__global__ __launch_bounds__(WAVES * 64, WAVES == 8 && NG == 1 && VEC ? 4 : 2) void rows_dz_kernel(GroupedParams p) {
+    __shared__ float s[WAVES][4 * C][65];
+    const int blocks = (p.K + 16 * C - 1) / (16 * C), slot = blockIdx.x / blocks;
+    const int k0 = (blockIdx.x - slot * blocks) * 16 * C;
     int r0, end;
     const int e = find_rows(p.offsets, p.E, p.R, 16 * NG, slot, r0, end);
-    if (e >= 0) dz_rows<NG, VEC>(p, e, k0, r0, end, s);
+    if (e >= 0) dz_rows<WAVES, NG, C, VEC>(p, e, k0, r0, end, s);
 }
 
 // ---------------------------------------------------------------------------
@@ -335,16 +349,29 @@ __global__ __launch_bounds__(DW_WAVES * 64) void rows_dw_kernel(GroupedParams p)
     if (n0 >= N) return;
     const int rows_n = min(DW_ROWS, N - n0);
     const float *__restrict__ d0 = p.x0, *__restrict__ d1 = p.x1;
-    if (p.db0 != nullptr && kb == 0 && lane < rows_n) {
+    // the factors of the result are on their way first
+    floatx4 w[DW_ROWS];
+#pragma unroll
+    for (int n = 0; n < DW_ROWS; n++)
+        w[n] = load4<VEC>(p.e0 + ((size_t)e * N + n0 + min(n, rows_n - 1)) * K, min(k, K - 1), K);
+    if (p.db0 != nullptr && kb == 0) {   // lane: row n0 + lane % 8, every eighth row of the batch
         float m = 0.f, v = 0.f;
-        for (int r = first; r < end; r++) {
-            m += d0[(size_t)r * N + n0 + lane];
-            v += d1[(size_t)r * N + n0 + lane];
+        const int n = n0 + min(lane & 7, rows_n - 1);
+        for (int r = first + (lane >> 3); r < end; r += 8) {
+            m += d0[(size_t)r * N + n];
+            v += d1[(size_t)r * N + n];
         }
-        const size_t at = (size_t)e * N + n0 + lane;
-        const float vb = p.e1[at];
-        p.db0[at] = vb * m;
-        p.db1[at] = vb * vb * v;
+#pragma unroll
+        for (int off = 8; off < 64; off <<= 1) {
+            m += __shfl_xor(m, off, 64);
+            v += __shfl_xor(v, off, 64);
+        }
+        if (lane < rows_n) {
+            const size_t at = (size_t)e * N + n0 + lane;
+            const float vb = p.e1[at];
+            p.db0[at] = vb * m;
+            p.db1[at] = vb * vb * v;
+        }
     }
     if (k >= K) return;
     floatx4 acc0[DW_ROWS], acc1[DW_ROWS];
@@ -380,32 +407,26 @@ __global__ __launch_bounds__(DW_WAVES * 64) void rows_dw_kernel(GroupedParams p)
             }
         }
     }
-    for (int n = 0; n < rows_n; n++) {
+#pragma unroll
+    for (int n = 0; n < DW_ROWS; n++) {
+        if (n >= rows_n) break;
         const size_t at = ((size_t)e * N + n0 + n) * K + k;
-        floatx4 x = acc0[0], y = acc1[0];
+        const floatx4 f = settle<VEC>(w[n], k, K);
+        float4_any m, v;
 #pragma unroll
-        for (int i = 1; i < DW_ROWS; i++)
-            if (i == n) {
-                x = acc0[i];
-                y = acc1[i];
-            }
+        for (int c = 0; c < 4; c++) {
+            m[c] = acc0[n][c] * f[c];
+            v[c] = acc1[n][c] * f[c] * f[c];
+        }
         if (k + 4 <= K) {
-            const float4_any w = *reinterpret_cast<const float4_any *>(p.e0 + at);
-            float4_any m, v;
-#pragma unroll
-            for (int c = 0; c < 4; c++) {
-                m[c] = x[c] * w[c];
-                v[c] = y[c] * w[c] * w[c];
-            }
             *reinterpret_cast<float4_any *>(p.out0 + at) = m;
             *reinterpret_cast<float4_any *>(p.out1 + at) = v;
         } else {
 #pragma unroll
-            for (int c = 0; c < 4; c++)
+            for (int c = 0; c < 3; c++)
                 if (k + c < K) {
-                    const float w = p.e0[at + c];
-                    p.out0[at + c] = x[c] * w;
-                    p.out1[at + c] = y[c] * w * w;
+                    p.out0[at + c] = m[c];
+                    p.out1[at + c] = v[c];
                 }
         }
     }
@@ -415,9 +436,10 @@ template <int WAVES, int NG, bool VEC>
 void rows_fwd(const GroupedParams &p, unsigned grid, hipStream_t stream) {
     hipLaunchKernelGGL((rows_fwd_kernel<WAVES, NG, VEC>), dim3(grid), dim3(WAVES * 64), 0, stream, p);
 }
-template <int NG, bool VEC>
-void rows_dz(const GroupedParams &p, unsigned grid, hipStream_t stream) {
-    hipLaunchKernelGGL((rows_dz_kernel<NG, VEC>), dim3(grid), dim3(DZ_WAVES * 64), 0, stream, p);
+template <int WAVES, int NG, int C, bool VEC>
+void rows_dz(const GroupedParams &p, unsigned slots, hipStream_t stream) {
+    const unsigned blocks = (p.K + 16 * C - 1) / (16 * C);
+    hipLaunchKernelGGL((rows_dz_kernel<WAVES, NG, C, VEC>), dim3(blocks * slots), dim3(WAVES * 64), 0, stream, p);
 }
 
 }  // namespace
@@ -437,8 +459,12 @@ hipError_t launch_grouped_rows(GroupedMode mode, const GroupedParams &p, bool ve
         const long long working = (long long)used * blocks;
         if (!vec)
             one ? rows_fwd<8, 1, false>(p, grid, stream) : rows_fwd<8, 2, false>(p, grid, stream);
-        else if (!one)   // (a wave needs some 32-element pieces to be worth its join)
-            p.K > 512 ? rows_fwd<8, 2, true>(p, grid, stream) : rows_fwd<4, 2, true>(p, grid, stream);
+        // (a wave needs some 32-element pieces to be worth its join. 32 rows: 4 / 8 waves 177 /
+        // 221 us at 8 x 256 blocks of 2048, 59 / 76 at 16 x 64 of 1024, 28 / 28 at 2 x 128 of
+        // 2048, 48 / 43 at 2 x 32 of 4096)
+        else if (!one)
+            p.K <= 512 || working > 256 ? rows_fwd<4, 2, true>(p, grid, stream)
+                                        : rows_fwd<8, 2, true>(p, grid, stream);
         else if (working > 1024)
             rows_fwd<4, 1, true>(p, grid, stream);
         else if (working > 256)
@@ -446,13 +472,18 @@ hipError_t launch_grouped_rows(GroupedMode mode, const GroupedParams &p, bool ve
         else
             rows_fwd<16, 1, true>(p, grid, stream);
     } else if (mode == GROUPED_DZ) {
-        const unsigned blocks = (p.K + 63) / 64, grid = blocks * slots;
+        // Blocks of 16 inputs, by sixteen waves, while those of 64 are too few: wide / narrow
+        // for blocks of 64 inputs x groups of rows, N = 2048, one row per expert 4: 27 / 13,
+        // 64: 32 / 15, 128: 32 / 21, 256: 33 / 31 us; twelve rows 4: 38 / 18, 128: 41 / 39,
+        // 256: 43 / 74 us.
+        const long long groups = p.R / 32 + used / 2;
+        const bool narrow = (groups > used ? groups : used) * ((p.K + 63) / 64) <= 128;
         if (!vec)
-            one ? rows_dz<1, false>(p, grid, stream) : rows_dz<2, false>(p, grid, stream);
-        else if (!one)
-            rows_dz<2, true>(p, grid, stream);
+            one ? rows_dz<8, 1, 4, false>(p, slots, stream) : rows_dz<8, 2, 4, false>(p, slots, stream);
+        else if (narrow)
+            one ? rows_dz<16, 1, 1, true>(p, slots, stream) : rows_dz<16, 2, 1, true>(p, slots, stream);
         else
-            rows_dz<1, true>(p, grid, stream);
+            one ? rows_dz<8, 1, 4, true>(p, slots, stream) : rows_dz<8, 2, 4, true>(p, slots, stream);
     } else {
         const int rows = DW_ROWS * DW_WAVES;
         const dim3 grid((unsigned)((p.K + DW_COLS - 1) / DW_COLS) * ((p.N + rows - 1) / rows) * p.E);
