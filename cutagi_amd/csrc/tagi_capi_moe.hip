@@ -38,10 +38,9 @@ int moe_sizes(int T, int k, int R, int N) {
     return (long long)T * k > MAX_INT ? TAGI_ERR_UNSUPPORTED : TAGI_OK;
 }
 
-// whether the scratch that a call needs is there
-bool grouped_scratch_ok(int K, int N, int E, int R, const void *scratch) {
-    return scratch != nullptr ? (reinterpret_cast<size_t>(scratch) & 15u) == 0
-                              : grouped_scratch_floats(K, N, E, R) == 0;
+// whether the scratch that a call needs is there, 16-byte aligned
+bool scratch_ok(const void *scratch, size_t floats) {
+    return scratch != nullptr ? (reinterpret_cast<size_t>(scratch) & 15u) == 0 : floats == 0;
 }
 
 int grouped_fwd(const float *mu_w, const float *var_w, const float *mu_b, const float *var_b,
@@ -52,7 +51,7 @@ int grouped_fwd(const float *mu_w, const float *var_w, const float *mu_b, const 
     if (bias && (!mu_b || !var_b)) return TAGI_ERR_INVALID_ARG;
     const int rc = grouped_sizes(K, N, E, R, T, rows, N, false);
     if (rc != TAGI_OK) return rc;
-    if (!grouped_scratch_ok(K, N, E, R, scratch)) return TAGI_ERR_INVALID_ARG;
+    if (!scratch_ok(scratch, grouped_scratch_floats(K, N, E, R))) return TAGI_ERR_INVALID_ARG;
     GroupedParams p = {};
     p.x0 = mu_a, p.x1 = var_a, p.y0 = mu_w, p.y1 = var_w;
     p.e0 = bias ? mu_b : nullptr, p.e1 = bias ? var_b : nullptr;
@@ -97,13 +96,12 @@ int tagi_layernorm_bwd(const float *mu_w, const float *var_w, const float *var_b
     if (!mu_w || !var_w || !mu_s || !var_s || !delta_mu_out || !delta_var_out)
         return TAGI_ERR_INVALID_ARG;
     if (state_update && (!delta_mu || !delta_var)) return TAGI_ERR_INVALID_ARG;
-    if (param_update && (!mu_a || !delta_mu_w || !delta_var_w || !scratch))
-        return TAGI_ERR_INVALID_ARG;
-    if (param_update && (reinterpret_cast<size_t>(scratch) & 15u)) return TAGI_ERR_INVALID_ARG;
+    if (param_update && (!mu_a || !delta_mu_w || !delta_var_w)) return TAGI_ERR_INVALID_ARG;
     if (param_update && bias && (!var_b || !delta_mu_b || !delta_var_b))
         return TAGI_ERR_INVALID_ARG;
     if (n < 2 || B <= 0) return TAGI_ERR_INVALID_ARG;
     if (!state_update && !param_update) return TAGI_OK;
+    if (param_update && !scratch_ok(scratch, layernorm_bwd_scratch_floats(n, B))) return TAGI_ERR_INVALID_ARG;
     TAGI_TRY(launch_layernorm_bwd(mu_w, var_w, bias ? var_b : nullptr, mu_a, jcb, mu_s, var_s,
                                   delta_mu_out, delta_var_out, epsilon, n, B, state_update,
                                   param_update, static_cast<float *>(scratch), delta_mu, delta_var,
@@ -155,7 +153,7 @@ int tagi_grouped_linear_bwd(const float *mu_w, const float *var_w, const float *
         return TAGI_ERR_INVALID_ARG;
     const int rc = grouped_sizes(K, N, E, R, T, rows, K, param_update != 0);
     if (rc != TAGI_OK) return rc;
-    if (!grouped_scratch_ok(K, N, E, R, scratch)) return TAGI_ERR_INVALID_ARG;
+    if (!scratch_ok(scratch, grouped_scratch_floats(K, N, E, R))) return TAGI_ERR_INVALID_ARG;
     GroupedParams p = {};
     p.scratch = static_cast<float *>(scratch);
     p.x0 = delta_mu, p.x1 = delta_var;

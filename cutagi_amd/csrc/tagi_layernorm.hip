@@ -148,14 +148,19 @@ __global__ __launch_bounds__(TPB) void ln_fwd_kernel(
 // Backward of one (block of columns, chunk of rows). 2^cw_log threads (up to a wave) hold
 // neighbouring groups of four columns, the other bits of the thread index are rows. A thread
 // keeps its columns' four sums over the rows it walks; the row threads of a wave are joined by
-// lane exchanges, the waves through LDS. part: [chunk][4][n].
+// lane exchanges, the waves through LDS. The sums go to part ([chunk][4][n]), or where there is
+// one chunk only to the innovations.
 // ---------------------------------------------------------------------------
+struct ParamOut {
+    const float *var_w, *var_b;
+    float *dmu_w, *dvar_w, *dmu_b, *dvar_b;
+};
 __global__ __launch_bounds__(TPB) void ln_bwd_kernel(
     const float *__restrict__ mu_w, const float *__restrict__ mu_a, const float *__restrict__ jcb,
     const float *__restrict__ mu_s, const float *__restrict__ var_s,
     const float *__restrict__ dmu_out, const float *__restrict__ dvar_out, float epsilon, int n,
     int B, int rows_per_chunk, int cw_log, int state_update, int param_update, bool past_cache,
-    float *__restrict__ dmu, float *__restrict__ dvar, float *__restrict__ part) {
+    float *__restrict__ dmu, float *__restrict__ dvar, float *__restrict__ part, ParamOut out) {
     __shared__ float s[TPB / 64][16][64];
     const int cw = 1 << cw_log, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int ct = threadIdx.x & (cw - 1), rt = threadIdx.x >> cw_log, row_step = TPB >> cw_log;
@@ -226,17 +231,25 @@ __global__ __launch_bounds__(TPB) void ln_bwd_kernel(
 #pragma unroll
         for (int c = 0; c < 4; c++)
             v[c] = (s[0][4 * k + c][at] + s[1][4 * k + c][at]) + (s[2][4 * k + c][at] + s[3][4 * k + c][at]);
-        store_group(part + ((size_t)blockIdx.y * 4 + k) * n + (size_t)(blockIdx.x * cw + at) * 4, have, v, false);
+        const size_t col = (size_t)(blockIdx.x * cw + at) * 4;
+        if (gridDim.y > 1) {
+            store_group(part + ((size_t)blockIdx.y * 4 + k) * n + col, have, v, false);
+            continue;
+        }
+        if (k >= 2 && out.var_b == nullptr) continue;
+        float f[4];
+        load_group((k < 2 ? out.var_w : out.var_b) + col, have, f);
+#pragma unroll
+        for (int c = 0; c < 4; c++) v[c] *= k & 1 ? f[c] * f[c] : f[c];
+        store_group((k == 0 ? out.dmu_w : k == 1 ? out.dvar_w : k == 2 ? out.dmu_b : out.dvar_b) + col, have, v, false);
     }
 }
 
 // The chunks of 2^cw_log (up to 64) columns: the other bits of the thread index share out the
 // chunks; their sums are joined like the row threads' above.
 constexpr int FINAL_WAVES = 16;
-__global__ __launch_bounds__(FINAL_WAVES * 64) void ln_bwd_final_kernel(
-    const float *__restrict__ part, const float *__restrict__ var_w,
-    const float *__restrict__ var_b, int n, int chunks, int cw_log, float *__restrict__ dmu_w,
-    float *__restrict__ dvar_w, float *__restrict__ dmu_b, float *__restrict__ dvar_b) {
+__global__ __launch_bounds__(FINAL_WAVES * 64) void ln_bwd_final_kernel(const float *__restrict__ part, int n,
+                                                                       int chunks, int cw_log, ParamOut out) {
     __shared__ float s[4][FINAL_WAVES][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, cw = 1 << cw_log;
     const int c = blockIdx.x * cw + (threadIdx.x & (cw - 1));
@@ -260,13 +273,13 @@ __global__ __launch_bounds__(FINAL_WAVES * 64) void ln_bwd_final_kernel(
 #pragma unroll
         for (int w = 0; w < FINAL_WAVES; w++) v[k] += s[k][w][lane];
     }
-    const float vw = var_w[c];
-    dmu_w[c] = vw * v[0];
-    dvar_w[c] = vw * vw * v[1];
-    if (var_b != nullptr) {
-        const float vb = var_b[c];
-        dmu_b[c] = vb * v[2];
-        dvar_b[c] = vb * vb * v[3];
+    const float vw = out.var_w[c];
+    out.dmu_w[c] = vw * v[0];
+    out.dvar_w[c] = vw * vw * v[1];
+    if (out.var_b != nullptr) {
+        const float vb = out.var_b[c];
+        out.dmu_b[c] = vb * v[2];
+        out.dvar_b[c] = vb * vb * v[3];
     }
 }
 
@@ -276,7 +289,10 @@ int ln_cw_log(int n) {
     while (l < 6 && (1 << l) < (n + 3) / 4) l++;
     return l;
 }
-int ln_rows_per_chunk(int n, int B) {
+struct LnChunks {
+    int rows, most;   // rows of a chunk, chunks at most (never more for fewer rows)
+};
+LnChunks ln_chunks(int n, int B) {
     // four workgroups per CU (16384 x 4096, forward and backward: 2 / 3 / 4 / 8 / 16 per CU take
     // 540 / 497 / 493 / 517 / 508 us; more of them also leave more partial sums), but four rows
     // for every row thread (sixteen in all at least)
@@ -284,7 +300,8 @@ int ln_rows_per_chunk(int n, int B) {
     const long long col_blocks = ((n + 3) / 4 + cw - 1) / cw;
     const long long chunks = (4LL * num_cu() + col_blocks - 1) / col_blocks;
     const long long rows = (B + chunks - 1) / chunks, least = 4 * (TPB / cw);
-    return (int)(rows > least ? rows : least);
+    const long long parts = (B + least - 1) / least;
+    return {(int)(rows > least ? rows : least), (int)(parts < chunks ? parts : chunks)};
 }
 
 template <int THREADS, int PER>
@@ -303,8 +320,8 @@ hipError_t fwd(const float *mu_w, const float *var_w, const float *mu_b, const f
 }  // namespace
 
 size_t layernorm_bwd_scratch_floats(int n, int B) {
-    const int rows = ln_rows_per_chunk(n, B);
-    return (size_t)((B + rows - 1) / rows) * 4 * n;
+    const int chunks = ln_chunks(n, B).most;
+    return chunks == 1 ? 0 : (size_t)chunks * 4 * n;
 }
 
 hipError_t launch_layernorm_fwd(const float *mu_w, const float *var_w, const float *mu_b,
@@ -329,18 +346,19 @@ hipError_t launch_layernorm_bwd(const float *mu_w, const float *var_w, const flo
                                 float epsilon, int n, int B, int state_update, int param_update,
                                 float *scratch, float *dmu, float *dvar, float *dmu_w,
                                 float *dvar_w, float *dmu_b, float *dvar_b, hipStream_t stream) {
-    const int rows = ln_rows_per_chunk(n, B), cw_log = ln_cw_log(n);
+    const int rows = ln_chunks(n, B).rows, cw_log = ln_cw_log(n);
     const int chunks = (B + rows - 1) / rows, groups = (n + 3) / 4;
     const dim3 grid((groups + (1 << cw_log) - 1) >> cw_log, chunks);
+    const ParamOut out = {var_w, var_b, dmu_w, dvar_w, dmu_b, dvar_b};
     hipLaunchKernelGGL(ln_bwd_kernel, grid, dim3(TPB), 0, stream, mu_w, mu_a, jcb, mu_s, var_s, dmu_out,
                        dvar_out, epsilon, n, B, rows, cw_log, state_update, param_update,
-                       goes_past_cache((size_t)2 * B * n), dmu, dvar, scratch);
+                       goes_past_cache((size_t)2 * B * n), dmu, dvar, scratch, out);
     hipError_t e = hipGetLastError();
-    if (e != hipSuccess || !param_update) return e;
+    if (e != hipSuccess || !param_update || chunks == 1) return e;
     int f_log = 0;
     while (f_log < 6 && (1 << f_log) < n) f_log++;
     hipLaunchKernelGGL(ln_bwd_final_kernel, dim3((n + (1 << f_log) - 1) >> f_log), dim3(FINAL_WAVES * 64), 0,
-                       stream, scratch, var_w, var_b, n, chunks, f_log, dmu_w, dvar_w, dmu_b, dvar_b);
+                       stream, scratch, n, chunks, f_log, out);
     return hipGetLastError();
 }
 

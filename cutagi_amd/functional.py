@@ -443,7 +443,8 @@ def layernorm_bwd(mu_w, var_w, var_b, mu_a, jcb, mu_s, var_s, delta_mu, delta_va
     if param_update:
         count = 2 if var_b is None else 4
         out[2:2 + count] = _new(delta_mu, count, n)
-        scratch = delta_mu.new_empty(capi.layernorm_bwd_scratch(n, B), dtype=torch.uint8)
+        size = capi.layernorm_bwd_scratch(n, B)
+        scratch = delta_mu.new_empty(size, dtype=torch.uint8) if size else None
     capi.check(capi.lib.tagi_layernorm_bwd(
         mu_w.data_ptr(), var_w.data_ptr(), _at(var_b), mu_a.data_ptr(), _at(jcb), mu_s.data_ptr(),
         var_s.data_ptr(), delta_mu.data_ptr(), delta_var.data_ptr(), eps, n, B,

@@ -455,7 +455,7 @@ int tagi_layernorm_fwd(const float *mu_w, const float *var_w, const float *mu_b,
                        float *var_s, float *mu_z, float *var_z, void *stream);
 
 /* Bytes of device memory that tagi_layernorm_bwd needs as scratch when param_update != 0
- * (on the current device). Host only. The caller owns it, so that calls recorded into
+ * (on the current device; 0 for few rows, and never more for fewer rows). Host only. The caller owns it, so that calls recorded into
  * several graphs need not share any. */
 int tagi_layernorm_bwd_scratch(int n, int B, size_t *bytes /* host, out */);
 
@@ -466,8 +466,8 @@ int tagi_layernorm_bwd_scratch(int n, int B, size_t *bytes /* host, out */);
  *   delta_mu_w = var_w * sum_b x * delta_mu_out, delta_var_w = var_w^2 * sum_b x^2 *
  *                delta_var_out, x = (mu_a - mu_s)/sqrt(var_s + eps); biases with x = 1
  * jcb may be NULL (one everywhere). Sums are taken in a fixed order: the same bits every
- * call. scratch: tagi_layernorm_bwd_scratch bytes, 16-byte aligned; may be NULL without
- * param_update. */
+ * call. scratch: tagi_layernorm_bwd_scratch bytes, 16-byte aligned; may be NULL where
+ * that is 0 and without param_update. */
 int tagi_layernorm_bwd(const float *mu_w, const float *var_w, const float *var_b,
                        const float *mu_a, const float *jcb, const float *mu_s,
                        const float *var_s, const float *delta_mu_out,

@@ -25,7 +25,8 @@ def test_layernorm_refuses():
         assert L.tagi_layernorm_fwd(*_without(fwd, i)) == capi.ERR_INVALID_ARG
     for n, B in ((1, 4), (0, 4), (8, 0), (8, -1)):     # one feature has no sample variance
         assert L.tagi_layernorm_fwd(*(fwd[:8] + [n, B] + fwd[10:])) == capi.ERR_INVALID_ARG
-    bwd = [one] * 9 + [1e-5, 8, 4, 1, 1, 1] + [one] * 7 + [None]
+    bwd = [one] * 9 + [1e-5, 8, 999, 1, 1, 1] + [one] * 7 + [None]
+    assert capi.layernorm_bwd_scratch(8, 999) > 0
     for i in [0, 1, 2, 3, 5, 6, 7, 8] + list(range(15, 22)):
         assert L.tagi_layernorm_bwd(*_without(bwd, i)) == capi.ERR_INVALID_ARG
     assert L.tagi_layernorm_bwd(*_without(bwd, 15, odd)) == capi.ERR_INVALID_ARG
@@ -35,6 +36,18 @@ def test_layernorm_refuses():
     assert L.tagi_layernorm_bwd_scratch(1, 4, ctypes.byref(size)) == capi.ERR_INVALID_ARG
     # nothing asked for: done
     assert L.tagi_layernorm_bwd(*([one] * 9 + [1e-5, 8, 4, 1, 0, 0] + [None] * 8)) == capi.OK
+
+
+def test_layernorm_scratch():
+    """What is held for a batch does for every smaller one."""
+    capi, _ = _lib()
+    for n in (2, 24, 300, 1023, 4096, 9001):
+        held = 0
+        for B in list(range(1, 2100)) + [4096, 9660, 65536, 1 << 20]:
+            now = capi.layernorm_bwd_scratch(n, B)
+            assert now >= held
+            held = now
+    assert capi.layernorm_bwd_scratch(4096, 16) == 0
 
 
 def test_grouped_linear_refuses():
