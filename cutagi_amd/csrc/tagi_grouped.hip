@@ -1,6 +1,7 @@
 // Linear layers grouped by expert: row r of expert e (offsets[e] <= r < offsets[e+1])
 // meets the weights [e][N][K]. gfx950.
 #include <algorithm>
+#include <cmath>
 #include <cstdint>
 #include <type_traits>
 
@@ -30,10 +31,10 @@ constexpr int MAX_GROUPS = 1024;
 // An infinity (or a magnitude beyond bf16's 3.39e38) has the residue NaN and gives NaN, where
 // fp32 arithmetic would give an infinity or NaN.
 //
-// A workgroup owns 128 x 128 tiles of an output pair and walks them one after the other. Four
+// A workgroup owns 128 x 128 tiles (64 x 128 where experts have few rows) of an output pair and walks them one after the other. Four
 // of its waves load the operands, form the sums and squares that the variance needs, split
 // them and write the pieces to LDS; the other four read fragments and issue matrix
-// instructions on 64 x 64 sub-tiles. Every SIMD holds one wave of each kind, so the vector
+// instructions on 64 x 64 (32 x 64) sub-tiles. Every SIMD holds one wave of each kind, so the vector
 // work of the split runs under the matrix instructions without any interleaving in the code,
 // and an element is split once for the two waves that read it.
 // The two kinds meet at one barrier per unit, 32 reduction elements of one product (mean;
@@ -59,7 +60,7 @@ __device__ __forceinline__ void split_pair(float a, float b, unsigned (&piece)[3
     }
 }
 
-constexpr int TM = 128;             // rows and columns of a tile
+constexpr int TM = 128;             // rows (64 XM of them: forward, state backward) and columns of a tile
 constexpr int TK = 32;              // reduction elements of a unit
 constexpr int TILE_THREADS = 512;   // 256 that stage, 256 that multiply
 // One piece of one operand of a unit: 64 bytes per row (or column) of the tile, four chunks of
@@ -132,7 +133,7 @@ struct Tile {
 //   DW: the same eighth of every expert's tiles, whatever its number of rows; an eighth of
 //            all experts' tiles in order where an expert has too few to divide
 // A divided reduction has all tiles once per part; the parts are whole units.
-template <int MODE>
+template <int MODE, int XM>
 struct TileList {
     int tiles_m, tiles_c, lo, count;   // this XCD's part of the list
     int per;                           // DW: tiles of it per expert and part, 0: of all in order
@@ -182,8 +183,8 @@ struct TileList {
         t.e = a;
         int first, end;
         group_rows(p.offsets, a, p.R, first, end);
-        t.m0 = first + (rt - prefix[a]) * TM;
-        t.m_end = min(end, t.m0 + TM);
+        t.m0 = first + (rt - prefix[a]) * (64 * XM);
+        t.m_end = min(end, t.m0 + 64 * XM);
         t.c_end = MODE == GROUPED_FWD ? p.N : p.K;
         t.r0 = 0;
         t.red = MODE == GROUPED_FWD ? p.K : p.N;
@@ -216,15 +217,16 @@ __device__ __forceinline__ float4_any to_front(float4_any v, int n) {
 }
 
 // Side with its reduction index contiguous: thread u holds the elements 4 (u % 8) .. + 3 of
-// the rows u / 8 + 16 i: eight lanes read a whole 128-byte line. At the end of a reduction
+// the NR rows u / 8 + 16 i: eight lanes read a whole 128-byte line. At the end of a reduction
 // that is no multiple of four the loads are moved to end with their row, and what they bring
 // is moved back before the split.
-template <int MODE, bool ROWS, bool FAR>
+template <int MODE, bool ROWS, bool FAR, int NR>
 struct SideK {
+    static constexpr int LOADS = NR;
     const float *q0, *q1;       // uniform
     static constexpr bool GATHER = ROWS && MODE == GROUPED_FWD;
-    unsigned row[8];            // element offset of the thread's rows
-    int source[GATHER ? 8 : 1]; // gather: the rows of the next tile
+    unsigned row[NR];           // element offset of the thread's rows
+    int source[GATHER ? NR : 1]; // gather: the rows of the next tile
     bool fresh, gather;
     unsigned dead;
     int k, red, at, first_row, last_row;
@@ -243,7 +245,7 @@ struct SideK {
         if constexpr (GATHER) {
             if (gather)
 #pragma unroll
-                for (int i = 0; i < 8; i++) source[i] = p.rows[t.m0 + min(first_row + 16 * i, last_row)];
+                for (int i = 0; i < NR; i++) source[i] = p.rows[t.m0 + min(first_row + 16 * i, last_row)];
         }
     }
     __device__ __forceinline__ void ahead(const GroupedParams &, int) {}
@@ -254,7 +256,7 @@ struct SideK {
             fresh = false;
             dead = 0u;
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
+            for (int i = 0; i < NR; i++) {
                 int s = min(first_row + 16 * i, last_row);
                 if constexpr (GATHER) {
                     if (gather) s = source[i];
@@ -281,7 +283,7 @@ struct SideK {
     // zeros behind the end of the reduction and in rows that are no rows
     __device__ __forceinline__ void mask(Batch &b) const {
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
+        for (int i = 0; i < NR; i++) {
             const int over = (b.dead >> i) & 1u ? 4 : min(max(4 - (b.left - k), 0), 4);
             b.v0[i] = to_front(b.v0[i], over);
             b.v1[i] = to_front(b.v1[i], over);
@@ -294,7 +296,7 @@ struct SideK {
     __device__ __forceinline__ void write(const Batch &b, char *side, int u, Batch *next) const {
         char *to = side + chunk_at(u >> 3, (u & 7) >> 1) + (u & 1) * 8;
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
+        for (int i = 0; i < NR; i++) {
             if (O < 2 && next != nullptr) load(*next, i, O == 1);
             const float4_any x = b.v0[i], y = b.v1[i];
             unsigned lo[3], hi[3];
@@ -311,6 +313,7 @@ struct SideK {
 // reduction elements 8 (u / 32) + i: 32 lanes read 512 bytes of one.
 template <int MODE, bool ROWS, bool FAR>
 struct SideM {
+    static constexpr int LOADS = 8;
     static constexpr bool GATHER = MODE == GROUPED_DW && !ROWS;
     const float *q0, *q1;     // element (reduction 0, column 0) of the operand, uniform
     int ld, red, r0, g, col, shift;
@@ -401,10 +404,10 @@ struct SideM {
 };
 
 // One of the two staging halves of a workgroup.
-template <int MODE, typename Side>
+template <int MODE, int XM, typename Side>
 struct Stager {
     const GroupedParams &p;
-    const TileList<MODE> &list;
+    const TileList<MODE, XM> &list;
     char *lds;
     int next, step, u;
     Side side;
@@ -458,7 +461,7 @@ struct Stager {
             side.begin(p, k0, a);
             advance();
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
+            for (int i = 0; i < Side::LOADS; i++) {
                 side.load(a, i, false);
                 side.load(a, i, true);
             }
@@ -475,14 +478,14 @@ struct Stager {
     }
 };
 
-template <int MODE, bool FAR>
+template <int MODE, int XM, bool FAR>
 __global__ __launch_bounds__(TILE_THREADS) void grouped_tile_kernel(GroupedParams p) {
     extern __shared__ __attribute__((aligned(16))) char tile_lds[];
     typedef TileShape<MODE> Shape;
     const int tid = threadIdx.x, lane = tid & 63;
     int *prefix = reinterpret_cast<int *>(tile_lds + RING * UNIT);
 
-    TileList<MODE> list;
+    TileList<MODE, XM> list;
     list.prefix = prefix;
     list.tiles_c = ((MODE == GROUPED_FWD ? p.N : p.K) + TM - 1) / TM;
     if (MODE == GROUPED_DW) {
@@ -502,7 +505,7 @@ __global__ __launch_bounds__(TILE_THREADS) void grouped_tile_kernel(GroupedParam
                 const int e = e0 + lane;
                 int first = 0, end = 0;
                 if (e < p.E) group_rows(p.offsets, e, p.R, first, end);
-                const int tiles = (end - first + TM - 1) / TM;
+                const int tiles = (end - first + 64 * XM - 1) / (64 * XM);
                 int inc = tiles;
 #pragma unroll
                 for (int off = 1; off < 64; off <<= 1) {
@@ -526,26 +529,26 @@ __global__ __launch_bounds__(TILE_THREADS) void grouped_tile_kernel(GroupedParam
         // ---- loads, splits, writes
         const int u = tid & 127;
         if (tid < 128) {
-            typedef std::conditional_t<Shape::AK, SideK<MODE, true, FAR>, SideM<MODE, true, FAR>> Side;
-            Stager<MODE, Side> s{p, list, tile_lds, first, step, u};
+            typedef std::conditional_t<Shape::AK, SideK<MODE, true, FAR, 4 * XM>, SideM<MODE, true, FAR>> Side;
+            Stager<MODE, XM, Side> s{p, list, tile_lds, first, step, u};
             s.run();
         } else {
-            typedef std::conditional_t<Shape::BK, SideK<MODE, false, FAR>, SideM<MODE, false, FAR>> Side;
-            Stager<MODE, Side> s{p, list, tile_lds + 3 * PIECE, first, step, u};
+            typedef std::conditional_t<Shape::BK, SideK<MODE, false, FAR, 8>, SideM<MODE, false, FAR>> Side;
+            Stager<MODE, XM, Side> s{p, list, tile_lds + 3 * PIECE, first, step, u};
             s.run();
         }
         return;
     }
     // ---- fragments, matrix instructions, results
     const int cw = (tid >> 6) - 4, wm = cw >> 1, wn = cw & 1;
-    const char *a_base = tile_lds + wm * 64 * TK * 2;
+    const char *a_base = tile_lds + wm * 32 * XM * TK * 2;
     const char *b_base = tile_lds + 3 * PIECE + wn * 64 * TK * 2;
     const int frag[2] = {chunk_at(lane & 31, lane >> 5), chunk_at(lane & 31, 2 + (lane >> 5))};
     // pieces of the half unit that is multiplied: [piece][sub-tile]
-    bf16x8 a[3][2], b[3][2];
-    auto fetch = [&](bf16x8(&f)[2], const char *base, int slot, int half, int piece) {
+    bf16x8 a[3][XM], b[3][2];
+    auto fetch = [&](auto &f, const char *base, int slot, int half, int piece) {
 #pragma unroll
-        for (int x = 0; x < 2; x++)
+        for (int x = 0; x < (int)(sizeof(f) / sizeof(f[0])); x++)
             f[x] = *reinterpret_cast<const bf16x8 *>(base + slot * UNIT + frag[half] + piece * PIECE + x * 32 * TK * 2);
     };
     reader_barrier();
@@ -558,11 +561,11 @@ __global__ __launch_bounds__(TILE_THREADS) void grouped_tile_kernel(GroupedParam
     int slot = 0;
     Tile t;
     for (int i = first; list.get(p, i, t); i += step) {
-        floatx16 acc[2][2][2];
+        floatx16 acc[2][XM][2];
 #pragma unroll
         for (int q = 0; q < 2; q++)
 #pragma unroll
-            for (int x = 0; x < 2; x++)
+            for (int x = 0; x < XM; x++)
 #pragma unroll
                 for (int y = 0; y < 2; y++)
 #pragma unroll
@@ -570,9 +573,9 @@ __global__ __launch_bounds__(TILE_THREADS) void grouped_tile_kernel(GroupedParam
         for (int k0 = 0; k0 < t.red; k0 += TK) {
 #pragma unroll
             for (int o = 0; o < Shape::OPS; o++) {
-                auto mul = [&](const bf16x8(&x)[2], const bf16x8(&y)[2]) {
+                auto mul = [&](const bf16x8(&x)[XM], const bf16x8(&y)[2]) {
 #pragma unroll
-                    for (int i = 0; i < 2; i++)
+                    for (int i = 0; i < XM; i++)
 #pragma unroll
                         for (int j = 0; j < 2; j++)
                             acc[o > 0][i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
@@ -584,7 +587,7 @@ __global__ __launch_bounds__(TILE_THREADS) void grouped_tile_kernel(GroupedParam
                     // the small products first; a piece is read anew, for the next half unit, as
                     // soon as its last product is issued (the high ones are needed to the end)
                     const int from = half == 0 ? slot : after, other = 1 - half;
-                    bf16x8 ah[2], bh[2];
+                    bf16x8 ah[XM], bh[2];
                     fetch(ah, a_base, from, other, 0);
                     fetch(bh, b_base, from, other, 0);
                     mul(a[2], b[0]);
@@ -602,10 +605,9 @@ __global__ __launch_bounds__(TILE_THREADS) void grouped_tile_kernel(GroupedParam
                     fetch(b[1], b_base, from, other, 1);
                     mul(a[0], b[0]);
 #pragma unroll
-                    for (int x = 0; x < 2; x++) {
-                        a[0][x] = ah[x];
-                        b[0][x] = bh[x];
-                    }
+                    for (int x = 0; x < XM; x++) a[0][x] = ah[x];
+#pragma unroll
+                    for (int y = 0; y < 2; y++) b[0][y] = bh[y];
                 }
                 slot = after;
                 reader_barrier();
@@ -620,11 +622,11 @@ __global__ __launch_bounds__(TILE_THREADS) void grouped_tile_kernel(GroupedParam
             const bool both = c + 1 < t.c_end;
             const size_t base = (MODE == GROUPED_DW ? (size_t)t.e * p.N * p.K : 0) + c;
 #pragma unroll
-            for (int x = 0; x < 2; x++)
+            for (int x = 0; x < XM; x++)
 #pragma unroll
                 for (int v0 = 0; v0 < 16; v0 += 4) {   // four rows at a time: registers
                     float2_any f[4];
-                    const int pos = wm * 64 + x * 32 + 2 * v0 + 4 * (lane >> 5);
+                    const int pos = (wm * XM + x) * 32 + 2 * v0 + 4 * (lane >> 5);
 #pragma unroll
                     for (int v = 0; v < 4; v++) {
                         const int m = min(t.m0 + row_at<Shape::AK>(pos + v), t.m_end - 1);
@@ -652,7 +654,7 @@ __global__ __launch_bounds__(TILE_THREADS) void grouped_tile_kernel(GroupedParam
                 }
         } else {
 #pragma unroll
-            for (int x = 0; x < 2; x++)
+            for (int x = 0; x < XM; x++)
 #pragma unroll
                 for (int y = 0; y < 2; y++) {
                     const int c = t.c0 + wn * 64 + y * 32 + (lane & 31);
@@ -664,7 +666,7 @@ __global__ __launch_bounds__(TILE_THREADS) void grouped_tile_kernel(GroupedParam
                     }
 #pragma unroll
                     for (int v = 0; v < 16; v++) {
-                        const int m = t.m0 + wm * 64 + x * 32 + 8 * (v >> 2) + 4 * (lane >> 5) + (v & 3);
+                        const int m = t.m0 + (wm * XM + x) * 32 + 8 * (v >> 2) + 4 * (lane >> 5) + (v & 3);
                         if (m >= t.m_end) continue;
                         store_activated(p.act, acc[0][x][y][v] + b0, acc[1][x][y][v] + b1,
                                         (size_t)m * p.N + c, out0, out1, p.out2);
@@ -781,48 +783,69 @@ __global__ __launch_bounds__(DB_WAVES * 64) void grouped_db_kernel(GroupedParams
 
 inline int ceil_div(int a, int b) { return (a + b - 1) / b; }
 
-template <int MODE, bool FAR>
+template <int MODE, int XM, bool FAR>
 hipError_t tile_launch(const GroupedParams &p, long long tiles, hipStream_t stream) {
     static PerDeviceOnce once;
     hipError_t e = allow_dynamic_lds(
-        once, reinterpret_cast<const void *>(&grouped_tile_kernel<MODE, FAR>), TILE_LDS);
+        once, reinterpret_cast<const void *>(&grouped_tile_kernel<MODE, XM, FAR>), TILE_LDS);
     if (e != hipSuccess) return e;
     // one workgroup per CU at most; every XCD the same number
     const long long most = num_cu() / 8 * 8, want = (tiles + 7) / 8 * 8;
-    hipLaunchKernelGGL((grouped_tile_kernel<MODE, FAR>), dim3((unsigned)(want < most ? want : most)),
+    hipLaunchKernelGGL((grouped_tile_kernel<MODE, XM, FAR>), dim3((unsigned)(want < most ? want : most)),
                        dim3(TILE_THREADS), TILE_LDS, stream, p);
     return hipGetLastError();
 }
 
-// How a call runs on the tiles: parts of the reduction, and the time in us that this is
-// expected to take. Few tiles of long reductions leave most of the chip idle: taken in parts /
-// in one piece, 8000 rows of 4096 -> 128: forward 158 / 367 us; 6826 rows, 2 experts of 529 ->
-// 20: weight backward 42 / 350 us.
+// Byte offsets from a tile's first row fit 32 bits (K, N <= 2^22), those of gathered rows while
+// the activations have fewer than 2^30 elements.
+bool far_offsets(const GroupedParams &p) {
+    return (p.rows != nullptr && (long long)p.T * p.K >= (1LL << 30)) || p.K > (1 << 22) || p.N > (1 << 22);
+}
+
+// How a call runs on the tiles: their height, parts of the reduction, and the time in us that
+// this is expected to take (fitted to the measurements here).
+//   Height: with up to 64 rows per expert a tile of 128 is half empty, with more it reads the
+//   weights half as often. 64 / 128 rows: 256 rows, 8 experts of 2048 -> 4096: forward 189 /
+//   255, state backward 123 / 170 us; 512 rows: 313 / 254, 206 / 177.
+//   Parts: few tiles of long reductions leave most of the chip idle. In parts / in one piece:
+//   8000 rows of 4096 -> 128: forward 158 / 367 us; 6826 rows, 2 experts of 529 -> 20: weight
+//   backward 42 / 350 us.
+// Groups of up to `rows` rows: of experts that are 30% smaller, average and 30% larger.
+double row_groups(int R, int used, int rows) {
+    const double each = (double)R / used / rows;
+    return used * (std::ceil(0.7 * each) + std::ceil(each) + std::ceil(1.3 * each)) / 3;
+}
+
 struct TilePlan {
-    long long tiles;
-    int splits;
+    int xm, splits;    // 64 xm rows to a tile
+    long long tiles;   // at most
     double us;
 };
 constexpr int MAX_SPLITS = 16;
 
-TilePlan plan_tiles(GroupedMode mode, int K, int N, int E, int R) {
-    const long long used = E < R ? E : R;
-    const long long cols = mode == GROUPED_FWD ? N : K;
-    // (tiles as they come: a part tile for most experts)
-    const long long row_tiles = std::max(R / TM + used / 2, used);
-    const long long tiles = mode == GROUPED_DW ? (long long)ceil_div(K, TM) * ceil_div(N, TM) * E
-                                               : row_tiles * ceil_div((int)cols, TM);
-    const double out = mode == GROUPED_DW ? (double)E * N * K : (double)R * cols;
-    const int red = mode == GROUPED_FWD ? K : mode == GROUPED_DZ ? N : (int)(R / used);
+TilePlan plan_tiles(GroupedMode mode, const GroupedParams &p) {
+    const int used = p.E < p.R ? p.E : p.R;
+    const int cols = mode == GROUPED_FWD ? p.N : p.K;
+    const int red = mode == GROUPED_FWD ? p.K : mode == GROUPED_DZ ? p.N : p.R / used;
     const int units = ceil_div(red, TK);
-    // (more where an expert's weights pass through one row of tiles only, all from memory)
-    const double unit_us = (mode == GROUPED_FWD ? 2.6 : 1.75) * (mode != GROUPED_DW && row_tiles <= used ? 1.4 : 1);
-    const double room = (double)grouped_scratch_floats(K, N, E, R);
-    TilePlan best = {tiles, 1, 12 + unit_us * ((tiles + num_cu() - 1) / num_cu()) * units};
-    // four units to a part at least; the parts are written and read once more
-    for (int s = 2; s <= MAX_SPLITS && tiles * s <= num_cu() && units / s >= 4 && 2 * out * s <= room; s++) {
-        const double us = 30 + unit_us * ceil_div(units, s) + 16 * out * s / 4e6;
-        if (us < best.us) best = {tiles, s, us};
+    const double out = mode == GROUPED_DW ? (double)p.E * p.N * p.K : (double)p.R * cols;
+    const double room = (double)grouped_scratch_floats(p.K, p.N, p.E, p.R);
+    TilePlan best = {2, 1, 0, 1e30};
+    const bool both = mode != GROUPED_DW && !far_offsets(p);
+    for (int xm = both ? 1 : 2; xm <= 2; xm++) {
+        const long long rows = (long long)row_groups(p.R, used, 64 * xm), most = p.R / (64 * xm) + used;
+        const long long blocks = ceil_div(cols, TM);
+        const long long tiles = mode == GROUPED_DW ? (long long)ceil_div(p.K, TM) * ceil_div(p.N, TM) * p.E : rows * blocks;
+        const double unit_us = mode == GROUPED_FWD ? (xm == 1 ? 2.4 : 3.2) : (xm == 1 ? 1.4 : 2.0);
+        // Four units to a part at least; the parts are written and read once more, and have to
+        // run at once (with some room, where the tiles depend on the experts' rows).
+        for (int s = 1; s <= MAX_SPLITS; s++) {
+            const long long wgs = tiles * s + (mode == GROUPED_DW || used == 1 ? 0 : tiles * s / 4);
+            if (s > 1 && (wgs > num_cu() || units / s < 4 || 2 * out * s > room)) break;
+            const double us = s == 1 ? 12 + unit_us * ((tiles + num_cu() - 1) / num_cu()) * units
+                                     : 22 + unit_us * ceil_div(units, s) + 16 * out * s / 4e6;
+            if (us < best.us) best = {xm, s, s * (mode == GROUPED_DW ? tiles : most * blocks), us};
+        }
     }
     return best;
 }
@@ -833,21 +856,22 @@ TilePlan plan_tiles(GroupedMode mode, int K, int N, int E, int R) {
 // chip, because their groups of 32 rows by 16 (forward) or 64 (state backward) outputs are
 // many more, and where the tiles would be mostly empty. Measured, few rows / tiles, and the
 // two formulas were fitted to these (us):
-//   forward         777 rows,  6 experts,  301 ->  415   15 /  45
-//                   192        8          2048 -> 4096  183 / 260
-//                   256        8          2048 -> 4096  264 / 265
-//                   512        8          2048 -> 4096  440 / 275
-//                   512        8          1024 -> 1024   61 /  57
-//                   256        4          2048 ->  512   49 /  42
-//                  2048        8           512 ->  512   58 /  62
-//                  1024        8          2048 -> 2048  393 / 216
-//                  8000        1          4096 ->  128  421 / 154
-//   state backward  777        6           301 ->  415   16 /  44
-//                   256        8          2048 -> 4096  155 / 177
-//                   512        8          2048 -> 4096  251 / 187
-//                  2048        8           512 ->  512   44 /  41
-//                  1024        8          2048 -> 2048  199 / 141
-//                  6826        2           529 ->   20   46 /  27
+//   forward         777 rows,  6 experts,  301 ->  415   15 /  33
+//                   192        8          2048 -> 4096  183 / 190
+//                   256        8          2048 -> 4096  251 / 189
+//                   512        8          2048 -> 4096  415 / 254
+//                   512        8          1024 -> 1024   60 /  54
+//                   256        4          2048 ->  512   48 /  34
+//                  2048        8           512 ->  512   58 /  47
+//                  1024        8          2048 -> 2048  383 / 206
+//                  8000        1          4096 ->  128  399 / 145
+//   state backward  777        6           301 ->  415   15 /  34
+//                   192        8          2048 -> 4096   83 / 117
+//                   256        8          2048 -> 4096  156 / 123
+//                   512        8          2048 -> 4096  249 / 172
+//                  2048        8           512 ->  512   43 /  32
+//                  1024        8          2048 -> 2048  198 / 136
+//                  6826        2           529 ->   20   46 /  24
 // The weight backward has as many tiles as the weights: few rows only (777 rows: 89 / 31 us).
 bool streams(GroupedMode mode, const GroupedParams &p) {
     // (its grid: one workgroup per sixteen outputs of every group of rows)
@@ -856,10 +880,10 @@ bool streams(GroupedMode mode, const GroupedParams &p) {
     if (cols * (p.R / 16 + used) >= 1LL << 26) return false;
     if ((long long)p.R <= 16LL * p.E) return true;
     if (mode == GROUPED_DW) return false;
-    const double groups = p.R / 32 + 0.5 * used;
+    const double groups = row_groups(p.R, (int)used, 32);
     const double rows_us = mode == GROUPED_FWD ? 8 + 2.4e-6 * groups * p.N * p.K
                                                : 8 + groups * (1.3e-6 * p.N * p.K + 0.02 * ceil_div(p.K, 64));
-    return rows_us < plan_tiles(mode, p.K, p.N, p.E, p.R).us;
+    return rows_us < plan_tiles(mode, p).us;
 }
 
 }  // namespace
@@ -878,7 +902,7 @@ hipError_t launch_grouped(GroupedMode mode, const GroupedParams &params, hipStre
     const bool vec = p.K >= 4 && p.N >= 4;
     if (!vec || (g_grouped_rows >= 0 ? g_grouped_rows != 0 : streams(mode, p)))
         return launch_grouped_rows(mode, p, vec, stream);
-    const TilePlan plan = plan_tiles(mode, p.K, p.N, p.E, p.R);
+    const TilePlan plan = plan_tiles(mode, p);
     const int cols = mode == GROUPED_FWD ? p.N : p.K;
     p.splits = plan.splits;
     p.part = 0;
@@ -890,19 +914,19 @@ hipError_t launch_grouped(GroupedMode mode, const GroupedParams &params, hipStre
         p.e0 = nullptr;
         p.act = ACT_NONE;
     }
-    // byte offsets from a tile's first row fit 32 bits (K, N <= 2^22), those of gathered rows
-    // while the activations have fewer than 2^30 elements
-    const bool far = (p.rows != nullptr && (long long)p.T * p.K >= (1LL << 30)) || p.K > (1 << 22) || p.N > (1 << 22);
-    // row tiles over all groups: every group ends with at most one part tile
-    const long long row_tiles = p.R / TM + (p.E < p.R ? p.E : p.R);
-    const long long tiles = p.splits * (mode == GROUPED_DW ? plan.tiles : row_tiles * ceil_div(cols, TM));
+    const bool far = far_offsets(p), low = plan.xm == 1;
     hipError_t e;
     if (mode == GROUPED_FWD)
-        e = far ? tile_launch<GROUPED_FWD, true>(p, tiles, stream) : tile_launch<GROUPED_FWD, false>(p, tiles, stream);
+        e = far   ? tile_launch<GROUPED_FWD, 2, true>(p, plan.tiles, stream)
+            : low ? tile_launch<GROUPED_FWD, 1, false>(p, plan.tiles, stream)
+                  : tile_launch<GROUPED_FWD, 2, false>(p, plan.tiles, stream);
     else if (mode == GROUPED_DZ)
-        e = far ? tile_launch<GROUPED_DZ, true>(p, tiles, stream) : tile_launch<GROUPED_DZ, false>(p, tiles, stream);
+        e = far   ? tile_launch<GROUPED_DZ, 2, true>(p, plan.tiles, stream)
+            : low ? tile_launch<GROUPED_DZ, 1, false>(p, plan.tiles, stream)
+                  : tile_launch<GROUPED_DZ, 2, false>(p, plan.tiles, stream);
     else
-        e = far ? tile_launch<GROUPED_DW, true>(p, tiles, stream) : tile_launch<GROUPED_DW, false>(p, tiles, stream);
+        e = far ? tile_launch<GROUPED_DW, 2, true>(p, plan.tiles, stream)
+                : tile_launch<GROUPED_DW, 2, false>(p, plan.tiles, stream);
     if (e != hipSuccess) return e;
     if (p.splits > 1) {
         const dim3 grid(p.R / JOIN_ROWS + (p.E < p.R ? p.E : p.R), ceil_div(JOIN_ROWS * ((cols + 3) / 4), TPB));

@@ -445,12 +445,16 @@ void rows_dz(const GroupedParams &p, unsigned slots, hipStream_t stream) {
 }  // namespace
 
 hipError_t launch_grouped_rows(GroupedMode mode, const GroupedParams &p, bool vec, hipStream_t stream) {
-    // two groups of sixteen rows share a pass over the weights where experts have more than
-    // eight rows on average; one group leaves registers for twice the waves
-    const bool one = (long long)p.R <= 8LL * p.E;
-    // groups of rows at most, experts that can have rows
+    // experts that can have rows
     const int used = p.E < p.R ? p.E : p.R;
-    const unsigned slots = p.R / (one ? 16 : 32) + used;
+    // Two groups of sixteen rows share a pass over the weights where experts have more than
+    // eight rows on average; one group leaves registers for twice the waves, which is also
+    // better where the forward's blocks are few (two groups / one: 87 rows, 3 experts of 3878
+    // -> 37: 37 / 24 us; 40 rows, 2 experts of 4096 -> 512: 43 / 33; 777 rows, 6 experts of 301
+    // -> 200: 12 / 17).
+    const bool one = (long long)p.R <= 8LL * p.E ||
+                     (mode == GROUPED_FWD && (p.R / 16 + used) * ((p.N + 15LL) / 16) <= 256);
+    const unsigned slots = p.R / (one ? 16 : 32) + used;   // groups of rows at most
     if (mode == GROUPED_FWD) {
         const unsigned blocks = (p.N + 15) / 16, grid = blocks * slots;
         // Waves that share a block: many blocks fill the chip with few waves each, which
