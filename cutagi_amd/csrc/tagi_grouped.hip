@@ -40,6 +40,13 @@ constexpr int MAX_GROUPS = 1024;
 // The two kinds meet at one barrier per unit, 32 reduction elements of one product (mean;
 // variance, one or two), 48 matrix instructions per wave: while unit u is multiplied, its
 // second half and the first half of unit u + 1 are read from LDS and unit u + 2 is written.
+//
+// Bound by the matrix instructions at the clock that the power limit leaves: the forward of
+// 8192 rows, 8 experts of 2048 -> 4096, takes 2070 us (1.20 PFLOP/s of bf16 products, 199 TFLOP/s
+// of fp32 ones, where the fp32 matrix instructions end at 157) and 1611 us with nothing but its
+// matrix instructions left; the backward of 4096 -> 2048 takes 3010 us. (2815 us for the forward
+// with 16-element units, half lines per load and fragments read when they were needed; 8105 us
+// with fp32 products on plain tiles.)
 // ---------------------------------------------------------------------------
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -724,10 +731,12 @@ __global__ __launch_bounds__(TPB) void grouped_join_kernel(GroupedParams p) {
     *reinterpret_cast<float4_any *>(p.out1 + at) = v * f * f;
 }
 
-// Bias innovations of one expert's columns, 2^cw_log (up to sixteen) groups of four of them to
+// Bias innovations of one expert's columns, 2^cw_log (up to eight) groups of four of them to
 // a workgroup: the other bits of the thread index are rows, four of them in flight each. The
 // row threads of a wave are joined by lane exchanges, the waves in their order.
-constexpr int DB_WAVES = 16, DB_GROUPS = 16;
+// Groups of a workgroup 4 / 8 / 16 / 32, with the weight backward of eight inputs before it: 8192
+// rows, 8 experts of 2048 outputs 140 / 120 / 122 / 133 us, of 512 50 / 47 / 54 / 70.
+constexpr int DB_WAVES = 16, DB_GROUPS = 8;
 __global__ __launch_bounds__(DB_WAVES * 64) void grouped_db_kernel(GroupedParams p, int cw_log) {
     __shared__ float s[2][DB_WAVES][DB_GROUPS * 4];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, cw = 1 << cw_log;

@@ -20,8 +20,10 @@ constexpr int TPB = 256;
 //   gate next to one keeps its slope
 // Lane j of the token keeps choice j (top_k <= 64, and <= the lanes where those are fewer).
 // A round is a chain of dependent instructions and bound by their latency: the maximum goes
-// through lane permutations inside the vector unit (16384 tokens, 64 experts, 4 choices: 123 us
-// with the ones through LDS and 128 tokens per workgroup, CHOOSE_US us with these and 32).
+// through lane permutations inside the vector unit (16384 tokens, 64 experts, 4 choices, whole
+// call: 129 us with the ones through LDS and 128 tokens per workgroup, 24 us with these and 32,
+// of which this kernel takes 15.5, the scan 5.9 and the rows 3.7). 32 tokens of 16 experts go
+// through one launch: 4.0 us.
 // ---------------------------------------------------------------------------
 constexpr int ROUTE_TOKENS = 32;   // tokens of a workgroup of the plan, a bit each
 
@@ -266,6 +268,8 @@ __global__ __launch_bounds__(TPB) void route_place_kernel(int T, int E, int k, R
 // The gated sum, four features of one token per thread. A choice without a row (slot < 0, or a
 // slot that is no row) adds nothing.
 //   mu_z = sum_j g y,  var_z = sum_j (g^2 + var_g) var_y + var_g y^2
+// Bound by memory: 8 bytes per choice and feature in, 8 per feature out. 8192 tokens, 2 choices
+// of 4096: 155 us, 5.2 TB/s.
 // ---------------------------------------------------------------------------
 __global__ __launch_bounds__(TPB) void combine_fwd_kernel(
     const float *__restrict__ mu_g, const float *__restrict__ var_g,
@@ -304,6 +308,9 @@ __global__ __launch_bounds__(TPB) void combine_fwd_kernel(
 //   rows    dmu_y = g dmu,  dvar_y = g^2 dvar
 //   scores  dmu_s[e] = jcb_g sum_n y dmu,  dvar_s[e] = jcb_g^2 sum_n y^2 dvar;
 //           zero for the experts that the token did not choose
+// A wave or a workgroup per token, so that its sums stay inside one. Bound by memory: 12 bytes
+// per choice and feature (innovations are read once, for further choices from cache), 8 per
+// feature. 8192 tokens, 2 choices of 4096: 214 us, 5.0 TB/s.
 template <int THREADS>
 __global__ __launch_bounds__(TPB) void combine_bwd_kernel(
     const float *__restrict__ mu_g, const float *__restrict__ jcb_g,
@@ -371,7 +378,8 @@ __global__ __launch_bounds__(TPB) void combine_bwd_kernel(
     }
 }
 
-// Rows back to tokens: (sum_j rows[slot] + res) * jcb, jcb^2.
+// Rows back to tokens: (sum_j rows[slot] + res) * jcb, jcb^2. Bound by memory. A token's rows
+// are few and known, so they are gathered in order and nothing has to be added atomically.
 __global__ __launch_bounds__(TPB) void gather_bwd_kernel(
     const float *__restrict__ dmu_r, const float *__restrict__ dvar_r,
     const int *__restrict__ slot, const float *__restrict__ jcb, const float *res_mu,
