@@ -14,12 +14,16 @@ using namespace tagi;
 namespace {
 
 constexpr int MAX_EXPERTS = 1024, MAX_TOP_K = 64;
-constexpr long long MAX_INT = 0x7fffffffLL;
 
 hipStream_t as_stream(void *s) { return static_cast<hipStream_t>(s); }
 
-// `columns`: width of the output, `weights`: whether it is [E][N][K]. The launches number
-// their tiles in one grid of fewer than 2^32 threads: 64 x 64 elements a tile, 256 threads.
+// Sizes that the kernels' indices hold with what is added to them.
+constexpr int MAX_SIZE = 1 << 30;
+
+// `columns`: width of the output, `weights`: whether it is [E][N][K]. A launch holds fewer than
+// 2^32 threads: the weight backward's kernels have up to 1024 for 32 outputs by 256 inputs, the
+// ones for few rows (and for fewer than four inputs or outputs any rows) up to 512 for sixteen
+// rows by sixteen columns.
 int grouped_sizes(int K, int N, int E, int R, int T, const int *rows, int columns, bool weights) {
     if (K <= 0 || N <= 0 || E <= 0 || R <= 0 || (rows != nullptr && T <= 0))
         return TAGI_ERR_INVALID_ARG;
@@ -28,14 +32,15 @@ int grouped_sizes(int K, int N, int E, int R, int T, const int *rows, int column
     if (K > (1 << 24) || N > (1 << 24)) return TAGI_ERR_UNSUPPORTED;
     if (rows != nullptr && (long long)T * K > (1LL << 32) - 1) return TAGI_ERR_UNSUPPORTED;
     const double tiles = (columns + 63) / 64 * ((double)R / 64 + E);
-    const double weight_tiles = weights ? (double)((K + 63) / 64) * ((N + 63) / 64) * E : 0;
-    const double most = (double)(1 << 24) - 1;
-    return tiles > most || weight_tiles > most ? TAGI_ERR_UNSUPPORTED : TAGI_OK;
+    const double weight_wgs = weights ? (double)((K + 255) / 256) * ((N + 31) / 32) * E : 0;
+    if (tiles > (1 << 24) - 1 || weight_wgs > (1 << 22) - 1) return TAGI_ERR_UNSUPPORTED;
+    const double few = K < 4 || N < 4 ? (columns + 15) / 16 * ((double)R / 16 + E) : 0;
+    return few > (1 << 23) - 1 ? TAGI_ERR_UNSUPPORTED : TAGI_OK;
 }
 
 int moe_sizes(int T, int k, int R, int N) {
     if (T <= 0 || k <= 0 || R <= 0 || N <= 0) return TAGI_ERR_INVALID_ARG;
-    return (long long)T * k > MAX_INT ? TAGI_ERR_UNSUPPORTED : TAGI_OK;
+    return (long long)T * k > MAX_SIZE || N > MAX_SIZE ? TAGI_ERR_UNSUPPORTED : TAGI_OK;
 }
 
 // whether the scratch that a call needs is there, 16-byte aligned
@@ -75,6 +80,7 @@ int tagi_layernorm_fwd(const float *mu_w, const float *var_w, const float *mu_b,
         return TAGI_ERR_INVALID_ARG;
     if (bias && (!mu_b || !var_b)) return TAGI_ERR_INVALID_ARG;
     if (n < 2 || B <= 0) return TAGI_ERR_INVALID_ARG;
+    if (n > MAX_SIZE || B > MAX_SIZE) return TAGI_ERR_UNSUPPORTED;
     TAGI_TRY(launch_layernorm_fwd(mu_w, var_w, bias ? mu_b : nullptr, bias ? var_b : nullptr, mu_a,
                                   var_a, epsilon, n, B, mu_s, var_s, mu_z, var_z,
                                   as_stream(stream)));
@@ -83,6 +89,7 @@ int tagi_layernorm_fwd(const float *mu_w, const float *var_w, const float *mu_b,
 
 int tagi_layernorm_bwd_scratch(int n, int B, size_t *bytes) {
     if (bytes == nullptr || n < 2 || B <= 0) return TAGI_ERR_INVALID_ARG;
+    if (n > MAX_SIZE || B > MAX_SIZE) return TAGI_ERR_UNSUPPORTED;
     *bytes = layernorm_bwd_scratch_floats(n, B) * sizeof(float);
     return TAGI_OK;
 }
@@ -100,6 +107,7 @@ int tagi_layernorm_bwd(const float *mu_w, const float *var_w, const float *var_b
     if (param_update && bias && (!var_b || !delta_mu_b || !delta_var_b))
         return TAGI_ERR_INVALID_ARG;
     if (n < 2 || B <= 0) return TAGI_ERR_INVALID_ARG;
+    if (n > MAX_SIZE || B > MAX_SIZE) return TAGI_ERR_UNSUPPORTED;
     if (!state_update && !param_update) return TAGI_OK;
     if (param_update && !scratch_ok(scratch, layernorm_bwd_scratch_floats(n, B))) return TAGI_ERR_INVALID_ARG;
     TAGI_TRY(launch_layernorm_bwd(mu_w, var_w, bias ? var_b : nullptr, mu_a, jcb, mu_s, var_s,
@@ -184,7 +192,8 @@ int tagi_moe_route(const float *mu_s, const float *var_s, int T, int E, int top_
     if (!mu_s || !var_s || !expert || !mu_g || !var_g || !jcb_g || !offsets || !token || !slot)
         return TAGI_ERR_INVALID_ARG;
     if (T <= 0 || E <= 0 || top_k <= 0 || top_k > E) return TAGI_ERR_INVALID_ARG;
-    if (E > MAX_EXPERTS || top_k > MAX_TOP_K || (long long)T * top_k > MAX_INT)
+    // (32 tokens to a workgroup of 256 threads)
+    if (E > MAX_EXPERTS || top_k > MAX_TOP_K || (long long)T * top_k > MAX_SIZE || T >= 1 << 29)
         return TAGI_ERR_UNSUPPORTED;
     if (moe_route_scratch_ints(T, E) > 0 && !scratch) return TAGI_ERR_INVALID_ARG;
     TAGI_TRY(launch_moe_route(mu_s, var_s, T, E, top_k, expert, mu_g, var_g, jcb_g, offsets, token,
@@ -214,6 +223,7 @@ int tagi_moe_combine_bwd(const float *mu_g, const float *jcb_g, const float *mu_
     const int rc = moe_sizes(T, top_k, R, N);
     if (rc != TAGI_OK) return rc;
     if (E <= 0) return TAGI_ERR_INVALID_ARG;
+    if (E > MAX_SIZE) return TAGI_ERR_UNSUPPORTED;
     TAGI_TRY(launch_moe_combine_bwd(mu_g, jcb_g, mu_y, expert, slot, delta_mu, delta_var, T, top_k,
                                     R, N, E, delta_mu_y, delta_var_y, delta_mu_s, delta_var_s,
                                     as_stream(stream)));

@@ -883,10 +883,10 @@ TilePlan plan_tiles(GroupedMode mode, const GroupedParams &p) {
 //                  6826        2           529 ->   20   46 /  24
 // The weight backward has as many tiles as the weights: few rows only (777 rows: 89 / 31 us).
 bool streams(GroupedMode mode, const GroupedParams &p) {
-    // (its grid: one workgroup per sixteen outputs of every group of rows)
+    // (their grids: up to 1024 threads for sixteen outputs of every group of rows)
     const long long used = p.E < p.R ? p.E : p.R;
     const long long cols = mode == GROUPED_FWD ? p.N : p.K;
-    if (cols * (p.R / 16 + used) >= 1LL << 26) return false;
+    if ((cols + 15) / 16 * (p.R / 16 + used) >= 1LL << 22) return false;
     if ((long long)p.R <= 16LL * p.E) return true;
     if (mode == GROUPED_DW) return false;
     const double groups = row_groups(p.R, (int)used, 32);

@@ -485,7 +485,9 @@ int tagi_layernorm_bwd(const float *mu_w, const float *var_w, const float *var_b
  * int[R]) row r takes its activations from row rows[r] of the T rows of mu_a / var_a, so a
  * token that several experts see is stored once; an entry outside 0..T-1 stands for a row
  * of zeros. Offsets outside 0..R are moved to its ends. E <= 1024, K and N <= 2^24, with
- * rows T K < 2^32 (TAGI_ERR_UNSUPPORTED beyond). The same bits every call. No counterpart in
+ * rows T K < 2^32, tiles of 64 x 64 outputs and of 32 x 256 weights that number fewer than
+ * 2^24 and 2^22 (TAGI_ERR_UNSUPPORTED beyond). The same bits every call. Infinities may come
+ * out as NaN: calls of many rows take fp32 numbers apart into three parts. No counterpart in
  * the reference, which has one Linear per layer; the arithmetic of a group is
  * tagi_linear_fwd's and tagi_linear_bwd's. */
 

@@ -142,3 +142,28 @@ def test_replays_of_a_graph():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(held, want)), "replay %d" % i
+
+
+def test_more_than_32_bit_offsets():
+    """The last rows of 2^31 elements and more: each row as in a call of its own, the parameter
+    innovations those of the only rows that have any (five of them)."""
+    import torch
+    import cutagi_amd.functional as F
+    n, few = 4100, 5
+    B = (1 << 19) + few
+    d = C.norm_inputs(few, n, seed=10)
+    t = _dev(d)
+    whole = {}
+    for name in ("mu_a", "var_a", "dmu", "dvar"):
+        whole[name] = torch.zeros(B, n, device="cuda")
+        whole[name][B - few:] = t[name]
+    args = (t["mu_w"], t["var_w"], t["mu_b"], t["var_b"])
+    want = F.layernorm_fwd(*args, t["mu_a"], t["var_a"], EPS)
+    got = F.layernorm_fwd(*args, whole["mu_a"], whole["var_a"], EPS)
+    for g, w in zip(got, want):
+        assert torch.equal(g[B - few:], w)
+    grads = F.layernorm_bwd(t["mu_w"], t["var_w"], t["var_b"], whole["mu_a"], None, got[2], got[3], whole["dmu"],
+                            whole["dvar"], EPS)
+    ref = C.norm_bwd(d, _host(want[2]), _host(want[3]), EPS, False)
+    for name, g in zip(("dz_mu", "dz_var", "dw_mu", "dw_var", "db_mu", "db_var"), grads):
+        C.check(_host(g[B - few:] if name[:2] == "dz" else g), *ref[name], name)

@@ -34,6 +34,10 @@ def test_layernorm_refuses():
     size = ctypes.c_size_t(0)
     assert L.tagi_layernorm_bwd_scratch(8, 4, None) == capi.ERR_INVALID_ARG
     assert L.tagi_layernorm_bwd_scratch(1, 4, ctypes.byref(size)) == capi.ERR_INVALID_ARG
+    for n, B in ((8, (1 << 30) + 1), ((1 << 30) + 1, 8)):
+        assert L.tagi_layernorm_fwd(*(fwd[:8] + [n, B] + fwd[10:])) == capi.ERR_UNSUPPORTED
+        assert L.tagi_layernorm_bwd(*(bwd[:10] + [n, B] + bwd[12:])) == capi.ERR_UNSUPPORTED
+        assert L.tagi_layernorm_bwd_scratch(n, B, ctypes.byref(size)) == capi.ERR_UNSUPPORTED
     # nothing asked for: done
     assert L.tagi_layernorm_bwd(*([one] * 9 + [1e-5, 8, 4, 1, 0, 0] + [None] * 8)) == capi.OK
 
@@ -72,6 +76,11 @@ def test_grouped_linear_refuses():
     assert L.tagi_grouped_linear_fwd(*huge) == capi.ERR_UNSUPPORTED
     huge = [one] * 9 + [1 << 30, 1 << 30, 1024, 16, 16, 1, 0, 1] + [one] * 7 + [None]
     assert L.tagi_grouped_linear_bwd(*huge) == capi.ERR_UNSUPPORTED
+    # more threads than a launch holds: weights in pieces of 32 x 256, rows of one or two inputs
+    huge = [one] * 9 + [4, 1 << 24, 1024, 16, 16, 1, 0, 1] + [one] * 7 + [None]
+    assert L.tagi_grouped_linear_bwd(*huge) == capi.ERR_UNSUPPORTED
+    huge = [one] * 8 + [1, 1, 4, 1 << 28, 16, 1] + [one] * 3 + [None]
+    assert L.tagi_grouped_linear_fwd(*huge) == capi.ERR_UNSUPPORTED
     # scratch that is needed and missing, or not 16-byte aligned
     size = capi.grouped_linear_scratch(256, 128, 4, 400)
     assert size > 0

@@ -171,6 +171,47 @@ def test_indices_outside_the_arrays_read_nothing(kernel_choice):
         C.check(_host(g), *C.grouped_bwd(d)[name], name)
 
 
+@pytest.mark.parametrize("sizes,K,N,tail", [([5, 0, 9], 40, 36, 6), ([100, 31], 130, 64, 90), ([300, 0, 90], 600, 130, 20)])
+def test_rows_behind_the_last_group_are_not_read(kernel_choice, sizes, K, N, tail):
+    import torch
+    import cutagi_amd.functional as F
+    d = C.grouped_inputs(sizes, K, N, seed=3, tail=tail)
+    t, total = _dev(d), sum(sizes)
+    for name in ("mu_a", "var_a", "jcb", "dmu", "dvar"):
+        t[name][total:] = float("nan")
+    out = F.grouped_linear_fwd(t["mu_w"], t["var_w"], t["mu_b"], t["var_b"], t["mu_a"], t["var_a"], t["offsets"])
+    want = {k: (v[0][:total], v[1][:total]) for k, v in C.grouped_fwd(d).items()}
+    for name, g in zip(("mu_z", "var_z"), out):
+        C.check(_host(g)[:total], *want[name], name)
+    got = F.grouped_linear_bwd(t["mu_w"], t["var_w"], t["var_b"], t["mu_a"], t["jcb"], t["dmu"], t["dvar"],
+                               t["offsets"])
+    for name, g in zip(BWD, got):
+        g = _host(g)
+        C.check(g[:total] if name[:2] == "dz" else g, *C.grouped_bwd(d)[name], name)
+
+
+def test_tokens_beyond_32_bit_offsets(kernel_choice):
+    """The last tokens of activations of more than 2^31 elements."""
+    import torch
+    import cutagi_amd.functional as F
+    K, N, held, T = 16, 24, 50, (1 << 27) + 9
+    d = C.grouped_inputs([150, 0, 40], K, N, seed=6, tokens=held)
+    t = _dev(d)
+    for name in ("mu_a", "var_a"):
+        whole = torch.zeros(T, K, device="cuda")
+        whole[T - held:] = t[name]
+        t[name] = whole
+    rows = t["rows"] + (T - held)
+    got = F.grouped_linear_fwd(t["mu_w"], t["var_w"], t["mu_b"], t["var_b"], t["mu_a"], t["var_a"],
+                               t["offsets"], rows)
+    for name, g in zip(("mu_z", "var_z"), got):
+        C.check(_host(g), *C.grouped_fwd(d)[name], name)
+    got = F.grouped_linear_bwd(t["mu_w"], t["var_w"], t["var_b"], t["mu_a"], t["jcb"], t["dmu"],
+                               t["dvar"], t["offsets"], rows)
+    for name, g in zip(BWD, got):
+        C.check(_host(g), *C.grouped_bwd(d)[name], name)
+
+
 def test_one_group_is_the_linear_layer(kernel_choice):
     """E = 1 against the ungrouped entry points (each is within its own bound of the exact
     result, so they are within twice that of one another)."""
@@ -318,6 +359,34 @@ def test_gated_sum(T, E, k, N):
                              [d[r] for r in res] if res else None)
             C.check(_host(g[0]), *w["mu"], "gathered mu")
             C.check(_host(g[1]), *w["var"], "gathered var")
+
+
+def test_gated_sum_of_rows_beyond_32_bit_offsets():
+    """The last rows of expert outputs of more than 2^31 elements."""
+    import torch
+    import cutagi_amd.functional as F
+    T, E, k, N = 6, 4, 2, 4100
+    d = _gated(T, E, k, N, seed=5)
+    t, held = _dev(d), T * k
+    R = (1 << 19) + held
+    for name in ("mu_y", "var_y"):
+        whole = torch.zeros(R, N, device="cuda")
+        whole[R - held:] = t[name]
+        t[name] = whole
+    slot = torch.where(t["slot"] >= 0, t["slot"] + (R - held), t["slot"])
+    got = F.moe_combine_fwd(t["mu_g"], t["var_g"], t["mu_y"], t["var_y"], slot)
+    for name, g in zip(("mu_z", "var_z"), got):
+        C.check(_host(g), *C.combine_fwd(d["mu_g"], d["var_g"], d["mu_y"], d["var_y"], d["slot"])[name], name)
+    g = F.moe_gather_bwd(t["mu_y"], t["var_y"], slot)
+    w = C.gather_bwd(d["mu_y"], d["var_y"], d["slot"])
+    C.check(_host(g[0]), *w["mu"], "gathered mu")
+    C.check(_host(g[1]), *w["var"], "gathered var")
+    got = F.moe_combine_bwd(t["mu_g"], t["jcb_g"], t["mu_y"], t["expert"], slot, t["dmu"], t["dvar"], E)
+    want = C.combine_bwd(d["mu_g"], d["jcb_g"], d["mu_y"], d["expert"], d["slot"], d["dmu"], d["dvar"], E)
+    for name, g in zip(("dy_mu", "dy_var", "ds_mu", "ds_var"), got):
+        value, bound = want[name]
+        g, live = _host(g[R - held:] if name[:2] == "dy" else g), ~np.isnan(value)
+        C.check(g[live], value[live], bound[live], name)
 
 
 # ---- as they are used ------------------------------------------------------------------------
