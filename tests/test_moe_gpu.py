@@ -212,6 +212,41 @@ def test_tokens_beyond_32_bit_offsets(kernel_choice):
         C.check(_host(g), *C.grouped_bwd(d)[name], name)
 
 
+@pytest.mark.parametrize("sizes,K,N", [([300, 0, 90], 600, 130), ([700, 31], 523, 20)])
+def test_two_graphs_replayed_side_by_side(sizes, K, N):
+    """Calls that take their reductions in parts, recorded twice: each recording holds scratch
+    memory of its own."""
+    import torch
+    import cutagi_amd.functional as F
+    from cutagi_amd import capi
+    assert capi.grouped_linear_scratch(K, N, len(sizes), sum(sizes)) > 0
+    t = _dev(C.grouped_inputs(sizes, K, N, seed=8, tokens=200))
+
+    def both():
+        z = F.grouped_linear_fwd(t["mu_w"], t["var_w"], t["mu_b"], t["var_b"], t["mu_a"], t["var_a"],
+                                 t["offsets"], t["rows"])
+        return z + F.grouped_linear_bwd(t["mu_w"], t["var_w"], t["var_b"], t["mu_a"], t["jcb"], t["dmu"],
+                                        t["dvar"], t["offsets"], t["rows"])
+    both()
+    torch.cuda.synchronize()
+    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+    held = []
+    for g in graphs:
+        with torch.cuda.graph(g):
+            held.append(both())
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for i in range(4):
+        t["mu_a"].mul_(-1.1)
+        want = both()
+        torch.cuda.synchronize()
+        for g, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                g.replay()
+        torch.cuda.synchronize()
+        for out in held:
+            assert all(torch.equal(a, b) for a, b in zip(out, want)), "replay %d" % i
+
+
 def test_one_group_is_the_linear_layer(kernel_choice):
     """E = 1 against the ungrouped entry points (each is within its own bound of the exact
     result, so they are within twice that of one another)."""
