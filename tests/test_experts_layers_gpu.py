@@ -175,6 +175,34 @@ def test_residual_block_and_evaluation_mode():
         assert np.array_equal(g.ravel(), x.cpu().numpy().ravel()), keys
 
 
+def test_two_blocks_through_the_python_layer():
+    """Blocks one behind the other, batches of different sizes: finite, and a step moves every
+    layer's parameters."""
+    from cutagi_amd import cutagi
+    from cutagi_amd.nn import (LayerBlock, LayerNorm, Linear, MixtureOfExperts, OutputUpdater, ReLU, ResNetBlock,
+                               Sequential)
+    cutagi.manual_seed(3)
+    experts = lambda: ResNetBlock(LayerBlock(LayerNorm(64), MixtureOfExperts(64, 256, 64, num_experts=8, top_k=2)))
+    net = Sequential(Linear(32, 64), ReLU(), experts(), experts(), LayerNorm(64), Linear(64, 10))
+    net.to_device("cuda")
+    updater = OutputUpdater(net.device)
+    rng = np.random.default_rng(3)
+    before = net.state_dict()
+    for batch in (16, 3, 64, 16):
+        mu, var = net(rng.standard_normal(batch * 32).astype(np.float32))
+        assert np.all(np.isfinite(mu)) and np.all(np.asarray(var) > 0)
+        updater.update(net.output_z_buffer, rng.standard_normal(batch * 10).astype(np.float32),
+                       np.full(batch * 10, 0.5, np.float32), net.input_delta_z_buffer)
+        net.backward()
+        net.step()
+    after = net.state_dict()
+    assert sorted(after) == sorted(before) and len(after) >= 6
+    for name in after:
+        for a, b in zip(after[name], before[name]):
+            assert len(a) == len(b) and np.all(np.isfinite(a))
+            assert len(a) == 0 or np.any(np.asarray(a) != np.asarray(b)), name
+
+
 def test_checkpoints(tmp_path):
     from cutagi_amd import cutagi
     net, other = _net(cutagi, seed=0), _net(cutagi, seed=1)
