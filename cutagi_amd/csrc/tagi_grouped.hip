@@ -623,59 +623,86 @@ __global__ __launch_bounds__(TILE_THREADS) void grouped_tile_kernel(GroupedParam
         float *out0 = p.out0 + t.part * p.part, *out1 = p.out1 + t.part * p.part;
         // register v of lane l: row 8 (v / 4) + 4 (l / 32) + v % 4, column l % 32
         if constexpr (!Shape::BK) {
-            // the two column sub-tiles hold neighbouring columns
+            // The two column sub-tiles hold neighbouring columns; four rows at a time. All sums are
+            // scaled before any is stored, with three groups of factors on their way: a load
+            // behind stores would be waited for together with them (256 rows, 8 experts of
+            // 2048 -> 2048, weight backward, loads and stores in turn / apart: 157 / 112 us).
             const int c = t.c0 + row_at<false>(wn * 64 + (lane & 31));
             if (c >= t.c_end) continue;
             const bool both = c + 1 < t.c_end;
             const size_t base = (MODE == GROUPED_DW ? (size_t)t.e * p.N * p.K : 0) + c;
+            constexpr int GROUPS = XM * 4;
+            auto row = [&](int g, int v, int half) {
+                return t.m0 + row_at<Shape::AK>((wm * XM + g / 4) * 32 + 8 * (g % 4) + 4 * half + v);
+            };
+            int half = lane >> 5;
+            if (p.e0 != nullptr) {
+                constexpr int AHEAD = 3;
+                float2_any f[AHEAD][4];
+                auto load = [&](int g) {
 #pragma unroll
-            for (int x = 0; x < XM; x++)
+                    for (int v = 0; v < 4; v++)   // (the last column alone: with the one before it)
+                        f[g % AHEAD][v] = *reinterpret_cast<const float2_any *>(
+                            p.e0 + base - (both ? 0 : 1) + (size_t)min(row(g, v, half), t.m_end - 1) * p.K);
+                };
 #pragma unroll
-                for (int v0 = 0; v0 < 16; v0 += 4) {   // four rows at a time: registers
-                    float2_any f[4];
-                    const int pos = (wm * XM + x) * 32 + 2 * v0 + 4 * (lane >> 5);
+                for (int g = 0; g < AHEAD; g++) load(g);
+#pragma unroll
+                for (int g = 0; g < GROUPS; g++) {
+                    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                     for (int v = 0; v < 4; v++) {
-                        const int m = min(t.m0 + row_at<Shape::AK>(pos + v), t.m_end - 1);
-                        const float *e = p.e0 + base + (size_t)m * p.K;
-                        f[v] = p.e0 == nullptr ? (float2_any){1.f, 1.f}
-                               : both          ? *reinterpret_cast<const float2_any *>(e)
-                                               : (float2_any){e[0], 1.f};
-                    }
-#pragma unroll
-                    for (int v = 0; v < 4; v++) {
-                        const int m = t.m0 + row_at<Shape::AK>(pos + v);
-                        if (m >= t.m_end) continue;
-                        const size_t at = base + (size_t)m * p.K;
-                        const float2_any s0 = (float2_any){acc[0][x][0][v0 + v], acc[0][x][1][v0 + v]} * f[v];
-                        const float2_any s1 = (float2_any){acc[1][x][0][v0 + v], acc[1][x][1][v0 + v]} * f[v] * f[v];
-                        if (both) {
-                            *reinterpret_cast<float2_any *>(out0 + at) = s0;
-                            *reinterpret_cast<float2_any *>(out1 + at) = s1;
-                        } else {
-                            out0[at] = s0[0];
-                            out1[at] = s1[0];
-                        }
+                        const float2_any w = f[g % AHEAD][v];
+                        const float w0 = both ? w[0] : w[1], w1 = w[1];
+                        const int x = g / 4, i = 4 * (g % 4) + v;
+                        acc[0][x][0][i] *= w0;
+                        acc[0][x][1][i] *= w1;
+                        acc[1][x][0][i] *= w0 * w0;
+                        acc[1][x][1][i] *= w1 * w1;
                     }
                     __builtin_amdgcn_sched_barrier(0);
+                    if (g + AHEAD < GROUPS) load(g + AHEAD);
                 }
+            }
+            asm volatile("" : "+v"(half));   // (the addresses are not worth keeping until here)
+#pragma unroll
+            for (int g = 0; g < GROUPS; g++) {
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int v = 0; v < 4; v++) {
+                    const int m = row(g, v, half), x = g / 4, i = 4 * (g % 4) + v;
+                    if (m >= t.m_end) continue;
+                    const size_t at = base + (size_t)m * p.K;
+                    if (both) {
+                        *reinterpret_cast<float2_any *>(out0 + at) = (float2_any){acc[0][x][0][i], acc[0][x][1][i]};
+                        *reinterpret_cast<float2_any *>(out1 + at) = (float2_any){acc[1][x][0][i], acc[1][x][1][i]};
+                    } else {
+                        out0[at] = acc[0][x][0][i];
+                        out1[at] = acc[1][x][0][i];
+                    }
+                }
+            }
         } else {
+            float b0[2] = {0.f, 0.f}, b1[2] = {0.f, 0.f};
+            const int c0 = t.c0 + wn * 64 + (lane & 31);
+            if (p.e0 != nullptr)   // (ahead of all stores, as above)
+#pragma unroll
+                for (int y = 0; y < 2; y++) {
+                    const size_t at = (size_t)t.e * p.N + min(c0 + y * 32, p.N - 1);
+                    b0[y] = p.e0[at];
+                    b1[y] = p.e1[at];
+                }
 #pragma unroll
             for (int x = 0; x < XM; x++)
 #pragma unroll
                 for (int y = 0; y < 2; y++) {
-                    const int c = t.c0 + wn * 64 + y * 32 + (lane & 31);
+                    const int c = c0 + y * 32;
                     if (c >= t.c_end) continue;
-                    float b0 = 0.f, b1 = 0.f;
-                    if (p.e0 != nullptr) {
-                        b0 = p.e0[(size_t)t.e * p.N + c];
-                        b1 = p.e1[(size_t)t.e * p.N + c];
-                    }
 #pragma unroll
                     for (int v = 0; v < 16; v++) {
                         const int m = t.m0 + (wm * XM + x) * 32 + 8 * (v >> 2) + 4 * (lane >> 5) + (v & 3);
                         if (m >= t.m_end) continue;
-                        store_activated(p.act, acc[0][x][y][v] + b0, acc[1][x][y][v] + b1,
+                        store_activated(p.act, acc[0][x][y][v] + b0[y], acc[1][x][y][v] + b1[y],
                                         (size_t)m * p.N + c, out0, out1, p.out2);
                     }
                 }
