@@ -44,7 +44,7 @@ constexpr int MAX_GROUPS = 1024;
 // Bound by the matrix instructions at the clock that the power limit leaves: the forward of
 // 8192 rows, 8 experts of 2048 -> 4096, takes 2070 us (1.20 PFLOP/s of bf16 products, 199 TFLOP/s
 // of fp32 ones, where the fp32 matrix instructions end at 157) and 1611 us with nothing but its
-// matrix instructions left; the backward of 4096 -> 2048 takes 3010 us. (2815 us for the forward
+// matrix instructions left; the backward of 4096 -> 2048 takes 2990 us. (2815 us for the forward
 // with 16-element units, half lines per load and fragments read when they were needed; 8105 us
 // with fp32 products on plain tiles.)
 // ---------------------------------------------------------------------------
@@ -908,14 +908,18 @@ TilePlan plan_tiles(GroupedMode mode, const GroupedParams &p) {
 //                  2048        8           512 ->  512   43 /  32
 //                  1024        8          2048 -> 2048  198 / 136
 //                  6826        2           529 ->   20   46 /  24
-// The weight backward has as many tiles as the weights: few rows only (777 rows: 89 / 31 us).
+// The weight backward has as many tiles as the weights: few rows only, the fewer where the
+// weights are many. 8 / 12 / 16 rows per expert, few rows / tiles: 8 experts of 2048 -> 2048
+// 104 / 103, 122 / 104, 139 / 105 us; 4 of 1024 -> 1024 16.5 / 22, 17.5 / 22, 20 / 22 us (with
+// the launch of the bias innovations, which the kernel for few rows does itself).
 bool streams(GroupedMode mode, const GroupedParams &p) {
     // (their grids: up to 1024 threads for sixteen outputs of every group of rows)
     const long long used = p.E < p.R ? p.E : p.R;
     const long long cols = mode == GROUPED_FWD ? p.N : p.K;
     if ((cols + 15) / 16 * (p.R / 16 + used) >= 1LL << 22) return false;
-    if ((long long)p.R <= 16LL * p.E) return true;
-    if (mode == GROUPED_DW) return false;
+    if (mode == GROUPED_DW)
+        return p.R <= 8LL * p.E || (p.R <= 16LL * p.E && (double)p.E * p.N * p.K <= 1 << 23);
+    if (p.R <= 16LL * p.E) return true;
     const double groups = row_groups(p.R, (int)used, 32);
     const double rows_us = mode == GROUPED_FWD ? 8 + 2.4e-6 * groups * p.N * p.K
                                                : 8 + groups * (1.3e-6 * p.N * p.K + 0.02 * ceil_div(p.K, 64));
