@@ -144,7 +144,15 @@ def test_replays_of_a_graph():
         assert all(torch.equal(a, b) for a, b in zip(held, want)), "replay %d" % i
 
 
-def test_more_than_32_bit_offsets():
+@pytest.fixture
+def large_memory():
+    """Gives the memory back to the device afterwards."""
+    import torch
+    yield
+    torch.cuda.empty_cache()
+
+
+def test_more_than_32_bit_offsets(large_memory):
     """The last rows of 2^31 elements and more: each row as in a call of its own, the parameter
     innovations those of the only rows that have any (five of them)."""
     import torch

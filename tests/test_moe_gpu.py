@@ -29,6 +29,14 @@ def kernel_choice(request):
     capi.tune("grouped.rows", -1)
 
 
+@pytest.fixture
+def large_memory():
+    """Gives the memory back to the device afterwards."""
+    import torch
+    yield
+    torch.cuda.empty_cache()
+
+
 # (rows of the experts, K, N, tokens or None, rows behind the last group)
 GROUPS = [
     ([1], 1, 1, None, 0),
@@ -50,6 +58,9 @@ GROUPS = [
     ([130, 700, 0, 450], 4100, 72, 300, 5),
     ([130, 700, 0, 450], 72, 4100, None, 5),
     ([33, 90, 40], 1300, 1284, 100, 0),
+    # the same with tiles of 64 rows
+    ([50, 64, 0, 33] * 9, 40, 1284, 60, 0),
+    ([50, 64, 0, 33] * 9, 1284, 40, None, 3),
     # long reductions of few tiles, taken in parts: of every pass, and parts of no rows
     ([700, 0, 300, 5], 523, 20, None, 3),
     ([40, 0, 200, 31], 2051, 37, 90, 0),
@@ -190,7 +201,7 @@ def test_rows_behind_the_last_group_are_not_read(kernel_choice, sizes, K, N, tai
         C.check(g[:total] if name[:2] == "dz" else g, *C.grouped_bwd(d)[name], name)
 
 
-def test_tokens_beyond_32_bit_offsets(kernel_choice):
+def test_tokens_beyond_32_bit_offsets(kernel_choice, large_memory):
     """The last tokens of activations of more than 2^31 elements."""
     import torch
     import cutagi_amd.functional as F
@@ -396,7 +407,7 @@ def test_gated_sum(T, E, k, N):
             C.check(_host(g[1]), *w["var"], "gathered var")
 
 
-def test_gated_sum_of_rows_beyond_32_bit_offsets():
+def test_gated_sum_of_rows_beyond_32_bit_offsets(large_memory):
     """The last rows of expert outputs of more than 2^31 elements."""
     import torch
     import cutagi_amd.functional as F
