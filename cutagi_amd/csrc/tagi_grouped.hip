@@ -485,11 +485,82 @@ struct Stager {
     }
 };
 
+// The functions below take four columns to a thread; the last four of a row start at its end less
+// four, so that some columns are taken twice, with the same result.
+__device__ __forceinline__ void add4(float4_any &sum, const float *p) {
+    sum += *reinterpret_cast<const float4_any *>(p);
+}
+
+// Bias innovations of one expert's columns, 2^db_log (up to eight) groups of four of them to a
+// workgroup: the other bits of the thread index are rows, four of them in flight each. The
+// row threads of a wave are joined by lane exchanges, the waves in their order. Groups of a
+// workgroup 4 / 8 / 16 / 32, with the weight backward of eight inputs before it: 8192 rows, 8
+// experts of 2048 outputs 140 / 120 / 122 / 133 us, of 512 50 / 47 / 54 / 70.
+constexpr int DB_GROUPS = 8;
+
+template <int WAVES>
+__device__ __forceinline__ void bias_sums(const GroupedParams &p, int block, float (*s)[WAVES][DB_GROUPS * 4]) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, cw = 1 << p.db_log;
+    const int blocks = ((p.N + 3) / 4 + cw - 1) >> p.db_log, e = block / blocks;
+    const int c0 = (block - e * blocks) * cw * 4;
+    int first, end;
+    group_rows(p.offsets, e, p.R, first, end);
+    float4_any m[4], v[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) m[i] = v[i] = (float4_any){0.f, 0.f, 0.f, 0.f};
+    const int step = (WAVES * 64) >> p.db_log;
+    const size_t col = min(c0 + 4 * ((int)threadIdx.x & (cw - 1)), p.N - 4);
+    const float *x = p.x0 + col, *y = p.x1 + col;
+    long long r = first + (threadIdx.x >> p.db_log);
+    for (; r + 3 * step < end; r += 4 * step)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            add4(m[i], x + (r + i * step) * p.N);
+            add4(v[i], y + (r + i * step) * p.N);
+        }
+    for (; r < end; r += step) {
+        add4(m[0], x + r * p.N);
+        add4(v[0], y + r * p.N);
+    }
+    m[0] = (m[0] + m[1]) + (m[2] + m[3]);
+    v[0] = (v[0] + v[1]) + (v[2] + v[3]);
+#pragma unroll
+    for (int c = 0; c < 4; c++) {
+        float sm = m[0][c], sv = v[0][c];
+        for (int off = 32; off >= cw; off >>= 1) {
+            sm += __shfl_xor(sm, off, 64);
+            sv += __shfl_xor(sv, off, 64);
+        }
+        if (lane < cw) {
+            s[0][wave][4 * lane + c] = sm;
+            s[1][wave][4 * lane + c] = sv;
+        }
+    }
+    __syncthreads();
+    const int t = threadIdx.x, want = c0 + (t & ~3);
+    if (t >= 4 * cw || want >= p.N) return;
+    float sm = 0.f, sv = 0.f;
+#pragma unroll
+    for (int w = 0; w < WAVES; w++) {
+        sm += s[0][w][t];
+        sv += s[1][w][t];
+    }
+    const size_t at = (size_t)e * p.N + min(want, p.N - 4) + (t & 3);
+    const float vb = p.e1[at];
+    p.db0[at] = vb * sm;
+    p.db1[at] = vb * vb * sv;
+}
+
 template <int MODE, int XM, bool FAR>
 __global__ __launch_bounds__(TILE_THREADS) void grouped_tile_kernel(GroupedParams p) {
     extern __shared__ __attribute__((aligned(16))) char tile_lds[];
     typedef TileShape<MODE> Shape;
     const int tid = threadIdx.x, lane = tid & 63;
+    if (MODE == GROUPED_DW && (int)blockIdx.x >= p.tile_wgs) {
+        bias_sums<TILE_THREADS / 64>(p, blockIdx.x - p.tile_wgs,
+                                     reinterpret_cast<float(*)[TILE_THREADS / 64][DB_GROUPS * 4]>(tile_lds));
+        return;
+    }
     int *prefix = reinterpret_cast<int *>(tile_lds + RING * UNIT);
 
     TileList<MODE, XM> list;
@@ -530,7 +601,7 @@ __global__ __launch_bounds__(TILE_THREADS) void grouped_tile_kernel(GroupedParam
         list.lo = (int)(total * (blockIdx.x & 7) / 8);
         list.count = (int)(total * ((blockIdx.x & 7) + 1) / 8) - list.lo;
     }
-    const int first = blockIdx.x >> 3, step = gridDim.x >> 3;
+    const int first = blockIdx.x >> 3, step = p.tile_wgs >> 3;
 
     if (tid < 256) {
         // ---- loads, splits, writes
@@ -710,12 +781,6 @@ __global__ __launch_bounds__(TILE_THREADS) void grouped_tile_kernel(GroupedParam
     }
 }
 
-// The kernels below take four columns to a thread; the last four of a row start at its end less
-// four, so that some columns are taken twice, with the same result.
-__device__ __forceinline__ void add4(float4_any &sum, const float *p) {
-    sum += *reinterpret_cast<const float4_any *>(p);
-}
-
 // The parts of a divided reduction, in order, and what the tile kernel would have done with
 // their sums (p.x0, p.x1: the parts' outputs).
 constexpr int JOIN_ROWS = 8;
@@ -758,77 +823,21 @@ __global__ __launch_bounds__(TPB) void grouped_join_kernel(GroupedParams p) {
     *reinterpret_cast<float4_any *>(p.out1 + at) = v * f * f;
 }
 
-// Bias innovations of one expert's columns, 2^cw_log (up to eight) groups of four of them to
-// a workgroup: the other bits of the thread index are rows, four of them in flight each. The
-// row threads of a wave are joined by lane exchanges, the waves in their order.
-// Groups of a workgroup 4 / 8 / 16 / 32, with the weight backward of eight inputs before it: 8192
-// rows, 8 experts of 2048 outputs 140 / 120 / 122 / 133 us, of 512 50 / 47 / 54 / 70.
-constexpr int DB_WAVES = 16, DB_GROUPS = 8;
-__global__ __launch_bounds__(DB_WAVES * 64) void grouped_db_kernel(GroupedParams p, int cw_log) {
+constexpr int DB_WAVES = 16;
+__global__ __launch_bounds__(DB_WAVES * 64) void grouped_db_kernel(GroupedParams p) {
     __shared__ float s[2][DB_WAVES][DB_GROUPS * 4];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, cw = 1 << cw_log;
-    const int blocks = ((p.N + 3) / 4 + cw - 1) >> cw_log, e = blockIdx.x / blocks;
-    const int c0 = (blockIdx.x - e * blocks) * cw * 4;
-    int first, end;
-    group_rows(p.offsets, e, p.R, first, end);
-    float4_any m[4], v[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) m[i] = v[i] = (float4_any){0.f, 0.f, 0.f, 0.f};
-    const int step = (DB_WAVES * 64) >> cw_log;
-    const size_t col = min(c0 + 4 * ((int)threadIdx.x & (cw - 1)), p.N - 4);
-    const float *x = p.x0 + col, *y = p.x1 + col;
-    long long r = first + (threadIdx.x >> cw_log);
-    for (; r + 3 * step < end; r += 4 * step)
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            add4(m[i], x + (r + i * step) * p.N);
-            add4(v[i], y + (r + i * step) * p.N);
-        }
-    for (; r < end; r += step) {
-        add4(m[0], x + r * p.N);
-        add4(v[0], y + r * p.N);
-    }
-    m[0] = (m[0] + m[1]) + (m[2] + m[3]);
-    v[0] = (v[0] + v[1]) + (v[2] + v[3]);
-#pragma unroll
-    for (int c = 0; c < 4; c++) {
-        float sm = m[0][c], sv = v[0][c];
-        for (int off = 32; off >= cw; off >>= 1) {
-            sm += __shfl_xor(sm, off, 64);
-            sv += __shfl_xor(sv, off, 64);
-        }
-        if (lane < cw) {
-            s[0][wave][4 * lane + c] = sm;
-            s[1][wave][4 * lane + c] = sv;
-        }
-    }
-    __syncthreads();
-    const int t = threadIdx.x, want = c0 + (t & ~3);
-    if (t >= 4 * cw || want >= p.N) return;
-    float sm = 0.f, sv = 0.f;
-#pragma unroll
-    for (int w = 0; w < DB_WAVES; w++) {
-        sm += s[0][w][t];
-        sv += s[1][w][t];
-    }
-    const size_t at = (size_t)e * p.N + min(want, p.N - 4) + (t & 3);
-    const float vb = p.e1[at];
-    p.db0[at] = vb * sm;
-    p.db1[at] = vb * vb * sv;
+    bias_sums<DB_WAVES>(p, blockIdx.x, s);
 }
 
 inline int ceil_div(int a, int b) { return (a + b - 1) / b; }
 
 template <int MODE, int XM, bool FAR>
-hipError_t tile_launch(const GroupedParams &p, long long tiles, hipStream_t stream) {
+hipError_t tile_launch(const GroupedParams &p, unsigned wgs, hipStream_t stream) {
     static PerDeviceOnce once;
     hipError_t e = allow_dynamic_lds(
         once, reinterpret_cast<const void *>(&grouped_tile_kernel<MODE, XM, FAR>), TILE_LDS);
     if (e != hipSuccess) return e;
-    // one workgroup per CU at most; every XCD the same number
-    const long long most = num_cu() / 8 * 8, want = (tiles + 7) / 8 * 8;
-    hipLaunchKernelGGL((grouped_tile_kernel<MODE, XM, FAR>), dim3((unsigned)(want < most ? want : most)),
-                       dim3(TILE_THREADS), TILE_LDS, stream, p);
+    hipLaunchKernelGGL((grouped_tile_kernel<MODE, XM, FAR>), dim3(wgs), dim3(TILE_THREADS), TILE_LDS, stream, p);
     return hipGetLastError();
 }
 
@@ -955,18 +964,32 @@ hipError_t launch_grouped(GroupedMode mode, const GroupedParams &params, hipStre
         p.act = ACT_NONE;
     }
     const bool far = far_offsets(p), low = plan.xm == 1;
+    // one workgroup per CU at most; every XCD the same number
+    p.tile_wgs = (int)std::min<long long>(num_cu() / 8 * 8, (plan.tiles + 7) / 8 * 8);
+    // The bias innovations go along where there are CUs left for all of them, and get a launch
+    // of their own, in larger workgroups, where not (apart / along, weight backward of 777 rows,
+    // 6 experts of 301 -> 415: 26 / 22 us, of 6826 rows, 2 experts of 529 -> 20: 41 / 31 us).
+    unsigned wgs = p.tile_wgs, db_wgs = 0;
+    if (mode == GROUPED_DW && p.db0 != nullptr) {
+        while ((1 << p.db_log) < DB_GROUPS && (4 << p.db_log) < p.N) p.db_log++;
+        db_wgs = (unsigned)ceil_div(ceil_div(p.N, 4), 1 << p.db_log) * p.E;
+        if (wgs + db_wgs <= (unsigned)num_cu()) {
+            wgs += db_wgs;
+            db_wgs = 0;
+        }
+    }
     hipError_t e;
     if (mode == GROUPED_FWD)
-        e = far   ? tile_launch<GROUPED_FWD, 2, true>(p, plan.tiles, stream)
-            : low ? tile_launch<GROUPED_FWD, 1, false>(p, plan.tiles, stream)
-                  : tile_launch<GROUPED_FWD, 2, false>(p, plan.tiles, stream);
+        e = far   ? tile_launch<GROUPED_FWD, 2, true>(p, wgs, stream)
+            : low ? tile_launch<GROUPED_FWD, 1, false>(p, wgs, stream)
+                  : tile_launch<GROUPED_FWD, 2, false>(p, wgs, stream);
     else if (mode == GROUPED_DZ)
-        e = far   ? tile_launch<GROUPED_DZ, 2, true>(p, plan.tiles, stream)
-            : low ? tile_launch<GROUPED_DZ, 1, false>(p, plan.tiles, stream)
-                  : tile_launch<GROUPED_DZ, 2, false>(p, plan.tiles, stream);
+        e = far   ? tile_launch<GROUPED_DZ, 2, true>(p, wgs, stream)
+            : low ? tile_launch<GROUPED_DZ, 1, false>(p, wgs, stream)
+                  : tile_launch<GROUPED_DZ, 2, false>(p, wgs, stream);
     else
-        e = far ? tile_launch<GROUPED_DW, 2, true>(p, plan.tiles, stream)
-                : tile_launch<GROUPED_DW, 2, false>(p, plan.tiles, stream);
+        e = far ? tile_launch<GROUPED_DW, 2, true>(p, wgs, stream)
+                : tile_launch<GROUPED_DW, 2, false>(p, wgs, stream);
     if (e != hipSuccess) return e;
     if (p.splits > 1) {
         const dim3 grid(p.R / JOIN_ROWS + (p.E < p.R ? p.E : p.R), ceil_div(JOIN_ROWS * ((cols + 3) / 4), TPB));
@@ -979,11 +1002,8 @@ hipError_t launch_grouped(GroupedMode mode, const GroupedParams &params, hipStre
             hipLaunchKernelGGL(grouped_join_kernel<GROUPED_DW>, flat, dim3(TPB), 0, stream, join);
         e = hipGetLastError();
     }
-    if (e != hipSuccess || mode != GROUPED_DW || p.db0 == nullptr) return e;
-    int cw_log = 0;
-    while ((1 << cw_log) < DB_GROUPS && (4 << cw_log) < p.N) cw_log++;
-    hipLaunchKernelGGL(grouped_db_kernel, dim3((unsigned)ceil_div(ceil_div(p.N, 4), 1 << cw_log) * p.E),
-                       dim3(DB_WAVES * 64), 0, stream, p, cw_log);
+    if (e != hipSuccess || db_wgs == 0) return e;
+    hipLaunchKernelGGL(grouped_db_kernel, dim3(db_wgs), dim3(DB_WAVES * 64), 0, stream, p);
     return hipGetLastError();
 }
 

@@ -352,7 +352,9 @@ struct GroupedParams {
     float *out0, *out1, *out2, *db0, *db1;
     float *scratch;   // grouped_scratch_floats of them
     int splits;       // set by launch_grouped: parts of the reduction,
-    size_t part;      // floats of one part's output
+    size_t part;      // floats of one part's output,
+    int tile_wgs;     // workgroups that walk tiles,
+    int db_log;       // groups of columns of one that sums bias innovations, log 2
 };
 // never more for fewer rows
 size_t grouped_scratch_floats(int K, int N, int E, int R);
