@@ -29,7 +29,8 @@ constexpr int MAX_GROUPS = 1024;
 // fp32's own half step. Products of two bf16 are exact in the fp32 accumulator. Six
 // instructions at 16 times the fp32 matrix rate leave 2.7 times that rate.
 // An infinity (or a magnitude beyond bf16's 3.39e38) has the residue NaN and gives NaN, where
-// fp32 arithmetic would give an infinity or NaN.
+// fp32 arithmetic would give an infinity or NaN. The last part of a number below 2^-108 (3e-33)
+// is below the normal numbers and may be lost, the middle one from 2^-117 on.
 //
 // A workgroup owns 128 x 128 tiles (64 x 128 where experts have few rows) of an output pair and walks them one after the other. Four
 // of its waves load the operands, form the sums and squares that the variance needs, split

@@ -487,7 +487,8 @@ int tagi_layernorm_bwd(const float *mu_w, const float *var_w, const float *var_b
  * of zeros. Offsets outside 0..R are moved to its ends. E <= 1024, K and N <= 2^24, with
  * rows T K < 2^32, tiles of 64 x 64 outputs and of 32 x 256 weights that number fewer than
  * 2^24 and 2^22 (TAGI_ERR_UNSUPPORTED beyond). The same bits every call. Infinities may come
- * out as NaN: calls of many rows take fp32 numbers apart into three parts. No counterpart in
+ * out as NaN, and numbers below 3e-33 count with less than fp32's precision: calls of many
+ * rows take fp32 numbers apart into three parts. No counterpart in
  * the reference, which has one Linear per layer; the arithmetic of a group is
  * tagi_linear_fwd's and tagi_linear_bwd's. */
 
