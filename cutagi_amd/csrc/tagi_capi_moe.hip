@@ -192,8 +192,8 @@ int tagi_moe_route(const float *mu_s, const float *var_s, int T, int E, int top_
     if (!mu_s || !var_s || !expert || !mu_g || !var_g || !jcb_g || !offsets || !token || !slot)
         return TAGI_ERR_INVALID_ARG;
     if (T <= 0 || E <= 0 || top_k <= 0 || top_k > E) return TAGI_ERR_INVALID_ARG;
-    // (32 tokens to a workgroup of 256 threads)
-    if (E > MAX_EXPERTS || top_k > MAX_TOP_K || (long long)T * top_k > MAX_SIZE || T >= 1 << 29)
+    // (32 tokens to a workgroup of 256 threads, and a launch holds fewer than 2^32 of them)
+    if (E > MAX_EXPERTS || top_k > MAX_TOP_K || (long long)T * top_k > MAX_SIZE || T > (1 << 29) - 32)
         return TAGI_ERR_UNSUPPORTED;
     if (moe_route_scratch_ints(T, E) > 0 && !scratch) return TAGI_ERR_INVALID_ARG;
     TAGI_TRY(launch_moe_route(mu_s, var_s, T, E, top_k, expert, mu_g, var_g, jcb_g, offsets, token,

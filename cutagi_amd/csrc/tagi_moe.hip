@@ -260,7 +260,9 @@ __global__ __launch_bounds__(TPB) void route_place_kernel(int T, int E, int k, R
         [&](int e) { return counts[(size_t)blockIdx.x * E + e]; }, s, base,
         blockIdx.x == 0 ? o.offsets : nullptr);
     place(k, t0, t1, o, mask, base);
-    for (int r = total + blockIdx.x * TPB + threadIdx.x; r < T * k; r += gridDim.x * TPB)
+    // (eight threads per token: their number alone passes 31 bits before T * k does)
+    for (long long r = total + (long long)blockIdx.x * TPB + threadIdx.x; r < (long long)T * k;
+         r += (long long)gridDim.x * TPB)
         o.token[r] = -1;
 }
 

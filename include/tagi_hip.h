@@ -540,7 +540,8 @@ int tagi_grouped_linear_bwd(const float *mu_w, const float *var_w, const float *
  *   offsets [E+1]     first row of every expert; offsets[E] rows in all
  *   token [T*top_k]   the token of every row, -1 behind the last
  * scratch: tagi_moe_route_scratch bytes of device memory, owned by the caller (may be NULL
- * where that is 0). E <= 1024, top_k <= 64 (TAGI_ERR_UNSUPPORTED beyond), top_k <= E. */
+ * where that is 0). E <= 1024, top_k <= 64, T top_k <= 2^30, T <= 2^29 - 32
+ * (TAGI_ERR_UNSUPPORTED beyond), top_k <= E. */
 int tagi_moe_route_scratch(int T, int E, size_t *bytes /* host, out */);
 int tagi_moe_route(const float *mu_s, const float *var_s, int T, int E, int top_k,
                    void *scratch, int *expert, float *mu_g, float *var_g, float *jcb_g,

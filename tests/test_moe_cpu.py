@@ -125,6 +125,17 @@ def test_router_refuses():
     assert L.tagi_moe_route_scratch(4, 4, None) == capi.ERR_INVALID_ARG
 
 
+def test_router_refuses_more_tokens_than_a_launch_holds():
+    """32 tokens to a workgroup of 256 threads: the largest plan whose launch stays below 2^32
+    threads has 2^29 - 32 tokens."""
+    capi, L = _lib()
+    route = [one, one, 0, 1, 1] + [one] * 8 + [None]
+    for T in ((1 << 29) - 31, (1 << 29) - 1, 1 << 29):
+        assert -(-T // 32) * 256 >= 1 << 32
+        assert L.tagi_moe_route(*_without(route, 2, T)) == capi.ERR_UNSUPPORTED
+
+
+
 def test_gated_sum_refuses():
     capi, L = _lib()
     fwd = [one] * 5 + [4, 2, 8, 16] + [one] * 2 + [None]

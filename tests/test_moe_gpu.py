@@ -344,6 +344,28 @@ def test_route_ties_and_masked_scores(T, E, k):
     assert _host(got.expert)[7, 0] == E - 1 and _host(got.mu_g)[7, 0] == 1
 
 
+def test_plan_of_more_tokens_than_31_bits_of_threads(large_memory):
+    """Eight threads per token look for places behind the last row: past 2^28 tokens their
+    numbers leave 31 bits."""
+    import torch
+    import cutagi_amd.functional as F
+    T = (1 << 28) + 33
+    mu = torch.zeros(T, 1, device="cuda")
+    mu[::1000] = -float("inf")
+    mu[-5:] = -float("inf")
+    live = (mu[:, 0] == 0).nonzero()[:, 0].int()
+    n = live.numel()
+    r = F.moe_route(mu, torch.full_like(mu, 0.1), 1)
+    assert r.offsets.tolist() == [0, n]
+    assert torch.equal(r.token[:n], live) and bool((r.token[n:] == -1).all())
+    slot = torch.full((T,), -1, dtype=torch.int32, device="cuda")
+    slot[live.long()] = torch.arange(n, dtype=torch.int32, device="cuda")
+    assert torch.equal(r.slot[:, 0], slot)
+    assert torch.equal(r.expert[:, 0], torch.where(slot >= 0, 0, -1).int())
+    assert torch.equal(r.mu_g, (r.expert >= 0).float())
+
+
+
 def test_slope_of_the_gates_against_differences():
     import torch
     import cutagi_amd.functional as F
