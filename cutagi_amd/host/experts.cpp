@@ -77,6 +77,30 @@ void LayerNormHip::init_weight_bias() {
     this->params_to_device();
 }
 
+void LayerNormHip::hold(int batch_size) {
+    if ((size_t)batch_size > rows_held) {
+        freed += d_mu_s != nullptr;
+        dev_free_t(d_mu_s);
+        dev_free_t(d_var_s);
+        rows_held = 0;
+        d_mu_s = dev_alloc_t<float>(batch_size, device_idx);
+        d_var_s = dev_alloc_t<float>(batch_size, device_idx);
+        rows_held = batch_size;
+    }
+    if (!training) return;
+    // the backward pass's scratch memory too: the recording of a pass allocates nothing
+    size_t bytes = 0;
+    TAGI_OK_OR_THROW(tagi_layernorm_bwd_scratch((int)input_size, batch_size, &bytes));
+    if (bytes > scratch_held) {
+        freed += d_scratch != nullptr;
+        dev_free_t(d_scratch);
+        scratch_held = 0;
+        d_scratch = dev_alloc_t<char>(bytes, device_idx);
+        scratch_held = bytes;
+    }
+    train_rows_held = std::max(train_rows_held, (size_t)batch_size);
+}
+
 // reference: LayerNormCuda::forward, src/layernorm_layer_cuda.cu
 void LayerNormHip::forward(BaseHiddenStates &input_states, BaseHiddenStates &output_states,
                            BaseTempStates &) {
@@ -90,14 +114,7 @@ void LayerNormHip::forward(BaseHiddenStates &input_states, BaseHiddenStates &out
     if (this->output_size * batch_size > out->size)
         LOG(LogLevel::ERROR, "Output state buffer too small for " + this->get_layer_info());
     if (d_mu_w == nullptr) LOG(LogLevel::ERROR, "Parameters of " + get_layer_info() + " are not on the device");
-    if ((size_t)batch_size > rows_held) {
-        dev_free_t(d_mu_s);
-        dev_free_t(d_var_s);
-        rows_held = 0;
-        d_mu_s = dev_alloc_t<float>(batch_size, device_idx);
-        d_var_s = dev_alloc_t<float>(batch_size, device_idx);
-        rows_held = batch_size;
-    }
+    this->hold(batch_size);
     TAGI_OK_OR_THROW(tagi_layernorm_fwd(d_mu_w, d_var_w, d_mu_b, d_var_b, in->d_mu_a, in->d_var_a,
                                         bias ? 1 : 0, epsilon, (int)input_size, batch_size, d_mu_s,
                                         d_var_s, out->d_mu_a, out->d_var_a, host_stream()));
@@ -119,18 +136,8 @@ void LayerNormHip::backward(BaseDeltaStates &input_delta_states, BaseDeltaStates
     const int batch_size = (int)input_delta_states.block_size;
     if (state_udapte && input_size * batch_size > dout->size)
         LOG(LogLevel::ERROR, "Delta state buffer too small for " + this->get_layer_info());
-    if ((size_t)batch_size > rows_held || bwd->d_mu_a == nullptr)
+    if ((size_t)batch_size > train_rows_held || bwd->d_mu_a == nullptr)
         LOG(LogLevel::ERROR, "Backward pass of " + this->get_layer_info() + " without its forward pass");
-    if (param_update) {
-        size_t bytes = 0;
-        TAGI_OK_OR_THROW(tagi_layernorm_bwd_scratch((int)input_size, batch_size, &bytes));
-        if (bytes > scratch_held) {
-            dev_free_t(d_scratch);
-            scratch_held = 0;
-            d_scratch = dev_alloc_t<char>(bytes, device_idx);
-            scratch_held = bytes;
-        }
-    }
     TAGI_OK_OR_THROW(tagi_layernorm_bwd(
         d_mu_w, d_var_w, d_var_b, bwd->d_mu_a, bwd->jcb_ones ? nullptr : bwd->d_jcb, d_mu_s, d_var_s,
         din->d_delta_mu, din->d_delta_var, epsilon, (int)input_size, batch_size, bias ? 1 : 0,
@@ -281,6 +288,7 @@ MixtureOfExpertsHip::Work MixtureOfExpertsHip::work(int batch) const {
 
 void MixtureOfExpertsHip::hold(int batch) {
     if ((size_t)batch <= batch_held) return;
+    freed += d_work != nullptr;
     dev_free_t(d_work);
     batch_held = 0;
     const size_t bytes = this->work(batch).bytes;

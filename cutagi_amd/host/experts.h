@@ -47,10 +47,11 @@ class LayerNormHip : public BaseLayerHip {
 
    private:
     // statistics of the rows of the last forward pass, sums of the backward pass; as large as
-    // the largest batch seen needs
+    // the largest batch seen (in training) needs
     float *d_mu_s = nullptr, *d_var_s = nullptr;
     char *d_scratch = nullptr;
-    size_t rows_held = 0, scratch_held = 0;
+    size_t rows_held = 0, train_rows_held = 0, scratch_held = 0;
+    void hold(int batch_size);
 };
 
 // ---- MixtureOfExperts --------------------------------------------------------------------

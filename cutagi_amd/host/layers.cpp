@@ -158,6 +158,7 @@ void BaseLayerHip::release_param_memory() {
 }
 
 void BaseLayerHip::allocate_param_memory() {
+    freed += d_mu_w != nullptr;
     dev_free_t(d_mu_w); dev_free_t(d_var_w); dev_free_t(d_mu_b); dev_free_t(d_var_b);
     d_mu_w = dev_alloc_t<float>(num_weights, device_idx);
     d_var_w = dev_alloc_t<float>(num_weights, device_idx);
@@ -173,6 +174,7 @@ void BaseLayerHip::allocate_param_memory() {
 
 void BaseLayerHip::allocate_param_delta() {
     BaseLayer::allocate_param_delta();
+    freed += d_delta_mu_w != nullptr;
     dev_free_t(d_delta_mu_w); dev_free_t(d_delta_var_w);
     dev_free_t(d_delta_mu_b); dev_free_t(d_delta_var_b);
     d_delta_mu_w = dev_alloc_t<float>(num_weights, device_idx);

@@ -66,6 +66,9 @@ class BaseLayer {
     std::vector<float> mu_w, var_w, mu_b, var_b;
     std::vector<float> delta_mu_w, delta_var_w, delta_mu_b, delta_var_b;
     std::unique_ptr<BaseBackwardStates> bwd_states;
+    // Device arrays of this layer, besides those of bwd_states, that were freed so far
+    // (as BaseHiddenStates::freed).
+    size_t freed = 0;
     // One-shot request to the next forward() of a layer that can_fuse_activation():
     // apply this activation (TAGI_ACT_*) in the kernel's epilogue and write its
     // moments and Jacobian instead of the layer's own output. Set by the owner of the

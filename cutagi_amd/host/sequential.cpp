@@ -340,9 +340,6 @@ void Sequential::prepare_buffers(int batch_size) {
     if (batch_size != this->z_buffer_block_size) {
         this->z_buffer_size = batch_size * (this->z_buffer_size / this->z_buffer_block_size);
         this->z_buffer_block_size = batch_size;
-        // Growing frees these buffers, and what the layers and the library hold for a batch:
-        // what was recorded refers to them, even where new ones come to lie in their place.
-        if ((size_t)this->z_buffer_size > this->input_z_buffer->size) this->clear_graphs();
         this->input_z_buffer->set_size(this->z_buffer_size, batch_size);
         this->output_z_buffer->set_size(this->z_buffer_size, batch_size);
         // a model first run in eval mode has no delta buffers yet: they are created
@@ -488,6 +485,18 @@ void Sequential::clear_graphs() {
     graphs_.clear();
 }
 
+// Arrays of the state and delta buffers and of the layers that were freed so far. They grow at
+// different times (the state buffers with the largest batch, what the layers keep for the
+// backward pass with the largest one in training, scratch memory with the pass that needs it).
+size_t Sequential::buffers_freed() const {
+    size_t n = 0;
+    for (const auto &layer : layers) n += layer->freed + layer->bwd_states->freed;
+    for (const auto *b : {input_z_buffer.get(), output_z_buffer.get()}) n += b != nullptr ? b->freed : 0;
+    for (const auto *b : {input_delta_z_buffer.get(), output_delta_z_buffer.get()})
+        n += b != nullptr ? b->freed : 0;
+    return n;
+}
+
 bool Sequential::only_plain_layers() const {
     for (const auto &layer : layers) {
         const LayerType t = layer->get_layer_type();
@@ -504,6 +513,11 @@ void Sequential::run_or_replay(const GraphKey &key, const std::function<void()> 
         body();
         return;
     }
+    // What was recorded refers to buffers that are gone, even where new ones came to lie in
+    // their place.
+    const size_t freed = this->buffers_freed();
+    if (freed != freed_when_recorded_) this->clear_graphs();
+    freed_when_recorded_ = freed;
     GraphEntry &e = graphs_[key];
     hipStream_t stream = host_stream();
     if (e.exec != nullptr) {

@@ -108,7 +108,9 @@ class Sequential {
     // ordinary stream (the null stream cannot be captured), and only networks of plain
     // layers (no LayerBlock / ResNetBlock, whose buffers trade contents) are replayed;
     // others run as before. Input transfers, the output update and step() are not part
-    // of a graph. Results are the same kernels' results either way.
+    // of a graph. A recording lasts until the model frees a buffer that it may refer to,
+    // as a batch larger than all before it does. Results are the same kernels' results
+    // either way.
     void enable_graphs(bool on);
     bool graphs_enabled() const { return graphs_on_; }
     int graphs_captured() const;  // graphs held at the moment (for tests)
@@ -155,6 +157,8 @@ class Sequential {
     using GraphKey = std::tuple<int, const void *, const void *, int, int>;
     std::map<GraphKey, GraphEntry> graphs_;
     bool graphs_on_ = false;
+    size_t freed_when_recorded_ = 0;
+    size_t buffers_freed() const;
     void clear_graphs();
     bool only_plain_layers() const;
     void run_or_replay(const GraphKey &key, const std::function<void()> &body);

@@ -272,6 +272,7 @@ void HiddenStateHip::allocate_memory() {
     this->to_device();
 }
 void HiddenStateHip::deallocate_memory() {
+    freed += d_mu_a != nullptr;
     dev_free(d_mu_a);
     dev_free(d_var_a);
     dev_free(d_jcb);
@@ -433,6 +434,7 @@ void DeltaStateHip::allocate_memory() {
     this->to_device();
 }
 void DeltaStateHip::deallocate_memory() {
+    freed += d_delta_mu != nullptr;
     dev_free(d_delta_mu);
     d_delta_var = nullptr;
 }
@@ -507,6 +509,7 @@ void BackwardStateHip::allocate_memory() {
     d_jcb = dev_alloc(size, device_idx);
 }
 void BackwardStateHip::deallocate_memory() {
+    freed += d_mu_a != nullptr;
     if (borrowed) {
         d_mu_a = d_jcb = nullptr;
         borrowed = false;

@@ -25,6 +25,9 @@ class BaseHiddenStates {
     size_t actual_size = 0;  // features per sample currently held
     size_t width = 0, height = 0, depth = 0;
     int device_idx = 0;
+    // Device arrays of this object that were freed so far (here and in the two classes
+    // below): what a recorded graph had of them is gone.
+    size_t freed = 0;
 
     BaseHiddenStates(size_t n, size_t m, int device_idx = 0);
     BaseHiddenStates() = default;
@@ -42,6 +45,7 @@ class BaseDeltaStates {
     std::vector<float> delta_mu, delta_var;
     size_t size = 0, block_size = 0, actual_size = 0;
     int device_idx = 0;
+    size_t freed = 0;
 
     BaseDeltaStates(size_t n, size_t m, int device_idx = 0);
     BaseDeltaStates() = default;
@@ -71,6 +75,7 @@ class BaseBackwardStates {
     std::vector<float> mu_a, jcb;
     size_t size = 0;
     int device_idx = 0;
+    size_t freed = 0;
 
     explicit BaseBackwardStates(int num);
     BaseBackwardStates() = default;

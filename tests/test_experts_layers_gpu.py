@@ -131,6 +131,39 @@ def test_replay_gives_the_eager_bits():
     assert all(np.all(np.isfinite(u)) for a in eager for u in a)
 
 
+@pytest.mark.parametrize("first", ["forward", "eval"])
+def test_backward_scratch_that_grows_later_drops_the_recordings(first):
+    """1024 features: 100 and 200 rows need different amounts of scratch memory for the layer
+    norm's parameter sums, and a pass of 512 rows before them leaves nothing else to grow."""
+    from cutagi_amd import capi, cutagi
+    assert 0 < capi.layernorm_bwd_scratch(1024, 100) < capi.layernorm_bwd_scratch(1024, 200)
+    rng = np.random.default_rng(5)
+    sizes = [100] * 5 + [200] + [100] * 5
+    xs = [rng.standard_normal((b, 16)).astype(np.float32) for b in sizes]
+    ys = [rng.standard_normal(b * N_OUT).astype(np.float32) for b in sizes]
+    large = rng.standard_normal((512, 16)).astype(np.float32)
+
+    def run(graphs):
+        cutagi.manual_seed(0)
+        net = cutagi.Sequential([cutagi.Linear(16, 1024), cutagi.MixtureReLU(), cutagi.LayerNorm([1024]),
+                                 cutagi.MixtureOfExperts(1024, 24, N_OUT, 4, 2)])
+        net.to_device("cuda")
+        net.enable_graphs(graphs)
+        if first == "eval":
+            net.eval()
+        net.forward(large)
+        net.train()
+        trace, params = _train(net, cutagi, xs, ys)
+        captured = net.graphs_captured()
+        net.enable_graphs(False)
+        return trace, params, captured
+    (eager, p0, _), (replay, p1, captured) = run(False), run(True)
+    for i, (a, b) in enumerate(zip(eager, replay)):
+        assert all(np.array_equal(u, w) for u, w in zip(a, b)), "outputs differ at step %d" % i
+    assert p0 == p1 and captured >= 2
+    assert all(np.all(np.isfinite(u)) for a in eager for u in a)
+
+
 def test_residual_block_and_evaluation_mode():
     """x + experts(norm(x)): the block adds the shortcut forward and its innovations back."""
     from cutagi_amd import cutagi

@@ -102,6 +102,58 @@ def test_mode_switches_and_reloads_drop_the_recordings():
     assert all(np.array_equal(p[0], q[0]) for p, q in zip(a, b)) and pa == pb
 
 
+def _eager_and_replayed(make, cutagi, steps, n_in, n_out):
+    """Runs `steps` - ("train" | "forward", batch) or "eval" / "train" - on a network with
+    graphs and on one without, and compares outputs and parameters. Returns the graphs held
+    before every step."""
+    rng = np.random.default_rng(4)
+    data = [s if isinstance(s, str) else
+            (s[0], rng.normal(0, 1, (s[1], n_in)).astype(np.float32),
+             rng.normal(0, 1, s[1] * n_out).astype(np.float32)) for s in steps]
+    held = []
+
+    def run(net, note):
+        updater = cutagi.OutputUpdater(net.device)
+        trace = []
+        for s in data:
+            if note:
+                held.append(net.graphs_captured())
+            if isinstance(s, str):
+                getattr(net, s)()
+                continue
+            kind, x, y = s
+            net.forward(x)
+            trace.append([a.copy() for a in net.get_outputs()])
+            if kind == "train":
+                updater.update(net.output_z_buffer, y, np.full(y.size, 0.5, np.float32),
+                               net.input_delta_z_buffer)
+                net.backward()
+                net.step()
+        return trace, net.state_dict()
+    eager, eager_params = run(make(cutagi), False)
+    net = make(cutagi)
+    net.enable_graphs(True)
+    replay, replay_params = run(net, True)
+    net.enable_graphs(False)
+    for i, (a, b) in enumerate(zip(eager, replay)):
+        assert all(np.array_equal(u, w) for u, w in zip(a, b)), "outputs differ at step %d" % i
+    assert all(np.all(np.isfinite(u)) for a in eager for u in a)
+    assert eager_params == replay_params
+    return held
+
+
+@pytest.mark.parametrize("make,n_in,n_out", [(_mlp, 784, 11), (_cnn, 3 * 8 * 8, 5)])
+def test_training_buffers_that_grow_later_drop_the_recordings(make, n_in, n_out):
+    """An evaluation of a larger batch first: the state buffers do not grow with the training
+    batches any more, but what the layers keep for the backward pass does."""
+    from cutagi_amd import cutagi
+    steps = ["eval", ("forward", 256), "train"] + [("train", b) for b in [32] * 5 + [64] * 2 + [32] * 5 + [64] * 4]
+    held = _eager_and_replayed(make, cutagi, steps, n_in, n_out)
+    assert held[7] == 2      # recorded at 32
+    assert held[9] == 0      # after the first step at 64: dropped
+    assert max(held[10:]) >= 2
+
+
 def test_networks_with_blocks_stay_eager():
     from cutagi_amd import cutagi
     cutagi.manual_seed(2)
