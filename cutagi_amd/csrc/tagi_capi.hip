@@ -1,5 +1,6 @@
 // C ABI of the backend (include/tagi_hip.h): argument checks, kernel selection
 // by shape, and the per-device workspace for split-reduction partial sums.
+#include <algorithm>
 #include <cstdint>
 #include <cstring>
 #include <mutex>
@@ -38,13 +39,15 @@ struct Workspace {
 // Calls on one stream are ordered by the stream and share theirs.
 struct DeviceWorkspaces {
     std::vector<std::pair<hipStream_t, Workspace>> by_stream;
+    std::vector<float *> outgrown;
 };
 DeviceWorkspaces g_ws[MAX_DEVICES];
 std::mutex g_ws_mutex;
 int g_num_cu[MAX_DEVICES];
 
-// Grow-only. Reallocation waits for the device, so buffers still in use by
-// queued kernels are never freed under them.
+// Grow-only, and an outgrown array is kept: kernels that are queued use it, and so does every
+// graph that was recorded with it, at each replay. Sizes double at least, so that all outgrown
+// ones together are no larger than the one in use.
 int workspace_get(size_t bytes, hipStream_t stream, float **out) {
     int dev = 0;
     TAGI_TRY(hipGetDevice(&dev));
@@ -58,12 +61,17 @@ int workspace_get(size_t bytes, hipStream_t stream, float **out) {
         w = &g_ws[dev].by_stream.back().second;
     }
     if (w->bytes < bytes) {
-        TAGI_TRY(hipDeviceSynchronize());
-        if (w->ptr != nullptr) TAGI_TRY(hipFree(w->ptr));
-        w->ptr = nullptr;
-        w->bytes = 0;
-        const size_t want = (bytes + ((size_t)1 << 20) - 1) & ~(((size_t)1 << 20) - 1);
-        TAGI_TRY(hipMalloc(reinterpret_cast<void **>(&w->ptr), want));
+        constexpr size_t MIB = (size_t)1 << 20;
+        const size_t least = (bytes + MIB - 1) & ~(MIB - 1);
+        size_t want = std::max(least, 2 * w->bytes);
+        float *p = nullptr;
+        if (want > least && hipMalloc(reinterpret_cast<void **>(&p), want) != hipSuccess) {
+            (void)hipGetLastError();
+            p = nullptr;
+        }
+        if (p == nullptr) TAGI_TRY(hipMalloc(reinterpret_cast<void **>(&p), want = least));
+        if (w->ptr != nullptr) g_ws[dev].outgrown.push_back(w->ptr);
+        w->ptr = p;
         w->bytes = want;
     }
     *out = w->ptr;
@@ -316,7 +324,9 @@ int tagi_hip_shutdown(void) {
         TAGI_TRY(hipDeviceSynchronize());
         for (auto &entry : g_ws[d].by_stream)
             if (entry.second.ptr != nullptr) TAGI_TRY(hipFree(entry.second.ptr));
+        for (float *p : g_ws[d].outgrown) TAGI_TRY(hipFree(p));
         g_ws[d].by_stream.clear();
+        g_ws[d].outgrown.clear();
     }
     TAGI_TRY(hipSetDevice(cur));
     return TAGI_OK;

@@ -122,9 +122,9 @@ const float *device_ones(size_t n, int device_idx) {
     static size_t cap[16] = {};
     if (device_idx < 0 || device_idx >= 16) LOG(LogLevel::ERROR, "Invalid device index");
     if (n > cap[device_idx]) {
-        HIP_OK(hipSetDevice(device_idx));
-        HIP_OK(hipDeviceSynchronize());  // kernels in flight may still read the old array
-        dev_free(ones[device_idx]);
+        // (an outgrown array is kept: kernels in flight and recorded graphs read it. Sizes
+        // double at least, so that those together are no larger than the one in use.)
+        n = std::max(n, 2 * cap[device_idx]);
         ones[device_idx] = dev_alloc(n, device_idx);
         cap[device_idx] = n;
         if (tagi_store_states(nullptr, nullptr, 0, nullptr, nullptr, ones[device_idx], n,

@@ -100,8 +100,8 @@ class BaseObservation {
 
 // ---- device side ---------------------------------------------------------------
 
-// A device array of ones, at least n long, on the given device (grow-only, shared):
-// what a consumer reads for a Jacobian that is known to be one everywhere.
+// A device array of ones, at least n long, on the given device (grow-only, shared, never
+// freed): what a consumer reads for a Jacobian that is known to be one everywhere.
 const float *device_ones(size_t n, int device_idx);
 
 class HiddenStateHip : public BaseHiddenStates {

@@ -21,7 +21,8 @@
  *   - the library owns no user buffer. It keeps one grow-only device workspace
  *     per (GPU, stream) for split-reduction partial sums (see
  *     tagi_hip_workspace_reserve), so calls on different streams never share
- *     scratch memory; calls issued to ONE stream from several host threads must be
+ *     scratch memory; an outgrown workspace stays allocated until
+ *     tagi_hip_shutdown, because graphs that were recorded with it use it; calls issued to ONE stream from several host threads must be
  *     serialised by the caller, as with any stream-ordered API.
  */
 #ifndef TAGI_HIP_H
@@ -46,11 +47,10 @@ int tagi_hip_version(void);
  * Sequential::to_device (src/sequential.cpp:32-73). */
 int tagi_hip_device_count(int *count /* host, out */);
 const char *tagi_hip_error_string(int code);
-/* Grow the workspace of `stream` on the current device to at least `bytes` now
- * (synchronises the device if it has to reallocate). Optional: entry points grow it
- * on demand. */
+/* Grow the workspace of `stream` on the current device to at least `bytes` now (and to
+ * twice its size where it has to grow and that fits). Optional: entry points grow it on demand. */
 int tagi_hip_workspace_reserve(size_t bytes, void *stream);
-/* Free the workspaces of all devices. */
+/* Free the workspaces of all devices, those too that recorded graphs use. */
 int tagi_hip_shutdown(void);
 /* Compute units, peak engine clock (MHz) and name of the current device, as the
  * runtime reports them (hipGetDeviceProperties); any pointer may be NULL. The

@@ -154,6 +154,49 @@ def test_training_buffers_that_grow_later_drop_the_recordings(make, n_in, n_out)
     assert max(held[10:]) >= 2
 
 
+def test_workspace_of_a_recorded_call_outlives_its_growth():
+    """A sliced reduction recorded with the workspace of its stream, which then grows: the
+    recording still owns the memory that its partial sums go to."""
+    import torch
+    import cutagi_amd.functional as F
+    from cutagi_amd import capi
+    torch.cuda.synchronize()
+    capi.check(capi.lib.tagi_hip_shutdown())
+    K, N, B = 4096, 2048, 256        # eight reduction slices: 32 MiB of partial sums
+    mk = lambda *s: torch.rand(*s, device="cuda")
+    w, v, a, q = mk(N, K) - 0.5, mk(N, K), mk(B, K), mk(B, K)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    free = [torch.cuda.mem_get_info()[0]]
+    with torch.cuda.stream(stream):
+        want = F.linear_fwd(w, v, None, None, a, q)
+    stream.synchronize()
+    free.append(torch.cuda.mem_get_info()[0])
+    assert free[0] - free[1] > 16 << 20, "no workspace grew"
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        got = F.linear_fwd(w, v, None, None, a, q)
+    free.append(torch.cuda.mem_get_info()[0])
+    capi.check(capi.lib.tagi_hip_workspace_reserve(1 << 30, stream.cuda_stream))
+    # 1 GiB where the old 32 MiB are kept, 32 MiB less where not (the runtime moves some pages
+    # of 2 MiB by itself: the limit lies halfway)
+    assert free[2] - torch.cuda.mem_get_info()[0] > (1 << 30) - (16 << 20), "the outgrown workspace was freed"
+    other = torch.full((64 << 20,), float("nan"), device="cuda")     # would lie where it was
+    for i in range(3):
+        a.mul_(1.01)
+        with torch.cuda.stream(stream):
+            stream.wait_stream(torch.cuda.default_stream())
+            want = F.linear_fwd(w, v, None, None, a, q)
+            graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(got, want)), "replay %d" % i
+    assert bool(torch.isnan(other).all())
+    del graph
+    free.append(torch.cuda.mem_get_info()[0])
+    capi.check(capi.lib.tagi_hip_shutdown())
+    assert torch.cuda.mem_get_info()[0] - free[3] > (1 << 30) + (16 << 20)
+
+
 def test_networks_with_blocks_stay_eager():
     from cutagi_amd import cutagi
     cutagi.manual_seed(2)
