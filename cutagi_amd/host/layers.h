@@ -115,6 +115,8 @@ class BaseLayer {
     // cannot describe its update that way performs it on the spot.
     virtual void collect_update_items(std::vector<tagi_update_item> &) { this->update_params(); }
     virtual void set_cap_factor_udapte(int batch_size);
+    // A recorded forward pass of this batch was replayed: what forward() leaves on the host.
+    virtual void forward_replayed(int /*batch_size*/) {}
     virtual void set_threads(int num) { num_threads = num; }
     virtual void compute_input_output_size(const InitArgs &args);
     virtual void train() { training = true; }
@@ -167,6 +169,7 @@ class BaseLayerHip : public BaseLayer {
     void update_biases() override;
     void update_params() override;
     void collect_update_items(std::vector<tagi_update_item> &items) override;
+    void forward_replayed(int batch_size) override { this->set_cap_factor_udapte(batch_size); }
     void raw_update_weights() override;
     void raw_update_biases() override;
     void set_cuda_threads(int num) { num_cuda_threads = (unsigned int)num; }

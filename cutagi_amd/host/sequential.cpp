@@ -507,7 +507,7 @@ bool Sequential::only_plain_layers() const {
 
 // `body` queues device work on host_stream() and moves the buffer pointers around; it
 // is run as it is, or recorded into a graph, or skipped in favour of the recorded graph
-// (whose effect on the buffer pointers is then repeated by hand).
+// (whose effect on the buffer pointers and on the host is then repeated by hand).
 void Sequential::run_or_replay(const GraphKey &key, const std::function<void()> &body) {
     if (!graphs_on_ || host_stream() == nullptr || !this->only_plain_layers()) {
         body();
@@ -524,6 +524,8 @@ void Sequential::run_or_replay(const GraphKey &key, const std::function<void()> 
         HIP_OK(hipGraphLaunch(static_cast<hipGraphExec_t>(e.exec), stream));
         if (e.swaps_state) std::swap(input_z_buffer, output_z_buffer);
         if (e.swaps_delta) std::swap(input_delta_z_buffer, output_delta_z_buffer);
+        if (std::get<0>(key) == 0)
+            for (auto &layer : layers) layer->forward_replayed(std::get<3>(key));
         return;
     }
     // the first runs allocate (workspaces, what layers keep for the backward pass):

@@ -127,6 +127,7 @@ def _eager_and_replayed(make, cutagi, steps, n_in, n_out):
             if kind == "train":
                 updater.update(net.output_z_buffer, y, np.full(y.size, 0.5, np.float32),
                                net.input_delta_z_buffer)
+            if kind != "forward":
                 net.backward()
                 net.step()
         return trace, net.state_dict()
@@ -152,6 +153,15 @@ def test_training_buffers_that_grow_later_drop_the_recordings(make, n_in, n_out)
     assert held[7] == 2      # recorded at 32
     assert held[9] == 0      # after the first step at 64: dropped
     assert max(held[10:]) >= 2
+
+
+@pytest.mark.parametrize("make,n_in,n_out", [(_mlp, 784, 11), (_cnn, 3 * 8 * 8, 5)])
+def test_replayed_batches_are_capped_by_their_own_size(make, n_in, n_out):
+    """The cap of the parameter updates depends on the batch: one sample, up to 255, more."""
+    from cutagi_amd import cutagi
+    sizes = [300] * 5 + [32] * 5 + [300] * 2 + [1] * 5 + [32] * 2 + [1, 300, 1]
+    held = _eager_and_replayed(make, cutagi, [("train", b) for b in sizes], n_in, n_out)
+    assert max(held) >= 6
 
 
 def test_workspace_of_a_recorded_call_outlives_its_growth():
