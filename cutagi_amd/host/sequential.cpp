@@ -505,6 +505,18 @@ bool Sequential::only_plain_layers() const {
     return true;
 }
 
+// The host side of a forward pass that was replayed: the layers' and the output's.
+void Sequential::replayed_forward(const GraphEntry &e) {
+    for (auto &layer : layers) layer->forward_replayed((int)e.block_size);
+    auto *out = dynamic_cast<HiddenStateHip *>(output_z_buffer.get());
+    out->width = e.width;
+    out->height = e.height;
+    out->depth = e.depth;
+    out->block_size = e.block_size;
+    out->actual_size = e.actual_size;
+    out->jcb_ones = e.jcb_ones;
+}
+
 // `body` queues device work on host_stream() and moves the buffer pointers around; it
 // is run as it is, or recorded into a graph, or skipped in favour of the recorded graph
 // (whose effect on the buffer pointers and on the host is then repeated by hand).
@@ -524,8 +536,7 @@ void Sequential::run_or_replay(const GraphKey &key, const std::function<void()> 
         HIP_OK(hipGraphLaunch(static_cast<hipGraphExec_t>(e.exec), stream));
         if (e.swaps_state) std::swap(input_z_buffer, output_z_buffer);
         if (e.swaps_delta) std::swap(input_delta_z_buffer, output_delta_z_buffer);
-        if (std::get<0>(key) == 0)
-            for (auto &layer : layers) layer->forward_replayed(std::get<3>(key));
+        if (std::get<0>(key) == 0) this->replayed_forward(e);
         return;
     }
     // the first runs allocate (workspaces, what layers keep for the backward pass):
@@ -574,6 +585,13 @@ void Sequential::run_or_replay(const GraphKey &key, const std::function<void()> 
     e.exec = exec;
     e.swaps_state = input_z_buffer != state_before;
     e.swaps_delta = input_delta_z_buffer != delta_before;
+    const auto *out = dynamic_cast<HiddenStateHip *>(output_z_buffer.get());
+    e.width = out->width;
+    e.height = out->height;
+    e.depth = out->depth;
+    e.block_size = out->block_size;
+    e.actual_size = out->actual_size;
+    e.jcb_ones = out->jcb_ones;
     HIP_OK(hipGraphLaunch(exec, stream));
 }
 

@@ -152,6 +152,9 @@ class Sequential {
         int warm_runs = 0;       // eager runs seen with this key (allocations happen in them)
         bool unusable = false;   // capture failed: stay eager
         bool swaps_state = false, swaps_delta = false;  // net effect on the buffer pointers
+        // what a forward pass says about its output
+        size_t width = 0, height = 0, depth = 0, block_size = 0, actual_size = 0;
+        bool jcb_ones = false;
     };
     // (kind, first buffer's arrays, second buffer's arrays, batch size, flags)
     using GraphKey = std::tuple<int, const void *, const void *, int, int>;
@@ -159,6 +162,7 @@ class Sequential {
     bool graphs_on_ = false;
     size_t freed_when_recorded_ = 0;
     size_t buffers_freed() const;
+    void replayed_forward(const GraphEntry &e);
     void clear_graphs();
     bool only_plain_layers() const;
     void run_or_replay(const GraphKey &key, const std::function<void()> &body);

@@ -103,7 +103,7 @@ def test_mode_switches_and_reloads_drop_the_recordings():
 
 
 def _eager_and_replayed(make, cutagi, steps, n_in, n_out):
-    """Runs `steps` - ("train" | "forward", batch) or "eval" / "train" - on a network with
+    """Runs `steps` - ("train" | "indexed" | "forward", batch) or "eval" / "train" - on a network with
     graphs and on one without, and compares outputs and parameters. Returns the graphs held
     before every step."""
     rng = np.random.default_rng(4)
@@ -127,6 +127,11 @@ def _eager_and_replayed(make, cutagi, steps, n_in, n_out):
             if kind == "train":
                 updater.update(net.output_z_buffer, y, np.full(y.size, 0.5, np.float32),
                                net.input_delta_z_buffer)
+            elif kind == "indexed":      # two observed outputs per sample
+                idx = np.tile(np.array([1, n_out], np.int32), len(x))
+                updater.update_using_indices(net.output_z_buffer, y[:2 * len(x)],
+                                             np.full(2 * len(x), 0.5, np.float32), idx,
+                                             net.input_delta_z_buffer)
             if kind != "forward":
                 net.backward()
                 net.step()
@@ -162,6 +167,23 @@ def test_replayed_batches_are_capped_by_their_own_size(make, n_in, n_out):
     sizes = [300] * 5 + [32] * 5 + [300] * 2 + [1] * 5 + [32] * 2 + [1, 300, 1]
     held = _eager_and_replayed(make, cutagi, [("train", b) for b in sizes], n_in, n_out)
     assert max(held) >= 6
+
+
+def _even(cutagi):
+    """Two passes: the output lies in the object that the input was written to."""
+    cutagi.manual_seed(3)
+    net = cutagi.Sequential([cutagi.Linear(24, 16), cutagi.ReLU(), cutagi.Linear(16, 6)])
+    net.to_device("cuda")
+    return net
+
+
+@pytest.mark.parametrize("make,n_in,n_out", [(_even, 24, 6), (_mlp, 784, 11), (_cnn, 3 * 8 * 8, 5)])
+def test_indexed_update_after_a_replay(make, n_in, n_out):
+    """The update finds the outputs of a sample by the size that the forward pass gave them."""
+    from cutagi_amd import cutagi
+    sizes = [32] * 9 + [16] * 9 + [32] * 3 + [16] * 2
+    held = _eager_and_replayed(make, cutagi, [("indexed", b) for b in sizes], n_in, n_out)
+    assert max(held) >= 4
 
 
 def test_workspace_of_a_recorded_call_outlives_its_growth():
