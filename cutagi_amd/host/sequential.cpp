@@ -342,14 +342,17 @@ void Sequential::prepare_buffers(int batch_size) {
         this->z_buffer_block_size = batch_size;
         this->input_z_buffer->set_size(this->z_buffer_size, batch_size);
         this->output_z_buffer->set_size(this->z_buffer_size, batch_size);
-        // a model first run in eval mode has no delta buffers yet: they are created
-        // below at the new size
-        if (this->training && this->input_delta_z_buffer) {
-            this->input_delta_z_buffer->set_size(this->z_buffer_size, batch_size);
-            this->output_delta_z_buffer->set_size(this->z_buffer_size, batch_size);
-        }
     }
-    if (this->training && !this->input_delta_z_buffer) this->init_delta_state_buffer();
+    if (!this->training) return;
+    // The innovation buffers follow the batches of training mode alone: a model first run in
+    // eval mode has none, one that was evaluated in between has those of an earlier batch.
+    if (!this->input_delta_z_buffer) {
+        this->init_delta_state_buffer();
+        return;
+    }
+    for (auto *d : {this->input_delta_z_buffer.get(), this->output_delta_z_buffer.get()})
+        if (d->block_size != (size_t)batch_size || d->size < (size_t)this->z_buffer_size)
+            d->set_size(this->z_buffer_size, batch_size);
 }
 
 void Sequential::set_threads(unsigned n) {

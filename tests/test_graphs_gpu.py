@@ -186,6 +186,56 @@ def test_indexed_update_after_a_replay(make, n_in, n_out):
     assert max(held) >= 4
 
 
+def _experts(cutagi):
+    cutagi.manual_seed(5)
+    net = cutagi.Sequential([cutagi.Linear(12, 20), cutagi.MixtureReLU(), cutagi.LayerNorm([20]),
+                             cutagi.MixtureOfExperts(20, 24, 6, 4, 2)])
+    net.to_device("cuda")
+    return net
+
+
+def _residual(cutagi):
+    cutagi.manual_seed(6)
+    block = cutagi.LayerBlock([cutagi.LayerNorm([20]), cutagi.MixtureOfExperts(20, 24, 20, 4, 2)])
+    net = cutagi.Sequential([cutagi.Linear(12, 20), cutagi.ResNetBlock(block), cutagi.Linear(20, 6)])
+    net.to_device("cuda")
+    return net
+
+
+@pytest.mark.parametrize("graphs", [False, True])
+@pytest.mark.parametrize("make,n_in,n_out", [(_mlp, 784, 11), (_cnn, 3 * 8 * 8, 5), (_experts, 12, 6),
+                                             (_residual, 12, 6)])
+def test_evaluations_between_training_steps_leave_the_steps_alone(make, n_in, n_out, graphs):
+    """An evaluation of another batch size, smaller or larger, and training steps of the size
+    of that evaluation: the same parameters as without the evaluations."""
+    from cutagi_amd import cutagi
+    rng = np.random.default_rng(7)
+    sizes = [32, 32, 16, 64, 64, 64, 64, 9, 64, 32]
+    data = [(rng.normal(0, 1, (b, n_in)).astype(np.float32), rng.normal(0, 1, b * n_out).astype(np.float32))
+            for b in sizes]
+    other = rng.normal(0, 1, (200, n_in)).astype(np.float32)
+
+    def run(evaluate):
+        net = make(cutagi)
+        net.enable_graphs(graphs)
+        updater = cutagi.OutputUpdater(net.device)
+        for i, (x, y) in enumerate(data):
+            net.forward(x)
+            updater.update(net.output_z_buffer, y, np.full(y.size, 0.5, np.float32), net.input_delta_z_buffer)
+            net.backward()
+            net.step()
+            if evaluate and i + 1 < len(sizes):
+                net.eval()
+                net.forward(other[:7])
+                net.forward(other[:sizes[i + 1]])
+                net.train()
+        net.enable_graphs(False)
+        return net.state_dict()
+    plain, evaluated = run(False), run(True)
+    assert plain == evaluated
+    assert all(np.all(np.isfinite(a)) for p in plain.values() for a in p)
+
+
 def test_workspace_of_a_recorded_call_outlives_its_growth():
     """A sliced reduction recorded with the workspace of its stream, which then grows: the
     recording still owns the memory that its partial sums go to."""
