@@ -144,7 +144,8 @@ def _eager_and_replayed(make, cutagi, steps, n_in, n_out):
     for i, (a, b) in enumerate(zip(eager, replay)):
         assert all(np.array_equal(u, w) for u, w in zip(a, b)), "outputs differ at step %d" % i
     assert all(np.all(np.isfinite(u)) for a in eager for u in a)
-    assert eager_params == replay_params
+    differ = [name for name in eager_params if eager_params[name] != replay_params[name]]
+    assert not differ
     return held
 
 
@@ -232,7 +233,8 @@ def test_evaluations_between_training_steps_leave_the_steps_alone(make, n_in, n_
         net.enable_graphs(False)
         return net.state_dict()
     plain, evaluated = run(False), run(True)
-    assert plain == evaluated
+    differ = [name for name in plain if plain[name] != evaluated[name]]
+    assert not differ
     assert all(np.all(np.isfinite(a)) for p in plain.values() for a in p)
 
 
