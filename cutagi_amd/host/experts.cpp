@@ -330,7 +330,7 @@ void MixtureOfExpertsHip::forward(BaseHiddenStates &input_states, BaseHiddenStat
         w.offsets, nullptr, H, N, E, R, R, has_b, w.scratch, w.mu_y, w.var_y, stream));
     TAGI_OK_OR_THROW(tagi_moe_combine_fwd(w.mu_g, w.var_g, w.mu_y, w.var_y, w.slot, T, k, R, N,
                                           out->d_mu_a, out->d_var_a, stream));
-    last_batch = T;
+    this->last_batch = T;
     output_states.width = this->out_width;
     output_states.height = this->out_height;
     output_states.depth = this->out_channels;
@@ -382,6 +382,11 @@ void MixtureOfExpertsHip::backward(BaseDeltaStates &input_delta_states,
                                              bwd->jcb_ones ? nullptr : bwd->d_jcb, dout->d_delta_mu,
                                              dout->d_delta_var, T, k, R, K, dout->d_delta_mu,
                                              dout->d_delta_var, stream));
+}
+
+void MixtureOfExpertsHip::forward_replayed(int batch_size) {
+    BaseLayerHip::forward_replayed(batch_size);
+    this->last_batch = batch_size;
 }
 
 std::vector<int> MixtureOfExpertsHip::get_expert_choices() {

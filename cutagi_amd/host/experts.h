@@ -105,13 +105,15 @@ class MixtureOfExpertsHip : public BaseLayerHip {
                   BaseTempStates &temp_states, bool state_udapte = true) override;
     // Expert of every choice of the last forward pass [samples][top_k], to the host.
     std::vector<int> get_expert_choices();
+    void forward_replayed(int batch_size) override;
 
    private:
+    // samples of the last forward pass; d_work is laid out for them
+    int last_batch = 0;
     // What the last forward pass chose and computed on the way, and what the backward pass
     // computes; one allocation, as large as the largest batch seen needs.
     char *d_work = nullptr;
     size_t batch_held = 0;
-    int last_batch = 0;
     struct Work;
     Work work(int batch) const;
     void hold(int batch);

@@ -164,6 +164,27 @@ def test_backward_scratch_that_grows_later_drops_the_recordings(first):
     assert all(np.all(np.isfinite(u)) for a in eager for u in a)
 
 
+def test_expert_choices_after_replays():
+    """Of the last pass, replayed or not, whatever batch ran last by itself."""
+    from cutagi_amd import cutagi
+    rng = np.random.default_rng(6)
+    xs = {b: rng.standard_normal((b, 16)).astype(np.float32) for b in (32, 9, 64)}
+    eager, net = _net(cutagi), _net(cutagi)
+    eager.eval()
+    net.eval()
+    net.enable_graphs(True)
+    net.forward(xs[64])
+    for b in [32] * 5 + [9] * 5 + [64, 32, 9, 64, 32, 64, 9, 32]:
+        x = xs[b] + rng.standard_normal(xs[b].shape).astype(np.float32)
+        net.forward(x)
+        eager.forward(x)
+        choices = net.layers[3].get_expert_choices()
+        assert len(choices) == b * TOP_K
+        assert choices == eager.layers[3].get_expert_choices()
+    assert net.graphs_captured() >= 2
+    net.enable_graphs(False)
+
+
 def test_residual_block_and_evaluation_mode():
     """x + experts(norm(x)): the block adds the shortcut forward and its innovations back."""
     from cutagi_amd import cutagi
