@@ -98,7 +98,11 @@ void LayerNormHip::hold(int batch_size) {
         d_scratch = dev_alloc_t<char>(bytes, device_idx);
         scratch_held = bytes;
     }
-    train_rows_held = std::max(train_rows_held, (size_t)batch_size);
+}
+
+void LayerNormHip::forward_replayed(int batch_size) {
+    BaseLayerHip::forward_replayed(batch_size);
+    trained_batch = training ? batch_size : 0;
 }
 
 // reference: LayerNormCuda::forward, src/layernorm_layer_cuda.cu
@@ -123,6 +127,7 @@ void LayerNormHip::forward(BaseHiddenStates &input_states, BaseHiddenStates &out
     output_states.depth = this->out_channels;
     output_states.block_size = batch_size;
     output_states.actual_size = this->output_size;
+    trained_batch = training ? batch_size : 0;
     out->jcb_ones = true;
     if (this->training) this->store_states_for_training_hip(*in, *out);
 }
@@ -136,8 +141,8 @@ void LayerNormHip::backward(BaseDeltaStates &input_delta_states, BaseDeltaStates
     const int batch_size = (int)input_delta_states.block_size;
     if (state_udapte && input_size * batch_size > dout->size)
         LOG(LogLevel::ERROR, "Delta state buffer too small for " + this->get_layer_info());
-    if ((size_t)batch_size > train_rows_held || bwd->d_mu_a == nullptr)
-        LOG(LogLevel::ERROR, "Backward pass of " + this->get_layer_info() + " without its forward pass");
+    if (batch_size > trained_batch || bwd->d_mu_a == nullptr)
+        LOG(LogLevel::ERROR, "Backward pass of " + this->get_layer_info() + " without its forward pass in training mode");
     TAGI_OK_OR_THROW(tagi_layernorm_bwd(
         d_mu_w, d_var_w, d_var_b, bwd->d_mu_a, bwd->jcb_ones ? nullptr : bwd->d_jcb, d_mu_s, d_var_s,
         din->d_delta_mu, din->d_delta_var, epsilon, (int)input_size, batch_size, bias ? 1 : 0,
@@ -330,7 +335,8 @@ void MixtureOfExpertsHip::forward(BaseHiddenStates &input_states, BaseHiddenStat
         w.offsets, nullptr, H, N, E, R, R, has_b, w.scratch, w.mu_y, w.var_y, stream));
     TAGI_OK_OR_THROW(tagi_moe_combine_fwd(w.mu_g, w.var_g, w.mu_y, w.var_y, w.slot, T, k, R, N,
                                           out->d_mu_a, out->d_var_a, stream));
-    this->last_batch = T;
+    last_batch = T;
+    trained_batch = training ? T : 0;
     output_states.width = this->out_width;
     output_states.height = this->out_height;
     output_states.depth = this->out_channels;
@@ -349,8 +355,8 @@ void MixtureOfExpertsHip::backward(BaseDeltaStates &input_delta_states,
     const int T = (int)input_delta_states.block_size;
     if (state_udapte && input_size * T > dout->size)
         LOG(LogLevel::ERROR, "Delta state buffer too small for " + this->get_layer_info());
-    if ((size_t)T > batch_held || bwd->d_mu_a == nullptr)
-        LOG(LogLevel::ERROR, "Backward pass of " + this->get_layer_info() + " without its forward pass");
+    if (T != trained_batch || bwd->d_mu_a == nullptr)
+        LOG(LogLevel::ERROR, "Backward pass of " + this->get_layer_info() + " without its forward pass in training mode");
     const Work w = this->work(T);
     const int K = (int)sizes.input, H = (int)sizes.hidden, N = (int)sizes.output;
     const int E = sizes.experts, k = sizes.top_k, R = T * k, has_b = bias ? 1 : 0;
@@ -386,7 +392,8 @@ void MixtureOfExpertsHip::backward(BaseDeltaStates &input_delta_states,
 
 void MixtureOfExpertsHip::forward_replayed(int batch_size) {
     BaseLayerHip::forward_replayed(batch_size);
-    this->last_batch = batch_size;
+    last_batch = batch_size;
+    trained_batch = training ? batch_size : 0;
 }
 
 std::vector<int> MixtureOfExpertsHip::get_expert_choices() {

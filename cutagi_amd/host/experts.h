@@ -44,13 +44,17 @@ class LayerNormHip : public BaseLayerHip {
                  BaseTempStates &temp_states) override;
     void backward(BaseDeltaStates &input_delta_states, BaseDeltaStates &output_delta_states,
                   BaseTempStates &temp_states, bool state_udapte = true) override;
+    void forward_replayed(int batch_size) override;
 
    private:
+    // rows that the backward pass finds: those of the last forward pass, none if that was an
+    // evaluation (whose statistics have taken their place)
+    int trained_batch = 0;
     // statistics of the rows of the last forward pass, sums of the backward pass; as large as
     // the largest batch seen (in training) needs
     float *d_mu_s = nullptr, *d_var_s = nullptr;
     char *d_scratch = nullptr;
-    size_t rows_held = 0, train_rows_held = 0, scratch_held = 0;
+    size_t rows_held = 0, scratch_held = 0;
     void hold(int batch_size);
 };
 
@@ -108,8 +112,9 @@ class MixtureOfExpertsHip : public BaseLayerHip {
     void forward_replayed(int batch_size) override;
 
    private:
-    // samples of the last forward pass; d_work is laid out for them
-    int last_batch = 0;
+    // samples of the last forward pass, for which d_work is laid out; and what of them the
+    // backward pass finds, none if that was an evaluation
+    int last_batch = 0, trained_batch = 0;
     // What the last forward pass chose and computed on the way, and what the backward pass
     // computes; one allocation, as large as the largest batch seen needs.
     char *d_work = nullptr;

@@ -185,6 +185,50 @@ def test_expert_choices_after_replays():
     net.enable_graphs(False)
 
 
+@pytest.mark.parametrize("make", ["norm", "experts"])
+@pytest.mark.parametrize("graphs", [False, True])
+def test_backward_needs_the_forward_pass_of_its_batch(make, graphs):
+    """What the two layers keep belongs to the last forward pass: a backward pass after an
+    evaluation is refused, and for the experts, whose rows lie elsewhere for every batch, one
+    of another batch."""
+    from cutagi_amd import cutagi
+    cutagi.manual_seed(0)
+    last = cutagi.LayerNorm([12]) if make == "norm" else cutagi.MixtureOfExperts(12, 8, 12, 3, 2)
+    net = cutagi.Sequential([cutagi.Linear(16, 12), cutagi.MixtureReLU(), last])
+    net.to_device("cuda")
+    net.enable_graphs(graphs)
+    rng = np.random.default_rng(8)
+    xs = [rng.standard_normal((10, 16)).astype(np.float32) for _ in range(4)]
+    ys = [rng.standard_normal(120).astype(np.float32) for _ in range(4)]
+    _train(net, cutagi, xs, ys)
+    before = net.state_dict()
+    for batch in (10, 4, 20):
+        net.forward(xs[0])
+        net.eval()
+        net.forward(np.resize(xs[1], (batch, 16)))
+        net.train()
+        with pytest.raises(RuntimeError, match="without its forward pass"):
+            net.backward()
+    net.forward(xs[0])
+    net.input_delta_z_buffer.block_size = 11
+    with pytest.raises(RuntimeError, match="without its forward pass"):
+        net.backward()
+    net.input_delta_z_buffer.block_size = 7
+    if make == "experts":
+        with pytest.raises(RuntimeError, match="without its forward pass"):
+            net.backward()
+    assert [n for n in before if before[n] != net.state_dict()[n]] == []
+    # and it goes on as if nothing had been
+    _, got = _train(net, cutagi, xs, ys)
+    net.enable_graphs(False)
+    other = cutagi.Sequential([cutagi.Linear(16, 12), cutagi.MixtureReLU(),
+                               cutagi.LayerNorm([12]) if make == "norm" else cutagi.MixtureOfExperts(12, 8, 12, 3, 2)])
+    other.to_device("cuda")
+    other.load_state_dict(before)
+    _, want = _train(other, cutagi, xs, ys)
+    assert [n for n in want if want[n] != got[n]] == []
+
+
 def test_residual_block_and_evaluation_mode():
     """x + experts(norm(x)): the block adds the shortcut forward and its innovations back."""
     from cutagi_amd import cutagi
