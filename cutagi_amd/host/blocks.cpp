@@ -777,6 +777,7 @@ void ResNetBlock::forward(BaseHiddenStates &input_states, BaseHiddenStates &outp
         batch_size_ = batch_size;
         this->init_buffers(want);
     }
+    trained_batch_ = training ? batch_size : 0;
     auto *kept = as<HiddenStateHip>(*input_z);
     auto *main_lb = dynamic_cast<LayerBlock *>(main_block.get());
     if (trade) {
@@ -828,6 +829,8 @@ void ResNetBlock::backward(BaseDeltaStates &input_delta_states,
                            bool state_update) {
     if (!on_device) no_cpu_path("backward");
     const int batch_size = (int)input_delta_states.block_size;
+    if (batch_size != trained_batch_)
+        LOG(LogLevel::ERROR, "Backward pass of " + this->get_layer_info() + " without its forward pass in training mode");
     // As in forward(): the incoming innovations are needed by both branches; trade arrays
     // with the buffer they arrive in where both branches can be told where to read.
     auto *din = as<DeltaStateHip>(input_delta_states);

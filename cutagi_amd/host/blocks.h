@@ -248,6 +248,9 @@ class ResNetBlock : public BaseLayer {
    protected:
     bool on_device = false;
     int batch_size_ = 0;
+    // samples that the backward pass finds: those of the last forward pass, none if that was
+    // an evaluation (whose input has taken the place that the first layers borrowed)
+    int trained_batch_ = 0;
     size_t buffer_size_ = 0;
     // buffers of `size` floats per array (0: what the block's own layers need)
     void init_buffers(size_t size = 0);

@@ -238,6 +238,40 @@ def test_evaluations_between_training_steps_leave_the_steps_alone(make, n_in, n_
     assert all(np.all(np.isfinite(a)) for p in plain.values() for a in p)
 
 
+def _conv_block(cutagi):
+    cutagi.manual_seed(7)
+    block = lambda: cutagi.LayerBlock([cutagi.Conv2d(2, 2, 3, padding=1, in_width=4, in_height=4), cutagi.ReLU(),
+                                       cutagi.Conv2d(2, 2, 3, padding=1)])
+    res = [cutagi.ResNetBlock(block()), cutagi.ResNetBlock(block(), block())]
+    res[0].in_width, res[0].in_height, res[0].in_channels = 4, 4, 2
+    net = cutagi.Sequential(res + [cutagi.Linear(32, 6)])
+    net.to_device("cuda")
+    net.preinit_layer()      # (the convolutions draw their weights here, not in the first pass)
+    return net
+
+
+@pytest.mark.parametrize("make,n_in", [(_residual, 12), (_conv_block, 32)])
+def test_blocks_refuse_a_backward_pass_after_an_evaluation(make, n_in):
+    """The first layers of a block borrow the input that it keeps, and an evaluation puts its
+    own there."""
+    from cutagi_amd import cutagi
+    rng = np.random.default_rng(9)
+    xs = [rng.normal(0, 1, (10, n_in)).astype(np.float32) for _ in range(3)]
+    ys = [rng.normal(0, 1, 60).astype(np.float32) for _ in range(3)]
+    net, twin = make(cutagi), make(cutagi)
+    _train(net, cutagi, xs, ys, 6)
+    for batch in (10, 4, 20):
+        net.forward(xs[0])
+        net.eval()
+        net.forward(np.resize(xs[1], (batch, n_in)))
+        net.train()
+        with pytest.raises(RuntimeError, match="without its forward pass"):
+            net.backward()
+    _train(twin, cutagi, xs, ys, 6)
+    (_, got), (_, want) = (_train(n, cutagi, xs, ys, 6) for n in (net, twin))
+    assert [n for n in want if want[n] != got[n]] == []
+
+
 def test_workspace_of_a_recorded_call_outlives_its_growth():
     """A sliced reduction recorded with the workspace of its stream, which then grows: the
     recording still owns the memory that its partial sums go to."""
