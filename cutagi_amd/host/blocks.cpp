@@ -566,10 +566,14 @@ void LayerBlock::compute_input_output_size(const InitArgs &args) {
     out_channels = layers.back()->out_channels;
     out_height = layers.back()->out_height;
     out_width = layers.back()->out_width;
-    input_size = in_width * in_width * in_channels;
-    output_size = out_width * out_height * out_channels;
-    // no image comes in (a block behind a Linear layer): the features of its layers
-    if (input_size == 0) this->add_layers();
+    // Features of the first and the last layer that know theirs (activations and BatchNorm2d
+    // do not yet): a Linear layer hands on the geometry of the image before it, so that says
+    // nothing about a block behind one.
+    input_size = output_size = 0;
+    for (auto it = layers.begin(); it != layers.end() && input_size == 0; ++it) input_size = (*it)->input_size;
+    for (auto it = layers.rbegin(); it != layers.rend() && output_size == 0; ++it) output_size = (*it)->output_size;
+    if (input_size == 0) input_size = in_width * in_width * in_channels;
+    if (output_size == 0) output_size = out_width * out_height * out_channels;
 }
 
 void LayerBlock::save(std::ofstream &file) {
@@ -694,12 +698,10 @@ void ResNetBlock::compute_input_output_size(const InitArgs &args) {
     out_channels = main_block->out_channels;
     out_height = main_block->out_height;
     out_width = main_block->out_width;
-    input_size = in_width * in_width * in_channels;
-    output_size = out_width * out_height * out_channels;
-    if (input_size == 0) {   // no image comes in: the features of the main block
-        input_size = main_block->input_size;
-        output_size = main_block->output_size;
-    }
+    input_size = main_block->input_size;
+    output_size = main_block->output_size;
+    if (input_size == 0) input_size = in_width * in_width * in_channels;
+    if (output_size == 0) output_size = out_width * out_height * out_channels;
     if (shortcut && shortcut->output_size != output_size)
         LOG(LogLevel::ERROR, "ResNetBlock: shortcut output " +
                                  std::to_string(shortcut->output_size) + " vs main block output " +

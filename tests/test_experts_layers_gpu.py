@@ -301,6 +301,38 @@ def test_two_blocks_through_the_python_layer():
             assert len(a) == 0 or np.any(np.asarray(a) != np.asarray(b)), name
 
 
+@pytest.mark.parametrize("features", [16, 64])
+def test_residual_block_of_features_behind_an_image(features):
+    """More and fewer features than the image has pixels: the same bits as from the block by
+    itself, given what the layers before it put out."""
+    from cutagi_amd import cutagi
+    rng = np.random.default_rng(10)
+    cutagi.manual_seed(4)
+    block = lambda: cutagi.ResNetBlock(cutagi.LayerBlock([cutagi.LayerNorm([features]),
+                                                          cutagi.MixtureOfExperts(features, 24, features, 4, 2)]))
+    head = lambda: [cutagi.Conv2d(1, 2, 3, padding=1, in_width=4, in_height=4), cutagi.ReLU(),
+                    cutagi.Linear(32, features)]
+    net, first, second = (cutagi.Sequential(layers) for layers in (head() + [block()], head(), [block()]))
+    for n in (net, first, second):
+        n.to_device("cuda")
+        n.preinit_layer()
+    sd = net.state_dict()
+    first.load_state_dict({k: v for k, v in sd.items() if "main" not in k})
+    second.load_state_dict({k.replace("main.3", "main.0"): v for k, v in sd.items() if "main" in k})
+    x = rng.standard_normal((10, 16)).astype(np.float32)
+    net.forward(x)
+    first.forward(x)
+    second.forward(*first.get_outputs())
+    got, want = net.get_outputs(), second.get_outputs()
+    assert got[0].size == 10 * features
+    assert all(np.array_equal(a, b) for a, b in zip(got, want))
+    before = net.state_dict()
+    _train(net, cutagi, [x] * 2, [rng.standard_normal(10 * features).astype(np.float32)] * 2)
+    after = net.state_dict()
+    assert all(np.all(np.isfinite(a)) for p in after.values() for a in p)
+    assert [k for k in after if after[k] == before[k]] == []
+
+
 def test_checkpoints(tmp_path):
     from cutagi_amd import cutagi
     net, other = _net(cutagi, seed=0), _net(cutagi, seed=1)

@@ -192,6 +192,24 @@ def test_tensor_calls_refuse():
     no("come together", F.moe_gather_bwd, f(8, 3), f(8, 3), i(4, 2), None, f(4, 3), None)
 
 
+def test_block_sizes_behind_an_image():
+    """A Linear layer hands the image's geometry on: a block behind it has the features of its
+    layers, not the image's pixels."""
+    from cutagi_amd import nn
+    block = lambda *tail: nn.ResNetBlock(nn.LayerBlock(nn.LayerNorm(20), nn.MixtureOfExperts(20, 24, 20, 4, 2), *tail))
+    image = lambda: nn.Conv2d(1, 2, 3, padding=1, in_width=4, in_height=4)
+    net = nn.Sequential(image(), nn.ReLU(), nn.Linear(32, 20), block(), nn.ReLU(), block(nn.BatchNorm2d(20), nn.ReLU()),
+                        nn.Linear(20, 3))
+    assert [(net.layers[i].input_size, net.layers[i].output_size) for i in (3, 5)] == [(20, 20)] * 2
+    shortcut = nn.LayerBlock(nn.Linear(20, 12), nn.ReLU(), nn.Linear(12, 12))
+    main = nn.LayerBlock(nn.ReLU(), nn.Linear(20, 30), nn.MixtureReLU(), nn.Linear(30, 12))
+    flat = nn.Sequential(image(), nn.Linear(32, 20), nn.ResNetBlock(main, shortcut), nn.Linear(12, 3))
+    assert (flat.layers[2].input_size, flat.layers[2].output_size) == (20, 12)
+    # and a block of convolutions still has the image's
+    conv = nn.ResNetBlock(nn.LayerBlock(nn.Conv2d(2, 2, 3, padding=1), nn.BatchNorm2d(2), nn.ReLU()))
+    net = nn.Sequential(image(), nn.ReLU(), conv, nn.Linear(32, 3))
+    assert (net.layers[2].input_size, net.layers[2].output_size) == (32, 32)
+
 
 def test_layer_descriptions():
     """The host layers without a GPU: sizes, parameters, refusals, no CPU compute path."""
