@@ -273,6 +273,108 @@ def test_residual_block_and_evaluation_mode():
         assert np.array_equal(g.ravel(), x.cpu().numpy().ravel()), keys
 
 
+@pytest.mark.parametrize("shortcut", [False, True])
+@pytest.mark.parametrize("batch", [10, 300])
+def test_training_through_a_residual_block_is_its_calls(batch, shortcut):
+    """Steps of x + experts(norm(x)) behind an activation, whose Jacobian meets the innovations of
+    both branches: every parameter has the bits of the tensor-level calls, step after step."""
+    import torch
+    import cutagi_amd.functional as F
+    from cutagi_amd import capi, cutagi
+    cutagi.manual_seed(12)
+    branch = [cutagi.LayerBlock([cutagi.Linear(N_IN, 20), cutagi.ReLU(), cutagi.Linear(20, N_IN)])] if shortcut else []
+    block = cutagi.LayerBlock([cutagi.LayerNorm([N_IN]), cutagi.MixtureOfExperts(N_IN, HIDDEN, N_IN, EXPERTS, TOP_K)])
+    net = cutagi.Sequential([cutagi.Linear(8, N_IN), cutagi.MixtureReLU(), cutagi.ResNetBlock(block, *branch),
+                             cutagi.Linear(N_IN, 3)])
+    net.to_device("cuda")
+    rng = np.random.default_rng(batch)
+    xs = [rng.standard_normal((batch, 8)).astype(np.float32) for _ in range(3)]
+    ys = [rng.standard_normal(batch * 3).astype(np.float32) for _ in range(3)]
+    names = {part: next(k for k in net.state_dict() if part in k)
+             for part in ("LinearCuda.0", "LayerNorm", "MixtureOfExperts", "LinearCuda.3")}
+    if shortcut:
+        names.update({"sc%d" % i: "LinearCuda.shortcut.2.%d" % i for i in (0, 2)})
+    p = {part: _params(net, name) for part, name in names.items()}
+    t = lambda a: torch.from_numpy(np.ascontiguousarray(a)).cuda()
+
+    def linear(part, N, K):
+        m, v, b, q = p[part]
+        return m.view(N, K), v.view(N, K), b, q
+
+    for x, y in zip(xs, ys):
+        a, zero = t(x), torch.zeros(batch, 8, device="cuda")
+        h, vh, jh = F.linear_fwd_act(*linear("LinearCuda.0", N_IN, 8), a, zero, "mixture_relu")
+        z, vz, m, s = F.layernorm_fwd(*p["LayerNorm"], h, vh, 1e-5)
+        parts = _split_square(p["MixtureOfExperts"])
+        router, up, down = parts
+        r = F.moe_route(*F.linear_fwd(*router, z, vz), TOP_K)
+        g, vg, jg = F.grouped_linear_fwd_act(*up, z, vz, r.offsets, "relu", rows=r.token)
+        e, ve = F.grouped_linear_fwd(*down, g, vg, r.offsets)
+        c, vc = F.moe_combine_fwd(r.mu_g, r.var_g, e, ve, r.slot)
+        if shortcut:
+            k, vk, jk = F.linear_fwd_act(*linear("sc0", 20, N_IN), h, vh, "relu")
+            F.add_shortcut(*F.linear_fwd(*linear("sc2", N_IN, 20), k, vk), c, vc)
+        else:
+            F.add_shortcut(h, vh, c, vc)
+        o, vo = F.linear_fwd(*linear("LinearCuda.3", 3, N_IN), c, vc)
+        net.forward(x)
+        for got, want in zip(net.get_outputs(), (o, vo)):
+            assert np.array_equal(np.asarray(got).ravel(), _host_flat(want))
+
+        one = torch.ones_like
+        dmu, dvar = torch.zeros_like(o), torch.zeros_like(o)
+        F.out_update_dense(o, vo, one(o), t(y), torch.full((batch * 3,), 0.5, device="cuda"), dmu, dvar)
+        w = linear("LinearCuda.3", 3, N_IN)
+        last = F.linear_bwd(w[0], w[1], w[3], c, one(c), dmu, dvar)
+        do = last[:2]
+        d = {"LinearCuda.3": last[2:]}
+        de, dve, ds, dvs = F.moe_combine_bwd(r.mu_g, r.jcb_g, e, r.expert, r.slot, *do, EXPERTS)
+        gd = F.grouped_linear_bwd(down[0], down[1], down[3], g, jg, de, dve, r.offsets)
+        gu = F.grouped_linear_bwd(up[0], up[1], up[3], z, None, gd[0], gd[1], r.offsets, rows=r.token)
+        gr = F.linear_bwd(router[0], router[1], router[3], z, one(z), ds, dvs)
+        dz = F.moe_gather_bwd(gu[0], gu[1], r.slot, None, gr[0], gr[1])
+        d["MixtureOfExperts"] = [torch.cat([q[i].reshape(-1) for q in (gr, gu, gd)]) for i in range(2, 6)]
+        norm = F.layernorm_bwd(p["LayerNorm"][0], p["LayerNorm"][1], p["LayerNorm"][3], h, jh, m, s, *dz, 1e-5)
+        d["LayerNorm"] = norm[2:]
+        dh = norm[:2]
+        if shortcut:
+            w = linear("sc2", N_IN, 20)
+            b2 = F.linear_bwd(w[0], w[1], w[3], k, jk, *do)
+            w = linear("sc0", 20, N_IN)
+            b0 = F.linear_bwd(w[0], w[1], w[3], h, jh, b2[0], b2[1])
+            d["sc2"], d["sc0"] = b2[2:], b0[2:]
+            F.add_shortcut(b0[0], b0[1], *dh)
+        else:
+            F.add_shortcut_delta(*do, jh, *dh)
+        w = linear("LinearCuda.0", N_IN, 8)
+        d["LinearCuda.0"] = F.linear_bwd(w[0], w[1], w[3], a, one(a), *dh, state_update=False)[2:]
+        cap = capi.cap_factor(batch)
+        for part, (m_w, v_w, m_b, v_b) in d.items():
+            F.param_update(m_w.reshape(-1), v_w.reshape(-1), cap, p[part][0], p[part][1])
+            F.param_update(m_b.reshape(-1), v_b.reshape(-1), cap, p[part][2], p[part][3])
+
+        updater = cutagi.OutputUpdater(net.device)
+        updater.update(net.output_z_buffer, y, np.full(y.size, 0.5, np.float32), net.input_delta_z_buffer)
+        net.backward()
+        net.step()
+        for part, name in names.items():
+            for i, (got, want) in enumerate(zip(_params(net, name), p[part])):
+                assert torch.equal(got, want), "%s, array %d" % (name, i)
+
+
+def _host_flat(t):
+    return t.cpu().numpy().ravel()
+
+
+def _split_square(p):
+    """_split for experts that put out as many features as they take."""
+    E, K, H = EXPERTS, N_IN, HIDDEN
+    ends, bends = [0, E * K, E * K + E * H * K, E * K + 2 * E * H * K], [0, E, E + E * H, E + E * H + E * K]
+    shapes, bshapes = [(E, K), (E, H, K), (E, K, H)], [(E,), (E, H), (E, K)]
+    return [[x[ends[i]:ends[i + 1]].view(shapes[i]) for x in p[:2]] +
+            [x[bends[i]:bends[i + 1]].view(bshapes[i]) for x in p[2:]] for i in range(3)]
+
+
 def test_two_blocks_through_the_python_layer():
     """Blocks one behind the other, batches of different sizes: finite, and a step moves every
     layer's parameters."""
