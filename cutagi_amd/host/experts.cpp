@@ -117,7 +117,7 @@ void LayerNormHip::forward(BaseHiddenStates &input_states, BaseHiddenStates &out
                                  std::to_string(input_states.actual_size));
     if (this->output_size * batch_size > out->size)
         LOG(LogLevel::ERROR, "Output state buffer too small for " + this->get_layer_info());
-    if (d_mu_w == nullptr) LOG(LogLevel::ERROR, "Parameters of " + get_layer_info() + " are not on the device");
+    this->require_params(input_size, input_size);
     this->hold(batch_size);
     TAGI_OK_OR_THROW(tagi_layernorm_fwd(d_mu_w, d_var_w, d_mu_b, d_var_b, in->d_mu_a, in->d_var_a,
                                         bias ? 1 : 0, epsilon, (int)input_size, batch_size, d_mu_s,
@@ -312,7 +312,7 @@ void MixtureOfExpertsHip::forward(BaseHiddenStates &input_states, BaseHiddenStat
                                  std::to_string(input_states.actual_size));
     if (this->output_size * T > out->size)
         LOG(LogLevel::ERROR, "Output state buffer too small for " + this->get_layer_info());
-    if (d_mu_w == nullptr) LOG(LogLevel::ERROR, "Parameters of " + get_layer_info() + " are not on the device");
+    this->require_params(sizes.weights(), sizes.biases());
     this->hold(T);
     const Work w = this->work(T);
     const int K = (int)sizes.input, H = (int)sizes.hidden, N = (int)sizes.output;

@@ -172,6 +172,14 @@ void BaseLayerHip::allocate_param_memory() {
     }
 }
 
+void BaseLayerHip::require_params(size_t weights, size_t biases) {
+    if (d_mu_w == nullptr) LOG(LogLevel::ERROR, "Parameters of " + get_layer_info() + " are not on the device");
+    if (alloc_w != weights || (bias && alloc_b != biases))
+        LOG(LogLevel::ERROR, "Parameters of " + get_layer_info() + ": " + std::to_string(alloc_w) + " weights and " +
+                                 std::to_string(alloc_b) + " biases, expected " + std::to_string(weights) +
+                                 " and " + std::to_string(bias ? biases : 0));
+}
+
 void BaseLayerHip::allocate_param_delta() {
     BaseLayer::allocate_param_delta();
     freed += d_delta_mu_w != nullptr;

@@ -194,6 +194,9 @@ class BaseLayerHip : public BaseLayer {
    protected:
     void allocate_param_memory();
     void release_param_memory();
+    // Raises unless the device parameters have these numbers (a state dict or another model
+    // may have brought any).
+    void require_params(size_t weights, size_t biases);
     void store_states_for_training_hip(HiddenStateHip &input_states, HiddenStateHip &output_states);
     size_t alloc_w = 0, alloc_b = 0;  // sizes the device parameter arrays were allocated for
     bool neg_var_dirty = false;

@@ -454,6 +454,37 @@ def test_checkpoints(tmp_path):
     assert all(np.array_equal(a, b) for a, b in zip(want, third.get_outputs()))
 
 
+@pytest.mark.parametrize("where", ["device", "host", "model"])
+def test_parameters_of_other_sizes_are_refused(where):
+    """A state dict, or a model, of layers with other sizes under the same names: the forward
+    pass raises, and the right parameters put it right again."""
+    from cutagi_amd import cutagi
+    x = np.zeros((3, 12), np.float32)
+
+    def make(norm, experts, hidden=8, bias=True, device=True):
+        cutagi.manual_seed(0)
+        net = cutagi.Sequential([cutagi.LayerNorm([norm], 1e-5, bias),
+                                 cutagi.MixtureOfExperts(norm, hidden, 12, experts, 2, "relu", bias)])
+        if device:
+            net.to_device("cuda")
+        return net
+    for wrong in (make(10, 3), make(12, 2), make(12, 3, hidden=7), make(14, 3), make(12, 3, bias=False)):
+        net = make(12, 3, device=where != "host")
+        right = net.state_dict()
+        if where == "model":
+            net.params_from(wrong)
+        elif where == "device":
+            net.load_state_dict(wrong.state_dict())
+        else:
+            net.load_state_dict({k.replace("Cuda", ""): v for k, v in wrong.state_dict().items()})
+            net.to_device("cuda")
+        with pytest.raises(RuntimeError, match="expected"):
+            net.forward(x)
+        net.load_state_dict({(k if "Cuda" in k else k.replace(".", "Cuda.")): v for k, v in right.items()})
+        net.forward(x)
+        assert all(np.all(np.isfinite(a)) for a in net.get_outputs())
+
+
 def test_refusals():
     from cutagi_amd import cutagi
     net = _net(cutagi, first=False)
