@@ -43,9 +43,9 @@ constexpr int MAX_GROUPS = 1024;
 // second half and the first half of unit u + 1 are read from LDS and unit u + 2 is written.
 //
 // Bound by the matrix instructions at the clock that the power limit leaves: the forward of
-// 8192 rows, 8 experts of 2048 -> 4096, takes 2070 us (1.20 PFLOP/s of bf16 products, 199 TFLOP/s
+// 8192 rows, 8 experts of 2048 -> 4096, takes 2085 us (1.19 PFLOP/s of bf16 products, 198 TFLOP/s
 // of fp32 ones, where the fp32 matrix instructions end at 157) and 1611 us with nothing but its
-// matrix instructions left; the backward of 4096 -> 2048 takes 2990 us. (2815 us for the forward
+// matrix instructions left; the backward of 4096 -> 2048 takes 2943 us. (2815 us for the forward
 // with 16-element units, half lines per load and fragments read when they were needed; 8105 us
 // with fp32 products on plain tiles.)
 // ---------------------------------------------------------------------------

@@ -53,8 +53,8 @@ __device__ __forceinline__ floatx4 settle(floatx4 v, int k, int end) {
 // [n0 + i][k + 4 s .. + 3] and row i's activations at the same k; component t of both meets in
 // MFMA t. A wave takes every WAVES-th 32-element piece (a 128-byte line of each weight row) and
 // has the next piece's loads in flight while it multiplies. Bound by the weights: 64 rows, 16
-// experts of 2048 -> 4096, in 180 us, 6.0 TB/s; one token's two of 8 experts of 4096 -> 4096 in
-// 58 us, 4.7 TB/s.
+// experts of 2048 -> 4096, in 178 us back to back, 6.0 TB/s (239 us, 195 at best, where a pause
+// precedes every call); one token's two of 8 experts of 4096 -> 4096 in 58 us, 4.6 TB/s.
 // ---------------------------------------------------------------------------
 template <int NG, bool VEC>
 struct FwdPiece {

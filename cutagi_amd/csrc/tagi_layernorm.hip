@@ -37,8 +37,8 @@ __device__ __forceinline__ void row_sum(float (&v)[NV], float (*s)[TPB / 64]) {
 
 // ---------------------------------------------------------------------------
 // Forward. THREADS threads hold one row, PER groups of four features each; PER == 0: a row of
-// any length, read three times. Bound by memory, 16 bytes per element: 16384 x 4096 in 200 us,
-// 5.4 TB/s.
+// any length, read three times. Bound by memory, 16 bytes per element: 16384 x 4096 in 195 us,
+// 5.5 TB/s.
 // ---------------------------------------------------------------------------
 template <int THREADS, int PER>
 __global__ __launch_bounds__(TPB) void ln_fwd_kernel(
@@ -150,7 +150,7 @@ __global__ __launch_bounds__(TPB) void ln_fwd_kernel(
 // neighbouring groups of four columns, the other bits of the thread index are rows. A thread
 // keeps its columns' four sums over the rows it walks; the row threads of a wave are joined by
 // lane exchanges, the waves through LDS. The sums go to part ([chunk][4][n]), or where there is
-// one chunk only to the innovations. Bound by memory, 24 bytes per element: 16384 x 4096 in 311
+// one chunk only to the innovations. Bound by memory, 24 bytes per element: 16384 x 4096 in 310
 // us, 5.2 TB/s.
 // ---------------------------------------------------------------------------
 struct ParamOut {

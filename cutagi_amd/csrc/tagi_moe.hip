@@ -22,8 +22,8 @@ constexpr int TPB = 256;
 // A round is a chain of dependent instructions and bound by their latency: the maximum goes
 // through lane permutations inside the vector unit (16384 tokens, 64 experts, 4 choices, whole
 // call: 129 us with the ones through LDS and 128 tokens per workgroup, 24 us with these and 32,
-// of which this kernel takes 15.5, the scan 5.9 and the rows 3.7). 32 tokens of 16 experts go
-// through one launch: 4.0 us.
+// of which this kernel takes 15.4, the scan 6.1 and the rows 4.1 when each is timed by itself). 32
+// tokens of 16 experts go through one launch: 3.9 us.
 // ---------------------------------------------------------------------------
 constexpr int ROUTE_TOKENS = 32;   // tokens of a workgroup of the plan, a bit each
 

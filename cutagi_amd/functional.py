@@ -457,7 +457,10 @@ def grouped_linear_fwd(mu_w, var_w, mu_b, var_b, mu_a, var_a, offsets, rows=None
     """Linear layers [E, N, K], rows grouped by expert: rows offsets[e] .. offsets[e+1] meet
     the weights of expert e (offsets: int32 [E+1]). rows (int32 [R]): row r is row rows[r] of
     mu_a / var_a; without it mu_a / var_a [R, K] hold the rows in order. Returns (mu_z, var_z)
-    [R, N]; rows from offsets[E] on are left as `out` held them (unset without `out`)."""
+    [R, N]; rows from offsets[E] on are left as `out` held them (unset without `out`).
+    Which kernels a call runs on depends on all of its sizes; some take fp32 numbers apart into
+    three bf16 parts, and there (here and in grouped_linear_bwd) an infinity may come out as
+    NaN and numbers below 3e-33 count with less than fp32's precision."""
     return _grouped_fwd(mu_w, var_w, mu_b, var_b, mu_a, var_a, offsets, rows, None, out)
 
 
