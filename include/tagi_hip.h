@@ -22,8 +22,9 @@
  *     per (GPU, stream) for split-reduction partial sums (see
  *     tagi_hip_workspace_reserve), so calls on different streams never share
  *     scratch memory; an outgrown workspace stays allocated until
- *     tagi_hip_shutdown, because graphs that were recorded with it use it; calls issued to ONE stream from several host threads must be
- *     serialised by the caller, as with any stream-ordered API.
+ *     tagi_hip_shutdown, because graphs that were recorded with it use it; calls
+ *     issued to ONE stream from several host threads must be serialised by the
+ *     caller, as with any stream-ordered API.
  */
 #ifndef TAGI_HIP_H
 #define TAGI_HIP_H
@@ -48,7 +49,8 @@ int tagi_hip_version(void);
 int tagi_hip_device_count(int *count /* host, out */);
 const char *tagi_hip_error_string(int code);
 /* Grow the workspace of `stream` on the current device to at least `bytes` now (and to
- * twice its size where it has to grow and that fits). Optional: entry points grow it on demand. */
+ * twice its size where it has to grow and that fits). Optional: entry points grow it
+ * on demand. */
 int tagi_hip_workspace_reserve(size_t bytes, void *stream);
 /* Free the workspaces of all devices, those too that recorded graphs use. */
 int tagi_hip_shutdown(void);
